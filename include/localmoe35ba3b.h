@@ -315,6 +315,77 @@ int lm_rmsnorm(const void *x, const float *w, void *y, int64_t rows,
                int64_t n, float eps, void *stream);
 
 /* ---------------------------------------------------------------------
+ * Attention between the MoE blocks.  No counterpart among the reference's
+ * operators (it runs the Transformers modules): for rows of heads of 64, 128
+ * or 256 channels, bf16 or fp16, whose channels are contiguous; token and head
+ * strides are in elements and multiples of 8, and every data pointer is
+ * 16-byte aligned.
+ *
+ * Norms of queries and keys for each head, and the position rotation, in one
+ * pass:
+ *   n = x * rsqrt(mean_d x^2 + eps) * (1 + w)          (weight NULL: n = x)
+ *   y_i = n_i cos a - n_{i+pairs} sin a, y_{i+pairs} = n_{i+pairs} cos a + n_i sin a
+ * with a = positions[t] * inv_freq[i] for i < pairs (formed in fp64), the
+ * channels from 2 * pairs on y = n; fp32 throughout, rounded once.  pairs is a
+ * multiple of 8 (inv_freq NULL and pairs 0: no rotation).  Outputs are
+ * contiguous [tokens, heads, head_dim]; heads 0 leaves a side out. */
+int lm_qk_norm_rope(const void *q, int64_t q_token_stride, int64_t q_head_stride,
+                    int64_t q_heads, const float *q_weight, void *q_out,
+                    const void *k, int64_t k_token_stride, int64_t k_head_stride,
+                    int64_t k_heads, const float *k_weight, void *k_out,
+                    const int64_t *positions, const float *inv_freq, int64_t pairs,
+                    int64_t tokens, int64_t head_dim, float eps, int dtype,
+                    void *stream);
+
+/* Appends keys and values to a paged cache, the keys normed and rotated on the
+ * way as in lm_qk_norm_rope, and gives the queries of the same tokens the same
+ * treatment (q_heads 0: none).
+ * The batch: sequence s's new tokens are rows starts[s] .. starts[s+1] - 1
+ * (starts ascending, [sequences + 1]) and the last of its lengths[s] positions;
+ * position p lives in row p % page_size of page table[s * table_stride +
+ * p / page_size], table_pages entries a sequence.  A page holds [kv_heads,
+ * page_size, head_dim] values, pages lie page_stride elements apart, page_size
+ * is a power of two from 16 to 1024.  Rows of no sequence are left as they
+ * were, in q_out and the cache; a position outside the table is not written.
+ * Page numbers are clamped into [0, pages).  The pages written by one call
+ * belong to one sequence each. */
+int lm_paged_append(const void *k, int64_t k_token_stride, int64_t k_head_stride,
+                    const float *k_weight, const void *v, int64_t v_token_stride,
+                    int64_t v_head_stride, const void *q, int64_t q_token_stride,
+                    int64_t q_head_stride, int64_t q_heads, const float *q_weight,
+                    void *q_out, void *k_pages, void *v_pages, int64_t pages,
+                    int64_t page_stride, int64_t kv_heads, int64_t page_size,
+                    int64_t head_dim, const int32_t *starts, const int32_t *lengths,
+                    const int32_t *table, int64_t table_stride, int64_t table_pages,
+                    int64_t sequences, const float *inv_freq, int64_t pairs,
+                    int64_t tokens, float eps, int dtype, void *stream);
+
+/* Attention of the new tokens over the cache (the batch of lm_paged_append):
+ * the row at position p of its sequence sees the positions up to p,
+ *   o = sum_j softmax_j(scale * q . k_j) v_j, times sigmoid(gate) if gate != NULL
+ * in fp32 (the weights rounded to dtype for their product with the values),
+ * rounded once; a row that sees no key is 0, rows of no sequence are left as
+ * they were.  q_heads is a multiple of kv_heads; out is contiguous [tokens,
+ * q_heads, head_dim].  max_new bounds the new tokens of a sequence: sequences
+ * with more get results for the first max_new only.  workspace holds
+ * lm_paged_attention_workspace_bytes (0: none is needed), 16-byte aligned; its
+ * contents need no initialization.  A call's result does not depend on what
+ * else is in the batch's unused pages, nor on other rows' values. */
+int64_t lm_paged_attention_workspace_bytes(int64_t tokens, int64_t sequences,
+                                           int64_t q_heads, int64_t kv_heads,
+                                           int64_t head_dim, int64_t max_new);
+int lm_paged_attention(const void *q, int64_t q_token_stride, int64_t q_head_stride,
+                       int64_t q_heads, const void *k_pages, const void *v_pages,
+                       int64_t pages, int64_t page_stride, int64_t kv_heads,
+                       int64_t page_size, int64_t head_dim, const int32_t *starts,
+                       const int32_t *lengths, const int32_t *table,
+                       int64_t table_stride, int64_t table_pages, int64_t sequences,
+                       int64_t tokens, int64_t max_new, float scale, const void *gate,
+                       int64_t gate_token_stride, int64_t gate_head_stride, void *out,
+                       void *workspace, int64_t workspace_bytes, int dtype,
+                       void *stream);
+
+/* ---------------------------------------------------------------------
  * Fused MoE-FFN block of the synthetic stack (router + 256 routed experts
  * top-8 + shared expert + RMSNorm + residual; HF:779-798, 801-815, 866-875).
  * One layer's weights:

@@ -61,6 +61,13 @@ SIGNATURES = {
     'lm_router_workspace_pays': (I32, [I64, I64, I64]),
     'lm_router_topk_ws': (I32, [P, P, P, P, P, P, I64, I64, I64, I64, P, I64, P]),
     'lm_rmsnorm': (I32, [P, P, P, I64, I64, F32, P]),
+    'lm_qk_norm_rope': (I32, [P, I64, I64, I64, P, P, P, I64, I64, I64, P, P, P, P, I64, I64, I64,
+                              F32, I32, P]),
+    'lm_paged_append': (I32, [P, I64, I64, P, P, I64, I64, P, I64, I64, I64, P, P, P, P, I64, I64,
+                              I64, I64, I64, P, P, P, I64, I64, I64, P, I64, I64, F32, I32, P]),
+    'lm_paged_attention_workspace_bytes': (I64, [I64, I64, I64, I64, I64, I64]),
+    'lm_paged_attention': (I32, [P, I64, I64, I64, P, P, I64, I64, I64, I64, I64, P, P, P, I64,
+                                 I64, I64, I64, I64, F32, P, I64, I64, P, P, I64, I32, P]),
     'lm_moe_workspace_bytes': (I64, [I64, I64, I64, I64, I64]),
     'lm_moe_workspace_init': (I32, [P, I64, P]),
     'lm_moe_workspace_region': (I32, [I64, I32, P, P]),
@@ -131,6 +138,14 @@ def call(name, *args):
     rc = _fns[name](*args)
     if rc:
         check(rc)
+
+
+def call_on(device, name, *args):
+    """call with `device` current, for streams and the null stream of that device."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return call(name, *args)
+    with torch.cuda.device(device):
+        call(name, *args)
 
 
 def ptr(t):
