@@ -366,14 +366,17 @@ int lm_paged_append(const void *k, int64_t k_token_stride, int64_t k_head_stride
  * in fp32 (the weights rounded to dtype for their product with the values),
  * rounded once; a row that sees no key is 0, rows of no sequence are left as
  * they were.  q_heads is a multiple of kv_heads; out is contiguous [tokens,
- * q_heads, head_dim].  max_new bounds the new tokens of a sequence: sequences
- * with more get results for the first max_new only.  workspace holds
- * lm_paged_attention_workspace_bytes (0: none is needed), 16-byte aligned; its
- * contents need no initialization.  A call's result does not depend on what
- * else is in the batch's unused pages, nor on other rows' values. */
+ * q_heads, head_dim].  max_new bounds the new tokens of a sequence (tokens is
+ * always right); rows of sequences with more may be left unwritten.  workspace
+ * holds lm_paged_attention_workspace_bytes (max_keys = table_pages * page_size;
+ * 0: none is needed), 16-byte aligned; its contents need no initialization, and
+ * calls that overlap need one each.  Nothing that a row does not see reaches its
+ * result, infinities and NaN in unused rows of pages or later positions
+ * included. */
 int64_t lm_paged_attention_workspace_bytes(int64_t tokens, int64_t sequences,
                                            int64_t q_heads, int64_t kv_heads,
-                                           int64_t head_dim, int64_t max_new);
+                                           int64_t head_dim, int64_t max_new,
+                                           int64_t max_keys);
 int lm_paged_attention(const void *q, int64_t q_token_stride, int64_t q_head_stride,
                        int64_t q_heads, const void *k_pages, const void *v_pages,
                        int64_t pages, int64_t page_stride, int64_t kv_heads,

@@ -65,7 +65,7 @@ SIGNATURES = {
                               F32, I32, P]),
     'lm_paged_append': (I32, [P, I64, I64, P, P, I64, I64, P, I64, I64, I64, P, P, P, P, I64, I64,
                               I64, I64, I64, P, P, P, I64, I64, I64, P, I64, I64, F32, I32, P]),
-    'lm_paged_attention_workspace_bytes': (I64, [I64, I64, I64, I64, I64, I64]),
+    'lm_paged_attention_workspace_bytes': (I64, [I64, I64, I64, I64, I64, I64, I64]),
     'lm_paged_attention': (I32, [P, I64, I64, I64, P, P, I64, I64, I64, I64, I64, P, P, P, I64,
                                  I64, I64, I64, I64, F32, P, I64, I64, P, P, I64, I32, P]),
     'lm_moe_workspace_bytes': (I64, [I64, I64, I64, I64, I64]),

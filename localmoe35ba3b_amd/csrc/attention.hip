@@ -1,86 +1,915 @@
 // Attention of each sequence's new tokens over its paged cache (gfx950).
 //
-//   o_t = sum_{j <= p_t} e^{scale q_t.k_j - m_t} v_j / sum_j e^{scale q_t.k_j - m_t}
+//   o_t = sum_{j <= p_t} e^{x_j - m} v_j / sum_j e^{x_j - m},   x_j = scale q_t . k_j
 //
 // causal at the end of the sequence, times sigmoid(gate_t) where a gate is given;
-// a row without a visible key is 0.
+// a row without a visible key is 0.  One pass over the keys with a running m and
+// sum (exponentials in base 2, fp32); m follows the maximum only when that has
+// grown by more than 2^kSlack, so the accumulated rows are rarely rescaled.
 //
-// One wave takes one (token, query head) and walks its keys 64 at a time: lane j
-// forms key j's score, then the wave adds the weighted values, each lane its
-// D / 64 channels.
+// Both kernels form the transposed products.  S^T = K Q^T leaves a lane with one
+// query (its column) and a few consecutive keys, so a column's statistics are the
+// lane's own, and the weights are already the operand of O^T = V^T P^T: the keys
+// of a lane's C registers are the k indices its operand registers hold.  V^T comes
+// from the row-major V tile by the LDS transpose read, four keys of one channel a
+// lane.  K and V go from the cache into LDS by direct loads, whole rows at a time,
+// the 16-byte pieces of a row permuted (swizzle) so that neither read meets a bank
+// conflict.
+//
+//  attention_few_kernel   sequences of at most 16 rows (new tokens x query heads of
+//                         a key-value head): bound by the cache's bytes.  16-column
+//                         tiles; the waves of a workgroup split its keys, each with
+//                         a ring of its own in LDS, so nothing waits for another
+//                         wave; the keys of a sequence are split over workgroups by
+//                         their share of all keys of the call.
+//  attention_tile_kernel  longer ones: bound by the matrix cores.  128 rows a
+//                         workgroup, 32 a wave, over shared 32-key tiles; few tiles
+//                         split their keys over workgroups too.
+//  attention_combine_*    joins the parts of split keys.
 #include "paged.hpp"
 
 namespace lm {
 namespace {
+
+#define LDS __attribute__((address_space(3)))
+#define GLB __attribute__((address_space(1)))
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 struct Attention {
   const uint16_t *q, *gate;  // gate: null or a row for each row of q
   int64_t q_token, q_head, gate_token, gate_head;  // strides, elements
   const uint16_t *k_pages, *v_pages;
   uint16_t *out;  // [tokens][q_heads][D]
+  float *part;    // unscaled sums of split keys, then (m, l) of each row
+  float *part_ml;
   PagedBatch batch;
   int tokens, q_heads, group;
-  float scale;
+  int shares;  // few: parts a key-value head's keys are cut into, about
+  int splits;  // tile: parts of each tile's keys
+  bool few;    // tile: sequences of few rows are attention_few_kernel's
+  float scale2;  // scale * log2(e)
 };
 
-template <typename T, int D>
-__global__ __launch_bounds__(64) void attention_row_kernel(Attention a) {
-  const int t = blockIdx.x, head = blockIdx.y, lane = threadIdx.x;
-  const int s = paged_find(a.batch, t);
-  if (s < 0) return;  // a row of no sequence keeps its output
-  const PagedSequence seq = paged_sequence(a.batch, s, a.tokens);
-  const int keys = min(seq.base + (t - seq.first) + 1, seq.length);
-  const int kv = head / a.group, shift = a.batch.page_shift, mask = (1 << shift) - 1;
-  constexpr int C = D / 64;
-  __shared__ float qs[D], ps[64];
-  for (int i = lane; i < D; i += 64)
-    qs[i] = T::to_f32(a.q[t * a.q_token + head * a.q_head + i]) * a.scale;
-  __syncthreads();
-  float m = -INFINITY, l = 0.0f, o[C] = {};
-  for (int k0 = 0; k0 < keys; k0 += 64) {
-    const int j = k0 + lane;
-    float x = -INFINITY;
-    if (j < keys) {
-      const uint16_t *kr =
-          a.k_pages + paged_page(a.batch, s, j) + ((int64_t)(kv << shift) + (j & mask)) * D;
-      x = 0.0f;
-      for (int i = 0; i < D; ++i) x = __builtin_fmaf(qs[i], T::to_f32(kr[i]), x);
-    }
-    float mx = x;
-    for (int i = 32; i >= 1; i >>= 1) mx = fmaxf(mx, __shfl_xor(mx, i, 64));
-    const float mn = fmaxf(m, mx), at = mn == -INFINITY ? 0.0f : mn;
-    const float keep = expf(m - at), p = expf(x - at);
-    m = mn;
-    l = l * keep + wave_sum_f32(p);
-    ps[lane] = p;
-    __syncthreads();
-    for (int c = 0; c < C; ++c) o[c] *= keep;
-    for (int i = 0; i < min(64, keys - k0); ++i) {
-      const uint16_t *vr = a.v_pages + paged_page(a.batch, s, k0 + i) +
-                           ((int64_t)(kv << shift) + ((k0 + i) & mask)) * D;
-      for (int c = 0; c < C; ++c)
-        o[c] = __builtin_fmaf(ps[i], T::to_f32(vr[c * 64 + lane]), o[c]);
-    }
-    __syncthreads();
+constexpr int kFewRows = 16;    // columns of the few-row kernel
+constexpr int kTileRows = 128;  // rows of a tile
+constexpr float kSlack = 8.0f;  // weights stay below 2^8: exact sums in fp32, finite in fp16
+
+__device__ __forceinline__ f32x4 mfma16(BF16, u32x4 a, u32x4 b, f32x4 c) {
+  return BF16::mfma16x16x32(a, b, c);
+}
+__device__ __forceinline__ f32x4 mfma16(FP16, u32x4 a, u32x4 b, f32x4 c) {
+  return FP16::mfma16x16x32(a, b, c);
+}
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f32x4 mfma16k16(BF16, u32x2 a, u32x2 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a),
+                                                   __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16k16(FP16, u32x2 a, u32x2 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a),
+                                               __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma32(BF16, u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                 __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma32(FP16, u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Exchanges between the 16-lane rows (xor 16) and the halves (xor 32) of a wave.
+template <typename F>
+__device__ __forceinline__ float across16(float v, F f) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+template <typename F>
+__device__ __forceinline__ float across32(float v, F f) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+struct Max {
+  __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+struct Add {
+  __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+};
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+// 2^(m - n) of two running maxima, n >= m; both may be -inf.
+__device__ __forceinline__ float decay(float m, float n) { return m == n ? 1.0f : exp2_hw(m - n); }
+
+// Piece c (16 bytes) of row r of a tile lies at place c ^ swizzle(r) of the row: rows of
+// one bank group (a row is D * 2 bytes, the banks repeat every 256) get different places.
+// Linear over disjoint bits of r, so a read's lane part is formed once and its constant
+// part is one exclusive or.
+template <int D>
+__device__ __forceinline__ constexpr int swizzle(int r) {
+  return D == 64 ? (r >> 1) & 7 : r & 15;
+}
+
+// ROWS rows of a page, from `src` (row `row0` of the tile), into LDS: wave-wide loads of
+// 1 KB, lane-linear in LDS, so the swizzle permutes the source.  Rows behind a sequence's
+// end are loaded as they are (their page holds them) and masked later.  A loop, not
+// unrolled: the compiler tells apart the targets of a few such instructions only, and
+// waits for all of them before any LDS read when there are more.
+template <int D, int ROWS>
+__device__ __forceinline__ void load_rows(const uint16_t *src, int row0, LDS char *to, int lane) {
+  constexpr int PIECES = D / 8, PER = 64 / PIECES;
+  const int own = lane / PIECES;
+  const uint32_t off = own * (D * 2) + (((lane % PIECES) ^ swizzle<D>(own)) << 4);
+  const GLB char *from = (const GLB char *)src;
+#pragma clang loop unroll(disable)
+  for (int i = 0; i < ROWS / PER; ++i)
+    __builtin_amdgcn_global_load_lds(
+        (const GLB void *)(from + i * 1024 + (off ^ (swizzle<D>(row0 + i * PER) << 4))),
+        (LDS void *)(to + i * 1024), 16, 0, 0);
+}
+
+// Has v loaded here, so that no wait for it is placed in a loop over direct loads, where it
+// would wait for those too.
+template <typename V>
+__device__ __forceinline__ void settle(V &v) {
+  asm volatile("" : "+v"(v));
+}
+
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// Four keys of one channel, by the LDS transpose read: lane i of each 16 lanes gets channel
+// d0 + i of rows r .. r + 3, r = row + ROW and d0 = d + CH with the lane's own row (a multiple
+// of 4) and d (0 or 16) in `base` (transpose_base), the rest constant.
+template <int D>
+__device__ __forceinline__ int transpose_base(int row, int d, int lane) {
+  const int r = row + (lane & 15) / 4;
+  return r * (D * 2) + (((d / 8 + (lane & 3) / 2) ^ swizzle<D>(r)) << 4) + (lane & 1) * 8;
+}
+template <int D>
+__device__ __forceinline__ u32x2 read_transposed(const LDS char *tile, int base, int row, int ch) {
+  const LDS char *p = tile + (base ^ ((ch / 8 ^ swizzle<D>(row)) << 4)) + row * (D * 2);
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS s16x4 *)p));
+}
+
+// Keeps a lane's base from being expanded into one register for every constant part.
+__device__ __forceinline__ int opaque(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+// Values of keys that some row does not see: a weight of 0 must not meet an infinity or
+// NaN (0 * inf).  The products take the finite values of a pair, 0 for others; where there
+// were any, the rows that do see such a key get it added afterwards.
+template <typename T>
+struct Pair {
+  static constexpr uint32_t E = __is_same(T, BF16) ? 0x7F80u : 0x7C00u;  // infinity
+  static __device__ __forceinline__ uint32_t finite(uint32_t v, bool &odd) {
+    const bool lo = (v & E) == E, hi = (v & (E << 16)) == (E << 16);
+    odd |= lo || hi;
+    return (lo ? 0u : v & 0xFFFFu) | (hi ? 0u : v & 0xFFFF0000u);
   }
-  for (int c = 0; c < C; ++c) {
-    const int i = c * 64 + lane;
-    float y = keys > 0 ? o[c] / l : 0.0f;
-    if (a.gate) y *= sigmoid_f32(T::to_f32(a.gate[t * a.gate_token + head * a.gate_head + i]));
-    a.out[((int64_t)t * a.q_heads + head) * D + i] = T::from_f32(y);
+  static __device__ __forceinline__ float odd_part(uint32_t x) {
+    return (x & E) == E ? T::to_f32(x) : 0.0f;
+  }
+};
+
+// The infinities and NaN among four channels, 0 for others.
+template <typename T>
+__device__ __forceinline__ f32x4 odd_parts(const uint16_t *v) {
+  const uint2 w = ldg_u2(v);
+  return f32x4{Pair<T>::odd_part(w.x & 0xFFFFu), Pair<T>::odd_part(w.x >> 16),
+               Pair<T>::odd_part(w.y & 0xFFFFu), Pair<T>::odd_part(w.y >> 16)};
+}
+
+// Value row of key k of sequence s at the key-value head whose rows begin at `head`.
+template <int D>
+__device__ __forceinline__ const uint16_t *value_row(const Attention &a, int s, int64_t head, int k) {
+  return a.v_pages + paged_page(a.batch, s, k) + head +
+         (int64_t)(k & ((1 << a.batch.page_shift) - 1)) * D;
+}
+
+// ------------------------------------------------------------------ shares of keys
+// The keys of the sequences with few rows, in blocks of 64, are cut into about
+// `shares` parts: n_s = ceil(blocks_s * shares / all blocks) of sequence s, at most its
+// blocks.  Every workgroup works this out from the lengths, so the host needs to know
+// none of them and a captured call follows them.
+struct Share {
+  int s, split, n;  // part `split` of sequence s's n; s < 0: none
+  int slot;         // of part 0 among the parts of sequences with several
+};
+
+constexpr int kBlockKeys = 64;
+
+// count > 0 of a sequence whose rows fit the few-row kernel
+__device__ __forceinline__ bool few_rows(const PagedSequence &q, int group) {
+  return q.count > 0 && q.count <= kFewRows / group;
+}
+__device__ __forceinline__ int few_blocks(const Attention &a, int s) {
+  if (s >= a.batch.sequences) return 0;
+  const PagedSequence q = paged_sequence(a.batch, s, a.tokens);
+  return few_rows(q, a.group) ? max((q.length + kBlockKeys - 1) / kBlockKeys, 1) : 0;
+}
+
+// The share with index `index` (by_sequence: of sequence `index`, split 0).  All 256
+// threads; scratch (8 words of LDS) and found are free again afterwards.
+__device__ Share find_share(const Attention &a, int index, bool by_sequence, uint64_t *scratch,
+                            Share *found) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, S = a.batch.sequences;
+  if (tid == 0) found->s = -1;
+  const int mine = few_blocks(a, tid);
+  uint64_t all = mine;
+  for (int s = tid + 256; s < S; s += 256) all += few_blocks(a, s);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) all += __shfl_xor(all, o, 64);
+  if (lane == 0) scratch[wave] = all;
+  __syncthreads();
+  all = scratch[0] + scratch[1] + scratch[2] + scratch[3];
+  uint64_t base = 0;  // parts before this group of 256 sequences, those of split ones above
+  for (int c = 0; c < S; c += 256) {
+    const int s = c + tid;
+    const uint64_t blocks = c == 0 ? mine : few_blocks(a, s);
+    const uint64_t n = blocks ? min(blocks, (blocks * a.shares + all - 1) / all) : 0;
+    uint64_t sum = n | (n > 1 ? n << 32 : 0);
+    const uint64_t own = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint64_t v = __shfl_up(sum, o, 64);
+      if (lane >= o) sum += v;
+    }
+    __syncthreads();
+    if (lane == 63) scratch[4 + wave] = sum;
+    __syncthreads();
+    uint64_t before = base;
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) before += scratch[4 + w];
+      base += scratch[4 + w];
+    }
+    before += sum - own;
+    const int first = (int)(uint32_t)before, slot = (int)(before >> 32);
+    if (by_sequence ? s == index && n > 0 : index >= first && index < first + (int)n)
+      *found = {s, by_sequence ? 0 : index - first, (int)n, slot};
+  }
+  __syncthreads();
+  const Share got = *found;
+  __syncthreads();
+  return got;
+}
+
+// ------------------------------------------------------------------ few rows
+constexpr int kFewWaves = 4;
+
+// Ring of a wave: keys and values of two 16-key steps.
+template <int D>
+constexpr int few_ring() { return 4 * 16 * D * 2; }
+template <int D>
+constexpr int few_merge() { return kFewWaves * (kFewRows * (D + 4) + 2 * kFewRows) * 4; }
+template <int D>
+constexpr int few_lds() {
+  return kFewWaves * few_ring<D>() > few_merge<D>() ? kFewWaves * few_ring<D>() : few_merge<D>();
+}
+
+// The running state of a wave's 16 columns (column lane & 15 in each 16 lanes).
+template <int D>
+struct FewState {
+  float m = -INFINITY, l = 0.0f;  // l: this lane's keys only
+  f32x4 o[D / 16] = {};           // channels 16 i + 4 (lane >> 4) .. + 3
+  bool odd = false;               // infinities or NaN were left out
+};
+
+// Products of one 16-key step with the columns: the weights of keys 4 g .. 4 g + 3, packed.
+template <typename T, int D>
+__device__ __forceinline__ u32x2 few_scores(const LDS char *kt, const u32x4 (&q)[D / 32], int key0,
+                                            int limit, float scale2, FewState<D> &st, int lane) {
+  const int g = lane >> 4, r = lane & 15;
+  const int base = opaque(r * (D * 2) + ((g ^ swizzle<D>(r)) << 4));
+  f32x4 s[2] = {};
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    const u32x4 k = *(const LDS u32x4 *)(kt + (base ^ (i << 6)));
+    s[i & 1] = mfma16(T{}, k, q[i], s[i & 1]);
+  }
+  float x[4], mx = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[i] = key0 + g * 4 + i < limit ? (s[0][i] + s[1][i]) * scale2 : -INFINITY;
+    mx = fmaxf(mx, x[i]);
+  }
+  mx = across32(across16(mx, Max()), Max());
+  if (__any(mx > st.m + kSlack)) {
+    const float n = fmaxf(st.m, mx), keep = decay(st.m, n);
+    st.m = n;
+    st.l *= keep;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) st.o[i] *= keep;
+  }
+  const float at = st.m == -INFINITY ? 0.0f : st.m;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[i] = exp2_hw(x[i] - at);
+    st.l += x[i];
+  }
+  return u32x2{T::pack2(x[0], x[1]), T::pack2(x[2], x[3])};
+}
+
+// Adds the weighted values of a 16-key step; `mixed`: some row does not see all its keys.
+template <typename T, int D>
+__device__ __forceinline__ void few_values(const LDS char *vt, u32x2 p, bool mixed,
+                                           FewState<D> &st, int lane) {
+  const int base = opaque(transpose_base<D>((lane >> 4) * 4, 0, lane));
+  if (!mixed) {
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+      st.o[i] = mfma16k16(T{}, read_transposed<D>(vt, base, 0, i * 16), p, st.o[i]);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+    const u32x2 v = read_transposed<D>(vt, base, 0, i * 16);
+    st.o[i] = mfma16k16(T{}, u32x2{Pair<T>::finite(v[0], st.odd), Pair<T>::finite(v[1], st.odd)},
+                        p, st.o[i]);
   }
 }
 
+// The keys of a wave: steps of 16 keys, `stride` steps apart, and the pages they lie in.
+struct FewKeys {
+  const uint16_t *k, *v;  // of the key-value head, in page 0
+  const int32_t *table;
+  int64_t page_stride;
+  int shift, pages, entries;
+  int first, stride, steps;  // first step's number, and how many
+  int page_of;               // pages of 64 steps, one a lane
+};
+
+__device__ __forceinline__ void few_pages(FewKeys &f, int from, int lane) {
+  const int step = f.first + min(from + lane, max(f.steps - 1, 0)) * f.stride;
+  const int i = min((step * 16) >> f.shift, f.entries - 1);
+  f.page_of = clamp_index32(f.table[i], f.pages);
+  settle(f.page_of);
+}
+
+// Loads step i's rows of one side (a step past the end: again the last, never used).
+template <int D>
+__device__ __forceinline__ void few_load(const FewKeys &f, const uint16_t *side, int i,
+                                         LDS char *to, int lane) {
+  const int j = min(i, f.steps - 1), key = (f.first + j * f.stride) * 16;
+  const int page = __builtin_amdgcn_readlane(f.page_of, j & 63);
+  const uint16_t *src = side + page * f.page_stride + (int64_t)(key & ((1 << f.shift) - 1)) * D;
+  load_rows<D, 16>(src, 0, to, lane);
+}
+
+// Two steps, i and i + 1, each from its own half of the ring, refilled for i + 2 and
+// i + 3 as soon as it is read.  The four regions are disjoint (restrict), so the compiler
+// does not take a read of one to wait for the loads into the others; the counts of loads
+// that may still be out are stated here.
+template <typename T, int D>
+__device__ __forceinline__ void few_steps(LDS char *__restrict__ k0, LDS char *__restrict__ v0,
+                                          LDS char *__restrict__ k1, LDS char *__restrict__ v1,
+                                          const FewKeys &f, const u32x4 (&q)[D / 32], int i,
+                                          int limit, int all_see, float scale2, FewState<D> &st,
+                                          int lane) {
+  constexpr int N = 16 * D * 2 / 1024;  // loads of one side of a step
+  int key = (f.first + i * f.stride) * 16;
+  wait_loads<3 * N>();
+  u32x2 p = few_scores<T, D>(k0, q, key, limit, scale2, st, lane);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  few_load<D>(f, f.k, i + 2, k0, lane);
+  wait_loads<3 * N>();
+  few_values<T, D>(v0, p, key + 16 > all_see, st, lane);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  few_load<D>(f, f.v, i + 2, v0, lane);
+  if (i + 1 >= f.steps) return;
+  key += f.stride * 16;
+  wait_loads<3 * N>();
+  p = few_scores<T, D>(k1, q, key, limit, scale2, st, lane);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  few_load<D>(f, f.k, i + 3, k1, lane);
+  wait_loads<3 * N>();
+  few_values<T, D>(v1, p, key + 16 > all_see, st, lane);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  few_load<D>(f, f.v, i + 3, v1, lane);
+}
+
+// Row c of a sequence's rows at a key-value head: new token c / group, query head
+// kv * group + c % group.
+struct RowPlace {
+  int64_t token;
+  int head;
+};
+__device__ __forceinline__ RowPlace row_place(const Attention &a, const PagedSequence &q, int kv,
+                                              int c) {
+  return {q.first + c / a.group, kv * a.group + c % a.group};
+}
+
+// sigmoid(x) by the hardware's exp2 and reciprocal; the argument's rounding, which far from
+// 0 would show in the result, is put back.
+__device__ __forceinline__ float sigmoid_hw(float x) {
+  constexpr float kHi = 1.4426950408889634f, kLo = 1.9259629911266175e-8f;  // log2(e)
+  const float t = -x * kHi, e = __builtin_fmaf(-x, kHi, -t) - x * kLo;
+  const float p = exp2_hw(t);
+  return __builtin_amdgcn_rcpf(1.0f + (t < 126.0f ? __builtin_fmaf(p, e * 0.6931472f, p) : p));
+}
+
+// Four channels from d of a finished row: scaled, gated, rounded once.
+template <typename T, int D>
+__device__ __forceinline__ void write_row(const Attention &a, RowPlace at, int d, f32x4 o,
+                                          float inv) {
+  o *= inv;
+  if (a.gate) {
+    const uint2 g = ldg_u2(a.gate + at.token * a.gate_token + at.head * a.gate_head + d);
+    o[0] *= sigmoid_hw(T::to_f32(g.x & 0xFFFFu));
+    o[1] *= sigmoid_hw(T::to_f32(g.x >> 16));
+    o[2] *= sigmoid_hw(T::to_f32(g.y & 0xFFFFu));
+    o[3] *= sigmoid_hw(T::to_f32(g.y >> 16));
+  }
+  *reinterpret_cast<uint2 *>(a.out + (at.token * a.q_heads + at.head) * D + d) =
+      uint2{T::pack2(o[0], o[1]), T::pack2(o[2], o[3])};
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, 1) void attention_few_kernel(Attention a) {
+  // One array: with several, the compiler waits for all direct loads at each LDS read.
+  __shared__ __attribute__((aligned(16))) char lds[few_lds<D>()];
+  uint64_t *scratch = reinterpret_cast<uint64_t *>(lds);
+  Share *found = reinterpret_cast<Share *>(scratch + 8);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kv = blockIdx.x % a.batch.kv_heads;
+  const Share sh = find_share(a, blockIdx.x / a.batch.kv_heads, false, scratch, found);
+  const int s = __builtin_amdgcn_readfirstlane(sh.s);
+  if (s < 0) return;
+  const PagedSequence seq = paged_sequence(a.batch, s, a.tokens);
+  const int rows = seq.count * a.group;
+  const int blocks = (seq.length + kBlockKeys - 1) / kBlockKeys;
+  const int b0 = (int)((int64_t)blocks * sh.split / sh.n);
+  const int b1 = (int)((int64_t)blocks * (sh.split + 1) / sh.n);
+
+  const int col = min(lane & 15, rows - 1), g = lane >> 4;
+  const RowPlace at = row_place(a, seq, kv, col);
+  u32x4 q[D / 32];
+  const uint16_t *qr = a.q + at.token * a.q_token + at.head * a.q_head;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) q[i] = ldg16(qr + i * 32 + g * 8);
+
+  FewKeys f;
+  const int64_t head = (int64_t)(kv << a.batch.page_shift) * D;
+  f.k = a.k_pages + head, f.v = a.v_pages + head;
+  f.table = a.batch.table + s * a.batch.table_stride;
+  f.page_stride = a.batch.page_stride, f.shift = a.batch.page_shift;
+  f.pages = a.batch.pages, f.entries = a.batch.table_pages;
+  const int last = min(b1 * (kBlockKeys / 16), (seq.length + 15) / 16);
+  f.first = b0 * (kBlockKeys / 16) + wave, f.stride = kFewWaves;
+  f.steps = last > f.first ? (last - f.first + kFewWaves - 1) / kFewWaves : 0;
+  const int limit = min(seq.base + col / a.group + 1, seq.length);
+  const int all_see = min(seq.base + 1, seq.length);  // keys that every row sees
+
+  FewState<D> st;
+  if (f.steps > 0) {
+    few_pages(f, 0, lane);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) settle(q[i]);
+    LDS char *ring = (LDS char *)lds + wave * few_ring<D>();
+    constexpr int TILE = 16 * D * 2;
+    for (int j = 0; j < 2; ++j) {  // in this order: the waits count what was issued later
+      few_load<D>(f, f.k, j, ring + 2 * j * TILE, lane);
+      asm volatile("" ::: "memory");
+      few_load<D>(f, f.v, j, ring + (2 * j + 1) * TILE, lane);
+      asm volatile("" ::: "memory");
+    }
+    for (int i = 0; i < f.steps; i += 2) {
+      // steps i + 2 and i + 3 are loaded next: their pages from the next 64 on
+      if (((i + 2) & 63) == 0) few_pages(f, i + 2, lane);
+      few_steps<T, D>(ring, ring + TILE, ring + 2 * TILE, ring + 3 * TILE, f, q, i, limit, all_see,
+                      a.scale2, st, lane);
+    }
+    wait_loads<0>();  // the last refills, before the ring is used otherwise
+    if (__builtin_expect(__any(st.odd), 0)) {
+      for (int i = max(all_see / 16 - 1 - f.first, 0) / f.stride; i < f.steps; ++i) {
+        const int key = (f.first + i * f.stride) * 16;
+        if (key + 16 <= all_see) continue;
+        for (int k = key; k < min(key + 16, limit); ++k) {
+          const uint16_t *v = value_row<D>(a, s, head, k) + g * 4;
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j) st.o[j] += odd_parts<T>(v + j * 16);
+        }
+      }
+    }
+  }
+
+  // The waves' sums, scaled to the largest of their maxima.
+  __syncthreads();
+  float *sums = reinterpret_cast<float *>(lds);  // [wave][row][D + 4]
+  float *ml = sums + kFewWaves * kFewRows * (D + 4);  // [wave][row] maxima, then sums
+  st.l = across32(across16(st.l, Add()), Add());
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i)
+    *reinterpret_cast<f32x4 *>(sums + (wave * kFewRows + (lane & 15)) * (D + 4) + i * 16 + g * 4) =
+        st.o[i];
+  if (lane < 16) {
+    ml[wave * kFewRows + lane] = st.m;
+    ml[(kFewWaves + wave) * kFewRows + lane] = st.l;
+  }
+  __syncthreads();
+  for (int i = tid; i < rows * (D / 4); i += 256) {
+    const int c = i / (D / 4), d = i % (D / 4) * 4;
+    float m = ml[c], l = 0.0f;
+#pragma unroll
+    for (int w = 1; w < kFewWaves; ++w) m = fmaxf(m, ml[w * kFewRows + c]);
+    f32x4 o = {};
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w) {
+      const float k = decay(ml[w * kFewRows + c], m);
+      l += ml[(kFewWaves + w) * kFewRows + c] * k;
+      o += *reinterpret_cast<const f32x4 *>(sums + (w * kFewRows + c) * (D + 4) + d) * k;
+    }
+    if (sh.n == 1) {
+      write_row<T, D>(a, row_place(a, seq, kv, c), d, o, l > 0.0f || l != l ? 1.0f / l : 0.0f);
+    } else {
+      const int64_t row = ((int64_t)(sh.slot + sh.split) * a.batch.kv_heads + kv) * kFewRows + c;
+      *reinterpret_cast<f32x4 *>(a.part + row * D + d) = o;
+      if (d == 0) *reinterpret_cast<float2 *>(a.part_ml + row * 2) = float2{m, l};
+    }
+  }
+}
+
+// Joins `n` parts of one row, whose (m, l) and sums lie `step` rows apart; D / 4 threads
+// take a part's channels, the groups of threads different parts.
+template <typename T, int D>
+__device__ __forceinline__ void join_row(const Attention &a, int64_t row, int64_t step, int n,
+                                         RowPlace at, float *scratch) {
+  constexpr int LANES = D / 4, GROUPS = 256 / LANES;
+  const int tid = threadIdx.x, d = tid % LANES * 4, group = tid / LANES;
+  const float *ml = a.part_ml + row * 2;
+  float m = -INFINITY;
+  for (int j = tid & 63; j < n; j += 64) m = fmaxf(m, ml[j * step * 2]);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  float l = 0.0f;
+  f32x4 o = {};
+#pragma unroll 4
+  for (int j = group; j < n; j += GROUPS) {
+    const float2 p = *reinterpret_cast<const float2 *>(ml + j * step * 2);
+    const f32x4 v = *reinterpret_cast<const f32x4 *>(a.part + (row + j * step) * D + d);
+    const float k = decay(p.x, m);
+    l += p.y * k;
+    o += v * k;
+  }
+  float *sums = scratch;             // [group][D]
+  float *ls = scratch + GROUPS * D;  // [group]
+  *reinterpret_cast<f32x4 *>(sums + group * D + d) = o;
+  if (d == 0) ls[group] = l;
+  __syncthreads();
+  if (group == 0) {
+#pragma unroll
+    for (int w = 1; w < GROUPS; ++w) {
+      o += *reinterpret_cast<const f32x4 *>(sums + w * D + d);
+      l += ls[w];
+    }
+    write_row<T, D>(a, at, d, o, l > 0.0f || l != l ? 1.0f / l : 0.0f);
+  }
+}
+
+// Rows of sequences whose keys attention_few_kernel split: blockIdx.x is a sequence's
+// key-value head, blockIdx.y its row.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attention_combine_few_kernel(Attention a) {
+  __shared__ uint64_t scratch[8];
+  __shared__ Share found;
+  __shared__ __attribute__((aligned(16))) float buf[1024 + 256 / (D / 4)];
+  const int kv = blockIdx.x % a.batch.kv_heads;
+  const Share sh = find_share(a, blockIdx.x / a.batch.kv_heads, true, scratch, &found);
+  if (sh.s < 0 || sh.n < 2) return;
+  const PagedSequence seq = paged_sequence(a.batch, sh.s, a.tokens);
+  const int c = blockIdx.y;
+  if (c >= seq.count * a.group) return;
+  const int64_t step = (int64_t)a.batch.kv_heads * kFewRows;
+  join_row<T, D>(a, sh.slot * step + kv * kFewRows + c, step, sh.n, row_place(a, seq, kv, c), buf);
+}
+
+// ------------------------------------------------------------------ tiles
+// Rows of the sequences that the few-row kernel does not take, 128 a tile; the tile with
+// the most keys of a sequence first.
+__device__ __forceinline__ int tile_count(const Attention &a, int s) {
+  if (s >= a.batch.sequences) return 0;
+  const PagedSequence q = paged_sequence(a.batch, s, a.tokens);
+  if (a.few && few_rows(q, a.group)) return 0;
+  return (int)(((int64_t)q.count * a.group + kTileRows - 1) / kTileRows);
+}
+
+struct TilePlace {
+  int s, tile, count;  // s < 0: none
+};
+
+__device__ TilePlace find_tile(const Attention &a, int index, int *scratch, TilePlace *found) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (tid == 0) found->s = -1;
+  int base = 0;
+  for (int c = 0; c < a.batch.sequences; c += 256) {
+    const int n = tile_count(a, c + tid);
+    int sum = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(sum, o, 64);
+      if (lane >= o) sum += v;
+    }
+    __syncthreads();
+    if (lane == 63) scratch[wave] = sum;
+    __syncthreads();
+    int before = base;
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) before += scratch[w];
+      base += scratch[w];
+    }
+    before += sum - n;
+    if (index >= before && index < before + n) *found = {c + tid, n - 1 - (index - before), n};
+    if (base > index) break;  // the same for every thread
+  }
+  __syncthreads();
+  const TilePlace got = *found;
+  __syncthreads();
+  return got;
+}
+
+constexpr int kTileKeys = 32;
+
+template <int D>
+struct TileState {
+  float m = -INFINITY, l = 0.0f;  // of column lane & 31; l: this lane's keys only
+  f32x16 o[D / 32] = {};          // o[i][4 b + r]: channel 32 i + 8 b + 4 (lane >> 5) + r
+  bool odd = false;               // infinities or NaN were left out
+};
+
+// 32 keys and values into LDS by the workgroup's four waves: 8 rows of each a wave.
+template <int D>
+__device__ __forceinline__ void tile_load(const Attention &a, int s, int64_t head, int key,
+                                          LDS char *kt, LDS char *vt, int wave, int lane) {
+  const int k = key + wave * 8, to = wave * 8 * D * 2;
+  const int64_t at = paged_page(a.batch, s, k) + head +
+                     (int64_t)(k & ((1 << a.batch.page_shift) - 1)) * D;
+  load_rows<D, 8>(a.k_pages + at, wave * 8, kt + to, lane);
+  load_rows<D, 8>(a.v_pages + at, wave * 8, vt + to, lane);
+}
+
+// Operand of 16 keys from row `ks` of the tile, channels 32 i ..
+template <int D>
+__device__ __forceinline__ u32x4 tile_operand(const LDS char *vt, int base, int i, int ks) {
+  const u32x2 lo = read_transposed<D>(vt, base, ks, i * 32);
+  const u32x2 hi = read_transposed<D>(vt, base, ks + 8, i * 32);
+  return u32x4{lo[0], lo[1], hi[0], hi[1]};
+}
+
+// Adds the weighted values of 32 keys; MIXED: some row does not see all of them.
+template <typename T, int D, bool MIXED>
+__device__ __forceinline__ void tile_values(const LDS char *vt, const u32x4 (&p)[2],
+                                            TileState<D> &st, int lane) {
+  const int base = opaque(transpose_base<D>((lane >> 5) * 4, ((lane >> 4) & 1) * 16, lane));
+  if constexpr (!MIXED) {
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+        st.o[i] = mfma32(T{}, tile_operand<D>(vt, base, i, ks * 16), p[ks], st.o[i]);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      u32x4 v = tile_operand<D>(vt, base, i, ks * 16);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = Pair<T>::finite(v[j], st.odd);
+      st.o[i] = mfma32(T{}, v, p[ks], st.o[i]);
+    }
+}
+
+// One tile of 32 keys, the next one's loads started before it.  MIXED: some row does not
+// see all of the keys.
+template <typename T, int D, bool MIXED>
+__device__ __forceinline__ void tile_step(const LDS char *__restrict__ kt,
+                                          const LDS char *__restrict__ vt,
+                                          LDS char *__restrict__ next_k,
+                                          LDS char *__restrict__ next_v, const Attention &a, int s,
+                                          int64_t head, int key, int key1,
+                                          const u32x4 (&q)[D / 16], int limit, bool idle, TileState<D> &st, int wave, int lane) {
+  if (key + kTileKeys < key1)
+    tile_load<D>(a, s, head, key + kTileKeys, next_k, next_v, wave, lane);
+  if (idle) return;
+  const int h = lane >> 5, r = lane & 31;
+  const int base = opaque(r * (D * 2) + ((h ^ swizzle<D>(r)) << 4));
+  f32x16 x = {};
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+    const u32x4 k = *(const LDS u32x4 *)(kt + (base ^ (i << 5)));
+    x = mfma32(T{}, k, q[i], x);
+  }
+  float mx = -INFINITY;
+  x *= a.scale2;
+  if constexpr (MIXED) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (key + 8 * (i / 4) + 4 * h + i % 4 >= limit) x[i] = -INFINITY;
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[i]);
+  mx = across32(mx, Max());
+  if (__any(mx > st.m + kSlack)) {
+    const float n = fmaxf(st.m, mx), keep = decay(st.m, n);
+    st.m = n;
+    st.l *= keep;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) st.o[i] *= keep;
+  }
+  const float at = st.m == -INFINITY ? 0.0f : st.m;
+  u32x4 p[2];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float e0 = exp2_hw(x[2 * i] - at), e1 = exp2_hw(x[2 * i + 1] - at);
+    st.l += e0 + e1;
+    p[i / 4][i % 4] = T::pack2(e0, e1);
+  }
+  tile_values<T, D, MIXED>(vt, p, st, lane);
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void attention_tile_kernel(Attention a) {
+  constexpr int TILE = kTileKeys * D * 2;
+  // One array: with several, the compiler waits for all direct loads at each LDS read.
+  __shared__ __attribute__((aligned(16))) char lds[4 * TILE];
+  int *scratch = reinterpret_cast<int *>(lds);
+  TilePlace *found = reinterpret_cast<TilePlace *>(scratch + 4);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kv = blockIdx.x % a.batch.kv_heads, split = blockIdx.y;
+  const TilePlace place = find_tile(a, blockIdx.x / a.batch.kv_heads, scratch, found);
+  const int s = __builtin_amdgcn_readfirstlane(place.s);
+  if (s < 0) return;
+  const PagedSequence seq = paged_sequence(a.batch, s, a.tokens);
+  const int rows = seq.count * a.group, c0 = place.tile * kTileRows;
+  const int c = c0 + wave * 32 + (lane & 31);
+  const bool idle = c0 + wave * 32 >= rows;
+  const RowPlace at = row_place(a, seq, kv, min(c, rows - 1));
+  const int limit = min(seq.base + min(c, rows - 1) / a.group + 1, seq.length);
+  const int all_see = min(seq.base + c0 / a.group + 1, seq.length);  // seen by every row
+  // keys that the tile's last row sees, and this split's part of them
+  const int last = min(c0 + kTileRows, rows) - 1;
+  const int keys = max(min(seq.base + last / a.group + 1, seq.length), 0);
+  const int tiles = (keys + kTileKeys - 1) / kTileKeys;
+  const int key0 = (int)((int64_t)tiles * split / a.splits) * kTileKeys;
+  const int key1 = min((int)((int64_t)tiles * (split + 1) / a.splits) * kTileKeys, keys);
+
+  u32x4 q[D / 16];
+  const uint16_t *qr = a.q + at.token * a.q_token + at.head * a.q_head + (lane >> 5) * 8;
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) q[i] = ldg16(qr + i * 16);
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) settle(q[i]);
+  TileState<D> st;
+  LDS char *base = (LDS char *)lds;
+  const int64_t head = (int64_t)(kv << a.batch.page_shift) * D;
+  if (key0 < key1) {
+    tile_load<D>(a, s, head, key0, base, base + TILE, wave, lane);
+    wait_loads<0>();
+    __syncthreads();
+    int key = key0, half = 0;
+    const int whole = min(key1, all_see);
+    for (; key + kTileKeys <= whole; key += kTileKeys, half ^= 1) {
+      LDS char *cur = base + half * 2 * TILE, *next = base + (half ^ 1) * 2 * TILE;
+      tile_step<T, D, false>(cur, cur + TILE, next, next + TILE, a, s, head, key, key1, q, limit,
+                             idle, st, wave, lane);
+      wait_loads<0>();
+      __syncthreads();
+    }
+    const int mixed = key;
+    for (; key < key1; key += kTileKeys, half ^= 1) {
+      LDS char *cur = base + half * 2 * TILE, *next = base + (half ^ 1) * 2 * TILE;
+      tile_step<T, D, true>(cur, cur + TILE, next, next + TILE, a, s, head, key, key1, q, limit,
+                            idle, st, wave, lane);
+      wait_loads<0>();
+      __syncthreads();
+    }
+    if (__builtin_expect(__any(st.odd), 0)) {
+      for (int k = mixed; k < min(key1, limit); ++k) {
+        const uint16_t *v = value_row<D>(a, s, head, k) + (lane >> 5) * 4;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const f32x4 x = odd_parts<T>(v + i * 32 + b * 8);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) st.o[i][4 * b + j] += x[j];
+          }
+      }
+    }
+  }
+  if (c >= rows) return;
+  const float l = across32(st.l, Add());
+  const int h = lane >> 5;
+  if (a.splits == 1) {
+    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        write_row<T, D>(a, at, i * 32 + b * 8 + h * 4,
+                        f32x4{st.o[i][4 * b], st.o[i][4 * b + 1], st.o[i][4 * b + 2],
+                              st.o[i][4 * b + 3]},
+                        inv);
+  } else {
+    const int64_t row = ((int64_t)split * a.tokens + at.token) * a.q_heads + at.head;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        *reinterpret_cast<f32x4 *>(a.part + row * D + i * 32 + b * 8 + h * 4) =
+            f32x4{st.o[i][4 * b], st.o[i][4 * b + 1], st.o[i][4 * b + 2], st.o[i][4 * b + 3]};
+    if (h == 0) *reinterpret_cast<float2 *>(a.part_ml + row * 2) = float2{st.m, l};
+  }
+}
+
+// Rows of sequences in tiles, where their keys were split: blockIdx.x a token, y a head.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attention_combine_tile_kernel(Attention a) {
+  __shared__ __attribute__((aligned(16))) float buf[1024 + 256 / (D / 4)];
+  const int t = blockIdx.x, head = blockIdx.y, s = paged_find(a.batch, t);
+  if (s < 0) return;
+  const PagedSequence seq = paged_sequence(a.batch, s, a.tokens);
+  if (t < seq.first || t >= seq.first + seq.count || (a.few && few_rows(seq, a.group))) return;
+  const int64_t step = (int64_t)a.tokens * a.q_heads;
+  join_row<T, D>(a, (int64_t)t * a.q_heads + head, step, a.splits, {t, head}, buf);
+}
+
+// ------------------------------------------------------------------ host side
+// What a call launches, by its sizes alone.
+struct AttentionPlan {
+  bool few, tile;
+  int64_t shares, few_grid;          // few: parts per key-value head, workgroups
+  int64_t tiles, splits;             // tile: tiles at most, parts of each
+  int64_t few_rows, tile_rows;       // rows of partial sums
+};
+
+AttentionPlan attention_plan(int64_t tokens, int64_t sequences, int64_t q_heads, int64_t kv_heads,
+                             int64_t max_new, int64_t max_keys) {
+  AttentionPlan p = {};
+  const int64_t group = q_heads / kv_heads;
+  max_new = max_new < tokens ? max_new : tokens;
+  p.few = group <= kFewRows;
+  p.tile = max_new * group > kFewRows;
+  if (p.few) {
+    p.shares = 512 / kv_heads > 1 ? 512 / kv_heads : 1;
+    const int64_t some = sequences < tokens ? sequences : tokens;  // with new tokens
+    p.few_grid = (p.shares + some) * kv_heads;
+    p.few_rows = 2 * p.shares * kv_heads * kFewRows;
+  }
+  if (p.tile) {
+    const int64_t some = sequences < tokens ? sequences : tokens;
+    p.tiles = tokens * group / kTileRows + some;
+    int64_t n = 512 / (p.tiles * kv_heads);
+    if (n > max_keys / 256) n = max_keys / 256;
+    p.splits = n < 1 ? 1 : n;
+    if (p.splits > 1) p.tile_rows = p.splits * tokens * q_heads;
+  }
+  return p;
+}
+
+int64_t attention_bytes(const AttentionPlan &p, int64_t head_dim) {
+  return (p.few_rows + p.tile_rows) * (head_dim + 2) * 4;
+}
+
+template <typename T, int D>
+int launch_attention(const AttentionPlan &p, Attention a, float *workspace, hipStream_t st) {
+  a.few = p.few;
+  if (p.few) {
+    a.shares = (int)p.shares;
+    a.part = workspace, a.part_ml = workspace + p.few_rows * D;
+    attention_few_kernel<T, D><<<(unsigned)p.few_grid, 256, 0, st>>>(a);
+    if (const int rc = check_launch("attention_few_kernel")) return rc;
+    const dim3 grid((unsigned)(a.batch.sequences * a.batch.kv_heads),
+                    (unsigned)(kFewRows / a.group * a.group));
+    attention_combine_few_kernel<T, D><<<grid, 256, 0, st>>>(a);
+    if (const int rc = check_launch("attention_combine_few_kernel")) return rc;
+  }
+  if (p.tile) {
+    a.splits = (int)p.splits;
+    a.part = workspace + p.few_rows * (D + 2), a.part_ml = a.part + p.tile_rows * D;
+    const dim3 grid((unsigned)(p.tiles * a.batch.kv_heads), (unsigned)p.splits);
+    attention_tile_kernel<T, D><<<grid, 256, 0, st>>>(a);
+    if (const int rc = check_launch("attention_tile_kernel")) return rc;
+    if (p.splits > 1) {
+      attention_combine_tile_kernel<T, D>
+          <<<dim3((unsigned)a.tokens, (unsigned)a.q_heads), 256, 0, st>>>(a);
+      return check_launch("attention_combine_tile_kernel");
+    }
+  }
+  return LM_OK;
+}
+
 template <typename T>
-int launch_attention(const Attention &a, int head_dim, hipStream_t st) {
-  const dim3 grid(a.tokens, a.q_heads);
-  if (head_dim == 256)
-    attention_row_kernel<T, 256><<<grid, 64, 0, st>>>(a);
-  else if (head_dim == 128)
-    attention_row_kernel<T, 128><<<grid, 64, 0, st>>>(a);
-  else
-    attention_row_kernel<T, 64><<<grid, 64, 0, st>>>(a);
-  return check_launch("attention_row_kernel");
+int launch_attention(const AttentionPlan &p, const Attention &a, float *workspace, int head_dim,
+                     hipStream_t st) {
+  return head_dim == 256   ? launch_attention<T, 256>(p, a, workspace, st)
+         : head_dim == 128 ? launch_attention<T, 128>(p, a, workspace, st)
+                           : launch_attention<T, 64>(p, a, workspace, st);
 }
 
 }  // namespace
@@ -90,8 +919,13 @@ using namespace lm;
 
 extern "C" int64_t lm_paged_attention_workspace_bytes(int64_t tokens, int64_t sequences,
                                                       int64_t q_heads, int64_t kv_heads,
-                                                      int64_t head_dim, int64_t max_new) {
-  return 0;
+                                                      int64_t head_dim, int64_t max_new,
+                                                      int64_t max_keys) {
+  if (tokens < 1 || sequences < 1 || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads ||
+      max_new < 0)
+    return 0;
+  return attention_bytes(
+      attention_plan(tokens, sequences, q_heads, kv_heads, max_new, max_keys), head_dim);
 }
 
 extern "C" int lm_paged_attention(const void *q, int64_t q_token_stride, int64_t q_head_stride,
@@ -107,10 +941,11 @@ extern "C" int lm_paged_attention(const void *q, int64_t q_token_stride, int64_t
   if (const int rc = paged_check(pages, page_stride, kv_heads, page_size, head_dim, starts, lengths,
                                  table, table_stride, table_pages, sequences, tokens, dtype))
     return rc;
-  LM_REQUIRE(q_heads >= 1 && q_heads <= 65536 && q_heads % kv_heads == 0, LM_EINVAL,
+  LM_REQUIRE(q_heads >= 1 && q_heads <= 16384 && q_heads % kv_heads == 0, LM_EINVAL,
              "query heads must be a multiple of key-value heads");
   LM_REQUIRE(max_new >= 0, LM_EINVAL, "invalid number of new tokens");
   if (tokens == 0 || sequences == 0) return LM_OK;
+  LM_REQUIRE(tokens * q_heads < (1LL << 31), LM_EINVAL, "too many rows");
   LM_REQUIRE(q && k_pages && v_pages && out, LM_EINVAL, "null pointer");
   LM_REQUIRE(aligned16(q) && aligned16(k_pages) && aligned16(v_pages) && aligned16(out) &&
                  q_token_stride % 8 == 0 && q_head_stride % 8 == 0 && q_token_stride >= 0 &&
@@ -119,6 +954,12 @@ extern "C" int lm_paged_attention(const void *q, int64_t q_token_stride, int64_t
   LM_REQUIRE(!gate || (aligned16(gate) && gate_token_stride % 8 == 0 && gate_head_stride % 8 == 0 &&
                        gate_token_stride >= 0 && gate_head_stride >= 0),
              LM_EINVAL, "head rows must be 16-byte aligned");
+  const AttentionPlan plan = attention_plan(tokens, sequences, q_heads, kv_heads, max_new,
+                                            table_pages * page_size);
+  const int64_t need = attention_bytes(plan, head_dim);
+  LM_REQUIRE(need == 0 || (workspace && aligned16(workspace)), LM_EINVAL,
+             "attention needs a 16-byte aligned workspace");
+  LM_REQUIRE(workspace_bytes >= need, LM_ENOMEM, "the workspace is too small");
   Attention a = {};
   a.q = static_cast<const uint16_t *>(q), a.q_token = q_token_stride, a.q_head = q_head_stride;
   a.gate = static_cast<const uint16_t *>(gate);
@@ -130,7 +971,9 @@ extern "C" int lm_paged_attention(const void *q, int64_t q_token_stride, int64_t
              __builtin_ctzll((unsigned long long)page_size), (int)pages, page_stride,
              (int)kv_heads};
   a.tokens = (int)tokens, a.q_heads = (int)q_heads, a.group = (int)(q_heads / kv_heads);
-  a.scale = scale;
-  return dtype == LM_BF16 ? launch_attention<BF16>(a, (int)head_dim, as_stream(stream))
-                          : launch_attention<FP16>(a, (int)head_dim, as_stream(stream));
+  a.scale2 = scale * 1.4426950408889634f;
+  float *ws = static_cast<float *>(workspace);
+  return dtype == LM_BF16
+             ? launch_attention<BF16>(plan, a, ws, (int)head_dim, as_stream(stream))
+             : launch_attention<FP16>(plan, a, ws, (int)head_dim, as_stream(stream));
 }

@@ -36,7 +36,9 @@ COMMON = ['-O3', '-std=c++17', '-fPIC', f'--offload-arch={ARCH}', '-ffp-contract
 # left the prefill unchanged.  w8a8_gemm.hip: its main loops begin on a fetch
 # line; with the 128 x 128 one 8 bytes into a line, [1300, 2048] by [8192, 2048]
 # took 55.4 us instead of 50.7.
-EXTRA = {'w8a8_gemm.hip': ['-falign-loops=64'],
+# attention.hip: the VGPR form as well, its softmax works on MFMA results throughout.
+EXTRA = {'attention.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form=1'],
+         'w8a8_gemm.hip': ['-falign-loops=64'],
          'moe.hip': ['-mllvm', '-amdgpu-kernarg-preload-count=6',
                      '-mllvm', '-amdgpu-mfma-vgpr-form=1']}
 

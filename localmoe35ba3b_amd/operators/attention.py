@@ -185,7 +185,7 @@ def paged_attention(q, k_pages, v_pages, starts, lengths, table, scale=None, gat
     batch = _batch(q.device, starts, lengths, table)
     max_new = tokens if max_new is None else max_new
     need = _lib.lib().lm_paged_attention_workspace_bytes(tokens, batch[5], q_heads, heads, dim,
-                                                         max_new)
+                                                         max_new, batch[4] * size)
     workspace = q.new_empty(need, dtype=torch.uint8) if need > 0 else None
     _lib.call_on(q.device, 'lm_paged_attention', q.data_ptr(), q.stride(0), q.stride(1), q_heads,
               k_pages.data_ptr(), v_pages.data_ptr(), pages, stride, heads, size, dim, *batch,
