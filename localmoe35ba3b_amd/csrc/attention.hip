@@ -26,6 +26,8 @@
 //                         workgroup, 32 a wave, over shared 32-key tiles; few tiles
 //                         split their keys over workgroups too.
 //  attention_combine_*    joins the parts of split keys.
+#include <utility>
+
 #include "paged.hpp"
 
 namespace lm {
@@ -47,14 +49,14 @@ struct Attention {
   float *part_ml;
   PagedBatch batch;
   int tokens, q_heads, group;
-  int shares;  // few: parts a key-value head's keys are cut into, about
+  int shares;  // few: spans that a key-value head's keys are cut into, at most
   int splits;  // tile: parts of each tile's keys
   bool few;    // tile: sequences of few rows are attention_few_kernel's
-  float scale2;  // scale * log2(e)
+  float scale2;   // |scale| * log2(e), not 0
+  uint32_t flip;  // sign bits that queries are flipped by, for a negative scale
 };
 
 constexpr int kFewRows = 16;    // columns of the few-row kernel
-constexpr int kTileRows = 128;  // rows of a tile
 constexpr float kSlack = 8.0f;  // weights stay below 2^8: exact sums in fp32, finite in fp16
 
 __device__ __forceinline__ f32x4 mfma16(BF16, u32x4 a, u32x4 b, f32x4 c) {
@@ -102,31 +104,42 @@ __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2
 // 2^(m - n) of two running maxima, n >= m; both may be -inf.
 __device__ __forceinline__ float decay(float m, float n) { return m == n ? 1.0f : exp2_hw(m - n); }
 
-// Piece c (16 bytes) of row r of a tile lies at place c ^ swizzle(r) of the row: rows of
-// one bank group (a row is D * 2 bytes, the banks repeat every 256) get different places.
-// Linear over disjoint bits of r, so a read's lane part is formed once and its constant
-// part is one exclusive or.
-template <int D>
+// Piece c (16 bytes) of row r of a tile lies at place c ^ swizzle(r) of the row, so that the
+// rows that one LDS read touches use different banks (a row is D * 2 bytes, the banks repeat
+// every 256).  kRows: reads of one or two pieces of 16 rows; kQuads: of four pieces of 4 rows
+// (the transpose reads of 32 channels; with kRows they took 4 times as long).  Linear over
+// disjoint bits of r: a read's lane part is formed once, its constant part is one exclusive or.
+enum Swizzle { kRows, kQuads };
+template <int D, Swizzle S = kRows>
 __device__ __forceinline__ constexpr int swizzle(int r) {
-  return D == 64 ? (r >> 1) & 7 : r & 15;
+  return S == kRows ? (D == 64 ? (r >> 1) & 7 : r & 15) : (D == 64 ? (r & 2) << 1 : (r & 3) << 2);
 }
+
+// Cache policy of loads that are not read again (non-temporal): 262144 keys of one sequence
+// in 88 us instead of 96; the tiles, which other workgroups read too, take 10 % longer with it.
+constexpr int kStream = 2;
 
 // ROWS rows of a page, from `src` (row `row0` of the tile), into LDS: wave-wide loads of
 // 1 KB, lane-linear in LDS, so the swizzle permutes the source.  Rows behind a sequence's
-// end are loaded as they are (their page holds them) and masked later.  A loop, not
-// unrolled: the compiler tells apart the targets of a few such instructions only, and
-// waits for all of them before any LDS read when there are more.
-template <int D, int ROWS>
+// end are loaded as they are (their page holds them) and masked later.  An instruction's
+// offset counts for both addresses, so four share a pair of them.
+template <int D, int PER, Swizzle S, int POLICY, int... I>
+__device__ __forceinline__ void load_4k(const GLB char *from, uint32_t off, int row0, LDS char *to,
+                                        std::integer_sequence<int, I...>) {
+  (__builtin_amdgcn_global_load_lds(
+       (const GLB void *)(from + (off ^ (swizzle<D, S>(row0 + I * PER) << 4))), (LDS void *)to, 16,
+       I * 1024, POLICY),
+   ...);
+}
+template <int D, int ROWS, Swizzle S = kRows, int POLICY = 0>
 __device__ __forceinline__ void load_rows(const uint16_t *src, int row0, LDS char *to, int lane) {
-  constexpr int PIECES = D / 8, PER = 64 / PIECES;
+  constexpr int PIECES = D / 8, PER = 64 / PIECES, LOADS = ROWS / PER, GROUP = LOADS < 4 ? LOADS : 4;
   const int own = lane / PIECES;
-  const uint32_t off = own * (D * 2) + (((lane % PIECES) ^ swizzle<D>(own)) << 4);
-  const GLB char *from = (const GLB char *)src;
-#pragma clang loop unroll(disable)
-  for (int i = 0; i < ROWS / PER; ++i)
-    __builtin_amdgcn_global_load_lds(
-        (const GLB void *)(from + i * 1024 + (off ^ (swizzle<D>(row0 + i * PER) << 4))),
-        (LDS void *)(to + i * 1024), 16, 0, 0);
+  const uint32_t off = own * (D * 2) + (((lane % PIECES) ^ swizzle<D, S>(own)) << 4);
+#pragma unroll
+  for (int i = 0; i < LOADS / GROUP; ++i)
+    load_4k<D, PER, S, POLICY>((const GLB char *)src + i * 4096, off, row0 + i * 4 * PER, to + i * 4096,
+                       std::make_integer_sequence<int, GROUP>{});
 }
 
 // Has v loaded here, so that no wait for it is placed in a loop over direct loads, where it
@@ -144,15 +157,22 @@ __device__ __forceinline__ void wait_loads() {
 // Four keys of one channel, by the LDS transpose read: lane i of each 16 lanes gets channel
 // d0 + i of rows r .. r + 3, r = row + ROW and d0 = d + CH with the lane's own row (a multiple
 // of 4) and d (0 or 16) in `base` (transpose_base), the rest constant.
-template <int D>
+template <int D, Swizzle S>
 __device__ __forceinline__ int transpose_base(int row, int d, int lane) {
   const int r = row + (lane & 15) / 4;
-  return r * (D * 2) + (((d / 8 + (lane & 3) / 2) ^ swizzle<D>(r)) << 4) + (lane & 1) * 8;
+  return r * (D * 2) + (((d / 8 + (lane & 3) / 2) ^ swizzle<D, S>(r)) << 4) + (lane & 1) * 8;
 }
-template <int D>
-__device__ __forceinline__ u32x2 read_transposed(const LDS char *tile, int base, int row, int ch) {
-  const LDS char *p = tile + (base ^ ((ch / 8 ^ swizzle<D>(row)) << 4)) + row * (D * 2);
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS s16x4 *)p));
+// The address of piece `ch` (constant) of row `row` (constant) past a lane's base, in which
+// the piece's low four bits were swizzled.
+template <int D, Swizzle S>
+__device__ __forceinline__ int swizzled(int base, int row, int ch) {
+  return (base ^ (((ch & 15) ^ swizzle<D, S>(row)) << 4)) + (ch & 16) * 16 + row * (D * 2);
+}
+template <int D, Swizzle S>
+__device__ __forceinline__ u32x2 read_transposed(const LDS char *tile, int base, int row, int d) {
+  return __builtin_bit_cast(
+      u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                 (LDS s16x4 *)(tile + swizzled<D, S>(base, row, d / 8))));
 }
 
 // Keeps a lane's base from being expanded into one register for every constant part.
@@ -193,78 +213,96 @@ __device__ __forceinline__ const uint16_t *value_row(const Attention &a, int s, 
 }
 
 // ------------------------------------------------------------------ shares of keys
-// The keys of the sequences with few rows, in blocks of 64, are cut into about
-// `shares` parts: n_s = ceil(blocks_s * shares / all blocks) of sequence s, at most its
-// blocks.  Every workgroup works this out from the lengths, so the host needs to know
-// none of them and a captured call follows them.
-struct Share {
-  int s, split, n;  // part `split` of sequence s's n; s < 0: none
-  int slot;         // of part 0 among the parts of sequences with several
-};
-
+// The keys of the sequences with few rows, in blocks of 64 and one sequence after another,
+// are cut into `shares` equal spans, one for each workgroup of a key-value head: as much
+// work for each, whatever the lengths.  Every workgroup works the cuts out from the lengths,
+// so the host needs to know none of them and a captured call follows them.
 constexpr int kBlockKeys = 64;
 
 // count > 0 of a sequence whose rows fit the few-row kernel
 __device__ __forceinline__ bool few_rows(const PagedSequence &q, int group) {
   return q.count > 0 && q.count <= kFewRows / group;
 }
+// Blocks of sequence s: 0 of one that is not the few-row kernel's, at least 1 of others.
 __device__ __forceinline__ int few_blocks(const Attention &a, int s) {
   if (s >= a.batch.sequences) return 0;
   const PagedSequence q = paged_sequence(a.batch, s, a.tokens);
   return few_rows(q, a.group) ? max((q.length + kBlockKeys - 1) / kBlockKeys, 1) : 0;
 }
 
-// The share with index `index` (by_sequence: of sequence `index`, split 0).  All 256
-// threads; scratch (8 words of LDS) and found are free again afterwards.
-__device__ Share find_share(const Attention &a, int index, bool by_sequence, uint64_t *scratch,
-                            Share *found) {
+struct Spans {
+  int64_t blocks;  // of all sequences
+  int spans;       // at most `blocks`
+  __device__ __forceinline__ int64_t start(int span) const { return blocks * span / spans; }
+  __device__ __forceinline__ int of(int64_t block) const {  // the span that holds a block
+    return (int)(((block + 1) * spans - 1) / blocks);
+  }
+};
+struct Find {
+  int64_t first;  // of the found sequence: its first block
+  int s;          // < 0: none
+};
+
+// The spans, and the sequence that holds the first block of span `index` (BY_SEQUENCE:
+// sequence `index`).  All 256 threads; scratch (8 words of LDS) and found are free again
+// afterwards.
+template <bool BY_SEQUENCE>
+__device__ Spans find_span(const Attention &a, int index, int64_t *scratch, Find *found, Find &got) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, S = a.batch.sequences;
+  Spans sp;
+  if (S == 1) {
+    sp.blocks = few_blocks(a, 0);
+    sp.spans = (int)min((int64_t)a.shares, sp.blocks);
+    got = {0, index < (BY_SEQUENCE ? min(sp.spans, 1) : sp.spans) ? 0 : -1};
+    return sp;
+  }
   if (tid == 0) found->s = -1;
   const int mine = few_blocks(a, tid);
-  uint64_t all = mine;
+  int64_t all = mine;
   for (int s = tid + 256; s < S; s += 256) all += few_blocks(a, s);
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) all += __shfl_xor(all, o, 64);
   if (lane == 0) scratch[wave] = all;
   __syncthreads();
-  all = scratch[0] + scratch[1] + scratch[2] + scratch[3];
-  uint64_t base = 0;  // parts before this group of 256 sequences, those of split ones above
-  for (int c = 0; c < S; c += 256) {
-    const int s = c + tid;
-    const uint64_t blocks = c == 0 ? mine : few_blocks(a, s);
-    const uint64_t n = blocks ? min(blocks, (blocks * a.shares + all - 1) / all) : 0;
-    uint64_t sum = n | (n > 1 ? n << 32 : 0);
-    const uint64_t own = sum;
+  sp.blocks = scratch[0] + scratch[1] + scratch[2] + scratch[3];
+  sp.spans = (int)min((int64_t)a.shares, sp.blocks);
+  if (BY_SEQUENCE || index < sp.spans) {
+    const int64_t want = BY_SEQUENCE ? 0 : sp.start(index);
+    int64_t base = 0;  // blocks before this group of 256 sequences
+    for (int c = 0; c < S && (BY_SEQUENCE ? c <= index : base <= want); c += 256) {
+      const int n = c == 0 ? mine : few_blocks(a, c + tid);
+      int64_t sum = n;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint64_t v = __shfl_up(sum, o, 64);
-      if (lane >= o) sum += v;
+      for (int o = 1; o < 64; o <<= 1) {
+        const int64_t v = __shfl_up(sum, o, 64);
+        if (lane >= o) sum += v;
+      }
+      __syncthreads();
+      if (lane == 63) scratch[4 + wave] = sum;
+      __syncthreads();
+      int64_t before = base + sum - n;
+      for (int w = 0; w < 4; ++w) {
+        if (w < wave) before += scratch[4 + w];
+        base += scratch[4 + w];
+      }
+      if (n > 0 && (BY_SEQUENCE ? c + tid == index : want >= before && want < before + n))
+        *found = {before, c + tid};
     }
-    __syncthreads();
-    if (lane == 63) scratch[4 + wave] = sum;
-    __syncthreads();
-    uint64_t before = base;
-    for (int w = 0; w < 4; ++w) {
-      if (w < wave) before += scratch[4 + w];
-      base += scratch[4 + w];
-    }
-    before += sum - own;
-    const int first = (int)(uint32_t)before, slot = (int)(before >> 32);
-    if (by_sequence ? s == index && n > 0 : index >= first && index < first + (int)n)
-      *found = {s, by_sequence ? 0 : index - first, (int)n, slot};
   }
   __syncthreads();
-  const Share got = *found;
+  got = *found;
   __syncthreads();
-  return got;
+  return sp;
 }
 
 // ------------------------------------------------------------------ few rows
 constexpr int kFewWaves = 4;
 
-// Ring of a wave: keys and values of two 16-key steps.
+// Steps of 16 keys in a wave's ring: as many bytes for every head size.
 template <int D>
-constexpr int few_ring() { return 4 * 16 * D * 2; }
+constexpr int few_steps() { return 256 / D; }
+template <int D>
+constexpr int few_ring() { return few_steps<D>() * 2 * 16 * D * 2; }
 template <int D>
 constexpr int few_merge() { return kFewWaves * (kFewRows * (D + 4) + 2 * kFewRows) * 4; }
 template <int D>
@@ -289,16 +327,16 @@ __device__ __forceinline__ u32x2 few_scores(const LDS char *kt, const u32x4 (&q)
   f32x4 s[2] = {};
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) {
-    const u32x4 k = *(const LDS u32x4 *)(kt + (base ^ (i << 6)));
+    const u32x4 k = *(const LDS u32x4 *)(kt + swizzled<D, kRows>(base, 0, i * 4));
     s[i & 1] = mfma16(T{}, k, q[i], s[i & 1]);
   }
   float x[4], mx = -INFINITY;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    x[i] = key0 + g * 4 + i < limit ? (s[0][i] + s[1][i]) * scale2 : -INFINITY;
+    x[i] = key0 + g * 4 + i < limit ? s[0][i] + s[1][i] : -INFINITY;
     mx = fmaxf(mx, x[i]);
   }
-  mx = across32(across16(mx, Max()), Max());
+  mx = across32(across16(mx, Max()), Max()) * scale2;
   if (__any(mx > st.m + kSlack)) {
     const float n = fmaxf(st.m, mx), keep = decay(st.m, n);
     st.m = n;
@@ -309,7 +347,7 @@ __device__ __forceinline__ u32x2 few_scores(const LDS char *kt, const u32x4 (&q)
   const float at = st.m == -INFINITY ? 0.0f : st.m;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    x[i] = exp2_hw(x[i] - at);
+    x[i] = exp2_hw(__builtin_fmaf(x[i], scale2, -at));
     st.l += x[i];
   }
   return u32x2{T::pack2(x[0], x[1]), T::pack2(x[2], x[3])};
@@ -319,16 +357,16 @@ __device__ __forceinline__ u32x2 few_scores(const LDS char *kt, const u32x4 (&q)
 template <typename T, int D>
 __device__ __forceinline__ void few_values(const LDS char *vt, u32x2 p, bool mixed,
                                            FewState<D> &st, int lane) {
-  const int base = opaque(transpose_base<D>((lane >> 4) * 4, 0, lane));
+  const int base = opaque(transpose_base<D, kRows>((lane >> 4) * 4, 0, lane));
   if (!mixed) {
 #pragma unroll
     for (int i = 0; i < D / 16; ++i)
-      st.o[i] = mfma16k16(T{}, read_transposed<D>(vt, base, 0, i * 16), p, st.o[i]);
+      st.o[i] = mfma16k16(T{}, read_transposed<D, kRows>(vt, base, 0, i * 16), p, st.o[i]);
     return;
   }
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) {
-    const u32x2 v = read_transposed<D>(vt, base, 0, i * 16);
+    const u32x2 v = read_transposed<D, kRows>(vt, base, 0, i * 16);
     st.o[i] = mfma16k16(T{}, u32x2{Pair<T>::finite(v[0], st.odd), Pair<T>::finite(v[1], st.odd)},
                         p, st.o[i]);
   }
@@ -358,39 +396,27 @@ __device__ __forceinline__ void few_load(const FewKeys &f, const uint16_t *side,
   const int j = min(i, f.steps - 1), key = (f.first + j * f.stride) * 16;
   const int page = __builtin_amdgcn_readlane(f.page_of, j & 63);
   const uint16_t *src = side + page * f.page_stride + (int64_t)(key & ((1 << f.shift) - 1)) * D;
-  load_rows<D, 16>(src, 0, to, lane);
+  load_rows<D, 16, kRows, kStream>(src, 0, to, lane);
 }
 
-// Two steps, i and i + 1, each from its own half of the ring, refilled for i + 2 and
-// i + 3 as soon as it is read.  The four regions are disjoint (restrict), so the compiler
-// does not take a read of one to wait for the loads into the others; the counts of loads
-// that may still be out are stated here.
+// Step i, from its place in the ring, which is refilled as soon as it is read; the counts of
+// loads that may still be out are stated here.
 template <typename T, int D>
-__device__ __forceinline__ void few_steps(LDS char *__restrict__ k0, LDS char *__restrict__ v0,
-                                          LDS char *__restrict__ k1, LDS char *__restrict__ v1,
-                                          const FewKeys &f, const u32x4 (&q)[D / 32], int i,
-                                          int limit, int all_see, float scale2, FewState<D> &st,
-                                          int lane) {
-  constexpr int N = 16 * D * 2 / 1024;  // loads of one side of a step
-  int key = (f.first + i * f.stride) * 16;
-  wait_loads<3 * N>();
-  u32x2 p = few_scores<T, D>(k0, q, key, limit, scale2, st, lane);
+__device__ __forceinline__ void few_step(LDS char *ring, const FewKeys &f, const u32x4 (&q)[D / 32],
+                                         int i, int limit, int all_see, float scale2,
+                                         FewState<D> &st, int lane) {
+  constexpr int TILE = 16 * D * 2, N = TILE / 1024;  // bytes and loads of one side of a step
+  constexpr int STEPS = few_steps<D>(), OUT = (2 * STEPS - 1) * N;
+  LDS char *k = ring + i % STEPS * 2 * TILE, *v = k + TILE;
+  const int key = (f.first + i * f.stride) * 16;
+  wait_loads<OUT>();
+  const u32x2 p = few_scores<T, D>(k, q, key, limit, scale2, st, lane);
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  few_load<D>(f, f.k, i + 2, k0, lane);
-  wait_loads<3 * N>();
-  few_values<T, D>(v0, p, key + 16 > all_see, st, lane);
+  few_load<D>(f, f.k, i + STEPS, k, lane);
+  wait_loads<OUT>();
+  few_values<T, D>(v, p, key + 16 > all_see, st, lane);
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  few_load<D>(f, f.v, i + 2, v0, lane);
-  if (i + 1 >= f.steps) return;
-  key += f.stride * 16;
-  wait_loads<3 * N>();
-  p = few_scores<T, D>(k1, q, key, limit, scale2, st, lane);
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  few_load<D>(f, f.k, i + 3, k1, lane);
-  wait_loads<3 * N>();
-  few_values<T, D>(v1, p, key + 16 > all_see, st, lane);
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  few_load<D>(f, f.v, i + 3, v1, lane);
+  few_load<D>(f, f.v, i + STEPS, v, lane);
 }
 
 // Row c of a sequence's rows at a key-value head: new token c / group, query head
@@ -429,29 +455,26 @@ __device__ __forceinline__ void write_row(const Attention &a, RowPlace at, int d
       uint2{T::pack2(o[0], o[1]), T::pack2(o[2], o[3])};
 }
 
+// Where a span's part of a sequence goes, when it is not all of the sequence: place 0 of the
+// span for its first part, 1 for a later one (its last).
+__device__ __forceinline__ int64_t part_row(const Attention &a, int span, bool later, int kv) {
+  return ((int64_t)(2 * span + later) * a.batch.kv_heads + kv) * kFewRows;
+}
+
+// Blocks b0 .. b1 - 1 of sequence s at key-value head kv; `part`: its row among the parts, or
+// negative where these are all of its blocks.
 template <typename T, int D>
-__global__ __launch_bounds__(256, 1) void attention_few_kernel(Attention a) {
-  // One array: with several, the compiler waits for all direct loads at each LDS read.
-  __shared__ __attribute__((aligned(16))) char lds[few_lds<D>()];
-  uint64_t *scratch = reinterpret_cast<uint64_t *>(lds);
-  Share *found = reinterpret_cast<Share *>(scratch + 8);
+__device__ __forceinline__ void few_part(const Attention &a, int s, int kv, int b0, int b1,
+                                         int64_t part, char *lds) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int kv = blockIdx.x % a.batch.kv_heads;
-  const Share sh = find_share(a, blockIdx.x / a.batch.kv_heads, false, scratch, found);
-  const int s = __builtin_amdgcn_readfirstlane(sh.s);
-  if (s < 0) return;
   const PagedSequence seq = paged_sequence(a.batch, s, a.tokens);
   const int rows = seq.count * a.group;
-  const int blocks = (seq.length + kBlockKeys - 1) / kBlockKeys;
-  const int b0 = (int)((int64_t)blocks * sh.split / sh.n);
-  const int b1 = (int)((int64_t)blocks * (sh.split + 1) / sh.n);
-
   const int col = min(lane & 15, rows - 1), g = lane >> 4;
   const RowPlace at = row_place(a, seq, kv, col);
   u32x4 q[D / 32];
   const uint16_t *qr = a.q + at.token * a.q_token + at.head * a.q_head;
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) q[i] = ldg16(qr + i * 32 + g * 8);
+  for (int i = 0; i < D / 32; ++i) q[i] = ldg16(qr + i * 32 + g * 8) ^ a.flip;
 
   FewKeys f;
   const int64_t head = (int64_t)(kv << a.batch.page_shift) * D;
@@ -471,22 +494,20 @@ __global__ __launch_bounds__(256, 1) void attention_few_kernel(Attention a) {
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) settle(q[i]);
     LDS char *ring = (LDS char *)lds + wave * few_ring<D>();
-    constexpr int TILE = 16 * D * 2;
-    for (int j = 0; j < 2; ++j) {  // in this order: the waits count what was issued later
+    constexpr int TILE = 16 * D * 2, STEPS = few_steps<D>();
+    for (int j = 0; j < STEPS; ++j) {  // in this order: the waits count what was issued later
       few_load<D>(f, f.k, j, ring + 2 * j * TILE, lane);
       asm volatile("" ::: "memory");
       few_load<D>(f, f.v, j, ring + (2 * j + 1) * TILE, lane);
       asm volatile("" ::: "memory");
     }
-    for (int i = 0; i < f.steps; i += 2) {
-      // steps i + 2 and i + 3 are loaded next: their pages from the next 64 on
-      if (((i + 2) & 63) == 0) few_pages(f, i + 2, lane);
-      few_steps<T, D>(ring, ring + TILE, ring + 2 * TILE, ring + 3 * TILE, f, q, i, limit, all_see,
-                      a.scale2, st, lane);
+    for (int i = 0; i < f.steps; ++i) {
+      if (((i + STEPS) & 63) == 0) few_pages(f, i + STEPS, lane);  // that step is loaded next
+      few_step<T, D>(ring, f, q, i, limit, all_see, a.scale2, st, lane);
     }
     wait_loads<0>();  // the last refills, before the ring is used otherwise
     if (__builtin_expect(__any(st.odd), 0)) {
-      for (int i = max(all_see / 16 - 1 - f.first, 0) / f.stride; i < f.steps; ++i) {
+      for (int i = 0; i < f.steps; ++i) {
         const int key = (f.first + i * f.stride) * 16;
         if (key + 16 <= all_see) continue;
         for (int k = key; k < min(key + 16, limit); ++k) {
@@ -524,73 +545,129 @@ __global__ __launch_bounds__(256, 1) void attention_few_kernel(Attention a) {
       l += ml[(kFewWaves + w) * kFewRows + c] * k;
       o += *reinterpret_cast<const f32x4 *>(sums + (w * kFewRows + c) * (D + 4) + d) * k;
     }
-    if (sh.n == 1) {
+    if (part < 0) {
       write_row<T, D>(a, row_place(a, seq, kv, c), d, o, l > 0.0f || l != l ? 1.0f / l : 0.0f);
     } else {
-      const int64_t row = ((int64_t)(sh.slot + sh.split) * a.batch.kv_heads + kv) * kFewRows + c;
-      *reinterpret_cast<f32x4 *>(a.part + row * D + d) = o;
-      if (d == 0) *reinterpret_cast<float2 *>(a.part_ml + row * 2) = float2{m, l};
+      *reinterpret_cast<f32x4 *>(a.part + (part + c) * D + d) = o;
+      if (d == 0) *reinterpret_cast<float2 *>(a.part_ml + (part + c) * 2) = float2{m, l};
     }
   }
+  __syncthreads();  // before the ring is used again
 }
 
-// Joins `n` parts of one row, whose (m, l) and sums lie `step` rows apart; D / 4 threads
-// take a part's channels, the groups of threads different parts.
 template <typename T, int D>
-__device__ __forceinline__ void join_row(const Attention &a, int64_t row, int64_t step, int n,
-                                         RowPlace at, float *scratch) {
-  constexpr int LANES = D / 4, GROUPS = 256 / LANES;
-  const int tid = threadIdx.x, d = tid % LANES * 4, group = tid / LANES;
-  const float *ml = a.part_ml + row * 2;
-  float m = -INFINITY;
-  for (int j = tid & 63; j < n; j += 64) m = fmaxf(m, ml[j * step * 2]);
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  float l = 0.0f;
-  f32x4 o = {};
-#pragma unroll 4
-  for (int j = group; j < n; j += GROUPS) {
-    const float2 p = *reinterpret_cast<const float2 *>(ml + j * step * 2);
-    const f32x4 v = *reinterpret_cast<const f32x4 *>(a.part + (row + j * step) * D + d);
-    const float k = decay(p.x, m);
-    l += p.y * k;
-    o += v * k;
-  }
-  float *sums = scratch;             // [group][D]
-  float *ls = scratch + GROUPS * D;  // [group]
-  *reinterpret_cast<f32x4 *>(sums + group * D + d) = o;
-  if (d == 0) ls[group] = l;
-  __syncthreads();
-  if (group == 0) {
-#pragma unroll
-    for (int w = 1; w < GROUPS; ++w) {
-      o += *reinterpret_cast<const f32x4 *>(sums + w * D + d);
-      l += ls[w];
-    }
-    write_row<T, D>(a, at, d, o, l > 0.0f || l != l ? 1.0f / l : 0.0f);
+__global__ __launch_bounds__(256, 1) void attention_few_kernel(Attention a) {
+  // One array: with several, the compiler waits for all direct loads at each LDS read.
+  __shared__ __attribute__((aligned(16))) char lds[few_lds<D>()];
+  int64_t *scratch = reinterpret_cast<int64_t *>(lds);
+  const int kv = blockIdx.x % a.batch.kv_heads, span = blockIdx.x / a.batch.kv_heads;
+  Find at;
+  const Spans sp = find_span<false>(a, span, scratch, reinterpret_cast<Find *>(scratch + 8), at);
+  if (at.s < 0) return;
+  int64_t block = sp.start(span);
+  const int64_t end = sp.start(span + 1);
+  int s = __builtin_amdgcn_readfirstlane(at.s);
+  int done = __builtin_amdgcn_readfirstlane((int)(block - at.first));  // blocks of s before
+  bool later = false;
+  for (; block < end && s < a.batch.sequences; ++s, done = 0) {
+    const int all = __builtin_amdgcn_readfirstlane(few_blocks(a, s));
+    const int take = __builtin_amdgcn_readfirstlane((int)min((int64_t)(all - done), end - block));
+    if (take <= 0) continue;
+    few_part<T, D>(a, s, kv, done, done + take, take == all ? -1 : part_row(a, span, later, kv),
+                   lds);
+    block += take;
+    later = true;
   }
 }
 
-// Rows of sequences whose keys attention_few_kernel split: blockIdx.x is a sequence's
-// key-value head, blockIdx.y its row.
+// The sum of parts of a row: a thread's four channels, under the largest maximum so far.
+struct PartSum {
+  float m = -INFINITY, l = 0.0f;
+  f32x4 o = {};
+  __device__ __forceinline__ void add(float pm, float pl, f32x4 po) {
+    const float n = fmaxf(m, pm), mine = decay(m, n), theirs = decay(pm, n);
+    m = n;
+    l = l * mine + pl * theirs;
+    o = o * mine + po * theirs;
+  }
+  __device__ __forceinline__ float inverse() const { return l > 0.0f || l != l ? 1.0f / l : 0.0f; }
+};
+
+constexpr int kFewParts = 8;
+
+// Rows of sequences whose keys attention_few_kernel split; blockIdx.x is a sequence's
+// key-value head.  Up to kFewParts parts: a thread takes four channels of a row, all parts of
+// it loaded at once.  More (few sequences then): the workgroups of blockIdx.y share the rows
+// and their channels, 64 at a time, the 16 groups of 16 threads the parts.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attention_combine_few_kernel(Attention a) {
-  __shared__ uint64_t scratch[8];
-  __shared__ Share found;
-  __shared__ __attribute__((aligned(16))) float buf[1024 + 256 / (D / 4)];
-  const int kv = blockIdx.x % a.batch.kv_heads;
-  const Share sh = find_share(a, blockIdx.x / a.batch.kv_heads, true, scratch, &found);
-  if (sh.s < 0 || sh.n < 2) return;
-  const PagedSequence seq = paged_sequence(a.batch, sh.s, a.tokens);
-  const int c = blockIdx.y;
-  if (c >= seq.count * a.group) return;
-  const int64_t step = (int64_t)a.batch.kv_heads * kFewRows;
-  join_row<T, D>(a, sh.slot * step + kv * kFewRows + c, step, sh.n, row_place(a, seq, kv, c), buf);
+  __shared__ int64_t scratch[8];
+  __shared__ Find found;
+  __shared__ __attribute__((aligned(16))) float sums[16][64];
+  __shared__ float ms[16], ls[16];
+  const int kv = blockIdx.x % a.batch.kv_heads, s = blockIdx.x / a.batch.kv_heads;
+  const int tid = threadIdx.x, group = tid / 16;
+  Find at;
+  const Spans sp = find_span<true>(a, s, scratch, &found, at);
+  if (at.s < 0) return;
+  const int first = sp.of(at.first), n = sp.of(at.first + few_blocks(a, s) - 1) - first + 1;
+  if (n < 2 || (n <= kFewParts && blockIdx.y > 0)) return;
+  const bool later = sp.start(first) != at.first;  // part 0 is not its span's first
+  const PagedSequence seq = paged_sequence(a.batch, s, a.tokens);
+  const int rows = seq.count * a.group;
+  if (n <= kFewParts) {
+    for (int u = tid; u < rows * (D / 4); u += 256) {
+      const int c = u / (D / 4), d = u % (D / 4) * 4;
+      float2 ml[kFewParts];
+      f32x4 v[kFewParts];
+#pragma unroll
+      for (int j = 0; j < kFewParts; ++j) {
+        const int64_t row = part_row(a, first + min(j, n - 1), j == 0 && later, kv) + c;
+        ml[j] = *reinterpret_cast<const float2 *>(a.part_ml + row * 2);
+        v[j] = *reinterpret_cast<const f32x4 *>(a.part + row * D + d);
+      }
+      PartSum sum;
+#pragma unroll
+      for (int j = 0; j < kFewParts; ++j)
+        if (j < n) sum.add(ml[j].x, ml[j].y, v[j]);
+      write_row<T, D>(a, row_place(a, seq, kv, c), d, sum.o, sum.inverse());
+    }
+    return;
+  }
+  for (int u = blockIdx.y; u < rows * (D / 64); u += gridDim.y) {
+    const int c = u / (D / 64), d = u % (D / 64) * 64 + tid % 16 * 4;
+    PartSum sum;
+#pragma unroll 8
+    for (int j = group; j < n; j += 16) {
+      const int64_t row = part_row(a, first + j, j == 0 && later, kv) + c;
+      const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + row * 2);
+      sum.add(ml.x, ml.y, *reinterpret_cast<const f32x4 *>(a.part + row * D + d));
+    }
+    *reinterpret_cast<f32x4 *>(&sums[group][tid % 16 * 4]) = sum.o;
+    if (tid % 16 == 0) ms[group] = sum.m, ls[group] = sum.l;
+    __syncthreads();
+    if (group == 0) {
+#pragma unroll
+      for (int w = 1; w < 16; ++w)
+        sum.add(ms[w], ls[w], *reinterpret_cast<const f32x4 *>(&sums[w][tid * 4]));
+      write_row<T, D>(a, row_place(a, seq, kv, c), d, sum.o, sum.inverse());
+    }
+    __syncthreads();
+  }
 }
 
 // ------------------------------------------------------------------ tiles
-// Rows of the sequences that the few-row kernel does not take, 128 a tile; the tile with
-// the most keys of a sequence first.
+constexpr int kTileRows = 128;  // rows of a tile, 32 a wave
+
+// Key groups of a workgroup: as many waves more take other keys of a tile for the same rows,
+// and their sums are joined in LDS at the end.
+template <int D>
+struct TileForm {
+  static constexpr int kGroups = D == 256 ? 2 : 1;
+  static constexpr int kWaves = 4 * kGroups, kKeys = 32 * kGroups;
+};
+
+// Tiles of the rows of sequence s, unless the few-row kernel takes them.
 __device__ __forceinline__ int tile_count(const Attention &a, int s) {
   if (s >= a.batch.sequences) return 0;
   const PagedSequence q = paged_sequence(a.batch, s, a.tokens);
@@ -599,14 +676,21 @@ __device__ __forceinline__ int tile_count(const Attention &a, int s) {
 }
 
 struct TilePlace {
-  int s, tile, count;  // s < 0: none
+  int s, tile;  // s < 0: none
 };
 
+// The index-th tile; the tile with the most keys of a sequence comes first.
+// All THREADS threads; scratch (a word a wave) and found are free again afterwards.
+template <int THREADS>
 __device__ TilePlace find_tile(const Attention &a, int index, int *scratch, TilePlace *found) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (a.batch.sequences == 1) {
+    const int n = tile_count(a, 0);
+    return {index < n ? 0 : -1, n - 1 - index};
+  }
   if (tid == 0) found->s = -1;
   int base = 0;
-  for (int c = 0; c < a.batch.sequences; c += 256) {
+  for (int c = 0; c < a.batch.sequences; c += THREADS) {
     const int n = tile_count(a, c + tid);
     int sum = n;
 #pragma unroll
@@ -618,12 +702,12 @@ __device__ TilePlace find_tile(const Attention &a, int index, int *scratch, Tile
     if (lane == 63) scratch[wave] = sum;
     __syncthreads();
     int before = base;
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < THREADS / 64; ++w) {
       if (w < wave) before += scratch[w];
       base += scratch[w];
     }
     before += sum - n;
-    if (index >= before && index < before + n) *found = {c + tid, n - 1 - (index - before), n};
+    if (index >= before && index < before + n) *found = {c + tid, n - 1 - (index - before)};
     if (base > index) break;  // the same for every thread
   }
   __syncthreads();
@@ -632,8 +716,6 @@ __device__ TilePlace find_tile(const Attention &a, int index, int *scratch, Tile
   return got;
 }
 
-constexpr int kTileKeys = 32;
-
 template <int D>
 struct TileState {
   float m = -INFINITY, l = 0.0f;  // of column lane & 31; l: this lane's keys only
@@ -641,22 +723,44 @@ struct TileState {
   bool odd = false;               // infinities or NaN were left out
 };
 
-// 32 keys and values into LDS by the workgroup's four waves: 8 rows of each a wave.
-template <int D>
-__device__ __forceinline__ void tile_load(const Attention &a, int s, int64_t head, int key,
-                                          LDS char *kt, LDS char *vt, int wave, int lane) {
-  const int k = key + wave * 8, to = wave * 8 * D * 2;
-  const int64_t at = paged_page(a.batch, s, k) + head +
-                     (int64_t)(k & ((1 << a.batch.page_shift) - 1)) * D;
-  load_rows<D, 8>(a.k_pages + at, wave * 8, kt + to, lane);
-  load_rows<D, 8>(a.v_pages + at, wave * 8, vt + to, lane);
+// Where a wave finds the keys of a tile: the pages of 64 steps of 16 keys from `from` on, one
+// a lane.
+struct TilePages {
+  const int32_t *table;
+  int64_t page_stride;
+  const uint16_t *k, *v;  // of the key-value head, in page 0
+  int shift, pages, entries;
+  int from, page_of;
+};
+
+__device__ __forceinline__ void tile_pages(TilePages &f, int key, int lane) {
+  f.from = key;
+  const int i = min((key + lane * 16) >> f.shift, f.entries - 1);
+  f.page_of = clamp_index32(f.table[i], f.pages);
+  settle(f.page_of);
+}
+
+// Loads a tile of keys and values from `key` on into LDS: ROWS rows of each a wave.
+template <int D, int ROWS>
+__device__ __forceinline__ void tile_load(TilePages &f, int key, LDS char *kt, LDS char *vt,
+                                          int wave, int lane) {
+  if (key - f.from >= 1024) tile_pages(f, key, lane);
+#pragma unroll
+  for (int r = 0; r < ROWS; r += 16) {  // of one page each
+    constexpr int N = ROWS < 16 ? ROWS : 16;
+    const int row = wave * ROWS + r, k = key + row, to = row * D * 2;
+    const int page = __builtin_amdgcn_readlane(f.page_of, (k - f.from) >> 4);
+    const int64_t at = page * f.page_stride + (int64_t)(k & ((1 << f.shift) - 1)) * D;
+    load_rows<D, N>(f.k + at, row, kt + to, lane);
+    load_rows<D, N, kQuads>(f.v + at, row, vt + to, lane);
+  }
 }
 
 // Operand of 16 keys from row `ks` of the tile, channels 32 i ..
 template <int D>
 __device__ __forceinline__ u32x4 tile_operand(const LDS char *vt, int base, int i, int ks) {
-  const u32x2 lo = read_transposed<D>(vt, base, ks, i * 32);
-  const u32x2 hi = read_transposed<D>(vt, base, ks + 8, i * 32);
+  const u32x2 lo = read_transposed<D, kQuads>(vt, base, ks, i * 32);
+  const u32x2 hi = read_transposed<D, kQuads>(vt, base, ks + 8, i * 32);
   return u32x4{lo[0], lo[1], hi[0], hi[1]};
 }
 
@@ -664,7 +768,7 @@ __device__ __forceinline__ u32x4 tile_operand(const LDS char *vt, int base, int 
 template <typename T, int D, bool MIXED>
 __device__ __forceinline__ void tile_values(const LDS char *vt, const u32x4 (&p)[2],
                                             TileState<D> &st, int lane) {
-  const int base = opaque(transpose_base<D>((lane >> 5) * 4, ((lane >> 4) & 1) * 16, lane));
+  const int base = opaque(transpose_base<D, kQuads>((lane >> 5) * 4, ((lane >> 4) & 1) * 16, lane));
   if constexpr (!MIXED) {
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
@@ -684,36 +788,32 @@ __device__ __forceinline__ void tile_values(const LDS char *vt, const u32x4 (&p)
     }
 }
 
-// One tile of 32 keys, the next one's loads started before it.  MIXED: some row does not
-// see all of the keys.
+// 32 keys of a tile for a wave's 32 rows.  MIXED: some row does not see all of the keys.
+// The wave's priority is raised while it feeds the matrix cores, so that the other wave of
+// its SIMD does its softmax beside them.
 template <typename T, int D, bool MIXED>
-__device__ __forceinline__ void tile_step(const LDS char *__restrict__ kt,
-                                          const LDS char *__restrict__ vt,
-                                          LDS char *__restrict__ next_k,
-                                          LDS char *__restrict__ next_v, const Attention &a, int s,
-                                          int64_t head, int key, int key1,
-                                          const u32x4 (&q)[D / 16], int limit, bool idle, TileState<D> &st, int wave, int lane) {
-  if (key + kTileKeys < key1)
-    tile_load<D>(a, s, head, key + kTileKeys, next_k, next_v, wave, lane);
-  if (idle) return;
+__device__ __forceinline__ void tile_step(const LDS char *kt, const LDS char *vt,
+                                          const u32x4 (&q)[D / 16], int key, int limit,
+                                          float scale2, TileState<D> &st, int lane) {
   const int h = lane >> 5, r = lane & 31;
   const int base = opaque(r * (D * 2) + ((h ^ swizzle<D>(r)) << 4));
   f32x16 x = {};
+  __builtin_amdgcn_s_setprio(1);
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) {
-    const u32x4 k = *(const LDS u32x4 *)(kt + (base ^ (i << 5)));
+    const u32x4 k = *(const LDS u32x4 *)(kt + swizzled<D, kRows>(base, 0, i * 2));
     x = mfma32(T{}, k, q[i], x);
   }
-  float mx = -INFINITY;
-  x *= a.scale2;
+  __builtin_amdgcn_s_setprio(0);
   if constexpr (MIXED) {
 #pragma unroll
     for (int i = 0; i < 16; ++i)
       if (key + 8 * (i / 4) + 4 * h + i % 4 >= limit) x[i] = -INFINITY;
   }
+  float mx = x[0];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[i]);
-  mx = across32(mx, Max());
+  for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
+  mx = across32(mx, Max()) * scale2;
   if (__any(mx > st.m + kSlack)) {
     const float n = fmaxf(st.m, mx), keep = decay(st.m, n);
     st.m = n;
@@ -725,71 +825,154 @@ __device__ __forceinline__ void tile_step(const LDS char *__restrict__ kt,
   u32x4 p[2];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float e0 = exp2_hw(x[2 * i] - at), e1 = exp2_hw(x[2 * i + 1] - at);
+    const float e0 = exp2_hw(__builtin_fmaf(x[2 * i], scale2, -at));
+    const float e1 = exp2_hw(__builtin_fmaf(x[2 * i + 1], scale2, -at));
     st.l += e0 + e1;
     p[i / 4][i % 4] = T::pack2(e0, e1);
   }
+  __builtin_amdgcn_s_setprio(1);
   tile_values<T, D, MIXED>(vt, p, st, lane);
+  __builtin_amdgcn_s_setprio(0);
+}
+
+// One half of a wave's rows' channels, or all (HALF < 0), to the output or the parts.
+template <typename T, int D, int HALF>
+__device__ __forceinline__ void tile_write(const Attention &a, RowPlace at, int split, float l,
+                                           const TileState<D> &st, int lane) {
+  constexpr int FROM = HALF == 1 ? D / 64 : 0, TO = HALF == 0 ? D / 64 : D / 32;
+  const int h = lane >> 5;
+  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+  const int64_t row = ((int64_t)split * a.tokens + at.token) * a.q_heads + at.head;
+#pragma unroll
+  for (int i = FROM; i < TO; ++i)
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const int d = i * 32 + b * 8 + h * 4;
+      const f32x4 o = {st.o[i][4 * b], st.o[i][4 * b + 1], st.o[i][4 * b + 2], st.o[i][4 * b + 3]};
+      if (a.splits == 1)
+        write_row<T, D>(a, at, d, o, inv);
+      else
+        *reinterpret_cast<f32x4 *>(a.part + row * D + d) = o;
+    }
+  if (a.splits > 1 && h == 0 && HALF < 1)
+    *reinterpret_cast<float2 *>(a.part_ml + row * 2) = float2{st.m, l};
+}
+
+// Hands the other key group of the same rows half of the channels and takes its share of
+// this wave's own half: `room` is the wave's place in LDS, `other` the other wave's.
+template <int D, int HALF>
+__device__ __forceinline__ void tile_give(const TileState<D> &st, float l, LDS f32x4 *room, int lane) {
+  constexpr int FROM = HALF == 0 ? D / 64 : 0;
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+      room[(i * 4 + b) * 64 + lane] =
+          f32x4{st.o[FROM + i][4 * b], st.o[FROM + i][4 * b + 1], st.o[FROM + i][4 * b + 2],
+                st.o[FROM + i][4 * b + 3]};
+  ((LDS float *)(room + D / 16 * 64))[lane] = st.m;
+  ((LDS float *)(room + D / 16 * 64))[64 + lane] = l;
+}
+template <int D, int HALF>
+__device__ __forceinline__ void tile_take(TileState<D> &st, float &l, const LDS f32x4 *other,
+                                          int lane) {
+  constexpr int FROM = HALF == 1 ? D / 64 : 0;
+  const float om = ((const LDS float *)(other + D / 16 * 64))[lane];
+  const float ol = ((const LDS float *)(other + D / 16 * 64))[64 + lane];
+  const float m = fmaxf(st.m, om), mine = decay(st.m, m), theirs = decay(om, m);
+  l = l * mine + ol * theirs;
+  st.m = m;
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const f32x4 o = other[(i * 4 + b) * 64 + lane];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        st.o[FROM + i][4 * b + j] = st.o[FROM + i][4 * b + j] * mine + o[j] * theirs;
+    }
+}
+
+template <int D>
+constexpr int tile_lds() {
+  using F = TileForm<D>;
+  constexpr int ring = 4 * F::kKeys * D * 2, join = F::kWaves * (D / 16 * 64 * 16 + 512);
+  return F::kGroups > 1 && join > ring ? join : ring;
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(256, 2) void attention_tile_kernel(Attention a) {
-  constexpr int TILE = kTileKeys * D * 2;
+__global__ __launch_bounds__(TileForm<D>::kWaves * 64, 2) void attention_tile_kernel(Attention a) {
+  constexpr int WAVES = TileForm<D>::kWaves, KEYS = TileForm<D>::kKeys, ROWS = KEYS / WAVES;
+  constexpr int GROUPS = TileForm<D>::kGroups, TILE = KEYS * D * 2;
+  static_assert(GROUPS == 1 || GROUPS == 2, "two groups are joined");
   // One array: with several, the compiler waits for all direct loads at each LDS read.
-  __shared__ __attribute__((aligned(16))) char lds[4 * TILE];
+  __shared__ __attribute__((aligned(16))) char lds[tile_lds<D>()];
   int *scratch = reinterpret_cast<int *>(lds);
-  TilePlace *found = reinterpret_cast<TilePlace *>(scratch + 4);
+  TilePlace *found = reinterpret_cast<TilePlace *>(scratch + WAVES);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int set = wave & 3, group = wave >> 2;
   const int kv = blockIdx.x % a.batch.kv_heads, split = blockIdx.y;
-  const TilePlace place = find_tile(a, blockIdx.x / a.batch.kv_heads, scratch, found);
+  const TilePlace place =
+      find_tile<WAVES * 64>(a, blockIdx.x / a.batch.kv_heads, scratch, found);
   const int s = __builtin_amdgcn_readfirstlane(place.s);
   if (s < 0) return;
   const PagedSequence seq = paged_sequence(a.batch, s, a.tokens);
   const int rows = seq.count * a.group, c0 = place.tile * kTileRows;
-  const int c = c0 + wave * 32 + (lane & 31);
-  const bool idle = c0 + wave * 32 >= rows;
+  const int c = c0 + set * 32 + (lane & 31);
+  const bool idle = c0 + set * 32 >= rows;
   const RowPlace at = row_place(a, seq, kv, min(c, rows - 1));
   const int limit = min(seq.base + min(c, rows - 1) / a.group + 1, seq.length);
   const int all_see = min(seq.base + c0 / a.group + 1, seq.length);  // seen by every row
   // keys that the tile's last row sees, and this split's part of them
   const int last = min(c0 + kTileRows, rows) - 1;
   const int keys = max(min(seq.base + last / a.group + 1, seq.length), 0);
-  const int tiles = (keys + kTileKeys - 1) / kTileKeys;
-  const int key0 = (int)((int64_t)tiles * split / a.splits) * kTileKeys;
-  const int key1 = min((int)((int64_t)tiles * (split + 1) / a.splits) * kTileKeys, keys);
+  const int tiles = (keys + KEYS - 1) / KEYS;
+  const int key0 = (int)((int64_t)tiles * split / a.splits) * KEYS;
+  const int key1 = min((int)((int64_t)tiles * (split + 1) / a.splits) * KEYS, keys);
 
   u32x4 q[D / 16];
   const uint16_t *qr = a.q + at.token * a.q_token + at.head * a.q_head + (lane >> 5) * 8;
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i) q[i] = ldg16(qr + i * 16);
+  for (int i = 0; i < D / 16; ++i) q[i] = ldg16(qr + i * 16) ^ a.flip;
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) settle(q[i]);
   TileState<D> st;
   LDS char *base = (LDS char *)lds;
   const int64_t head = (int64_t)(kv << a.batch.page_shift) * D;
   if (key0 < key1) {
-    tile_load<D>(a, s, head, key0, base, base + TILE, wave, lane);
+    TilePages f;
+    f.table = a.batch.table + s * a.batch.table_stride, f.page_stride = a.batch.page_stride;
+    f.k = a.k_pages + head, f.v = a.v_pages + head, f.shift = a.batch.page_shift;
+    f.pages = a.batch.pages, f.entries = a.batch.table_pages;
+    tile_pages(f, key0, lane);
+    tile_load<D, ROWS>(f, key0, base, base + TILE, wave, lane);
     wait_loads<0>();
     __syncthreads();
+    // A tile, the next one's loads started before it into the other half.
     int key = key0, half = 0;
-    const int whole = min(key1, all_see);
-    for (; key + kTileKeys <= whole; key += kTileKeys, half ^= 1) {
+    const int whole = min(key1, all_see), own = group * 32;
+    for (; key + KEYS <= whole; key += KEYS, half ^= 1) {
       LDS char *cur = base + half * 2 * TILE, *next = base + (half ^ 1) * 2 * TILE;
-      tile_step<T, D, false>(cur, cur + TILE, next, next + TILE, a, s, head, key, key1, q, limit,
-                             idle, st, wave, lane);
+      if (key + KEYS < key1) tile_load<D, ROWS>(f, key + KEYS, next, next + TILE, wave, lane);
+      if (!idle)
+        tile_step<T, D, false>(cur + own * D * 2, cur + TILE + own * D * 2, q, key + own, limit,
+                               a.scale2, st, lane);
       wait_loads<0>();
       __syncthreads();
     }
     const int mixed = key;
-    for (; key < key1; key += kTileKeys, half ^= 1) {
+    for (; key < key1; key += KEYS, half ^= 1) {
       LDS char *cur = base + half * 2 * TILE, *next = base + (half ^ 1) * 2 * TILE;
-      tile_step<T, D, true>(cur, cur + TILE, next, next + TILE, a, s, head, key, key1, q, limit,
-                            idle, st, wave, lane);
+      if (key + KEYS < key1) tile_load<D, ROWS>(f, key + KEYS, next, next + TILE, wave, lane);
+      if (!idle)
+        tile_step<T, D, true>(cur + own * D * 2, cur + TILE + own * D * 2, q, key + own, limit,
+                              a.scale2, st, lane);
       wait_loads<0>();
       __syncthreads();
     }
     if (__builtin_expect(__any(st.odd), 0)) {
       for (int k = mixed; k < min(key1, limit); ++k) {
+        if (((k - mixed) / 32) % GROUPS != group) continue;
         const uint16_t *v = value_row<D>(a, s, head, k) + (lane >> 5) * 4;
 #pragma unroll
         for (int i = 0; i < D / 32; ++i)
@@ -802,41 +985,45 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(Attention a) {
       }
     }
   }
-  if (c >= rows) return;
-  const float l = across32(st.l, Add());
-  const int h = lane >> 5;
-  if (a.splits == 1) {
-    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-      for (int b = 0; b < 4; ++b)
-        write_row<T, D>(a, at, i * 32 + b * 8 + h * 4,
-                        f32x4{st.o[i][4 * b], st.o[i][4 * b + 1], st.o[i][4 * b + 2],
-                              st.o[i][4 * b + 3]},
-                        inv);
-  } else {
-    const int64_t row = ((int64_t)split * a.tokens + at.token) * a.q_heads + at.head;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-      for (int b = 0; b < 4; ++b)
-        *reinterpret_cast<f32x4 *>(a.part + row * D + i * 32 + b * 8 + h * 4) =
-            f32x4{st.o[i][4 * b], st.o[i][4 * b + 1], st.o[i][4 * b + 2], st.o[i][4 * b + 3]};
-    if (h == 0) *reinterpret_cast<float2 *>(a.part_ml + row * 2) = float2{st.m, l};
+  float l = across32(st.l, Add());
+  if constexpr (GROUPS == 1) {
+    if (c < rows) tile_write<T, D, -1>(a, at, split, l, st, lane);
+  } else {  // every wave has left the ring: the last barrier above, or no key at all
+    LDS f32x4 *room = (LDS f32x4 *)base;
+    constexpr int STEP = D / 16 * 64 + 32;
+    if (group == 0)
+      tile_give<D, 0>(st, l, room + wave * STEP, lane);
+    else
+      tile_give<D, 1>(st, l, room + wave * STEP, lane);
+    __syncthreads();
+    if (group == 0) {
+      tile_take<D, 0>(st, l, room + (wave + 4) * STEP, lane);
+      if (c < rows) tile_write<T, D, 0>(a, at, split, l, st, lane);
+    } else {
+      tile_take<D, 1>(st, l, room + (wave - 4) * STEP, lane);
+      if (c < rows) tile_write<T, D, 1>(a, at, split, l, st, lane);
+    }
   }
 }
 
-// Rows of sequences in tiles, where their keys were split: blockIdx.x a token, y a head.
+// Rows of sequences in tiles, where their keys were split: D / 4 threads a row.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attention_combine_tile_kernel(Attention a) {
-  __shared__ __attribute__((aligned(16))) float buf[1024 + 256 / (D / 4)];
-  const int t = blockIdx.x, head = blockIdx.y, s = paged_find(a.batch, t);
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = (int64_t)a.tokens * a.q_heads;
+  const int64_t row = i / (D / 4);
+  const int d = (int)(i % (D / 4)) * 4, t = (int)(row / a.q_heads);
+  if (row >= rows) return;
+  const int s = paged_find(a.batch, t);
   if (s < 0) return;
   const PagedSequence seq = paged_sequence(a.batch, s, a.tokens);
   if (t < seq.first || t >= seq.first + seq.count || (a.few && few_rows(seq, a.group))) return;
-  const int64_t step = (int64_t)a.tokens * a.q_heads;
-  join_row<T, D>(a, (int64_t)t * a.q_heads + head, step, a.splits, {t, head}, buf);
+  PartSum sum;
+#pragma unroll 4
+  for (int j = 0; j < a.splits; ++j) {
+    const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + (row + j * rows) * 2);
+    sum.add(ml.x, ml.y, *reinterpret_cast<const f32x4 *>(a.part + (row + j * rows) * D + d));
+  }
+  write_row<T, D>(a, {t, (int)(row % a.q_heads)}, d, sum.o, sum.inverse());
 }
 
 // ------------------------------------------------------------------ host side
@@ -849,22 +1036,21 @@ struct AttentionPlan {
 };
 
 AttentionPlan attention_plan(int64_t tokens, int64_t sequences, int64_t q_heads, int64_t kv_heads,
-                             int64_t max_new, int64_t max_keys) {
+                             int64_t head_dim, int64_t max_new, int64_t max_keys) {
   AttentionPlan p = {};
   const int64_t group = q_heads / kv_heads;
   max_new = max_new < tokens ? max_new : tokens;
-  p.few = group <= kFewRows;
   p.tile = max_new * group > kFewRows;
+  p.few = group <= kFewRows && !(p.tile && sequences == 1);  // one sequence: one of them
   if (p.few) {
     p.shares = 512 / kv_heads > 1 ? 512 / kv_heads : 1;
-    const int64_t some = sequences < tokens ? sequences : tokens;  // with new tokens
-    p.few_grid = (p.shares + some) * kv_heads;
+    p.few_grid = p.shares * kv_heads;
     p.few_rows = 2 * p.shares * kv_heads * kFewRows;
   }
   if (p.tile) {
     const int64_t some = sequences < tokens ? sequences : tokens;
     p.tiles = tokens * group / kTileRows + some;
-    int64_t n = 512 / (p.tiles * kv_heads);
+    int64_t n = (head_dim == 256 ? 512 : 1024) / (p.tiles * kv_heads);
     if (n > max_keys / 256) n = max_keys / 256;
     p.splits = n < 1 ? 1 : n;
     if (p.splits > 1) p.tile_rows = p.splits * tokens * q_heads;
@@ -884,8 +1070,10 @@ int launch_attention(const AttentionPlan &p, Attention a, float *workspace, hipS
     a.part = workspace, a.part_ml = workspace + p.few_rows * D;
     attention_few_kernel<T, D><<<(unsigned)p.few_grid, 256, 0, st>>>(a);
     if (const int rc = check_launch("attention_few_kernel")) return rc;
-    const dim3 grid((unsigned)(a.batch.sequences * a.batch.kv_heads),
-                    (unsigned)(kFewRows / a.group * a.group));
+    // Where there are few sequences, their rows and channels fill the chip.
+    const int64_t heads = (int64_t)a.batch.sequences * a.batch.kv_heads;
+    const int64_t units = kFewRows / a.group * a.group * (D / 64), some = 1024 / heads;
+    const dim3 grid((unsigned)heads, (unsigned)(some < 1 ? 1 : some < units ? some : units));
     attention_combine_few_kernel<T, D><<<grid, 256, 0, st>>>(a);
     if (const int rc = check_launch("attention_combine_few_kernel")) return rc;
   }
@@ -893,11 +1081,11 @@ int launch_attention(const AttentionPlan &p, Attention a, float *workspace, hipS
     a.splits = (int)p.splits;
     a.part = workspace + p.few_rows * (D + 2), a.part_ml = a.part + p.tile_rows * D;
     const dim3 grid((unsigned)(p.tiles * a.batch.kv_heads), (unsigned)p.splits);
-    attention_tile_kernel<T, D><<<grid, 256, 0, st>>>(a);
+    attention_tile_kernel<T, D><<<grid, TileForm<D>::kWaves * 64, 0, st>>>(a);
     if (const int rc = check_launch("attention_tile_kernel")) return rc;
     if (p.splits > 1) {
       attention_combine_tile_kernel<T, D>
-          <<<dim3((unsigned)a.tokens, (unsigned)a.q_heads), 256, 0, st>>>(a);
+          <<<cdiv((int64_t)a.tokens * a.q_heads * (D / 4), 256), 256, 0, st>>>(a);
       return check_launch("attention_combine_tile_kernel");
     }
   }
@@ -925,7 +1113,7 @@ extern "C" int64_t lm_paged_attention_workspace_bytes(int64_t tokens, int64_t se
       max_new < 0)
     return 0;
   return attention_bytes(
-      attention_plan(tokens, sequences, q_heads, kv_heads, max_new, max_keys), head_dim);
+      attention_plan(tokens, sequences, q_heads, kv_heads, head_dim, max_new, max_keys), head_dim);
 }
 
 extern "C" int lm_paged_attention(const void *q, int64_t q_token_stride, int64_t q_head_stride,
@@ -954,7 +1142,7 @@ extern "C" int lm_paged_attention(const void *q, int64_t q_token_stride, int64_t
   LM_REQUIRE(!gate || (aligned16(gate) && gate_token_stride % 8 == 0 && gate_head_stride % 8 == 0 &&
                        gate_token_stride >= 0 && gate_head_stride >= 0),
              LM_EINVAL, "head rows must be 16-byte aligned");
-  const AttentionPlan plan = attention_plan(tokens, sequences, q_heads, kv_heads, max_new,
+  const AttentionPlan plan = attention_plan(tokens, sequences, q_heads, kv_heads, head_dim, max_new,
                                             table_pages * page_size);
   const int64_t need = attention_bytes(plan, head_dim);
   LM_REQUIRE(need == 0 || (workspace && aligned16(workspace)), LM_EINVAL,
@@ -971,7 +1159,9 @@ extern "C" int lm_paged_attention(const void *q, int64_t q_token_stride, int64_t
              __builtin_ctzll((unsigned long long)page_size), (int)pages, page_stride,
              (int)kv_heads};
   a.tokens = (int)tokens, a.q_heads = (int)q_heads, a.group = (int)(q_heads / kv_heads);
-  a.scale2 = scale * 1.4426950408889634f;
+  // A scale of 0 as one too small to matter, so that a masked -inf stays one under it.
+  a.scale2 = fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-30f);
+  a.flip = scale < 0.0f ? 0x80008000u : 0u;
   float *ws = static_cast<float *>(workspace);
   return dtype == LM_BF16
              ? launch_attention<BF16>(plan, a, ws, (int)head_dim, as_stream(stream))
