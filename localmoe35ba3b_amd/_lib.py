@@ -140,14 +140,6 @@ def call(name, *args):
         check(rc)
 
 
-def call_on(device, name, *args):
-    """call with `device` current, for streams and the null stream of that device."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return call(name, *args)
-    with torch.cuda.device(device):
-        call(name, *args)
-
-
 def ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -168,6 +160,29 @@ def stream(device=None):
     if _raw_stream is not None and device is not None and device.index is not None:
         return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+# A tensor's get_device() and the current device, both without a device object.
+_current_device = getattr(torch._C, '_cuda_getDevice', torch.cuda.current_device)
+
+
+def launch(index, name, *args):
+    """call on the current stream of device `index`, the last argument of the entry point,
+    with that device current."""
+    if _lib is None:
+        lib()
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return launch(index, name, *args)
+    rc = _fns[name](*args, stream_of(index))
+    if rc:
+        check(rc)
+
+
+def stream_of(index):
+    if _raw_stream is not None:
+        return _raw_stream(index)
+    return torch.cuda.current_stream(index).cuda_stream
 
 
 _DTYPE_CODES = {torch.bfloat16: LM_BF16, torch.float16: LM_FP16, torch.float32: LM_FP32}

@@ -10,10 +10,11 @@
 // frequency is exact in fp64, and its turns are reduced there before sine and
 // cosine are taken in fp32.
 //
-// A workgroup takes the rows of a few tokens.  Its threads first form each
-// token's angles once, in LDS; then D / 8 lanes hold a row, 16 bytes each, so a
-// row is read once, its sum of squares is a lane reduction, and the rotation's
-// partner channel is a lane shuffle.
+// A workgroup takes the rows of a token; D / 8 lanes hold one.  A lane of the rotated
+// channels takes four of the first half and their four partners of the second, others eight
+// in a row, so the rotation needs no exchange and a row is read once.  The first rows are
+// requested at the start, beside the position, whose lookups (sequence, length, page) are
+// the longest chain of a small call.
 #include "paged.hpp"
 
 namespace lm {
@@ -33,124 +34,152 @@ struct HeadRows {
 };
 
 constexpr int kMaxHalf = 128;
+constexpr int kAhead = 3;  // rows of a thread that are requested together
 
-// LANES = D / 8 lanes hold a row.  TOKENS per workgroup.
-template <typename T, int LANES, int TOKENS, bool PAGED>
+// Sum over the LANES (8, 16 or 32) lanes of a row, in every lane.
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v) {
+  if constexpr (LANES == 8) return octet_sum_f32(v);
+  v = row_sum_f32(v);
+  if constexpr (LANES == 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  return v;
+}
+
+struct Row8 {
+  uint2 lo, hi;
+};
+
+template <typename T>
+__device__ __forceinline__ void unpack4(uint2 w, float x[4]) {
+  x[0] = T::to_f32(w.x & 0xFFFFu), x[1] = T::to_f32(w.x >> 16);
+  x[2] = T::to_f32(w.y & 0xFFFFu), x[3] = T::to_f32(w.y >> 16);
+}
+
+template <typename T, int LANES, bool PAGED>
 __global__ __launch_bounds__(256) void head_rows_kernel(HeadRows a) {
   constexpr int D = LANES * 8, ROWS = 256 / LANES;
-  __shared__ float cosines[TOKENS][kMaxHalf], sines[TOKENS][kMaxHalf];
-  __shared__ int64_t place[TOKENS];     // element offset of the token's row of head 0; < 0: none
-  __shared__ double position[TOKENS];
-  const int t0 = blockIdx.x * TOKENS, n = min(TOKENS, a.tokens - t0);
-  if (threadIdx.x < n) {
-    const int t = t0 + threadIdx.x;
-    if constexpr (PAGED) {
-      const int s = paged_find(a.batch, t);
-      int64_t at = -1;
-      int p = 0;
-      if (s >= 0) {
-        const int first = a.batch.starts[s], count = a.batch.starts[s + 1] - first;
-        p = a.batch.lengths[s] - count + (t - first);
-        const int64_t room = (int64_t)a.batch.table_pages << a.batch.page_shift;
-        at = -2;  // a token of the sequence without a place in the cache
-        if (p >= 0 && p < room)
-          at = paged_page(a.batch, s, p) + (int64_t)(p & ((1 << a.batch.page_shift) - 1)) * D;
-      }
-      place[threadIdx.x] = at;
-      position[threadIdx.x] = p;
-    } else {
-      place[threadIdx.x] = 0;
-      position[threadIdx.x] = (double)a.positions[t];
-    }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < n * a.half; i += 256) {
-    const int t = i / a.half, j = i - t * a.half;
-    constexpr double kTurns = 0.15915494309189533577;  // 1 / (2 pi)
-    const double turns = position[t] * (double)a.inv_freq[j] * kTurns;
-    const float r = (float)(turns - rint(turns));
-    sincospif(2.0f * r, &sines[t][j], &cosines[t][j]);
-  }
-  __syncthreads();
-
-  const int lane = threadIdx.x % LANES, e0 = lane * 8, half = a.half;
+  __shared__ __attribute__((aligned(16))) float cosines[kMaxHalf], sines[kMaxHalf];
+  __shared__ int64_t place;  // element offset of the token's row of head 0 in the cache; < 0: none
+  __shared__ int found, at;  // the token's sequence and position
+  const int t = blockIdx.x, tid = threadIdx.x, lane = tid % LANES, half = a.half;
   const int heads = a.q_heads + a.k_heads + (PAGED ? a.k_heads : 0);
-  const bool rotated = e0 < 2 * half;
-  const int partner = (threadIdx.x & 63) + (rotated ? (e0 < half ? half / 8 : -half / 8) : 0);
-  for (int r = threadIdx.x / LANES; r < n * heads; r += ROWS) {
-    const int tl = r / heads, t = t0 + tl;
-    int h = r - tl * heads;
-    const int64_t at = place[tl];
-    const uint16_t *src;
-    uint16_t *dst;
-    const float *w = nullptr;
-    bool turn = half > 0;
-    if (h < a.q_heads) {
-      src = a.q + t * a.q_token + h * a.q_head;
-      dst = a.q_out + ((int64_t)t * a.q_heads + h) * D;
-      if (at == -1) continue;  // a row of no sequence
-      w = a.q_w;
-    } else {
-      h -= a.q_heads;
-      const int64_t to = at + ((int64_t)h << a.batch.page_shift) * D;
-      if (h < a.k_heads) {
-        src = a.k + t * a.k_token + h * a.k_head;
-        dst = PAGED ? a.k_pages + to : a.k_out + ((int64_t)t * a.k_heads + h) * D;
-        w = a.k_w;
+  const bool rotated = lane * 8 < 2 * half;
+  const int lo = rotated ? lane * 4 : lane * 8, hi = rotated ? half + lane * 4 : lane * 8 + 4;
+
+  auto load = [&](int r) {  // row r of the token: its queries, then keys, then values
+    r = min(r, heads - 1);
+    const uint16_t *p = r < a.q_heads ? a.q + t * a.q_token + r * a.q_head
+                        : r < a.q_heads + a.k_heads
+                            ? a.k + t * a.k_token + (r - a.q_heads) * a.k_head
+                            : a.v + t * a.v_token + (r - a.q_heads - a.k_heads) * a.v_head;
+    return Row8{ldg_u2(p + lo), ldg_u2(p + hi)};
+  };
+  const int r0 = tid / LANES;
+  Row8 raw[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) raw[i] = load(r0 + i * ROWS);
+  const float freq = tid < half ? a.inv_freq[tid] : 0.0f;
+
+  double position;
+  int64_t to = 0;
+  if constexpr (PAGED) {
+    if (tid == 0) found = -1;
+    __syncthreads();
+    for (int s = tid; s < a.batch.sequences; s += 256) {
+      const int first = a.batch.starts[s], end = a.batch.starts[s + 1], n = a.batch.lengths[s];
+      if (first <= t && t < end) found = s, at = n - (end - first) + (t - first);
+    }
+    __syncthreads();
+    if (found < 0) return;  // a row of no sequence
+    const int p = at;
+    position = p;
+    if (tid == 255) {
+      const int64_t room = (int64_t)a.batch.table_pages << a.batch.page_shift;
+      place = p < 0 || p >= room ? -1
+                                 : paged_page(a.batch, found, p) +
+                                       (int64_t)(p & ((1 << a.batch.page_shift) - 1)) * D;
+    }
+  } else {
+    position = (double)a.positions[t];
+  }
+  if (tid < half) {
+    constexpr double kTurns = 0.15915494309189533577;  // 1 / (2 pi)
+    const double turns = position * (double)freq * kTurns;
+    sincospif(2.0f * (float)(turns - rint(turns)), &sines[tid], &cosines[tid]);
+  }
+  __syncthreads();
+  if constexpr (PAGED) to = place;
+
+  float c[4], s[4];
+  if (rotated) {
+    *reinterpret_cast<float4 *>(c) = *reinterpret_cast<const float4 *>(cosines + lo);
+    *reinterpret_cast<float4 *>(s) = *reinterpret_cast<const float4 *>(sines + lo);
+  }
+  for (int r = r0; r < heads;) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i, r += ROWS) {
+      if (r >= heads) break;
+      float x[4], y[4];
+      unpack4<T>(raw[i].lo, x);
+      unpack4<T>(raw[i].hi, y);
+      const bool value = PAGED && r >= a.q_heads + a.k_heads;
+      const float *w = r < a.q_heads ? a.q_w : value ? nullptr : a.k_w;
+      if (w) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ss = __builtin_fmaf(x[j], x[j], ss);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ss = __builtin_fmaf(y[j], y[j], ss);
+        const float n = 1.0f / sqrtf(lanes_sum<LANES>(ss) * (1.0f / D) + a.eps);
+        const float4 w0 = *reinterpret_cast<const float4 *>(w + lo);
+        const float4 w1 = *reinterpret_cast<const float4 *>(w + hi);
+        x[0] *= n * (1.0f + w0.x), x[1] *= n * (1.0f + w0.y);
+        x[2] *= n * (1.0f + w0.z), x[3] *= n * (1.0f + w0.w);
+        y[0] *= n * (1.0f + w1.x), y[1] *= n * (1.0f + w1.y);
+        y[2] *= n * (1.0f + w1.z), y[3] *= n * (1.0f + w1.w);
+      }
+      if (rotated && !value) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float u = x[j] * c[j] - y[j] * s[j];
+          y[j] = y[j] * c[j] + x[j] * s[j];
+          x[j] = u;
+        }
+      }
+      uint16_t *dst;
+      if (r < a.q_heads) {
+        dst = a.q_out + ((int64_t)t * a.q_heads + r) * D;
       } else {
-        h -= a.k_heads;
-        src = a.v + t * a.v_token + h * a.v_head;
-        dst = a.v_pages + (to - ((int64_t)a.k_heads << a.batch.page_shift) * D);
-        turn = false;
+        const int h = r - a.q_heads - (value ? a.k_heads : 0);
+        if constexpr (PAGED) {
+          if (to < 0) continue;
+          dst = (value ? a.v_pages : a.k_pages) + to + ((int64_t)h << a.batch.page_shift) * D;
+        } else {
+          dst = a.k_out + ((int64_t)t * a.k_heads + h) * D;
+        }
       }
-      if (at < 0) continue;
+      *reinterpret_cast<uint2 *>(dst + lo) = uint2{T::pack2(x[0], x[1]), T::pack2(x[2], x[3])};
+      *reinterpret_cast<uint2 *>(dst + hi) = uint2{T::pack2(y[0], y[1]), T::pack2(y[2], y[3])};
     }
-    const u32x4 raw = ldg16(src + e0);
-    float x[8];
+    if (r < heads) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = T::to_f32(raw[i] & 0xFFFFu);
-      x[2 * i + 1] = T::to_f32(raw[i] >> 16);
+      for (int i = 0; i < kAhead; ++i) raw[i] = load(r + i * ROWS);
     }
-    if (w) {
-      float ss = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(x[i], x[i], ss);
-#pragma unroll
-      for (int o = LANES / 2; o >= 1; o >>= 1) ss += __shfl_xor(ss, o, 64);
-      const float s = 1.0f / sqrtf(ss * (1.0f / D) + a.eps);
-      const float4 w0 = *reinterpret_cast<const float4 *>(w + e0);
-      const float4 w1 = *reinterpret_cast<const float4 *>(w + e0 + 4);
-      const float wv[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = x[i] * s * (1.0f + wv[i]);
-    }
-    if (turn) {
-      const int j = rotated ? (e0 < half ? e0 : e0 - half) : 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float other = __shfl(x[i], partner, 64);
-        const float c = cosines[tl][j + i], s = sines[tl][j + i];
-        if (rotated) x[i] = x[i] * c + (e0 < half ? -other * s : other * s);
-      }
-    }
-    u32x4 y;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = T::pack2(x[2 * i], x[2 * i + 1]);
-    *reinterpret_cast<u32x4 *>(dst + e0) = y;
   }
 }
 
 template <typename T, bool PAGED>
 void launch_rows(const HeadRows &a, int head_dim, hipStream_t st) {
-  constexpr int TOKENS = 4;
-  const unsigned grid = cdiv(a.tokens, TOKENS);
+  const unsigned grid = (unsigned)a.tokens;
   if (head_dim == 256)
-    head_rows_kernel<T, 32, TOKENS, PAGED><<<grid, 256, 0, st>>>(a);
+    head_rows_kernel<T, 32, PAGED><<<grid, 256, 0, st>>>(a);
   else if (head_dim == 128)
-    head_rows_kernel<T, 16, TOKENS, PAGED><<<grid, 256, 0, st>>>(a);
+    head_rows_kernel<T, 16, PAGED><<<grid, 256, 0, st>>>(a);
   else
-    head_rows_kernel<T, 8, TOKENS, PAGED><<<grid, 256, 0, st>>>(a);
+    head_rows_kernel<T, 8, PAGED><<<grid, 256, 0, st>>>(a);
 }
 
 // Checks of one input's rows, whose head_dim channels are contiguous.

@@ -17,6 +17,8 @@ Rows of no sequence (padding behind the last) are left as they were.
 The reference has no operators of this kind (its layers run the Transformers
 modules, HF:627-735).
 """
+import functools
+
 import torch
 
 from .. import _lib
@@ -25,7 +27,8 @@ _TYPES = (torch.bfloat16, torch.float16)
 
 
 def _rows(x, what):
-    """x [tokens, heads, head_dim] with contiguous, 16-byte aligned heads; a copy of others."""
+    """x [tokens, heads, head_dim] with contiguous, 16-byte aligned heads (a copy of others),
+    and its strides."""
     if not x.is_cuda or x.ndim != 3 or x.dtype not in _TYPES:
         raise ValueError(f'{what}: expected CUDA FP16/BF16 rows [tokens, heads, head_dim]')
     token, head, channel = x.stride()
@@ -33,37 +36,41 @@ def _rows(x, what):
         x = x.contiguous()
         if x.data_ptr() % 16:
             x = x.clone()
-    return x
+        token, head, _ = x.stride()
+    return x, token, head
 
 
-def _weight(w, x):
-    """fp32 norm weights on the device of x, or None."""
+def _same(x, dtype, device):
+    if x.dtype is not dtype or x.get_device() != device:
+        raise ValueError('attention tensors must share their type and device')
+
+
+def _weight(w, dim, device):
+    """fp32 norm weights [dim] on the device, 16-byte aligned, and their address (0: no norm)."""
     if w is None:
-        return None
-    if w.numel() != x.shape[-1]:
-        raise ValueError('norm weight does not match the head size')
-    if w.dtype is not torch.float32 or w.device != x.device or not w.is_contiguous():
-        w = w.to(device=x.device, dtype=torch.float32).contiguous()
-    return w if w.data_ptr() % 16 == 0 else w.clone()
-
-
-def _frequencies(inv_freq, x):
-    """fp32 frequencies on the device of x, or None, and how many."""
-    if inv_freq is None:
         return None, 0
+    if w.numel() != dim:
+        raise ValueError('norm weight does not match the head size')
+    if w.dtype is not torch.float32 or w.get_device() != device or not w.is_contiguous():
+        w = w.to(device=device, dtype=torch.float32).contiguous()
+    at = w.data_ptr()
+    if at % 16:
+        w = w.clone()
+        at = w.data_ptr()
+    return w, at
+
+
+def _frequencies(inv_freq, dim, device):
+    """fp32 frequencies on the device, their address (0: no rotation), and how many."""
+    if inv_freq is None:
+        return None, 0, 0
     pairs = inv_freq.numel()
-    if pairs < 8 or pairs % 8 or 2 * pairs > x.shape[-1]:
+    if pairs < 8 or pairs % 8 or 2 * pairs > dim:
         raise ValueError('rotated channels must be a multiple of 16 and fit the head')
-    if (inv_freq.dtype is not torch.float32 or inv_freq.device != x.device
+    if (inv_freq.dtype is not torch.float32 or inv_freq.get_device() != device
             or not inv_freq.is_contiguous()):
-        inv_freq = inv_freq.to(device=x.device, dtype=torch.float32).contiguous()
-    return inv_freq, pairs
-
-
-def _same(x, *others):
-    for o in others:
-        if o.dtype is not x.dtype or o.device != x.device:
-            raise ValueError('attention tensors must share their type and device')
+        inv_freq = inv_freq.to(device=device, dtype=torch.float32).contiguous()
+    return inv_freq, inv_freq.data_ptr(), pairs
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6):
@@ -73,52 +80,56 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6):
     and head strides); weights [D] (scale 1 + w) or None for no norm; positions int64
     [T]; inv_freq [R / 2] rotates channels i and i + R / 2 by positions * inv_freq[i]
     (None: no rotation)."""
-    q, k = _rows(q, 'queries'), _rows(k, 'keys')
-    _same(q, k)
+    q, q_token, q_head = _rows(q, 'queries')
+    k, k_token, k_head = _rows(k, 'keys')
+    dtype, device = q.dtype, q.get_device()
+    _same(k, dtype, device)
     tokens, q_heads, dim = q.shape
-    k_heads = k.shape[1]
-    if k.shape[0] != tokens or k.shape[2] != dim:
+    k_tokens, k_heads, k_dim = k.shape
+    if k_tokens != tokens or k_dim != dim:
         raise ValueError('queries and keys do not match')
-    if positions.device != q.device or positions.numel() != tokens:
+    if positions.get_device() != device or positions.numel() != tokens:
         raise ValueError('Expected a CUDA position of every token')
-    positions = positions.to(torch.int64).contiguous()
-    q_weight, k_weight = _weight(q_weight, q), _weight(k_weight, k)
-    inv_freq, pairs = _frequencies(inv_freq, q)
+    if positions.dtype is not torch.int64 or not positions.is_contiguous():
+        positions = positions.to(torch.int64).contiguous()
+    q_weight, q_w = _weight(q_weight, dim, device)
+    k_weight, k_w = _weight(k_weight, dim, device)
+    inv_freq, freq, pairs = _frequencies(inv_freq, dim, device)
     q_out, k_out = q.new_empty((tokens, q_heads, dim)), k.new_empty((tokens, k_heads, dim))
-    _lib.call_on(q.device, 'lm_qk_norm_rope', q.data_ptr(), q.stride(0), q.stride(1), q_heads,
-              _lib.ptr(q_weight), q_out.data_ptr(), k.data_ptr(), k.stride(0), k.stride(1),
-              k_heads, _lib.ptr(k_weight), k_out.data_ptr(), positions.data_ptr(),
-              _lib.ptr(inv_freq), pairs, tokens, dim, eps, _lib.dtype_code(q.dtype),
-              _lib.stream(q.device))
+    _lib.launch(device, 'lm_qk_norm_rope', q.data_ptr(), q_token, q_head, q_heads, q_w,
+                q_out.data_ptr(), k.data_ptr(), k_token, k_head, k_heads, k_w, k_out.data_ptr(),
+                positions.data_ptr(), freq, pairs, tokens, dim, eps, _lib.dtype_code(dtype))
     return q_out, k_out
 
 
-def _cache(k_pages, v_pages):
+def _cache(k_pages, v_pages, dtype, device):
     """(pages, page stride, kv_heads, page_size, head_dim) of a cache."""
-    if (k_pages.ndim != 4 or k_pages.shape != v_pages.shape or not k_pages.is_cuda
-            or k_pages.dtype not in _TYPES or k_pages.stride() != v_pages.stride()):
-        raise ValueError('Expected CUDA key and value pages [pages, kv_heads, page_size, head_dim]')
-    _same(k_pages, v_pages)
-    pages, heads, size, dim = k_pages.shape
-    stride, *inner = k_pages.stride()
-    if tuple(inner) != (size * dim, dim, 1):
+    shape, strides = k_pages.shape, k_pages.stride()
+    if len(shape) != 4 or v_pages.shape != shape or v_pages.stride() != strides:
+        raise ValueError('Expected key and value pages [pages, kv_heads, page_size, head_dim]')
+    _same(k_pages, dtype, device)
+    _same(v_pages, dtype, device)
+    pages, heads, size, dim = shape
+    if strides[1:] != (size * dim, dim, 1):
         raise ValueError('the values of a page must be contiguous')
-    return pages, stride if pages > 1 else heads * size * dim, heads, size, dim
+    return pages, strides[0] if pages > 1 else heads * size * dim, heads, size, dim
 
 
 def _batch(device, starts, lengths, table):
     """The C arguments of a batch: pointers, table stride, table pages, sequences."""
-    for t in (starts, lengths, table):
-        if t.dtype is not torch.int32 or t.device != device:
-            raise ValueError('Expected CUDA int32 starts, lengths and page table')
-    sequences = lengths.numel()
-    if starts.numel() != sequences + 1 or table.ndim != 2 or table.shape[0] != sequences:
+    i32 = torch.int32
+    if (starts.dtype is not i32 or lengths.dtype is not i32 or table.dtype is not i32
+            or starts.get_device() != device or lengths.get_device() != device
+            or table.get_device() != device):
+        raise ValueError('Expected CUDA int32 starts, lengths and page table')
+    sequences, shape = lengths.numel(), table.shape
+    if starts.numel() != sequences + 1 or len(shape) != 2 or shape[0] != sequences:
         raise ValueError('starts, lengths and page table do not match')
-    if not (starts.is_contiguous() and lengths.is_contiguous()) or (
-            table.shape[1] > 1 and table.stride(1) != 1):
+    stride, step = table.stride()
+    if not (starts.is_contiguous() and lengths.is_contiguous()) or (step != 1 and shape[1] > 1):
         raise ValueError('starts, lengths and the rows of the page table must be contiguous')
     return (starts.data_ptr(), lengths.data_ptr(), table.data_ptr(),
-            table.stride(0) if sequences > 1 else table.shape[1], table.shape[1], sequences)
+            stride if sequences > 1 else shape[1], shape[1], sequences)
 
 
 def append(k_pages, v_pages, k, v, starts, lengths, table, inv_freq=None, k_weight=None, q=None,
@@ -127,31 +138,36 @@ def append(k_pages, v_pages, k, v, starts, lengths, table, inv_freq=None, k_weig
     (k_weight and inv_freq as in qk_norm_rope, by its position in its sequence).
     With q [T, q_heads, D], returns the queries normed and rotated for
     paged_attention; rows of no sequence are not written there."""
-    pages, stride, heads, size, dim = _cache(k_pages, v_pages)
-    k, v = _rows(k, 'keys'), _rows(v, 'values')
-    _same(k_pages, k, v)
-    tokens = k.shape[0]
-    if k.shape != v.shape or k.shape[1] != heads or k.shape[2] != dim:
+    k, k_token, k_head = _rows(k, 'keys')
+    v, v_token, v_head = _rows(v, 'values')
+    dtype, device, shape = k.dtype, k.get_device(), k.shape
+    _same(v, dtype, device)
+    pages, stride, heads, size, dim = _cache(k_pages, v_pages, dtype, device)
+    tokens = shape[0]
+    if v.shape != shape or shape[1] != heads or shape[2] != dim:
         raise ValueError('keys and values do not match the cache')
-    q_args = (None, 0, 0, 0, None, None)
-    q_out = None
+    q_args, q_out = (0, 0, 0, 0, 0, 0), None
     if q is not None:
-        q = _rows(q, 'queries')
-        _same(k, q)
-        if q.shape[0] != tokens or q.shape[2] != dim:
+        q, q_token, q_head = _rows(q, 'queries')
+        _same(q, dtype, device)
+        q_tokens, q_heads, q_dim = q.shape
+        if q_tokens != tokens or q_dim != dim:
             raise ValueError('queries and keys do not match')
-        q_weight = _weight(q_weight, q)
-        q_out = q.new_empty(q.shape)
-        q_args = (q.data_ptr(), q.stride(0), q.stride(1), q.shape[1], _lib.ptr(q_weight),
-                  q_out.data_ptr())
-    k_weight = _weight(k_weight, k)
-    inv_freq, pairs = _frequencies(inv_freq, k)
-    batch = _batch(k.device, starts, lengths, table)
-    _lib.call_on(k.device, 'lm_paged_append', k.data_ptr(), k.stride(0), k.stride(1), _lib.ptr(k_weight),
-              v.data_ptr(), v.stride(0), v.stride(1), *q_args, k_pages.data_ptr(),
-              v_pages.data_ptr(), pages, stride, heads, size, dim, *batch, _lib.ptr(inv_freq),
-              pairs, tokens, eps, _lib.dtype_code(k.dtype), _lib.stream(k.device))
+        q_weight, q_w = _weight(q_weight, dim, device)
+        q_out = q.new_empty((tokens, q_heads, dim))
+        q_args = (q.data_ptr(), q_token, q_head, q_heads, q_w, q_out.data_ptr())
+    k_weight, k_w = _weight(k_weight, dim, device)
+    inv_freq, freq, pairs = _frequencies(inv_freq, dim, device)
+    _lib.launch(device, 'lm_paged_append', k.data_ptr(), k_token, k_head, k_w, v.data_ptr(),
+                v_token, v_head, *q_args, k_pages.data_ptr(), v_pages.data_ptr(), pages, stride,
+                heads, size, dim, *_batch(device, starts, lengths, table), freq, pairs, tokens, eps,
+                _lib.dtype_code(dtype))
     return q_out
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(*sizes):
+    return _lib.lib().lm_paged_attention_workspace_bytes(*sizes)
 
 
 def paged_attention(q, k_pages, v_pages, starts, lengths, table, scale=None, gate=None,
@@ -163,33 +179,32 @@ def paged_attention(q, k_pages, v_pages, starts, lengths, table, scale=None, gat
     max_new bounds the new tokens of one sequence (default: T); a close bound saves
     time.  out [T, q_heads, D], contiguous, receives the result; rows of no sequence
     keep what they hold there."""
-    pages, stride, heads, size, dim = _cache(k_pages, v_pages)
-    q = _rows(q, 'queries')
-    _same(k_pages, q)
-    tokens, q_heads = q.shape[:2]
-    if q.shape[2] != dim or q_heads % heads:
+    q, q_token, q_head = _rows(q, 'queries')
+    dtype, device, shape = q.dtype, q.get_device(), q.shape
+    pages, stride, heads, size, dim = _cache(k_pages, v_pages, dtype, device)
+    tokens, q_heads, q_dim = shape
+    if q_dim != dim or q_heads % heads:
         raise ValueError('queries do not match the cache')
-    gate_args = (None, 0, 0)
+    gate_args = (0, 0, 0)
     if gate is not None:
-        gate = _rows(gate, 'gate')
-        _same(q, gate)
-        if gate.shape != q.shape:
+        gate, gate_token, gate_head = _rows(gate, 'gate')
+        _same(gate, dtype, device)
+        if gate.shape != shape:
             raise ValueError('gate does not match the queries')
-        gate_args = (gate.data_ptr(), gate.stride(0), gate.stride(1))
+        gate_args = (gate.data_ptr(), gate_token, gate_head)
     if out is None:
-        out = q.new_empty(q.shape)
+        out = q.new_empty(shape)
     else:
-        _same(q, out)
-        if out.shape != q.shape or not out.is_contiguous() or out.data_ptr() % 16:
+        _same(out, dtype, device)
+        if out.shape != shape or not out.is_contiguous() or out.data_ptr() % 16:
             raise ValueError('Expected a contiguous output of the shape of the queries')
-    batch = _batch(q.device, starts, lengths, table)
-    max_new = tokens if max_new is None else max_new
-    need = _lib.lib().lm_paged_attention_workspace_bytes(tokens, batch[5], q_heads, heads, dim,
-                                                         max_new, batch[4] * size)
-    workspace = q.new_empty(need, dtype=torch.uint8) if need > 0 else None
-    _lib.call_on(q.device, 'lm_paged_attention', q.data_ptr(), q.stride(0), q.stride(1), q_heads,
-              k_pages.data_ptr(), v_pages.data_ptr(), pages, stride, heads, size, dim, *batch,
-              tokens, max_new, dim ** -0.5 if scale is None else scale, *gate_args,
-              out.data_ptr(), _lib.ptr(workspace), need, _lib.dtype_code(q.dtype),
-              _lib.stream(q.device))
+    batch = _batch(device, starts, lengths, table)
+    if max_new is None:
+        max_new = tokens
+    need = _workspace_bytes(tokens, batch[5], q_heads, heads, dim, max_new, batch[4] * size)
+    workspace = q.new_empty(need // 2) if need > 0 else None
+    _lib.launch(device, 'lm_paged_attention', q.data_ptr(), q_token, q_head, q_heads,
+                k_pages.data_ptr(), v_pages.data_ptr(), pages, stride, heads, size, dim, *batch,
+                tokens, max_new, dim ** -0.5 if scale is None else scale, *gate_args,
+                out.data_ptr(), _lib.ptr(workspace), need, _lib.dtype_code(dtype))
     return out

@@ -22,8 +22,7 @@ def gpu(*shape, dtype=torch.bfloat16):
 @pytest.fixture
 def calls(monkeypatch):
     got = []
-    monkeypatch.setattr(_lib, 'call_on', lambda device, name, *args: got.append((name, args)))
-    monkeypatch.setattr(_lib, 'stream', lambda device=None: 0)
+    monkeypatch.setattr(_lib, 'launch', lambda device, name, *args: got.append((name, args)))
     return got
 
 
