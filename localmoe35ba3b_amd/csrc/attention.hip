@@ -40,6 +40,11 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
+// The parts of a sequence at a key-value head: their first span, its place there, their count.
+struct Parts {
+  int span, later, count;
+};
+
 struct Attention {
   const uint16_t *q, *gate;  // gate: null or a row for each row of q
   int64_t q_token, q_head, gate_token, gate_head;  // strides, elements
@@ -47,6 +52,7 @@ struct Attention {
   uint16_t *out;  // [tokens][q_heads][D]
   float *part;    // unscaled sums of split keys, then (m, l) of each row
   float *part_ml;
+  Parts *parts;   // few: [sequences][kv_heads]
   PagedBatch batch;
   int tokens, q_heads, group;
   int shares;  // few: spans that a key-value head's keys are cut into, at most
@@ -243,17 +249,27 @@ struct Find {
   int s;          // < 0: none
 };
 
-// The spans, and the sequence that holds the first block of span `index` (BY_SEQUENCE:
-// sequence `index`).  All 256 threads; scratch (8 words of LDS) and found are free again
-// afterwards.
-template <bool BY_SEQUENCE>
+// The spans, and the sequence that holds the first block of span `index`.  All 256 threads;
+// scratch (8 words of LDS) and found are free again afterwards.
 __device__ Spans find_span(const Attention &a, int index, int64_t *scratch, Find *found, Find &got) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, S = a.batch.sequences;
   Spans sp;
-  if (S == 1) {
-    sp.blocks = few_blocks(a, 0);
+  got = {0, -1};
+  if (S <= 64) {  // every wave by itself: a sequence a lane
+    const uint32_t n = few_blocks(a, lane);  // 64 of at most 2^25
+    uint32_t sum = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t v = __shfl_up(sum, o, 64);
+      if (lane >= o) sum += v;
+    }
+    sp.blocks = (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
     sp.spans = (int)min((int64_t)a.shares, sp.blocks);
-    got = {0, index < (BY_SEQUENCE ? min(sp.spans, 1) : sp.spans) ? 0 : -1};
+    if (index < sp.spans) {
+      const int64_t want = sp.start(index);
+      const int s = __builtin_ctzll(__ballot(want < (int64_t)sum));  // the first that ends after it
+      got = {(uint32_t)__builtin_amdgcn_readlane((int)(sum - n), s), s};
+    }
     return sp;
   }
   if (tid == 0) found->s = -1;
@@ -266,10 +282,10 @@ __device__ Spans find_span(const Attention &a, int index, int64_t *scratch, Find
   __syncthreads();
   sp.blocks = scratch[0] + scratch[1] + scratch[2] + scratch[3];
   sp.spans = (int)min((int64_t)a.shares, sp.blocks);
-  if (BY_SEQUENCE || index < sp.spans) {
-    const int64_t want = BY_SEQUENCE ? 0 : sp.start(index);
+  if (index < sp.spans) {
+    const int64_t want = sp.start(index);
     int64_t base = 0;  // blocks before this group of 256 sequences
-    for (int c = 0; c < S && (BY_SEQUENCE ? c <= index : base <= want); c += 256) {
+    for (int c = 0; c < S && base <= want; c += 256) {
       const int n = c == 0 ? mine : few_blocks(a, c + tid);
       int64_t sum = n;
 #pragma unroll
@@ -285,8 +301,7 @@ __device__ Spans find_span(const Attention &a, int index, int64_t *scratch, Find
         if (w < wave) before += scratch[4 + w];
         base += scratch[4 + w];
       }
-      if (n > 0 && (BY_SEQUENCE ? c + tid == index : want >= before && want < before + n))
-        *found = {before, c + tid};
+      if (n > 0 && want >= before && want < before + n) *found = {before, c + tid};
     }
   }
   __syncthreads();
@@ -562,7 +577,7 @@ __global__ __launch_bounds__(256, 1) void attention_few_kernel(Attention a) {
   int64_t *scratch = reinterpret_cast<int64_t *>(lds);
   const int kv = blockIdx.x % a.batch.kv_heads, span = blockIdx.x / a.batch.kv_heads;
   Find at;
-  const Spans sp = find_span<false>(a, span, scratch, reinterpret_cast<Find *>(scratch + 8), at);
+  const Spans sp = find_span(a, span, scratch, reinterpret_cast<Find *>(scratch + 8), at);
   if (at.s < 0) return;
   int64_t block = sp.start(span);
   const int64_t end = sp.start(span + 1);
@@ -573,6 +588,8 @@ __global__ __launch_bounds__(256, 1) void attention_few_kernel(Attention a) {
     const int all = __builtin_amdgcn_readfirstlane(few_blocks(a, s));
     const int take = __builtin_amdgcn_readfirstlane((int)min((int64_t)(all - done), end - block));
     if (take <= 0) continue;
+    if (done == 0 && threadIdx.x == 0)  // where its parts are, for the kernel that joins them
+      a.parts[s * a.batch.kv_heads + kv] = {span, later, sp.of(block + all - 1) - span + 1};
     few_part<T, D>(a, s, kv, done, done + take, take == all ? -1 : part_row(a, span, later, kv),
                    lds);
     block += take;
@@ -593,43 +610,42 @@ struct PartSum {
   __device__ __forceinline__ float inverse() const { return l > 0.0f || l != l ? 1.0f / l : 0.0f; }
 };
 
-constexpr int kFewParts = 8;
+constexpr int kFewParts = 16;
 
 // Rows of sequences whose keys attention_few_kernel split; blockIdx.x is a sequence's
-// key-value head.  Up to kFewParts parts: a thread takes four channels of a row, all parts of
-// it loaded at once.  More (few sequences then): the workgroups of blockIdx.y share the rows
-// and their channels, 64 at a time, the 16 groups of 16 threads the parts.
+// key-value head.  Up to kFewParts parts: a thread takes four channels of a row, eight parts
+// of it loaded at a time.  More: the workgroups of blockIdx.y share the rows and their
+// channels, 64 at a time, the 16 groups of 16 threads the parts.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attention_combine_few_kernel(Attention a) {
-  __shared__ int64_t scratch[8];
-  __shared__ Find found;
   __shared__ __attribute__((aligned(16))) float sums[16][64];
   __shared__ float ms[16], ls[16];
   const int kv = blockIdx.x % a.batch.kv_heads, s = blockIdx.x / a.batch.kv_heads;
   const int tid = threadIdx.x, group = tid / 16;
-  Find at;
-  const Spans sp = find_span<true>(a, s, scratch, &found, at);
-  if (at.s < 0) return;
-  const int first = sp.of(at.first), n = sp.of(at.first + few_blocks(a, s) - 1) - first + 1;
-  if (n < 2 || (n <= kFewParts && blockIdx.y > 0)) return;
-  const bool later = sp.start(first) != at.first;  // part 0 is not its span's first
+  const Parts parts = a.parts[blockIdx.x];
   const PagedSequence seq = paged_sequence(a.batch, s, a.tokens);
-  const int rows = seq.count * a.group;
+  if (!few_rows(seq, a.group) || parts.count < 2) return;
+  const int rows = seq.count * a.group, n = parts.count;
+  auto part = [&](int j, int c) {
+    return part_row(a, parts.span + j, j == 0 && parts.later, kv) + c;
+  };
   if (n <= kFewParts) {
-    for (int u = tid; u < rows * (D / 4); u += 256) {
+    for (int u = blockIdx.y * 256 + tid; u < rows * (D / 4); u += gridDim.y * 256) {
       const int c = u / (D / 4), d = u % (D / 4) * 4;
-      float2 ml[kFewParts];
-      f32x4 v[kFewParts];
-#pragma unroll
-      for (int j = 0; j < kFewParts; ++j) {
-        const int64_t row = part_row(a, first + min(j, n - 1), j == 0 && later, kv) + c;
-        ml[j] = *reinterpret_cast<const float2 *>(a.part_ml + row * 2);
-        v[j] = *reinterpret_cast<const f32x4 *>(a.part + row * D + d);
-      }
       PartSum sum;
+      for (int j0 = 0; j0 < n; j0 += 8) {
+        float2 ml[8];
+        f32x4 v[8];
 #pragma unroll
-      for (int j = 0; j < kFewParts; ++j)
-        if (j < n) sum.add(ml[j].x, ml[j].y, v[j]);
+        for (int j = 0; j < 8; ++j) {
+          const int64_t row = part(min(j0 + j, n - 1), c);
+          ml[j] = *reinterpret_cast<const float2 *>(a.part_ml + row * 2);
+          v[j] = *reinterpret_cast<const f32x4 *>(a.part + row * D + d);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j0 + j < n) sum.add(ml[j].x, ml[j].y, v[j]);
+      }
       write_row<T, D>(a, row_place(a, seq, kv, c), d, sum.o, sum.inverse());
     }
     return;
@@ -639,7 +655,7 @@ __global__ __launch_bounds__(256) void attention_combine_few_kernel(Attention a)
     PartSum sum;
 #pragma unroll 8
     for (int j = group; j < n; j += 16) {
-      const int64_t row = part_row(a, first + j, j == 0 && later, kv) + c;
+      const int64_t row = part(j, c);
       const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + row * 2);
       sum.add(ml.x, ml.y, *reinterpret_cast<const f32x4 *>(a.part + row * D + d));
     }
@@ -1006,24 +1022,39 @@ __global__ __launch_bounds__(TileForm<D>::kWaves * 64, 2) void attention_tile_ke
   }
 }
 
-// Rows of sequences in tiles, where their keys were split: D / 4 threads a row.
+// Rows of sequences in tiles, where their keys were split: D / 4 threads a row, `chunks`
+// workgroups a token.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void attention_combine_tile_kernel(Attention a) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = (int64_t)a.tokens * a.q_heads;
-  const int64_t row = i / (D / 4);
-  const int d = (int)(i % (D / 4)) * 4, t = (int)(row / a.q_heads);
-  if (row >= rows) return;
-  const int s = paged_find(a.batch, t);
-  if (s < 0) return;
+__global__ __launch_bounds__(256) void attention_combine_tile_kernel(Attention a, int chunks) {
+  const int t = blockIdx.x / chunks, lane = threadIdx.x & 63;
+  const int i = blockIdx.x % chunks * 256 + threadIdx.x;
+  const int head = i / (D / 4), d = i % (D / 4) * 4;
+  int s = -1;  // the token's sequence: a lane looks at one of 64
+  for (int c = 0; c < a.batch.sequences && s < 0; c += 64) {
+    const int k = c + lane;
+    const uint64_t hit = __ballot(k < a.batch.sequences && a.batch.starts[min(k, a.batch.sequences - 1)] <= t &&
+                                  t < a.batch.starts[min(k, a.batch.sequences - 1) + 1]);
+    if (hit) s = c + __builtin_ctzll(hit);
+  }
+  if (s < 0 || head >= a.q_heads) return;
   const PagedSequence seq = paged_sequence(a.batch, s, a.tokens);
   if (t < seq.first || t >= seq.first + seq.count || (a.few && few_rows(seq, a.group))) return;
+  const int64_t rows = (int64_t)a.tokens * a.q_heads, row = (int64_t)t * a.q_heads + head;
   PartSum sum;
-#pragma unroll 4
-  for (int j = 0; j < a.splits; ++j) {
-    const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + (row + j * rows) * 2);
-    sum.add(ml.x, ml.y, *reinterpret_cast<const f32x4 *>(a.part + (row + j * rows) * D + d));
+  for (int j0 = 0; j0 < a.splits; j0 += 4) {
+    float2 ml[4];
+    f32x4 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t r = row + min(j0 + j, a.splits - 1) * rows;
+      ml[j] = *reinterpret_cast<const float2 *>(a.part_ml + r * 2);
+      v[j] = *reinterpret_cast<const f32x4 *>(a.part + r * D + d);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j0 + j < a.splits) sum.add(ml[j].x, ml[j].y, v[j]);
   }
-  write_row<T, D>(a, {t, (int)(row % a.q_heads)}, d, sum.o, sum.inverse());
+  write_row<T, D>(a, {t, head}, d, sum.o, sum.inverse());
 }
 
 // ------------------------------------------------------------------ host side
@@ -1032,7 +1063,7 @@ struct AttentionPlan {
   bool few, tile;
   int64_t shares, few_grid;          // few: parts per key-value head, workgroups
   int64_t tiles, splits;             // tile: tiles at most, parts of each
-  int64_t few_rows, tile_rows;       // rows of partial sums
+  int64_t few_rows, tile_rows, parts;  // rows of partial sums, Parts
 };
 
 AttentionPlan attention_plan(int64_t tokens, int64_t sequences, int64_t q_heads, int64_t kv_heads,
@@ -1046,6 +1077,7 @@ AttentionPlan attention_plan(int64_t tokens, int64_t sequences, int64_t q_heads,
     p.shares = 512 / kv_heads > 1 ? 512 / kv_heads : 1;
     p.few_grid = p.shares * kv_heads;
     p.few_rows = 2 * p.shares * kv_heads * kFewRows;
+    p.parts = sequences * kv_heads;
   }
   if (p.tile) {
     const int64_t some = sequences < tokens ? sequences : tokens;
@@ -1059,7 +1091,7 @@ AttentionPlan attention_plan(int64_t tokens, int64_t sequences, int64_t q_heads,
 }
 
 int64_t attention_bytes(const AttentionPlan &p, int64_t head_dim) {
-  return (p.few_rows + p.tile_rows) * (head_dim + 2) * 4;
+  return (p.few_rows + p.tile_rows) * (head_dim + 2) * 4 + (p.parts * sizeof(Parts) + 15) / 16 * 16;
 }
 
 template <typename T, int D>
@@ -1068,11 +1100,12 @@ int launch_attention(const AttentionPlan &p, Attention a, float *workspace, hipS
   if (p.few) {
     a.shares = (int)p.shares;
     a.part = workspace, a.part_ml = workspace + p.few_rows * D;
+    a.parts = reinterpret_cast<Parts *>(workspace + (p.few_rows + p.tile_rows) * (D + 2));
     attention_few_kernel<T, D><<<(unsigned)p.few_grid, 256, 0, st>>>(a);
     if (const int rc = check_launch("attention_few_kernel")) return rc;
     // Where there are few sequences, their rows and channels fill the chip.
     const int64_t heads = (int64_t)a.batch.sequences * a.batch.kv_heads;
-    const int64_t units = kFewRows / a.group * a.group * (D / 64), some = 1024 / heads;
+    const int64_t units = kFewRows / a.group * a.group * (D / 64), some = 4096 / heads;
     const dim3 grid((unsigned)heads, (unsigned)(some < 1 ? 1 : some < units ? some : units));
     attention_combine_few_kernel<T, D><<<grid, 256, 0, st>>>(a);
     if (const int rc = check_launch("attention_combine_few_kernel")) return rc;
@@ -1084,8 +1117,8 @@ int launch_attention(const AttentionPlan &p, Attention a, float *workspace, hipS
     attention_tile_kernel<T, D><<<grid, TileForm<D>::kWaves * 64, 0, st>>>(a);
     if (const int rc = check_launch("attention_tile_kernel")) return rc;
     if (p.splits > 1) {
-      attention_combine_tile_kernel<T, D>
-          <<<cdiv((int64_t)a.tokens * a.q_heads * (D / 4), 256), 256, 0, st>>>(a);
+      const int chunks = (a.q_heads * (D / 4) + 255) / 256;
+      attention_combine_tile_kernel<T, D><<<a.tokens * chunks, 256, 0, st>>>(a, chunks);
       return check_launch("attention_combine_tile_kernel");
     }
   }
