@@ -188,15 +188,19 @@ __device__ __forceinline__ int opaque(int v) {
 }
 
 // Values of keys that some row does not see: a weight of 0 must not meet an infinity or
-// NaN (0 * inf).  The products take the finite values of a pair, 0 for others; where there
-// were any, the rows that do see such a key get it added afterwards.
+// NaN (0 * inf).  The products of such keys take the finite values, 0 for others, and where
+// there were others, the rows that do see the key get them added afterwards.
 template <typename T>
 struct Pair {
-  static constexpr uint32_t E = __is_same(T, BF16) ? 0x7F80u : 0x7C00u;  // infinity
-  static __device__ __forceinline__ uint32_t finite(uint32_t v, bool &odd) {
-    const bool lo = (v & E) == E, hi = (v & (E << 16)) == (E << 16);
-    odd |= lo || hi;
-    return (lo ? 0u : v & 0xFFFFu) | (hi ? 0u : v & 0xFFFF0000u);
+  static constexpr uint32_t E = __is_same(T, BF16) ? 0x7F80u : 0x7C00u;     // infinity
+  static constexpr uint32_t STEP = 0x8000u - E;  // carries it, and NaN, into the sign bit
+  static __device__ __forceinline__ uint32_t odd(uint32_t v) {  // sign bits set where odd
+    return (v & 0x7FFF7FFFu) + (STEP | STEP << 16);
+  }
+  static __device__ __forceinline__ uint32_t finite(uint32_t v, uint32_t &any) {
+    const uint32_t s = odd(v) & 0x80008000u;
+    any |= s;
+    return v & ~(s | (s - (s >> 15)));  // all bits of the halves where odd
   }
   static __device__ __forceinline__ float odd_part(uint32_t x) {
     return (x & E) == E ? T::to_f32(x) : 0.0f;
@@ -373,18 +377,20 @@ template <typename T, int D>
 __device__ __forceinline__ void few_values(const LDS char *vt, u32x2 p, bool mixed,
                                            FewState<D> &st, int lane) {
   const int base = opaque(transpose_base<D, kRows>((lane >> 4) * 4, 0, lane));
-  if (!mixed) {
+  if (mixed) {
+    uint32_t any = 0;
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i)
-      st.o[i] = mfma16k16(T{}, read_transposed<D, kRows>(vt, base, 0, i * 16), p, st.o[i]);
+    for (int i = 0; i < D / 16; ++i) {
+      const u32x2 v = read_transposed<D, kRows>(vt, base, 0, i * 16);
+      st.o[i] = mfma16k16(T{}, u32x2{Pair<T>::finite(v[0], any), Pair<T>::finite(v[1], any)}, p,
+                          st.o[i]);
+    }
+    st.odd |= __any(any != 0);
     return;
   }
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i) {
-    const u32x2 v = read_transposed<D, kRows>(vt, base, 0, i * 16);
-    st.o[i] = mfma16k16(T{}, u32x2{Pair<T>::finite(v[0], st.odd), Pair<T>::finite(v[1], st.odd)},
-                        p, st.o[i]);
-  }
+  for (int i = 0; i < D / 16; ++i)
+    st.o[i] = mfma16k16(T{}, read_transposed<D, kRows>(vt, base, 0, i * 16), p, st.o[i]);
 }
 
 // The keys of a wave: steps of 16 keys, `stride` steps apart, and the pages they lie in.
@@ -437,36 +443,36 @@ __device__ __forceinline__ void few_step(LDS char *ring, const FewKeys &f, const
 // Row c of a sequence's rows at a key-value head: new token c / group, query head
 // kv * group + c % group.
 struct RowPlace {
-  int64_t token;
-  int head;
+  int token, head;
 };
 __device__ __forceinline__ RowPlace row_place(const Attention &a, const PagedSequence &q, int kv,
                                               int c) {
   return {q.first + c / a.group, kv * a.group + c % a.group};
 }
 
-// sigmoid(x) by the hardware's exp2 and reciprocal; the argument's rounding, which far from
-// 0 would show in the result, is put back.
+// sigmoid(x) by the hardware's exp2 and reciprocal: (|x| + 4) 2^-24 of it at most, as the
+// exponent's rounding shows in a small result.
 __device__ __forceinline__ float sigmoid_hw(float x) {
-  constexpr float kHi = 1.4426950408889634f, kLo = 1.9259629911266175e-8f;  // log2(e)
-  const float t = -x * kHi, e = __builtin_fmaf(-x, kHi, -t) - x * kLo;
-  const float p = exp2_hw(t);
-  return __builtin_amdgcn_rcpf(1.0f + (t < 126.0f ? __builtin_fmaf(p, e * 0.6931472f, p) : p));
+  return __builtin_amdgcn_rcpf(1.0f + exp2_hw(x * -1.4426950408889634f));
 }
 
-// Four channels from d of a finished row: scaled, gated, rounded once.
+// Four channels from d of a row's gate, if there is one.
+__device__ __forceinline__ uint2 load_gate(const Attention &a, RowPlace at, int d) {
+  if (!a.gate) return uint2{0, 0};
+  return ldg_u2(a.gate + (int64_t)at.token * a.gate_token + (int64_t)at.head * a.gate_head + d);
+}
+
+// Four channels from d of a finished row: gated, rounded once.
 template <typename T, int D>
 __device__ __forceinline__ void write_row(const Attention &a, RowPlace at, int d, f32x4 o,
-                                          float inv) {
-  o *= inv;
+                                          uint2 g) {
   if (a.gate) {
-    const uint2 g = ldg_u2(a.gate + at.token * a.gate_token + at.head * a.gate_head + d);
     o[0] *= sigmoid_hw(T::to_f32(g.x & 0xFFFFu));
     o[1] *= sigmoid_hw(T::to_f32(g.x >> 16));
     o[2] *= sigmoid_hw(T::to_f32(g.y & 0xFFFFu));
     o[3] *= sigmoid_hw(T::to_f32(g.y >> 16));
   }
-  *reinterpret_cast<uint2 *>(a.out + (at.token * a.q_heads + at.head) * D + d) =
+  *reinterpret_cast<uint2 *>(a.out + ((int64_t)at.token * a.q_heads + at.head) * D + d) =
       uint2{T::pack2(o[0], o[1]), T::pack2(o[2], o[3])};
 }
 
@@ -487,7 +493,7 @@ __device__ __forceinline__ void few_part(const Attention &a, int s, int kv, int 
   const int col = min(lane & 15, rows - 1), g = lane >> 4;
   const RowPlace at = row_place(a, seq, kv, col);
   u32x4 q[D / 32];
-  const uint16_t *qr = a.q + at.token * a.q_token + at.head * a.q_head;
+  const uint16_t *qr = a.q + (int64_t)at.token * a.q_token + (int64_t)at.head * a.q_head;
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) q[i] = ldg16(qr + i * 32 + g * 8) ^ a.flip;
 
@@ -521,7 +527,7 @@ __device__ __forceinline__ void few_part(const Attention &a, int s, int kv, int 
       few_step<T, D>(ring, f, q, i, limit, all_see, a.scale2, st, lane);
     }
     wait_loads<0>();  // the last refills, before the ring is used otherwise
-    if (__builtin_expect(__any(st.odd), 0)) {
+    if (__builtin_expect(st.odd, 0)) {
       for (int i = 0; i < f.steps; ++i) {
         const int key = (f.first + i * f.stride) * 16;
         if (key + 16 <= all_see) continue;
@@ -561,7 +567,8 @@ __device__ __forceinline__ void few_part(const Attention &a, int s, int kv, int 
       o += *reinterpret_cast<const f32x4 *>(sums + (w * kFewRows + c) * (D + 4) + d) * k;
     }
     if (part < 0) {
-      write_row<T, D>(a, row_place(a, seq, kv, c), d, o, l > 0.0f || l != l ? 1.0f / l : 0.0f);
+      const RowPlace to = row_place(a, seq, kv, c);
+      write_row<T, D>(a, to, d, o * (l > 0.0f || l != l ? 1.0f / l : 0.0f), load_gate(a, to, d));
     } else {
       *reinterpret_cast<f32x4 *>(a.part + (part + c) * D + d) = o;
       if (d == 0) *reinterpret_cast<float2 *>(a.part_ml + (part + c) * 2) = float2{m, l};
@@ -632,6 +639,8 @@ __global__ __launch_bounds__(256) void attention_combine_few_kernel(Attention a)
   if (n <= kFewParts) {
     for (int u = blockIdx.y * 256 + tid; u < rows * (D / 4); u += gridDim.y * 256) {
       const int c = u / (D / 4), d = u % (D / 4) * 4;
+      const RowPlace to = row_place(a, seq, kv, c);
+      const uint2 gate = load_gate(a, to, d);
       PartSum sum;
       for (int j0 = 0; j0 < n; j0 += 8) {
         float2 ml[8];
@@ -646,12 +655,14 @@ __global__ __launch_bounds__(256) void attention_combine_few_kernel(Attention a)
         for (int j = 0; j < 8; ++j)
           if (j0 + j < n) sum.add(ml[j].x, ml[j].y, v[j]);
       }
-      write_row<T, D>(a, row_place(a, seq, kv, c), d, sum.o, sum.inverse());
+      write_row<T, D>(a, to, d, sum.o * sum.inverse(), gate);
     }
     return;
   }
   for (int u = blockIdx.y; u < rows * (D / 64); u += gridDim.y) {
     const int c = u / (D / 64), d = u % (D / 64) * 64 + tid % 16 * 4;
+    const RowPlace to = row_place(a, seq, kv, c);
+    const uint2 gate = load_gate(a, to, d);
     PartSum sum;
 #pragma unroll 8
     for (int j = group; j < n; j += 16) {
@@ -666,7 +677,7 @@ __global__ __launch_bounds__(256) void attention_combine_few_kernel(Attention a)
 #pragma unroll
       for (int w = 1; w < 16; ++w)
         sum.add(ms[w], ls[w], *reinterpret_cast<const f32x4 *>(&sums[w][tid * 4]));
-      write_row<T, D>(a, row_place(a, seq, kv, c), d, sum.o, sum.inverse());
+      write_row<T, D>(a, to, d, sum.o * sum.inverse(), gate);
     }
     __syncthreads();
   }
@@ -785,26 +796,30 @@ template <typename T, int D, bool MIXED>
 __device__ __forceinline__ void tile_values(const LDS char *vt, const u32x4 (&p)[2],
                                             TileState<D> &st, int lane) {
   const int base = opaque(transpose_base<D, kQuads>((lane >> 5) * 4, ((lane >> 4) & 1) * 16, lane));
-  if constexpr (!MIXED) {
+  if constexpr (MIXED) {
+    uint32_t any = 0;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
-        st.o[i] = mfma32(T{}, tile_operand<D>(vt, base, i, ks * 16), p[ks], st.o[i]);
+      for (int ks = 0; ks < 2; ++ks) {
+        u32x4 v = tile_operand<D>(vt, base, i, ks * 16);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = Pair<T>::finite(v[j], any);
+        st.o[i] = mfma32(T{}, v, p[ks], st.o[i]);
+      }
+    st.odd |= __any(any != 0);
     return;
   }
+  __builtin_amdgcn_s_setprio(1);
 #pragma unroll
   for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      u32x4 v = tile_operand<D>(vt, base, i, ks * 16);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = Pair<T>::finite(v[j], st.odd);
-      st.o[i] = mfma32(T{}, v, p[ks], st.o[i]);
-    }
+    for (int ks = 0; ks < 2; ++ks)
+      st.o[i] = mfma32(T{}, tile_operand<D>(vt, base, i, ks * 16), p[ks], st.o[i]);
+  __builtin_amdgcn_s_setprio(0);
 }
 
-// 32 keys of a tile for a wave's 32 rows.  MIXED: some row does not see all of the keys.
+// 32 keys of a tile for a wave's 32 rows.  MIXED: some row does not see all of them.
 // The wave's priority is raised while it feeds the matrix cores, so that the other wave of
 // its SIMD does its softmax beside them.
 template <typename T, int D, bool MIXED>
@@ -846,74 +861,18 @@ __device__ __forceinline__ void tile_step(const LDS char *kt, const LDS char *vt
     st.l += e0 + e1;
     p[i / 4][i % 4] = T::pack2(e0, e1);
   }
-  __builtin_amdgcn_s_setprio(1);
   tile_values<T, D, MIXED>(vt, p, st, lane);
-  __builtin_amdgcn_s_setprio(0);
 }
 
-// One half of a wave's rows' channels, or all (HALF < 0), to the output or the parts.
-template <typename T, int D, int HALF>
-__device__ __forceinline__ void tile_write(const Attention &a, RowPlace at, int split, float l,
-                                           const TileState<D> &st, int lane) {
-  constexpr int FROM = HALF == 1 ? D / 64 : 0, TO = HALF == 0 ? D / 64 : D / 32;
-  const int h = lane >> 5;
-  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-  const int64_t row = ((int64_t)split * a.tokens + at.token) * a.q_heads + at.head;
-#pragma unroll
-  for (int i = FROM; i < TO; ++i)
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const int d = i * 32 + b * 8 + h * 4;
-      const f32x4 o = {st.o[i][4 * b], st.o[i][4 * b + 1], st.o[i][4 * b + 2], st.o[i][4 * b + 3]};
-      if (a.splits == 1)
-        write_row<T, D>(a, at, d, o, inv);
-      else
-        *reinterpret_cast<f32x4 *>(a.part + row * D + d) = o;
-    }
-  if (a.splits > 1 && h == 0 && HALF < 1)
-    *reinterpret_cast<float2 *>(a.part_ml + row * 2) = float2{st.m, l};
-}
-
-// Hands the other key group of the same rows half of the channels and takes its share of
-// this wave's own half: `room` is the wave's place in LDS, `other` the other wave's.
-template <int D, int HALF>
-__device__ __forceinline__ void tile_give(const TileState<D> &st, float l, LDS f32x4 *room, int lane) {
-  constexpr int FROM = HALF == 0 ? D / 64 : 0;
-#pragma unroll
-  for (int i = 0; i < D / 64; ++i)
-#pragma unroll
-    for (int b = 0; b < 4; ++b)
-      room[(i * 4 + b) * 64 + lane] =
-          f32x4{st.o[FROM + i][4 * b], st.o[FROM + i][4 * b + 1], st.o[FROM + i][4 * b + 2],
-                st.o[FROM + i][4 * b + 3]};
-  ((LDS float *)(room + D / 16 * 64))[lane] = st.m;
-  ((LDS float *)(room + D / 16 * 64))[64 + lane] = l;
-}
-template <int D, int HALF>
-__device__ __forceinline__ void tile_take(TileState<D> &st, float &l, const LDS f32x4 *other,
-                                          int lane) {
-  constexpr int FROM = HALF == 1 ? D / 64 : 0;
-  const float om = ((const LDS float *)(other + D / 16 * 64))[lane];
-  const float ol = ((const LDS float *)(other + D / 16 * 64))[64 + lane];
-  const float m = fmaxf(st.m, om), mine = decay(st.m, m), theirs = decay(om, m);
-  l = l * mine + ol * theirs;
-  st.m = m;
-#pragma unroll
-  for (int i = 0; i < D / 64; ++i)
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const f32x4 o = other[(i * 4 + b) * 64 + lane];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        st.o[FROM + i][4 * b + j] = st.o[FROM + i][4 * b + j] * mine + o[j] * theirs;
-    }
-}
-
+// The waves' sums on their way out, half of the channels at a time: rows of D / 2 channels
+// and a pad of four, then each row's maximum and sum.
+template <int D>
+constexpr int tile_pitch() { return D / 2 + 4; }
 template <int D>
 constexpr int tile_lds() {
   using F = TileForm<D>;
-  constexpr int ring = 4 * F::kKeys * D * 2, join = F::kWaves * (D / 16 * 64 * 16 + 512);
-  return F::kGroups > 1 && join > ring ? join : ring;
+  constexpr int ring = 4 * F::kKeys * D * 2, out = F::kWaves * 32 * (tile_pitch<D>() + 2) * 4;
+  return out > ring ? out : ring;
 }
 
 template <typename T, int D>
@@ -947,11 +906,7 @@ __global__ __launch_bounds__(TileForm<D>::kWaves * 64, 2) void attention_tile_ke
   const int key1 = min((int)((int64_t)tiles * (split + 1) / a.splits) * KEYS, keys);
 
   u32x4 q[D / 16];
-  const uint16_t *qr = a.q + at.token * a.q_token + at.head * a.q_head + (lane >> 5) * 8;
-#pragma unroll
-  for (int i = 0; i < D / 16; ++i) q[i] = ldg16(qr + i * 16) ^ a.flip;
-#pragma unroll
-  for (int i = 0; i < D / 16; ++i) settle(q[i]);
+  const uint16_t *qr = a.q + (int64_t)at.token * a.q_token + (int64_t)at.head * a.q_head + (lane >> 5) * 8;
   TileState<D> st;
   LDS char *base = (LDS char *)lds;
   const int64_t head = (int64_t)(kv << a.batch.page_shift) * D;
@@ -962,6 +917,10 @@ __global__ __launch_bounds__(TileForm<D>::kWaves * 64, 2) void attention_tile_ke
     f.pages = a.batch.pages, f.entries = a.batch.table_pages;
     tile_pages(f, key0, lane);
     tile_load<D, ROWS>(f, key0, base, base + TILE, wave, lane);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) q[i] = ldg16(qr + i * 16) ^ a.flip;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) settle(q[i]);
     wait_loads<0>();
     __syncthreads();
     // A tile, the next one's loads started before it into the other half.
@@ -976,7 +935,6 @@ __global__ __launch_bounds__(TileForm<D>::kWaves * 64, 2) void attention_tile_ke
       wait_loads<0>();
       __syncthreads();
     }
-    const int mixed = key;
     for (; key < key1; key += KEYS, half ^= 1) {
       LDS char *cur = base + half * 2 * TILE, *next = base + (half ^ 1) * 2 * TILE;
       if (key + KEYS < key1) tile_load<D, ROWS>(f, key + KEYS, next, next + TILE, wave, lane);
@@ -986,9 +944,9 @@ __global__ __launch_bounds__(TileForm<D>::kWaves * 64, 2) void attention_tile_ke
       wait_loads<0>();
       __syncthreads();
     }
-    if (__builtin_expect(__any(st.odd), 0)) {
-      for (int k = mixed; k < min(key1, limit); ++k) {
-        if (((k - mixed) / 32) % GROUPS != group) continue;
+    if (__builtin_expect(st.odd, 0)) {
+      for (int k = key0 + max(all_see - key0, 0) / KEYS * KEYS; k < min(key1, limit); ++k) {
+        if (((k - key0) / 32) % GROUPS != group) continue;
         const uint16_t *v = value_row<D>(a, s, head, k) + (lane >> 5) * 4;
 #pragma unroll
         for (int i = 0; i < D / 32; ++i)
@@ -1001,23 +959,88 @@ __global__ __launch_bounds__(TileForm<D>::kWaves * 64, 2) void attention_tile_ke
       }
     }
   }
-  float l = across32(st.l, Add());
-  if constexpr (GROUPS == 1) {
-    if (c < rows) tile_write<T, D, -1>(a, at, split, l, st, lane);
-  } else {  // every wave has left the ring: the last barrier above, or no key at all
-    LDS f32x4 *room = (LDS f32x4 *)base;
-    constexpr int STEP = D / 16 * 64 + 32;
-    if (group == 0)
-      tile_give<D, 0>(st, l, room + wave * STEP, lane);
-    else
-      tile_give<D, 1>(st, l, room + wave * STEP, lane);
-    __syncthreads();
-    if (group == 0) {
-      tile_take<D, 0>(st, l, room + (wave + 4) * STEP, lane);
-      if (c < rows) tile_write<T, D, 0>(a, at, split, l, st, lane);
+
+  // Through LDS, which every wave has left: the last barrier above, or no key at all.  The
+  // key groups' sums are joined on the way, and rows are written whole.
+  constexpr int PITCH = tile_pitch<D>(), C = D / 2;
+  float *sums = reinterpret_cast<float *>(lds), *ml = sums + WAVES * 32 * PITCH;
+  const float l = across32(st.l, Add());
+  if (lane < 32) {
+    ml[(wave * 32 + lane) * 2] = st.m;
+    ml[(wave * 32 + lane) * 2 + 1] = l;
+  }
+  __syncthreads();
+  if (threadIdx.x < kTileRows) {  // what each group's sum of a row counts for
+    PartSum sum;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+      const float *p = ml + (g * kTileRows + threadIdx.x) * 2;
+      sum.add(p[0], p[1], f32x4{});
+    }
+    const float inv = a.splits == 1 ? sum.inverse() : 1.0f;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+      float *p = ml + (g * kTileRows + threadIdx.x) * 2;
+      p[0] = decay(p[0], sum.m) * inv;
+    }
+    if (a.splits > 1 && c0 + threadIdx.x < rows) {
+      const RowPlace to = row_place(a, seq, kv, c0 + threadIdx.x);
+      const int64_t row = ((int64_t)split * a.tokens + to.token) * a.q_heads + to.head;
+      *reinterpret_cast<float2 *>(a.part_ml + row * 2) = float2{sum.m, sum.l};
+    }
+  }
+  // A thread's units of four channels lie STEP rows apart; four at a time, their gates first.
+  // Little code, as it runs once: unrolled, it took longer to fetch than to run.
+  constexpr int STEP = WAVES * 64 / (C / 4), BATCH = 4;
+  const int first = threadIdx.x / (C / 4), d = threadIdx.x % (C / 4) * 4;
+  const int live = min(rows - c0, kTileRows), step_t = STEP / a.group, step_h = STEP % a.group;
+  const int t0 = (c0 + first) / a.group, h0 = (c0 + first) % a.group;
+  auto put = [&](const f32x16 &o, int i) {
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+      *reinterpret_cast<f32x4 *>(sums + (wave * 32 + (lane & 31)) * PITCH + i * 32 + b * 8 +
+                                 (lane >> 5) * 4) =
+          f32x4{o[4 * b], o[4 * b + 1], o[4 * b + 2], o[4 * b + 3]};
+  };
+#pragma unroll 1
+  for (int side = 0; side < 2; ++side) {
+    if (side == 0) {
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) put(st.o[i], i);
     } else {
-      tile_take<D, 1>(st, l, room + (wave - 4) * STEP, lane);
-      if (c < rows) tile_write<T, D, 1>(a, at, split, l, st, lane);
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) put(st.o[D / 64 + i], i);
+    }
+    __syncthreads();
+    int t = t0, h = h0;
+#pragma unroll 1
+    for (int r0 = first; r0 < live; r0 += BATCH * STEP) {
+      uint2 gate[BATCH];
+      RowPlace to[BATCH];
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        to[i] = {seq.first + min(t, seq.count - 1), kv * a.group + h};
+        if (a.splits == 1) gate[i] = load_gate(a, to[i], side * C + d);
+        t += step_t, h += step_h;
+        if (h >= a.group) h -= a.group, ++t;
+      }
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const int r = r0 + i * STEP;
+        if (r >= live) break;
+        f32x4 o = *reinterpret_cast<const f32x4 *>(sums + r * PITCH + d) * ml[r * 2];
+        if constexpr (GROUPS == 2) {
+          const int w = kTileRows + r;
+          o += *reinterpret_cast<const f32x4 *>(sums + w * PITCH + d) * ml[w * 2];
+        }
+        if (a.splits == 1) {
+          write_row<T, D>(a, to[i], side * C + d, o, gate[i]);
+        } else {
+          const int64_t row = ((int64_t)split * a.tokens + to[i].token) * a.q_heads + to[i].head;
+          *reinterpret_cast<f32x4 *>(a.part + row * D + side * C + d) = o;
+        }
+      }
     }
   }
 }
@@ -1040,6 +1063,7 @@ __global__ __launch_bounds__(256) void attention_combine_tile_kernel(Attention a
   const PagedSequence seq = paged_sequence(a.batch, s, a.tokens);
   if (t < seq.first || t >= seq.first + seq.count || (a.few && few_rows(seq, a.group))) return;
   const int64_t rows = (int64_t)a.tokens * a.q_heads, row = (int64_t)t * a.q_heads + head;
+  const uint2 gate = load_gate(a, {t, head}, d);
   PartSum sum;
   for (int j0 = 0; j0 < a.splits; j0 += 4) {
     float2 ml[4];
@@ -1054,7 +1078,7 @@ __global__ __launch_bounds__(256) void attention_combine_tile_kernel(Attention a
     for (int j = 0; j < 4; ++j)
       if (j0 + j < a.splits) sum.add(ml[j].x, ml[j].y, v[j]);
   }
-  write_row<T, D>(a, {t, head}, d, sum.o, sum.inverse());
+  write_row<T, D>(a, {t, head}, d, sum.o * sum.inverse(), gate);
 }
 
 // ------------------------------------------------------------------ host side

@@ -93,8 +93,10 @@ def attention(q, k_pages, v_pages, starts, lengths, table, scale=None, gate=None
                     lost = lost + 2.0 ** -25 * v[:seen].abs().sum(0)
                 out[t, h * g:(h + 1) * g], tol[t, h * g:(h + 1) * g] = o, lost
     if gate is not None:
-        s = torch.sigmoid(gate.double())
-        out, tol = out * s, tol * s + out.nan_to_num().abs() * s * 2.0 ** -21
+        # the exponent -x log2(e) is off by half a step of its size, |x| 2^-24 of e^-x; exp2, the
+        # sum, the reciprocal (a step each) and the product add 4 steps of 2^-24 (of 1 ulp: 2^-23)
+        s, x = torch.sigmoid(gate.double()), gate.double().abs()
+        out, tol = out * s, tol * s + out.nan_to_num().abs() * s * (2 * x + 8) * 2.0 ** -24
     return out, tol
 
 
