@@ -93,7 +93,13 @@ __global__ __launch_bounds__(256) void head_rows_kernel(HeadRows a) {
       if (first <= t && t < end) found = s, at = n - (end - first) + (t - first);
     }
     __syncthreads();
-    if (found < 0) return;  // a row of no sequence
+    if (found < 0) {  // a row of no sequence
+      for (int r = r0; r < a.q_heads; r += ROWS) {
+        uint16_t *dst = a.q_out + ((int64_t)t * a.q_heads + r) * D;
+        *reinterpret_cast<uint2 *>(dst + lo) = *reinterpret_cast<uint2 *>(dst + hi) = uint2{0, 0};
+      }
+      return;
+    }
     const int p = at;
     position = p;
     if (tid == 255) {

@@ -12,7 +12,8 @@ step and may rewrite between replays of a captured step:
   starts  [sequences + 1]  the rows of sequence s are starts[s] .. starts[s + 1] - 1
   lengths [sequences]      its positions, the new ones (its last) among them
   table   [sequences, n]   the page of its positions i * page_size ..
-Rows of no sequence (padding behind the last) are left as they were.
+Rows of no sequence (padding behind the last) touch neither the cache nor an output
+that the caller gave.
 
 The reference has no operators of this kind (its layers run the Transformers
 modules, HF:627-735).
@@ -137,7 +138,7 @@ def append(k_pages, v_pages, k, v, starts, lengths, table, inv_freq=None, k_weig
     """Appends k and v [T, kv_heads, D] to the cache, k normed and rotated on the way
     (k_weight and inv_freq as in qk_norm_rope, by its position in its sequence).
     With q [T, q_heads, D], returns the queries normed and rotated for
-    paged_attention; rows of no sequence are not written there."""
+    paged_attention, 0 in rows of no sequence."""
     k, k_token, k_head = _rows(k, 'keys')
     v, v_token, v_head = _rows(v, 'values')
     dtype, device, shape = k.dtype, k.get_device(), k.shape
@@ -177,8 +178,8 @@ def paged_attention(q, k_pages, v_pages, starts, lengths, table, scale=None, gat
     The token at position p of its sequence sees the positions up to p.  scale
     defaults to D ** -0.5; gate [T, q_heads, D] multiplies the result by sigmoid(gate).
     max_new bounds the new tokens of one sequence (default: T); a close bound saves
-    time.  out [T, q_heads, D], contiguous, receives the result; rows of no sequence
-    keep what they hold there."""
+    time.  out [T, q_heads, D], contiguous, receives the result, and rows of no sequence
+    keep what they hold there; without it they are 0."""
     q, q_token, q_head = _rows(q, 'queries')
     dtype, device, shape = q.dtype, q.get_device(), q.shape
     pages, stride, heads, size, dim = _cache(k_pages, v_pages, dtype, device)
@@ -193,7 +194,7 @@ def paged_attention(q, k_pages, v_pages, starts, lengths, table, scale=None, gat
             raise ValueError('gate does not match the queries')
         gate_args = (gate.data_ptr(), gate_token, gate_head)
     if out is None:
-        out = q.new_empty(shape)
+        out = q.new_zeros(shape)
     else:
         _same(out, dtype, device)
         if out.shape != shape or not out.is_contiguous() or out.data_ptr() % 16:

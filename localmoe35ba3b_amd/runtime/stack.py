@@ -28,6 +28,7 @@ import torch
 
 from .. import _lib
 from ..convert import quantize_g128
+from .attention import Batch
 
 HIDDEN, INTER, EXPERTS, TOP_K = 2048, 512, 256, 8
 EPS = 1e-6
@@ -86,6 +87,7 @@ class MoEStack:
         self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         _lib.call('lm_moe_workspace_init', self.workspace.data_ptr(), nbytes, _lib.stream(dev))
         self._structs = [self._layer_struct(l) for l in range(layers)]
+        self.attention = {}  # layer -> AttentionBlock that runs before its MoE block
         self._side = self._side_ws = None  # second stream and workspace of prefill_
         self.gu_q_tiles = self.dn_q_tiles = None  # see build_prefill_tiles
         self._tiles_of = None  # versions of gu_q / dn_q the tile copies were built from
@@ -253,24 +255,37 @@ class MoEStack:
                       _lib.ptr(ids_out), _lib.ptr(weights_out), None, _lib.stream(h.device))
         return h
 
-    def forward(self, h, layers=None, workspace=None, chain=True):
+    def forward(self, h, layers=None, workspace=None, chain=True, batch=None):
         """All (or the first `layers`) layers over h in place, one workspace;
         with chain, each layer's combine prepares the next layer's normalized
-        rows (layer_forward's next_layer / input_normed)."""
+        rows (layer_forward's next_layer / input_normed).  Layers with an
+        attention block run it first, on the sequences of `batch`
+        (runtime.attention.Batch)."""
         n = self.L if layers is None else layers
+        self._check_batch(batch, n)
         for l in range(n):
-            self.layer_forward(h, l, workspace=workspace,
-                               next_layer=l + 1 if chain and l + 1 < n else None,
-                               input_normed=chain and l > 0)
+            if l in self.attention:
+                self.attention[l].forward_(h, batch)
+            self.layer_forward(h, l, workspace=workspace, **self._chained(l, n, chain))
         return h
 
-    def prefill(self, x, chunk=2048, overlap=True):
+    def _check_batch(self, batch, layers):
+        if batch is None and any(l < layers for l in self.attention):
+            raise ValueError('layers with attention need the batch of their sequences')
+
+    def _chained(self, l, n, chain):
+        """layer_forward's chain arguments: attention between two layers changes the rows that
+        the first one's combine would have normed."""
+        return dict(next_layer=l + 1 if chain and l + 1 < n and l + 1 not in self.attention
+                    else None, input_normed=chain and l > 0 and l not in self.attention)
+
+    def prefill(self, x, chunk=2048, overlap=True, batch=None):
         """Runs all layers over x [T, H] in chunks of `chunk` tokens; returns h."""
         out = x.clone()
-        self.prefill_(out, chunk, overlap)
+        self.prefill_(out, chunk, overlap, batch)
         return out
 
-    def prefill_(self, h, chunk=2048, overlap=True):
+    def prefill_(self, h, chunk=2048, overlap=True, batch=None):
         """In-place chunked prefill of h [T, H], as the reference's chunked
         profile runs the model over consecutive `chunk`-token slices of the
         prompt (generation.py:39-42).
@@ -284,6 +299,11 @@ class MoEStack:
         other's grouped GEMMs.  Every chunk computes exactly what it computes
         alone, so the result is bit-identical to overlap=False.  The schedule
         is stream-ordered and HIP-graph capturable.
+
+        Layers with an attention block need `batch` (runtime.attention.Batch) of
+        one sequence, whose lengths count the whole prompt: chunk c sees the
+        positions before it and, at layer l, waits for chunk c-1's keys and
+        values of that layer.
         """
         if h.dtype != torch.bfloat16 or not h.is_contiguous() or h.dim() != 2 or h.shape[-1] != self.H:
             raise ValueError('expected contiguous bf16 [tokens, 2048] hidden states')
@@ -291,12 +311,15 @@ class MoEStack:
             raise ValueError('chunk must be positive')
         if min(chunk, h.shape[0]) > self.max_tokens:  # before anything is queued
             raise MemoryError('token count exceeds the workspace of this stack')
+        self._check_batch(batch, self.L)
         starts = list(range(0, h.shape[0], chunk))
         if not starts:  # no tokens: nothing to queue, no second workspace
             return h
+        batches = self._chunk_batches(batch, h.shape[0], chunk) if self.attention else [None] * len(
+            starts)
         if not overlap or len(starts) == 1:
-            for c0 in starts:
-                self.forward(h[c0:c0 + chunk])
+            for c0, part in zip(starts, batches):
+                self.forward(h[c0:c0 + chunk], batch=part)
             return h
         if self._side is None:
             if torch.cuda.is_current_stream_capturing():
@@ -308,6 +331,7 @@ class MoEStack:
         streams, spaces = (cur, self._side), (self.workspace, self._side_ws)
         self._side.wait_stream(cur)
         done = [[torch.cuda.Event() for _ in range(self.L)] for _ in starts]
+        kept = [{l: torch.cuda.Event() for l in self.attention} for _ in starts]
         # chained layers need a workspace per chunk (two chunks, two workspaces)
         chain = len(starts) == 2
         for l in range(self.L):
@@ -316,13 +340,28 @@ class MoEStack:
                 with torch.cuda.stream(st):
                     if c and l:
                         st.wait_event(done[c - 1][l - 1])
-                    self.layer_forward(h[c0:c0 + chunk], l, workspace=spaces[c % 2],
-                                       next_layer=l + 1 if chain and l + 1 < self.L else None,
-                                       input_normed=chain and l > 0, beside=chunk)
+                    if l in self.attention:
+                        if c:
+                            st.wait_event(kept[c - 1][l])
+                        self.attention[l].forward_(h[c0:c0 + chunk], batches[c])
+                        kept[c][l].record(st)
+                    self.layer_forward(h[c0:c0 + chunk], l, workspace=spaces[c % 2], beside=chunk,
+                                       **self._chained(l, self.L, chain))
                     done[c][l].record(st)
         cur.wait_stream(self._side)
-        self._done_events = done  # kept alive until the next call
+        self._done_events = done, kept, batches  # kept alive until the next call
         return h
+
+    def _chunk_batches(self, batch, tokens, chunk):
+        """The batch of each chunk of one sequence's prompt, made on the GPU."""
+        if batch.lengths.numel() != 1:
+            raise ValueError('chunked prefill takes the batch of one sequence')
+        out = []
+        for c0 in range(0, tokens, chunk):
+            n = min(chunk, tokens - c0)
+            starts = torch.arange(2, dtype=torch.int32, device=self.device) * n
+            out.append(Batch(starts, batch.lengths - (tokens - c0 - n), batch.table, n))
+        return out
 
     # ------------------------------------------------------------------ oracle views
     def layer_host(self, l, experts=None):

@@ -113,6 +113,7 @@ def test_append(dev, lens, page, q_heads, heads, dim, pairs, dtype):
         assert got is None
     else:
         U.assert_rows(got[:live], *U.norm_rope(q[:live], qw, positions, freq), dtype, 'queries')
+        assert not got[live:].any()
 
 
 def test_append_outside_the_table_is_not_written(dev):
