@@ -65,7 +65,7 @@ class AttentionBlock:
         tokens, dim = h.shape[0], self.head_dim
         x = int8.linear(router.rmsnorm(h, self.norm, self.eps), self.qkv['q'], self.qkv['scale'])
         q, k, v = x.split([self.q_width, self.kv_width, self.kv_width], dim=1)
-        q, gate = q.view(tokens, self.q_heads, -1), None
+        q, gate = q.view(tokens, self.q_heads, self.q_width // self.q_heads), None
         if self.gated:
             q, gate = q[..., :dim], q[..., dim:]
         k, v = (t.view(tokens, self.kv_heads, dim) for t in (k, v))
@@ -74,5 +74,5 @@ class AttentionBlock:
                              k_weight=self.k_norm, q=q, q_weight=self.q_norm, eps=self.eps)
         o = attention.paged_attention(q, self.k_pages, self.v_pages, *place, gate=gate,
                                       max_new=batch.max_new)
-        h += int8.linear(o.view(tokens, -1), self.o['q'], self.o['scale'])
+        h += int8.linear(o.view(tokens, self.q_heads * dim), self.o['q'], self.o['scale'])
         return h

@@ -353,14 +353,15 @@ class MoEStack:
         return h
 
     def _chunk_batches(self, batch, tokens, chunk):
-        """The batch of each chunk of one sequence's prompt, made on the GPU."""
+        """The batch of each chunk of one sequence's prompt, made on the GPU: the sequence's rows
+        within the chunk (none of rows before it or behind it) and its positions up to them."""
         if batch.lengths.numel() != 1:
             raise ValueError('chunked prefill takes the batch of one sequence')
         out = []
         for c0 in range(0, tokens, chunk):
             n = min(chunk, tokens - c0)
-            starts = torch.arange(2, dtype=torch.int32, device=self.device) * n
-            out.append(Batch(starts, batch.lengths - (tokens - c0 - n), batch.table, n))
+            later = (batch.starts[1:] - (c0 + n)).clamp(min=0)
+            out.append(Batch((batch.starts - c0).clamp(0, n), batch.lengths - later, batch.table, n))
         return out
 
     # ------------------------------------------------------------------ oracle views

@@ -171,3 +171,33 @@ def test_stack_refusals(dev, stack):
         block(dev, 1).forward_(x, two)
     with pytest.raises(ValueError, match='heads'):
         AttentionBlock(stack.attention[0].qkv, stack.attention[0].o, 8, 2, 256)
+
+
+@pytest.mark.parametrize('tokens,chunk,first,end', [(100, 64, 0, 90), (100, 32, 5, 60), (90, 64, 70, 71)])
+def test_stack_chunked_prefill_of_padded_rows(dev, stack, tokens, chunk, first, end):
+    """Rows before and behind the sequence, whole chunks of them too, are none of its positions:
+    bit for bit the chunks with batches written out by hand."""
+    n = end - first
+    table = ints(dev, [5, 0, 2, 7, 1, 4, 6])
+    x = prompt(dev, tokens, tokens)
+    past = prompt(dev, 3, 7)  # positions 0 .. 2
+    stack.forward(past, batch=Batch(ints(dev, 0, 3), ints(dev, 3), table, 3))
+    want = x.clone()
+    for c0 in range(0, tokens, chunk):
+        rows = min(chunk, tokens - c0)
+        lo, hi = (min(max(v - c0, 0), rows) for v in (first, end))
+        done = 3 + max(min(end, c0 + rows) - first, 0)
+        stack.forward(want[c0:c0 + rows], batch=Batch(ints(dev, lo, hi), ints(dev, done), table, rows))
+    batch = Batch(ints(dev, first, end), ints(dev, 3 + n), table)
+    for overlap in (False, True):
+        for b in stack.attention.values():
+            b.k_pages.index_fill_(0, table[0, 1:].long(), 0)
+        got = stack.prefill(x, chunk, overlap=overlap, batch=batch)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+def test_stack_without_rows(dev, stack):
+    """A step of no token passes through the attention blocks."""
+    batch = Batch(ints(dev, 0, 0), ints(dev, 5), ints(dev, [0]), 1)
+    assert stack.attention[0].forward_(prompt(dev, 0, 1), batch).shape == (0, H)
