@@ -26,6 +26,7 @@
 //                         workgroup, 32 a wave, over shared 32-key tiles; few tiles
 //                         split their keys over workgroups too.
 //  attention_combine_*    joins the parts of split keys.
+#include <cmath>
 #include <utility>
 
 #include "paged.hpp"
@@ -1189,6 +1190,7 @@ extern "C" int lm_paged_attention(const void *q, int64_t q_token_stride, int64_t
   LM_REQUIRE(q_heads >= 1 && q_heads <= 16384 && q_heads % kv_heads == 0, LM_EINVAL,
              "query heads must be a multiple of key-value heads");
   LM_REQUIRE(max_new >= 0, LM_EINVAL, "invalid number of new tokens");
+  LM_REQUIRE(std::isfinite(scale), LM_EINVAL, "the scale must be finite");
   if (tokens == 0 || sequences == 0) return LM_OK;
   LM_REQUIRE(tokens * q_heads < (1LL << 31), LM_EINVAL, "too many rows");
   LM_REQUIRE(q && k_pages && v_pages && out, LM_EINVAL, "null pointer");
@@ -1201,6 +1203,9 @@ extern "C" int lm_paged_attention(const void *q, int64_t q_token_stride, int64_t
              LM_EINVAL, "head rows must be 16-byte aligned");
   const AttentionPlan plan = attention_plan(tokens, sequences, q_heads, kv_heads, head_dim, max_new,
                                             table_pages * page_size);
+  // threads of the largest launches, below 2^32
+  LM_REQUIRE(sequences * kv_heads < (1LL << 24) && plan.tiles * kv_heads < (1LL << 23), LM_EINVAL,
+             "too many rows");
   const int64_t need = attention_bytes(plan, head_dim);
   LM_REQUIRE(need == 0 || (workspace && aligned16(workspace)), LM_EINVAL,
              "attention needs a 16-byte aligned workspace");

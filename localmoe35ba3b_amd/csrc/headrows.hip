@@ -222,7 +222,7 @@ extern "C" int lm_qk_norm_rope(const void *q, int64_t q_token_stride, int64_t q_
              "attention supports heads of 64, 128 or 256");
   LM_REQUIRE(q_heads >= 0 && q_heads <= 65536 && k_heads >= 0 && k_heads <= 65536, LM_EINVAL,
              "invalid number of heads");
-  LM_REQUIRE(tokens >= 0 && tokens < (1LL << 31), LM_EINVAL, "invalid token count");
+  LM_REQUIRE(tokens >= 0 && tokens < kMaxTokens, LM_EINVAL, "invalid token count");
   if (const int rc = check_rotation(inv_freq, pairs, head_dim)) return rc;
   if (tokens == 0 || q_heads + k_heads == 0) return LM_OK;
   if (q_heads)

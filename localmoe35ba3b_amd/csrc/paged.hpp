@@ -56,6 +56,9 @@ __device__ __forceinline__ int64_t paged_page(const PagedBatch &b, int s, int p)
   return clamp_index32(b.table[s * b.table_stride + i], b.pages) * b.page_stride;
 }
 
+// A launch has fewer than 2^32 threads; the kernels take at most 256 for a token.
+constexpr int64_t kMaxTokens = 1LL << 24;
+
 // Host checks of what the entry points of the paged cache share; LM_OK or the status.
 inline int paged_check(int64_t pages, int64_t page_stride, int64_t kv_heads, int64_t page_size,
                        int64_t head_dim, const void *starts, const void *lengths,
@@ -70,7 +73,7 @@ inline int paged_check(int64_t pages, int64_t page_stride, int64_t kv_heads, int
   LM_REQUIRE(pages >= 1 && pages < (1LL << 31) && page_stride >= kv_heads * page_size * head_dim &&
                  page_stride % 8 == 0,
              LM_EINVAL, "invalid pages");
-  LM_REQUIRE(tokens >= 0 && tokens < (1LL << 31), LM_EINVAL, "invalid token count");
+  LM_REQUIRE(tokens >= 0 && tokens < kMaxTokens, LM_EINVAL, "invalid token count");
   LM_REQUIRE(sequences >= 0 && sequences <= 65536, LM_EINVAL, "invalid number of sequences");
   LM_REQUIRE(table_pages >= 1 && table_pages * page_size < (1LL << 31) &&
                  table_stride >= 0,

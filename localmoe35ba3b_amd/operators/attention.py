@@ -138,7 +138,8 @@ def append(k_pages, v_pages, k, v, starts, lengths, table, inv_freq=None, k_weig
     """Appends k and v [T, kv_heads, D] to the cache, k normed and rotated on the way
     (k_weight and inv_freq as in qk_norm_rope, by its position in its sequence).
     With q [T, q_heads, D], returns the queries normed and rotated for
-    paged_attention, 0 in rows of no sequence."""
+    paged_attention, 0 in rows of no sequence.  The rows that a call writes must differ:
+    no page twice among the new positions of its sequences."""
     k, k_token, k_head = _rows(k, 'keys')
     v, v_token, v_head = _rows(v, 'values')
     dtype, device, shape = k.dtype, k.get_device(), k.shape
@@ -155,7 +156,7 @@ def append(k_pages, v_pages, k, v, starts, lengths, table, inv_freq=None, k_weig
         if q_tokens != tokens or q_dim != dim:
             raise ValueError('queries and keys do not match')
         q_weight, q_w = _weight(q_weight, dim, device)
-        q_out = q.new_empty((tokens, q_heads, dim))
+        q_out = (q.new_empty if lengths.numel() else q.new_zeros)((tokens, q_heads, dim))
         q_args = (q.data_ptr(), q_token, q_head, q_heads, q_w, q_out.data_ptr())
     k_weight, k_w = _weight(k_weight, dim, device)
     inv_freq, freq, pairs = _frequencies(inv_freq, dim, device)
@@ -179,7 +180,8 @@ def paged_attention(q, k_pages, v_pages, starts, lengths, table, scale=None, gat
     defaults to D ** -0.5; gate [T, q_heads, D] multiplies the result by sigmoid(gate).
     max_new bounds the new tokens of one sequence (default: T); a close bound saves
     time.  out [T, q_heads, D], contiguous, receives the result, and rows of no sequence
-    keep what they hold there; without it they are 0."""
+    keep what they hold there; without it they are 0.  It may be q or the gate itself, and
+    shares no memory with them, or with the cache, in another way."""
     q, q_token, q_head = _rows(q, 'queries')
     dtype, device, shape = q.dtype, q.get_device(), q.shape
     pages, stride, heads, size, dim = _cache(k_pages, v_pages, dtype, device)

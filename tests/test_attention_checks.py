@@ -190,3 +190,26 @@ def test_c_calls_without_work(entry):
     assert rows_call(entry, tokens=0, q=None, k=None)[0] == _lib.LM_OK
     if entry != 'norm':
         assert rows_call(entry, sequences=0, q=None, k=None, starts=None)[0] == _lib.LM_OK
+
+
+def test_c_sizes_of_a_launch():
+    """More rows than a launch has threads for, and a scale that is none."""
+    for entry in ALL:
+        rc, error = rows_call(entry, tokens=1 << 24)
+        assert rc == _lib.LM_EINVAL and 'token count' in error
+    rc, error = rows_call('attend', k_heads=1024, q_heads=1024, q_token=1 << 17, page_stride=1 << 21,
+                          sequences=65536)
+    assert rc == _lib.LM_EINVAL and 'too many rows' in error
+    rc, error = rows_call('attend', k_heads=1024, q_heads=1024, q_token=1 << 17, page_stride=1 << 21,
+                          tokens=1 << 20, sequences=1 << 13, max_new=1 << 10)
+    assert rc == _lib.LM_EINVAL and 'too many rows' in error
+
+
+@pytest.mark.parametrize('scale', [float('nan'), float('inf')])
+def test_c_scale_is_finite(scale, monkeypatch):
+    def launch(device, name, *args):
+        assert getattr(_lib.lib(), name)(*args, None) == _lib.LM_EINVAL
+        raise ValueError(_lib.lib().lm_last_error().decode())
+    monkeypatch.setattr(_lib, 'launch', launch)
+    with pytest.raises(ValueError, match='finite'):
+        attend(scale=scale)

@@ -377,3 +377,131 @@ def test_calls_on_two_streams(dev):
     torch.cuda.synchronize()
     for g, want in zip(got, alone):
         assert all(torch.equal(x, want) for x in g)
+
+
+def test_append_without_sequences(dev):
+    """Every row is one of no sequence: zeros for the queries, the cache as it was."""
+    kp = rand(seeded(1), 4, 2, 16, 64).to(dev)
+    q, k = rand(seeded(2), 5, 4, 64).to(dev), rand(seeded(3), 5, 2, 64).to(dev)
+    none, before = torch.zeros(1, dtype=torch.int32, device=dev), kp.clone()
+    torch.full((5, 4, 64), 3.0, dtype=BF16, device=dev)  # memory that is not 0
+    got = A.append(kp, kp.clone(), k, k, none, none[:0], none[:0].view(0, 1), q=q)
+    assert not got.any() and torch.equal(kp, before)
+    assert not A.paged_attention(q, kp, kp, none, none[:0], none[:0].view(0, 1)).any()
+
+
+@pytest.mark.parametrize('sequences', [70, 300, 600])
+@pytest.mark.parametrize('chunks', [False, True])
+def test_attention_many_sequences(dev, sequences, chunks):
+    """More sequences than a wave or a workgroup looks at together; some without new tokens,
+    some without a visible key, with chunks among them."""
+    gen = torch.Generator().manual_seed(sequences)
+    length = torch.randint(0, 90, (sequences,), generator=gen).tolist()
+    lens = [(i % 4 if i % 7 else 30 * chunks, n) for i, n in enumerate(length)]
+    lens = [(new, max(n, new - 1)) for new, n in lens]
+    attend(dev, lens, 16, 4, 2, 64, BF16, gate=chunks, pad=2, seed=sequences,
+           max_new=max(n for n, _ in lens))
+
+
+def long_cache(dev, heads, keys, dim, seed):
+    """A cache of one sequence in random pages, made on the GPU, and its CPU copy."""
+    gen = torch.Generator(device=dev)
+    gen.manual_seed(seed)
+    pages = -(-keys // 64)
+    kp, vp = (torch.randn(pages, heads, 64, dim, generator=gen, device=dev).to(BF16) for _ in range(2))
+    table = torch.randperm(pages, generator=seeded(seed)).to(torch.int32)[None]
+    return kp, vp, table
+
+
+@pytest.mark.parametrize('new,heads,keys,dim', [(2, 128, 18000, 64), (1, 128, 9000, 256),
+                                                (20, 128, 10000, 64), (20, 128, 4700, 256)])
+def test_attention_long_parts(dev, new, heads, keys, dim):
+    """Parts of a sequence longer than the pages that a wave looks up at a time: as many heads
+    as this leave each few parts."""
+    kp, vp, table = long_cache(dev, heads, keys, dim, keys)
+    q = rand(seeded(keys), new, heads, dim)
+    batch = torch.tensor([0, new], dtype=torch.int32), torch.tensor([keys], dtype=torch.int32), table
+    got = A.paged_attention(q.to(dev), kp, vp, *to(dev, *batch))
+    some = [0, heads // 2, heads - 1]  # heads are independent: three of them in 64 bits
+    want = U.attention(q[:, some], kp[:, some].cpu(), vp[:, some].cpu(), *batch)
+    U.assert_attention(got[:, some], want, f'{new} {heads} {keys} {dim}')
+    assert got.isfinite().all()
+
+
+@TYPES
+@pytest.mark.parametrize('dim', [128, 256])
+@pytest.mark.parametrize('new', [1, 40])
+def test_attention_odd_values_of_all_types(dev, new, dim, dtype):
+    """Infinities and NaN among the values of a position that only the last rows see."""
+    lens = [(new, 100), (new, 70)]
+    gen = seeded(dim + new)
+    starts, lengths, table, pages = U.batch(lens, 16)
+    q = rand(gen, 2 * new, 4, dim, dtype=dtype)
+    kp, vp = (rand(gen, pages, 2, 16, dim, dtype=dtype) for _ in range(2))
+    clean = U.attention(q, kp, vp, starts, lengths, table)
+    bad = 100 - max(1, new // 2)
+    at = int(table[0, bad // 16])
+    vp[at, 0, bad % 16, 3], vp[at, 0, bad % 16, dim - 2] = math.inf, math.nan
+    vp[at, 1, bad % 16, 64] = -math.inf
+    kp[at, 1, bad % 16, 9] = math.nan
+    got = A.paged_attention(*to(dev, q, kp, vp, starts, lengths, table)).cpu()
+    sees = torch.zeros(2 * new, 4, dim, dtype=torch.bool)
+    rows = slice(max(0, new - (100 - bad)), new)
+    sees[rows, :2, 3] = sees[rows, :2, dim - 2] = True
+    sees[rows, 2:] = True
+    assert not got[sees].isfinite().any()
+    U.assert_rows(got[~sees], clean[0][~sees], clean[1][~sees], dtype, 'rows before it')
+
+
+@pytest.mark.parametrize('lens,max_new', [([(1, 900), (2, 40), (1, 0)], 2), ([(130, 700)], 130),
+                                          ([(40, 40), (1, 3000), (300, 300)], 300)])
+def test_attention_in_place(dev, lens, max_new):
+    """The output may be the queries or the gate themselves."""
+    gen = seeded(21)
+    starts, lengths, table, pages = U.batch(lens, 64)
+    q, g = (rand(gen, int(starts[-1]), 16, 256).to(dev) for _ in range(2))
+    cache = to(dev, *(rand(gen, pages, 2, 64, 256) for _ in range(2)), starts, lengths, table)
+    want = A.paged_attention(q, *cache, gate=g, max_new=max_new)
+    for pick in (0, 1):
+        a = [q.clone(), g.clone()]
+        got = A.paged_attention(a[0], *cache, gate=a[1], max_new=max_new, out=a[pick])
+        assert got is a[pick] and torch.equal(got, want)
+
+
+def test_attention_on_another_stream_than_its_tensors(dev):
+    """A call on a stream that has waited for its inputs' stream; the output is made there."""
+    gen = seeded(23)
+    starts, lengths, table, pages = U.batch([(1, 500), (70, 300)], 16)
+    args = to(dev, rand(gen, 71, 8, 128), *(rand(gen, pages, 2, 16, 128) for _ in range(2)), starts,
+              lengths, table)
+    want = A.paged_attention(*args)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = A.paged_attention(*args)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+
+
+def test_two_captured_calls_replayed_in_turn(dev):
+    """Two graphs of one pool, one after another: each call's workspace is its own."""
+    gen = seeded(25)
+    graphs, outs, wants = [], [], []
+    args = []
+    for seed, lens in ((1, [(1, 2000)] * 3), (2, [(50, 400), (1, 900)])):
+        starts, lengths, table, pages = U.batch(lens, 64, seed)
+        args.append(to(dev, rand(gen, int(starts[-1]), 16, 256),
+                       *(rand(gen, pages, 2, 64, 256) for _ in range(2)), starts, lengths, table))
+    wants = [A.paged_attention(*a) for a in args]
+    torch.cuda.synchronize()
+    for a in args:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=graphs[0].pool() if graphs else None):
+            outs.append(A.paged_attention(*a))
+        graphs.append(graph)
+    for _ in range(3):
+        for graph, out, want, a in zip(graphs, outs, wants, args):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+            A.paged_attention(*a)  # eager work between replays
