@@ -51,8 +51,8 @@ struct Attention {
   int64_t q_token, q_head, gate_token, gate_head;  // strides, elements
   const uint16_t *k_pages, *v_pages;
   uint16_t *out;  // [tokens][q_heads][D]
-  float *part;    // unscaled sums of split keys, then (m, l) of each row
-  float *part_ml;
+  float *part, *part_ml;  // few: unscaled sums of split keys, and (m, l) of each row
+  float *tile_part, *tile_ml;  // the same of tiles
   Parts *parts;   // few: [sequences][kv_heads]
   PagedBatch batch;
   int tokens, q_heads, group;
@@ -620,17 +620,17 @@ struct PartSum {
 
 constexpr int kFewParts = 16;
 
-// Rows of sequences whose keys attention_few_kernel split; blockIdx.x is a sequence's
-// key-value head.  Up to kFewParts parts: a thread takes four channels of a row, eight parts
-// of it loaded at a time.  More: the workgroups of blockIdx.y share the rows and their
-// channels, 64 at a time, the 16 groups of 16 threads the parts.
+// Rows of sequences whose keys attention_few_kernel split, by `ys` workgroups for a sequence's
+// key-value head (`pair`).  Up to kFewParts parts: a thread takes four channels of a row, eight
+// parts of it loaded at a time.  More: the workgroups share the rows and their channels, 64 at
+// a time, the 16 groups of 16 threads the parts.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void attention_combine_few_kernel(Attention a) {
+__device__ __forceinline__ void combine_few(const Attention &a, int pair, int y, int ys) {
   __shared__ __attribute__((aligned(16))) float sums[16][64];
   __shared__ float ms[16], ls[16];
-  const int kv = blockIdx.x % a.batch.kv_heads, s = blockIdx.x / a.batch.kv_heads;
+  const int kv = pair % a.batch.kv_heads, s = pair / a.batch.kv_heads;
   const int tid = threadIdx.x, group = tid / 16;
-  const Parts parts = a.parts[blockIdx.x];
+  const Parts parts = a.parts[pair];
   const PagedSequence seq = paged_sequence(a.batch, s, a.tokens);
   if (!few_rows(seq, a.group) || parts.count < 2) return;
   const int rows = seq.count * a.group, n = parts.count;
@@ -638,7 +638,7 @@ __global__ __launch_bounds__(256) void attention_combine_few_kernel(Attention a)
     return part_row(a, parts.span + j, j == 0 && parts.later, kv) + c;
   };
   if (n <= kFewParts) {
-    for (int u = blockIdx.y * 256 + tid; u < rows * (D / 4); u += gridDim.y * 256) {
+    for (int u = y * 256 + tid; u < rows * (D / 4); u += ys * 256) {
       const int c = u / (D / 4), d = u % (D / 4) * 4;
       const RowPlace to = row_place(a, seq, kv, c);
       const uint2 gate = load_gate(a, to, d);
@@ -660,7 +660,7 @@ __global__ __launch_bounds__(256) void attention_combine_few_kernel(Attention a)
     }
     return;
   }
-  for (int u = blockIdx.y; u < rows * (D / 64); u += gridDim.y) {
+  for (int u = y; u < rows * (D / 64); u += ys) {
     const int c = u / (D / 64), d = u % (D / 64) * 64 + tid % 16 * 4;
     const RowPlace to = row_place(a, seq, kv, c);
     const uint2 gate = load_gate(a, to, d);
@@ -987,7 +987,7 @@ __global__ __launch_bounds__(TileForm<D>::kWaves * 64, 2) void attention_tile_ke
     if (a.splits > 1 && c0 + threadIdx.x < rows) {
       const RowPlace to = row_place(a, seq, kv, c0 + threadIdx.x);
       const int64_t row = ((int64_t)split * a.tokens + to.token) * a.q_heads + to.head;
-      *reinterpret_cast<float2 *>(a.part_ml + row * 2) = float2{sum.m, sum.l};
+      *reinterpret_cast<float2 *>(a.tile_ml + row * 2) = float2{sum.m, sum.l};
     }
   }
   // A thread's units of four channels lie STEP rows apart; four at a time, their gates first.
@@ -1039,7 +1039,7 @@ __global__ __launch_bounds__(TileForm<D>::kWaves * 64, 2) void attention_tile_ke
           write_row<T, D>(a, to[i], side * C + d, o, gate[i]);
         } else {
           const int64_t row = ((int64_t)split * a.tokens + to[i].token) * a.q_heads + to[i].head;
-          *reinterpret_cast<f32x4 *>(a.part + row * D + side * C + d) = o;
+          *reinterpret_cast<f32x4 *>(a.tile_part + row * D + side * C + d) = o;
         }
       }
     }
@@ -1049,9 +1049,9 @@ __global__ __launch_bounds__(TileForm<D>::kWaves * 64, 2) void attention_tile_ke
 // Rows of sequences in tiles, where their keys were split: D / 4 threads a row, `chunks`
 // workgroups a token.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void attention_combine_tile_kernel(Attention a, int chunks) {
-  const int t = blockIdx.x / chunks, lane = threadIdx.x & 63;
-  const int i = blockIdx.x % chunks * 256 + threadIdx.x;
+__device__ __forceinline__ void combine_tile(const Attention &a, int block, int chunks) {
+  const int t = block / chunks, lane = threadIdx.x & 63;
+  const int i = block % chunks * 256 + threadIdx.x;
   const int head = i / (D / 4), d = i % (D / 4) * 4;
   int s = -1;  // the token's sequence: a lane looks at one of 64
   for (int c = 0; c < a.batch.sequences && s < 0; c += 64) {
@@ -1072,14 +1072,26 @@ __global__ __launch_bounds__(256) void attention_combine_tile_kernel(Attention a
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t r = row + min(j0 + j, a.splits - 1) * rows;
-      ml[j] = *reinterpret_cast<const float2 *>(a.part_ml + r * 2);
-      v[j] = *reinterpret_cast<const f32x4 *>(a.part + r * D + d);
+      ml[j] = *reinterpret_cast<const float2 *>(a.tile_ml + r * 2);
+      v[j] = *reinterpret_cast<const f32x4 *>(a.tile_part + r * D + d);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (j0 + j < a.splits) sum.add(ml[j].x, ml[j].y, v[j]);
   }
   write_row<T, D>(a, {t, head}, d, sum.o * sum.inverse(), gate);
+}
+
+// Joins the parts of both kernels in one launch (one for each took 6 us longer where a call
+// has both): `ys` workgroups for each of the few rows' pairs, then those of the tiles.  The
+// pairs' first workgroups come first, as in many pairs only those have work.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attention_combine_kernel(Attention a, int pairs, int ys, int chunks) {
+  const int block = blockIdx.x;
+  if (block < pairs * ys)
+    combine_few<T, D>(a, block % pairs, block / pairs, ys);
+  else
+    combine_tile<T, D>(a, block - pairs * ys, chunks);
 }
 
 // ------------------------------------------------------------------ host side
@@ -1122,32 +1134,29 @@ int64_t attention_bytes(const AttentionPlan &p, int64_t head_dim) {
 template <typename T, int D>
 int launch_attention(const AttentionPlan &p, Attention a, float *workspace, hipStream_t st) {
   a.few = p.few;
+  a.part = workspace, a.part_ml = workspace + p.few_rows * D;
+  a.tile_part = workspace + p.few_rows * (D + 2), a.tile_ml = a.tile_part + p.tile_rows * D;
+  a.parts = reinterpret_cast<Parts *>(a.tile_ml + p.tile_rows * 2);
+  a.shares = (int)p.shares, a.splits = (int)p.splits;
+  int64_t ys = 0, tile = 0;  // workgroups that join parts: ys for each of p.parts, and tile
   if (p.few) {
-    a.shares = (int)p.shares;
-    a.part = workspace, a.part_ml = workspace + p.few_rows * D;
-    a.parts = reinterpret_cast<Parts *>(workspace + (p.few_rows + p.tile_rows) * (D + 2));
     attention_few_kernel<T, D><<<(unsigned)p.few_grid, 256, 0, st>>>(a);
     if (const int rc = check_launch("attention_few_kernel")) return rc;
     // Where there are few sequences, their rows and channels fill the chip.
-    const int64_t heads = (int64_t)a.batch.sequences * a.batch.kv_heads;
-    const int64_t units = kFewRows / a.group * a.group * (D / 64), some = 4096 / heads;
-    const dim3 grid((unsigned)heads, (unsigned)(some < 1 ? 1 : some < units ? some : units));
-    attention_combine_few_kernel<T, D><<<grid, 256, 0, st>>>(a);
-    if (const int rc = check_launch("attention_combine_few_kernel")) return rc;
+    const int64_t units = kFewRows / a.group * a.group * (D / 64), some = 4096 / p.parts;
+    ys = some < 1 ? 1 : some < units ? some : units;
   }
+  const int chunks = (a.q_heads * (D / 4) + 255) / 256;
   if (p.tile) {
-    a.splits = (int)p.splits;
-    a.part = workspace + p.few_rows * (D + 2), a.part_ml = a.part + p.tile_rows * D;
     const dim3 grid((unsigned)(p.tiles * a.batch.kv_heads), (unsigned)p.splits);
     attention_tile_kernel<T, D><<<grid, TileForm<D>::kWaves * 64, 0, st>>>(a);
     if (const int rc = check_launch("attention_tile_kernel")) return rc;
-    if (p.splits > 1) {
-      const int chunks = (a.q_heads * (D / 4) + 255) / 256;
-      attention_combine_tile_kernel<T, D><<<a.tokens * chunks, 256, 0, st>>>(a, chunks);
-      return check_launch("attention_combine_tile_kernel");
-    }
+    if (p.splits > 1) tile = (int64_t)a.tokens * chunks;
   }
-  return LM_OK;
+  const int64_t all = p.parts * ys + tile;
+  if (all == 0) return LM_OK;
+  attention_combine_kernel<T, D><<<(unsigned)all, 256, 0, st>>>(a, (int)p.parts, (int)ys, chunks);
+  return check_launch("attention_combine_kernel");
 }
 
 template <typename T>
