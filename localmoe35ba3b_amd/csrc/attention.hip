@@ -57,7 +57,9 @@ struct Attention {
   PagedBatch batch;
   int tokens, q_heads, group;
   int shares;  // few: spans that a key-value head's keys are cut into, at most
-  int splits;  // tile: parts of each tile's keys
+  int splits;  // tile: parts of a tile's keys, at most
+  int room;    // tile: workgroups at a time for a key-value head, 0: every tile has `splits` parts
+  int *row_parts;  // tile, if room > 0: parts of each row, [tokens][q_heads]
   bool few;    // tile: sequences of few rows are attention_few_kernel's
   float scale2;   // |scale| * log2(e), not 0
   uint32_t flip;  // sign bits that queries are flipped by, for a negative scale
@@ -703,43 +705,94 @@ __device__ __forceinline__ int tile_count(const Attention &a, int s) {
   return (int)(((int64_t)q.count * a.group + kTileRows - 1) / kTileRows);
 }
 
+// Keys that the last row of a sequence's tile sees, the most of its rows.
+__device__ __forceinline__ int tile_keys(const PagedSequence &q, int group, int tile) {
+  const int last = min((int64_t)(tile + 1) * kTileRows, (int64_t)q.count * group) - 1;
+  return max(min(q.base + last / group + 1, q.length), 0);
+}
+
+// Keys of n tiles of sequence s together (their mean is that of the first and the last).
+__device__ __forceinline__ int64_t all_keys(const Attention &a, int s, int n) {
+  if (n == 0) return 0;
+  const PagedSequence q = paged_sequence(a.batch, s, a.tokens);
+  return ((int64_t)tile_keys(q, a.group, 0) + tile_keys(q, a.group, n - 1)) * n / 2;
+}
+
 struct TilePlace {
-  int s, tile;  // s < 0: none
+  int s, tile;   // s < 0: none
+  // where tiles are split each in its own way: all tiles of the call, and their keys
+  int tiles;
+  int64_t keys;
 };
 
+// Parts of a tile that sees `keys` keys, where sequences differ: about equal parts, as many as
+// the tiles, which take one or more each, leave of so many rounds of workgroups that they fill
+// two thirds at most; none below 256 keys.  Against as many parts for every tile, 12 sequences of
+// up to 700 new tokens took 52 us instead of 61 (heads of 128) and 61 instead of 77 (256), 24 of
+// 8 to 24 tokens 46 instead of 55; parts of 128 or 512 keys and fewer or more rounds took up to
+// 30 % more in one case or another.
+__device__ __forceinline__ int tile_parts(const Attention &a, const TilePlace &place, int keys) {
+  const int rounds = (int)((float)place.tiles * 1.5f / (float)a.room) + 1;
+  const float all = (float)max(place.keys, (int64_t)1);
+  const float n = (float)keys * (float)(rounds * a.room - place.tiles) / all + 0.5f;
+  return max(min(min((int)fminf(n, 65536.0f), a.splits), keys / 256), 1);
+}
+
 // The index-th tile; the tile with the most keys of a sequence comes first.
-// All THREADS threads; scratch (a word a wave) and found are free again afterwards.
+// All THREADS threads; scratch (a word and a long word a wave) and found are free again
+// afterwards.
 template <int THREADS>
-__device__ TilePlace find_tile(const Attention &a, int index, int *scratch, TilePlace *found) {
+__device__ TilePlace find_tile(const Attention &a, int index, int *scratch, int64_t *sums,
+                               TilePlace *found) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const bool split = a.room > 0;
   if (a.batch.sequences == 1) {
     const int n = tile_count(a, 0);
-    return {index < n ? 0 : -1, n - 1 - index};
+    return {index < n ? 0 : -1, n - 1 - index, 0, 0};
   }
-  if (tid == 0) found->s = -1;
-  int base = 0;
-  for (int c = 0; c < a.batch.sequences; c += THREADS) {
-    const int n = tile_count(a, c + tid);
-    int sum = n;
+  auto scan = [&](int &sum, int64_t &keys) {  // counts up to the lane's, keys of all lanes
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const int v = __shfl_up(sum, o, 64);
       if (lane >= o) sum += v;
     }
+    if (split)
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) keys += __shfl_xor(keys, o, 64);
+  };
+  if (a.batch.sequences <= 64) {  // each wave for itself
+    const int n = tile_count(a, lane);
+    int sum = n;
+    int64_t keys = split ? all_keys(a, lane, n) : 0;
+    scan(sum, keys);
+    const uint64_t hit = __ballot(index >= sum - n && index < sum);
+    if (!hit) return {-1, 0, 0, 0};
+    const int at = __builtin_ctzll(hit);
+    return {at, __shfl(sum, at, 64) - 1 - index, __shfl(sum, 63, 64), keys};
+  }
+  if (tid == 0) found->s = -1;
+  int base = 0;
+  int64_t all = 0;
+  for (int c = 0; c < a.batch.sequences; c += THREADS) {
+    const int n = tile_count(a, c + tid);
+    int sum = n;
+    int64_t keys = split ? all_keys(a, c + tid, n) : 0;
+    scan(sum, keys);
     __syncthreads();
-    if (lane == 63) scratch[wave] = sum;
+    if (lane == 63) scratch[wave] = sum, sums[wave] = keys;
     __syncthreads();
     int before = base;
     for (int w = 0; w < THREADS / 64; ++w) {
       if (w < wave) before += scratch[w];
-      base += scratch[w];
+      base += scratch[w], all += sums[w];
     }
     before += sum - n;
-    if (index >= before && index < before + n) *found = {c + tid, n - 1 - (index - before)};
-    if (base > index) break;  // the same for every thread
+    if (index >= before && index < before + n) *found = {c + tid, n - 1 - (index - before), 0, 0};
+    if (base > index && !split) break;  // the same for every thread
   }
   __syncthreads();
-  const TilePlace got = *found;
+  TilePlace got = *found;
+  got.tiles = base, got.keys = all;
   __syncthreads();
   return got;
 }
@@ -884,27 +937,29 @@ __global__ __launch_bounds__(TileForm<D>::kWaves * 64, 2) void attention_tile_ke
   // One array: with several, the compiler waits for all direct loads at each LDS read.
   __shared__ __attribute__((aligned(16))) char lds[tile_lds<D>()];
   int *scratch = reinterpret_cast<int *>(lds);
-  TilePlace *found = reinterpret_cast<TilePlace *>(scratch + WAVES);
+  int64_t *key_sums = reinterpret_cast<int64_t *>(scratch + 8);
+  TilePlace *found = reinterpret_cast<TilePlace *>(key_sums + 8);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int set = wave & 3, group = wave >> 2;
   const int kv = blockIdx.x % a.batch.kv_heads, split = blockIdx.y;
   const TilePlace place =
-      find_tile<WAVES * 64>(a, blockIdx.x / a.batch.kv_heads, scratch, found);
+      find_tile<WAVES * 64>(a, blockIdx.x / a.batch.kv_heads, scratch, key_sums, found);
   const int s = __builtin_amdgcn_readfirstlane(place.s);
   if (s < 0) return;
   const PagedSequence seq = paged_sequence(a.batch, s, a.tokens);
-  const int rows = seq.count * a.group, c0 = place.tile * kTileRows;
+  const int tile = __builtin_amdgcn_readfirstlane(place.tile);
+  const int rows = seq.count * a.group, c0 = tile * kTileRows;
   const int c = c0 + set * 32 + (lane & 31);
   const bool idle = c0 + set * 32 >= rows;
   const RowPlace at = row_place(a, seq, kv, min(c, rows - 1));
   const int limit = min(seq.base + min(c, rows - 1) / a.group + 1, seq.length);
   const int all_see = min(seq.base + c0 / a.group + 1, seq.length);  // seen by every row
-  // keys that the tile's last row sees, and this split's part of them
-  const int last = min(c0 + kTileRows, rows) - 1;
-  const int keys = max(min(seq.base + last / a.group + 1, seq.length), 0);
-  const int tiles = (keys + KEYS - 1) / KEYS;
-  const int key0 = (int)((int64_t)tiles * split / a.splits) * KEYS;
-  const int key1 = min((int)((int64_t)tiles * (split + 1) / a.splits) * KEYS, keys);
+  // keys that the tile's last row sees, and this part of them
+  const int keys = tile_keys(seq, a.group, tile), tiles = (keys + KEYS - 1) / KEYS;
+  const int splits = __builtin_amdgcn_readfirstlane(a.room ? tile_parts(a, place, keys) : a.splits);
+  if (split >= splits) return;
+  const int key0 = (int)((int64_t)tiles * split / splits) * KEYS;
+  const int key1 = min((int)((int64_t)tiles * (split + 1) / splits) * KEYS, keys);
 
   u32x4 q[D / 16];
   const uint16_t *qr = a.q + (int64_t)at.token * a.q_token + (int64_t)at.head * a.q_head + (lane >> 5) * 8;
@@ -978,7 +1033,7 @@ __global__ __launch_bounds__(TileForm<D>::kWaves * 64, 2) void attention_tile_ke
       const float *p = ml + (g * kTileRows + threadIdx.x) * 2;
       sum.add(p[0], p[1], f32x4{});
     }
-    const float inv = a.splits == 1 ? sum.inverse() : 1.0f;
+    const float inv = splits == 1 ? sum.inverse() : 1.0f;
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) {
       float *p = ml + (g * kTileRows + threadIdx.x) * 2;
@@ -986,8 +1041,11 @@ __global__ __launch_bounds__(TileForm<D>::kWaves * 64, 2) void attention_tile_ke
     }
     if (a.splits > 1 && c0 + threadIdx.x < rows) {
       const RowPlace to = row_place(a, seq, kv, c0 + threadIdx.x);
-      const int64_t row = ((int64_t)split * a.tokens + to.token) * a.q_heads + to.head;
-      *reinterpret_cast<float2 *>(a.tile_ml + row * 2) = float2{sum.m, sum.l};
+      const int64_t row = (int64_t)to.token * a.q_heads + to.head;
+      if (a.room && split == 0) a.row_parts[row] = splits;
+      if (splits > 1)
+        *reinterpret_cast<float2 *>(a.tile_ml + ((int64_t)split * a.tokens * a.q_heads + row) * 2) =
+            float2{sum.m, sum.l};
     }
   }
   // A thread's units of four channels lie STEP rows apart; four at a time, their gates first.
@@ -1022,7 +1080,7 @@ __global__ __launch_bounds__(TileForm<D>::kWaves * 64, 2) void attention_tile_ke
 #pragma unroll
       for (int i = 0; i < BATCH; ++i) {
         to[i] = {seq.first + min(t, seq.count - 1), kv * a.group + h};
-        if (a.splits == 1) gate[i] = load_gate(a, to[i], side * C + d);
+        if (splits == 1) gate[i] = load_gate(a, to[i], side * C + d);
         t += step_t, h += step_h;
         if (h >= a.group) h -= a.group, ++t;
       }
@@ -1035,7 +1093,7 @@ __global__ __launch_bounds__(TileForm<D>::kWaves * 64, 2) void attention_tile_ke
           const int w = kTileRows + r;
           o += *reinterpret_cast<const f32x4 *>(sums + w * PITCH + d) * ml[w * 2];
         }
-        if (a.splits == 1) {
+        if (splits == 1) {
           write_row<T, D>(a, to[i], side * C + d, o, gate[i]);
         } else {
           const int64_t row = ((int64_t)split * a.tokens + to[i].token) * a.q_heads + to[i].head;
@@ -1064,20 +1122,22 @@ __device__ __forceinline__ void combine_tile(const Attention &a, int block, int 
   const PagedSequence seq = paged_sequence(a.batch, s, a.tokens);
   if (t < seq.first || t >= seq.first + seq.count || (a.few && few_rows(seq, a.group))) return;
   const int64_t rows = (int64_t)a.tokens * a.q_heads, row = (int64_t)t * a.q_heads + head;
+  const int parts = a.room ? min(a.row_parts[row], a.splits) : a.splits;
+  if (parts < 2) return;  // written by its tile
   const uint2 gate = load_gate(a, {t, head}, d);
   PartSum sum;
-  for (int j0 = 0; j0 < a.splits; j0 += 4) {
+  for (int j0 = 0; j0 < parts; j0 += 4) {
     float2 ml[4];
     f32x4 v[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int64_t r = row + min(j0 + j, a.splits - 1) * rows;
+      const int64_t r = row + min(j0 + j, parts - 1) * rows;
       ml[j] = *reinterpret_cast<const float2 *>(a.tile_ml + r * 2);
       v[j] = *reinterpret_cast<const f32x4 *>(a.tile_part + r * D + d);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (j0 + j < a.splits) sum.add(ml[j].x, ml[j].y, v[j]);
+      if (j0 + j < parts) sum.add(ml[j].x, ml[j].y, v[j]);
   }
   write_row<T, D>(a, {t, head}, d, sum.o * sum.inverse(), gate);
 }
@@ -1099,8 +1159,8 @@ __global__ __launch_bounds__(256) void attention_combine_kernel(Attention a, int
 struct AttentionPlan {
   bool few, tile;
   int64_t shares, few_grid;          // few: parts per key-value head, workgroups
-  int64_t tiles, splits;             // tile: tiles at most, parts of each
-  int64_t few_rows, tile_rows, parts;  // rows of partial sums, Parts
+  int64_t tiles, splits, room;       // tile: tiles at most, parts of each, see Attention
+  int64_t few_rows, tile_rows, parts, row_parts;  // rows of partial sums, Parts, rows' parts
 };
 
 AttentionPlan attention_plan(int64_t tokens, int64_t sequences, int64_t q_heads, int64_t kv_heads,
@@ -1119,16 +1179,27 @@ AttentionPlan attention_plan(int64_t tokens, int64_t sequences, int64_t q_heads,
   if (p.tile) {
     const int64_t some = sequences < tokens ? sequences : tokens;
     p.tiles = tokens * group / kTileRows + some;
-    int64_t n = (head_dim == 256 ? 512 : 1024) / (p.tiles * kv_heads);
-    if (n > max_keys / 256) n = max_keys / 256;
-    p.splits = n < 1 ? 1 : n;
-    if (p.splits > 1) p.tile_rows = p.splits * tokens * q_heads;
+    // One sequence's tiles have nearly the same keys: as many parts for each as keep the
+    // workgroups within two rounds.  Others differ: see tile_parts.
+    const int64_t round = (head_dim == 256 ? 256 : 512), pairs = p.tiles * kv_heads;
+    int64_t n = 2 * round / pairs, most = max_keys / 256;
+    if (sequences > 1 && n > 0) n = 4 * round / pairs + 1;
+    p.splits = n < most ? n : most;
+    if (p.splits < 1) p.splits = 1;
+    if (p.splits > 1) {
+      p.tile_rows = p.splits * tokens * q_heads;
+      if (sequences > 1) {
+        p.room = round / 2 / kv_heads > 1 ? round / 2 / kv_heads : 1;
+        p.row_parts = tokens * q_heads;
+      }
+    }
   }
   return p;
 }
 
 int64_t attention_bytes(const AttentionPlan &p, int64_t head_dim) {
-  return (p.few_rows + p.tile_rows) * (head_dim + 2) * 4 + (p.parts * sizeof(Parts) + 15) / 16 * 16;
+  return (p.few_rows + p.tile_rows) * (head_dim + 2) * 4 + p.row_parts * 4 +
+         (p.parts * sizeof(Parts) + 15) / 16 * 16;
 }
 
 template <typename T, int D>
@@ -1137,7 +1208,8 @@ int launch_attention(const AttentionPlan &p, Attention a, float *workspace, hipS
   a.part = workspace, a.part_ml = workspace + p.few_rows * D;
   a.tile_part = workspace + p.few_rows * (D + 2), a.tile_ml = a.tile_part + p.tile_rows * D;
   a.parts = reinterpret_cast<Parts *>(a.tile_ml + p.tile_rows * 2);
-  a.shares = (int)p.shares, a.splits = (int)p.splits;
+  a.row_parts = reinterpret_cast<int *>(a.parts + p.parts);
+  a.shares = (int)p.shares, a.splits = (int)p.splits, a.room = (int)p.room;
   int64_t ys = 0, tile = 0;  // workgroups that join parts: ys for each of p.parts, and tile
   if (p.few) {
     attention_few_kernel<T, D><<<(unsigned)p.few_grid, 256, 0, st>>>(a);

@@ -505,3 +505,16 @@ def test_two_captured_calls_replayed_in_turn(dev):
             torch.cuda.synchronize()
             assert torch.equal(out, want)
             A.paged_attention(*a)  # eager work between replays
+
+
+@pytest.mark.parametrize('sequences,longest,dim', [(70, 900, 64), (70, 700, 256), (5, 5000, 128),
+                                                   (270, 600, 64)])
+def test_attention_unequal_tiles(dev, sequences, longest, dim):
+    """Tiles whose keys differ by far, split into different counts of parts, some into none; more
+    sequences than a wave or a workgroup looks at together."""
+    gen = torch.Generator().manual_seed(longest)
+    lens = []
+    for i in range(sequences):
+        n = longest if i % 17 == 3 else int(torch.randint(1, 120, (1,), generator=gen))
+        lens.append((min(n, 10 + i % 13), n))
+    attend(dev, lens, 16, 6, 2, dim, BF16, gate=True, pad=1, seed=longest)
