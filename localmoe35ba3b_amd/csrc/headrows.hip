@@ -15,6 +15,10 @@
 // in a row, so the rotation needs no exchange and a row is read once.  The first rows are
 // requested at the start, beside the position, whose lookups (sequence, length, page) are
 // the longest chain of a small call.
+//
+// Bound by the rows' bytes where there are many, by that chain where there are few.  18 heads
+// of 256: 4096 tokens 16 us (75.5 MB, 4.7 TB/s), one token 3 us; 64 tokens into a cache 5 us;
+// 3310 tokens into a cache (48 heads of 128) 18 us (81 MB, 4.6 TB/s).
 #include "paged.hpp"
 
 namespace lm {
