@@ -318,8 +318,8 @@ int lm_rmsnorm(const void *x, const float *w, void *y, int64_t rows,
  * Attention between the MoE blocks.  No counterpart among the reference's
  * operators (it runs the Transformers modules): for rows of heads of 64, 128
  * or 256 channels, bf16 or fp16, whose channels are contiguous; token and head
- * strides are in elements and multiples of 8, and every data pointer is
- * 16-byte aligned.
+ * strides are in elements and multiples of 8, every data pointer is 16-byte
+ * aligned, and a call has fewer than 2^24 tokens.
  *
  * Norms of queries and keys for each head, and the position rotation, in one
  * pass:
@@ -348,7 +348,8 @@ int lm_qk_norm_rope(const void *q, int64_t q_token_stride, int64_t q_head_stride
  * is a power of two from 16 to 1024.  Rows of no sequence are not appended and
  * are 0 in q_out; a position outside the table is not written.  Page numbers
  * are clamped into [0, pages).  Rows that one call writes lie in different
- * places (its sequences share no page that it writes). */
+ * places (its sequences share no page that it writes).  A call of no sequence
+ * writes nothing. */
 int lm_paged_append(const void *k, int64_t k_token_stride, int64_t k_head_stride,
                     const float *k_weight, const void *v, int64_t v_token_stride,
                     int64_t v_head_stride, const void *q, int64_t q_token_stride,
@@ -366,7 +367,8 @@ int lm_paged_append(const void *k, int64_t k_token_stride, int64_t k_head_stride
  * in fp32 (the weights rounded to dtype for their product with the values),
  * rounded once; a row that sees no key is 0, rows of no sequence are left as
  * they were.  q_heads is a multiple of kv_heads; out is contiguous [tokens,
- * q_heads, head_dim].  max_new bounds the new tokens of a sequence (tokens is
+ * q_heads, head_dim], may be q or gate itself and overlaps no other operand.
+ * scale is finite.  max_new bounds the new tokens of a sequence (tokens is
  * always right); rows of sequences with more may be left unwritten.  workspace
  * holds lm_paged_attention_workspace_bytes (max_keys = table_pages * page_size;
  * 0: none is needed), 16-byte aligned; its contents need no initialization, and

@@ -27,7 +27,7 @@
 //                         heads: 262144 keys of one sequence 88 us (6.1 TB/s), 64
 //                         sequences of 400 to 13000 keys 92 us (5.8 TB/s); 16 heads
 //                         of 64, 24 sequences of 300 to 5000 keys with 2 to 9 rows
-//                         37 us (4.1 TB/s).
+//                         32 us (4.7 TB/s).
 //  attention_tile_kernel  longer ones: bound by the matrix cores and the softmax
 //                         beside them.  128 rows a workgroup, 32 a wave.  Heads of
 //                         256 leave a wave no registers for a second one of its kind
@@ -334,9 +334,12 @@ __device__ Spans find_span(const Attention &a, int index, int64_t *scratch, Find
 // ------------------------------------------------------------------ few rows
 constexpr int kFewWaves = 4;
 
-// Steps of 16 keys in a wave's ring: as many bytes for every head size.
+// Steps of 16 keys in a wave's ring: 64 KB for a workgroup, two of which share a CU, or 32 KB
+// with heads of 64, of which three do: of 24 sequences of 300 to 5000 keys 37 instead
+// of 41 us, of 200 up to 1000 keys 76 instead of 94 (16 heads each), one long one 3 % more.
+// Four workgroups, or three with 48 KB, took up to 6 % more than three with 32.
 template <int D>
-constexpr int few_steps() { return 256 / D; }
+constexpr int few_steps() { return D == 256 ? 1 : 2; }
 template <int D>
 constexpr int few_ring() { return few_steps<D>() * 2 * 16 * D * 2; }
 template <int D>
@@ -1202,7 +1205,8 @@ AttentionPlan attention_plan(int64_t tokens, int64_t sequences, int64_t q_heads,
   p.tile = max_new * group > kFewRows;
   p.few = group <= kFewRows && !(p.tile && sequences == 1);  // one sequence: one of them
   if (p.few) {
-    p.shares = 512 / kv_heads > 1 ? 512 / kv_heads : 1;
+    const int64_t all = head_dim == 64 ? 768 : 512;  // workgroups that run at a time
+    p.shares = all / kv_heads > 1 ? all / kv_heads : 1;
     p.few_grid = p.shares * kv_heads;
     p.few_rows = 2 * p.shares * kv_heads * kFewRows;
     p.parts = sequences * kv_heads;

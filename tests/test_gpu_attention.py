@@ -413,7 +413,7 @@ def long_cache(dev, heads, keys, dim, seed):
     return kp, vp, table
 
 
-@pytest.mark.parametrize('new,heads,keys,dim', [(2, 128, 18000, 64), (1, 128, 9000, 256),
+@pytest.mark.parametrize('new,heads,keys,dim', [(2, 128, 18000, 64), (2, 128, 27000, 64), (1, 128, 9000, 256),
                                                 (20, 128, 10000, 64), (20, 128, 4700, 256)])
 def test_attention_long_parts(dev, new, heads, keys, dim):
     """Parts of a sequence longer than the pages that a wave looks up at a time: as many heads
