@@ -27,7 +27,7 @@
 //                         heads: 262144 keys of one sequence 88 us (6.1 TB/s), 64
 //                         sequences of 400 to 13000 keys 92 us (5.8 TB/s); 16 heads
 //                         of 64, 24 sequences of 300 to 5000 keys with 2 to 9 rows
-//                         32 us (4.7 TB/s).
+//                         29 us (5.3 TB/s).
 //  attention_tile_kernel  longer ones: bound by the matrix cores and the softmax
 //                         beside them.  128 rows a workgroup, 32 a wave.  Heads of
 //                         256 leave a wave no registers for a second one of its kind
@@ -198,6 +198,34 @@ __device__ __forceinline__ u32x2 read_transposed(const LDS char *tile, int base,
                  (LDS s16x4 *)(tile + swizzled<D, S>(base, row, d / 8))));
 }
 
+// Eight or four such reads at once, waited for here: before the builtin's read the compiler waits
+// for every direct load in flight, which emptied the few-row kernel's rings at each step (24
+// sequences of 300 to 5000 keys, 16 heads of 64: 33 us instead of 37, 64 of 400 to 13000 keys, 8
+// heads of 128: 127 instead of 134).  The tiles keep the builtin: their loads are due by then,
+// and reads waited for in groups took 4 % more there.
+template <int OFFSET>
+__device__ __forceinline__ void read_transposed8(u32x2 (&v)[8], const LDS char *const (&at)[8]) {
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8 offset:%16\n\tds_read_b64_tr_b16 %1, %9 offset:%16\n\t"
+      "ds_read_b64_tr_b16 %2, %10 offset:%16\n\tds_read_b64_tr_b16 %3, %11 offset:%16\n\t"
+      "ds_read_b64_tr_b16 %4, %12 offset:%16\n\tds_read_b64_tr_b16 %5, %13 offset:%16\n\t"
+      "ds_read_b64_tr_b16 %6, %14 offset:%16\n\tds_read_b64_tr_b16 %7, %15 offset:%16\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]),
+        "=&v"(v[6]), "=&v"(v[7])
+      : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "v"(at[4]), "v"(at[5]), "v"(at[6]),
+        "v"(at[7]), "n"(OFFSET)
+      : "memory");
+}
+__device__ __forceinline__ void read_transposed4(u32x2 (&v)[4], const LDS char *const (&at)[4]) {
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %5\n\t"
+      "ds_read_b64_tr_b16 %2, %6\n\tds_read_b64_tr_b16 %3, %7\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3])
+      : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3])
+      : "memory");
+}
+
 // Keeps a lane's base from being expanded into one register for every constant part.
 __device__ __forceinline__ int opaque(int v) {
   asm volatile("" : "+v"(v));
@@ -335,9 +363,9 @@ __device__ Spans find_span(const Attention &a, int index, int64_t *scratch, Find
 constexpr int kFewWaves = 4;
 
 // Steps of 16 keys in a wave's ring: 64 KB for a workgroup, two of which share a CU, or 32 KB
-// with heads of 64, of which three do: of 24 sequences of 300 to 5000 keys 37 instead
-// of 41 us, of 200 up to 1000 keys 76 instead of 94 (16 heads each), one long one 3 % more.
-// Four workgroups, or three with 48 KB, took up to 6 % more than three with 32.
+// with heads of 64, of which three do: of 24 sequences of 300 to 5000 keys 33 instead of 37 us,
+// of 200 up to 1000 keys 69 instead of 77 (16 heads each), one of 100000 keys 25 instead of
+// 23.5.  Four workgroups, or three with 48 KB, took 1 to 5 % more than three with 32.
 template <int D>
 constexpr int few_steps() { return D == 256 ? 1 : 2; }
 template <int D>
@@ -392,25 +420,37 @@ __device__ __forceinline__ u32x2 few_scores(const LDS char *kt, const u32x4 (&q)
   return u32x2{T::pack2(x[0], x[1]), T::pack2(x[2], x[3])};
 }
 
+// The values of a 16-key step as operands, 16 channels each.
+template <int D>
+__device__ __forceinline__ void few_operands(const LDS char *vt, u32x2 (&v)[D / 16], int lane) {
+  const int base = opaque(transpose_base<D, kRows>((lane >> 4) * 4, 0, lane));
+  constexpr int N = D == 64 ? 4 : 8;
+  const LDS char *at[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) at[i] = vt + swizzled<D, kRows>(base, 0, i * 2);
+  if constexpr (D == 64) {
+    read_transposed4(v, at);
+  } else {
+    read_transposed8<0>(*reinterpret_cast<u32x2(*)[8]>(&v[0]), at);
+    if constexpr (D == 256) read_transposed8<256>(*reinterpret_cast<u32x2(*)[8]>(&v[8]), at);
+  }
+}
+
 // Adds the weighted values of a 16-key step; `mixed`: some row does not see all its keys.
 template <typename T, int D>
 __device__ __forceinline__ void few_values(const LDS char *vt, u32x2 p, bool mixed,
                                            FewState<D> &st, int lane) {
-  const int base = opaque(transpose_base<D, kRows>((lane >> 4) * 4, 0, lane));
+  u32x2 v[D / 16];
+  few_operands<D>(vt, v, lane);
   if (mixed) {
     uint32_t any = 0;
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      const u32x2 v = read_transposed<D, kRows>(vt, base, 0, i * 16);
-      st.o[i] = mfma16k16(T{}, u32x2{Pair<T>::finite(v[0], any), Pair<T>::finite(v[1], any)}, p,
-                          st.o[i]);
-    }
+    for (int i = 0; i < D / 16; ++i)
+      v[i] = u32x2{Pair<T>::finite(v[i][0], any), Pair<T>::finite(v[i][1], any)};
     st.odd |= __any(any != 0);
-    return;
   }
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i)
-    st.o[i] = mfma16k16(T{}, read_transposed<D, kRows>(vt, base, 0, i * 16), p, st.o[i]);
+  for (int i = 0; i < D / 16; ++i) st.o[i] = mfma16k16(T{}, v[i], p, st.o[i]);
 }
 
 // The keys of a wave: steps of 16 keys, `stride` steps apart, and the pages they lie in.
