@@ -36,8 +36,9 @@
 //                         four waves on 32-key tiles.  Two tiles in LDS, one read
 //                         and one loaded.  Few tiles split their keys over workgroups
 //                         too.  2048 tokens of 16 heads of 256 (2 key-value heads)
-//                         behind 8192 keys: 322 to 339 us, 911 to 960 TFLOP/s (1371
-//                         for a large library product); without a history 70 us.
+//                         behind 8192 keys: 293 to 302 us in a long run of calls,
+//                         1024 to 1054 TFLOP/s (1371 for a large library product);
+//                         without a history 64 us.
 //  attention_combine_kernel  joins the parts of split keys, 4 to 12 us: the partial
 //                         sums are fp32, written and read once.
 #include <cmath>
