@@ -4,8 +4,9 @@
 //
 // causal at the end of the sequence, times sigmoid(gate_t) where a gate is given;
 // a row without a visible key is 0.  One pass over the keys with a running m and
-// sum (exponentials in base 2, fp32); m follows the maximum only when that has
-// grown by more than 2^kSlack, so the accumulated rows are rarely rescaled.
+// sum (exponentials in base 2, fp32); m follows the maximum (in fp16 2^kLift below
+// it) only when that has grown by more than 2^kSlack, so the accumulated rows are
+// rarely rescaled.
 //
 // Both kernels form the transposed products.  S^T = K Q^T leaves a lane with one
 // query (its column) and a few consecutive keys, so a column's statistics are the
@@ -81,7 +82,12 @@ struct Attention {
 };
 
 constexpr int kFewRows = 16;    // columns of the few-row kernel
-constexpr float kSlack = 8.0f;  // weights stay below 2^8: exact sums in fp32, finite in fp16
+constexpr float kSlack = 8.0f;  // weights stay below 2^(8 + kLift)
+// How far m stays below the maximum.  fp16 ends at 2^-24: with weights of at most 1 a tail of keys
+// 2^-25 below one of them is lost from the products, but not from the sum of the weights; 2^7 more
+// keeps it to 2^-32, and the largest weight at 2^15, finite in fp16.  bf16 has fp32's exponents.
+template <typename T>
+constexpr float kLift = __is_same(T, FP16) ? 7.0f : 0.0f;
 
 __device__ __forceinline__ f32x4 mfma16(BF16, u32x4 a, u32x4 b, f32x4 c) {
   return BF16::mfma16x16x32(a, b, c);
@@ -404,7 +410,7 @@ __device__ __forceinline__ u32x2 few_scores(const LDS char *kt, const u32x4 (&q)
     x[i] = key0 + g * 4 + i < limit ? s[0][i] + s[1][i] : -INFINITY;
     mx = fmaxf(mx, x[i]);
   }
-  mx = across32(across16(mx, Max()), Max()) * scale2;
+  mx = __builtin_fmaf(across32(across16(mx, Max()), Max()), scale2, -kLift<T>);
   if (__any(mx > st.m + kSlack)) {
     const float n = fmaxf(st.m, mx), keep = decay(st.m, n);
     st.m = n;
@@ -973,7 +979,7 @@ __device__ __forceinline__ void tile_step(const LDS char *kt, const LDS char *vt
   float mx = x[0];
 #pragma unroll
   for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
-  mx = across32(mx, Max()) * scale2;
+  mx = __builtin_fmaf(across32(mx, Max()), scale2, -kLift<T>);
   if (__any(mx > st.m + kSlack)) {
     const float n = fmaxf(st.m, mx), keep = decay(st.m, n);
     st.m = n;

@@ -518,3 +518,39 @@ def test_attention_unequal_tiles(dev, sequences, longest, dim):
         n = longest if i % 17 == 3 else int(torch.randint(1, 120, (1,), generator=gen))
         lens.append((min(n, 10 + i % 13), n))
     attend(dev, lens, 16, 6, 2, dim, BF16, gate=True, pad=1, seed=longest)
+
+
+@pytest.mark.parametrize('dim', [64, 128, 256])
+@pytest.mark.parametrize('new,past,sink', [(1, 3000, 0), (1, 3000, 1500), (3, 2000, 5), (40, 2000, 0),
+                                           (150, 4000, 700)])
+def test_attention_fp16_tails_of_small_weights(dev, new, past, sink, dim):
+    """One key far above the rest, whose own values are 0: the result is the others' weights, which
+    are 2^-25 of the largest.  They stay apart from 0 although fp16 ends at 2^-24.
+
+    attention()'s fp16 tolerance takes a weight as off by half of fp16's smallest step, 2^-25, in a
+    sum of at least 1.  The kernels' weights are 2^7 times as large, so that half step is 2^-32 of
+    the sum: that is what a value counts for here."""
+    gen = seeded(dim + new)
+    n = past + new
+    starts, lengths, table, pages = U.batch([(new, n)], 64, dim)
+    q, kp, vp = torch.zeros(new, 4, dim), torch.zeros(pages, 2, 64, dim), torch.zeros(pages, 2, 64, dim)
+    q[..., 0] = 4.0
+    vp[:] = 1.0 + 0.25 * torch.randn(vp.shape, generator=gen)
+    at = int(table[0, sink // 64])
+    kp[at, 0, sink % 64, 0], kp[at, 1, sink % 64, 0] = 17.25 / 4, 17.5 / 4  # 2^-24.9 and 2^-25.2
+    vp[at, :, sink % 64] = 0
+    q, kp, vp = q.to(FP16), kp.to(FP16), vp.to(FP16)
+    for extra in (0, 1):  # alone, and beside a sequence of its own length
+        if extra:
+            starts = torch.tensor([0, new, new + 1], dtype=torch.int32)
+            lengths, table = torch.tensor([n, n], dtype=torch.int32), table.expand(2, -1)
+            q = torch.cat([q, q[-1:]])
+        got = A.paged_attention(*to(dev, q, kp, vp, starts, lengths, table), scale=1.0)
+        ref, slack = U.attention(q, kp, vp, starts, lengths, table, 1.0)
+        sums = [U.gather(vp, table[0], n, 64, h).double().abs().cumsum(0) for h in range(2)]
+        for t in range(new + extra):
+            seen = past + min(t, new - 1)
+            for h in range(4):
+                slack[t, h] -= (2.0 ** -25 - 2.0 ** -32) * sums[h // 2][seen]
+        assert (slack > 0).all()
+        U.assert_attention(got, (ref, slack), f'{new} {past} {sink} {dim}')
