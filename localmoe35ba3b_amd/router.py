@@ -45,10 +45,14 @@ def router_topk(hidden, weight, top_k, bias=None):
 
 def rmsnorm(x, weight=None, eps=1e-6):
     """Qwen3_5MoeRMSNorm (HF:801-815): bf16(x * rsqrt(mean(x^2) + eps) * (1 + w))."""
+    if not x.is_cuda or x.dtype != torch.bfloat16:
+        raise ValueError('rmsnorm expects CUDA bf16 rows')
     x = x.contiguous()
     out = torch.empty_like(x)
     n = x.shape[-1]
     if weight is not None:
+        if weight.numel() != n:
+            raise ValueError('norm weight does not match the rows')
         weight = weight.to(device=x.device, dtype=torch.float32).contiguous()
     _lib.call('lm_rmsnorm', x.data_ptr(), _lib.ptr(weight), out.data_ptr(), x.numel() // n, n,
               float(eps), _lib.stream(x.device))

@@ -1,0 +1,65 @@
+"""CPU checks of the attention block and of the norm before it: what is refused before
+anything is launched."""
+import pytest
+import torch
+
+from localmoe35ba3b_amd import _lib, router
+from localmoe35ba3b_amd.runtime.attention import AttentionBlock, Batch
+from tests.test_attention_checks import gpu
+
+F32, I32, FP16, H = torch.float32, torch.int32, torch.float16, 256
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """The names of the entry points that are called; nothing is launched."""
+    got = []
+    monkeypatch.setattr(_lib, 'call', lambda name, *args: got.append(name))
+    monkeypatch.setattr(_lib, 'launch', lambda device, name, *args: got.append(name))
+    monkeypatch.setattr(_lib, 'stream', lambda device=None: 0)
+    return got
+
+
+def block(**change):
+    a = dict(q_heads=4, kv_heads=2, head_dim=64, gated=False)
+    a.update(change)
+    rows = (a['q_heads'] * (2 if a['gated'] else 1) + 2 * a['kv_heads']) * a['head_dim']
+    wide = a['q_heads'] * a['head_dim']
+    qkv = {'q': gpu(rows, H, dtype=torch.int8), 'scale': gpu(rows, H // 128, dtype=F32)}
+    o = {'q': gpu(H, wide, dtype=torch.int8), 'scale': gpu(H, wide // 128, dtype=F32)}
+    return AttentionBlock(qkv, o, **a)
+
+
+def pages(b, dtype=torch.bfloat16):
+    b.k_pages, b.v_pages = gpu(3, 2, 16, 64, dtype=dtype), gpu(3, 2, 16, 64, dtype=dtype)
+    return b
+
+
+def batch(**change):
+    a = dict(starts=gpu(2, dtype=I32), lengths=gpu(1, dtype=I32), table=gpu(1, 3, dtype=I32))
+    a.update(change)
+    return Batch(**a)
+
+
+@pytest.mark.parametrize('x,weight', [
+    (gpu(5, H, dtype=FP16), None), (gpu(5, H, dtype=F32), None),
+    (torch.zeros(5, H, dtype=torch.bfloat16), None),
+    (gpu(5, H), gpu(H - 1, dtype=F32)), (gpu(5, H), gpu(2 * H, dtype=F32))])
+def test_rmsnorm_refusals(calls, x, weight):
+    """Rows of other types would be read as bf16, host memory and weights that are too short by
+    the GPU."""
+    router.rmsnorm(gpu(5, H), gpu(H, dtype=F32))
+    router.rmsnorm(gpu(5, H))
+    assert calls == ['lm_rmsnorm'] * 2
+    with pytest.raises(ValueError, match='rows'):
+        router.rmsnorm(x, weight)
+    assert len(calls) == 2
+
+
+@pytest.mark.parametrize('h', [gpu(5, H, dtype=FP16), torch.zeros(5, H, dtype=torch.bfloat16)])
+@pytest.mark.parametrize('dtype', [torch.bfloat16, FP16])
+def test_block_refuses_rows_that_its_norm_cannot_read(calls, h, dtype):
+    b = pages(block(), dtype)
+    with pytest.raises(ValueError, match='bf16'):
+        b.forward_(h, batch())
+    assert not calls
