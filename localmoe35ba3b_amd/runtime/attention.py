@@ -50,7 +50,12 @@ class AttentionBlock:
         self.k_pages = self.v_pages = None
 
     def allocate(self, pages, page_size=64, dtype=torch.bfloat16):
-        """An empty cache of `pages` pages for this layer."""
+        """An empty cache of `pages` pages for this layer, of bf16 like the rows that forward_
+        takes."""
+        if dtype is not torch.bfloat16:
+            raise ValueError('the block appends bf16 keys and values')
+        if not 16 <= page_size <= 1024 or page_size & (page_size - 1):
+            raise ValueError('page size must be a power of two from 16 to 1024')
         shape = (pages, self.kv_heads, page_size, self.head_dim)
         device = self.qkv['q'].device
         self.k_pages = torch.empty(shape, dtype=dtype, device=device)

@@ -63,3 +63,25 @@ def test_block_refuses_rows_that_its_norm_cannot_read(calls, h, dtype):
     with pytest.raises(ValueError, match='bf16'):
         b.forward_(h, batch())
     assert not calls
+
+
+@pytest.mark.parametrize('dtype', [FP16, F32])
+def test_allocate_refuses_types_that_the_block_never_writes(dtype):
+    """The block's rows are bf16, so are the keys and values it appends."""
+    with pytest.raises(ValueError, match='bf16'):
+        block().allocate(3, 16, dtype=dtype)
+    with pytest.raises(ValueError, match='bf16'):
+        block().allocate(3, 16, dtype)
+
+
+@pytest.mark.parametrize('size', [0, 8, 24, 2048])
+def test_allocate_refuses_pages_that_the_operators_do(size):
+    with pytest.raises(ValueError, match='page size'):
+        block().allocate(3, size)
+
+
+def test_allocate():
+    b = block().allocate(3, 16, torch.bfloat16)
+    assert b.k_pages.shape == b.v_pages.shape == (3, 2, 16, 64)
+    assert b.k_pages.dtype == b.v_pages.dtype == torch.bfloat16
+    assert block().allocate(2).k_pages.shape == (2, 2, 64, 64)
