@@ -334,22 +334,24 @@ class MoEStack:
         kept = [{l: torch.cuda.Event() for l in self.attention} for _ in starts]
         # chained layers need a workspace per chunk (two chunks, two workspaces)
         chain = len(starts) == 2
-        for l in range(self.L):
-            for c, c0 in enumerate(starts):
-                st = streams[c % 2]
-                with torch.cuda.stream(st):
-                    if c and l:
-                        st.wait_event(done[c - 1][l - 1])
-                    if l in self.attention:
-                        if c:
-                            st.wait_event(kept[c - 1][l])
-                        self.attention[l].forward_(h[c0:c0 + chunk], batches[c])
-                        kept[c][l].record(st)
-                    self.layer_forward(h[c0:c0 + chunk], l, workspace=spaces[c % 2], beside=chunk,
-                                       **self._chained(l, self.L, chain))
-                    done[c][l].record(st)
-        cur.wait_stream(self._side)
-        self._done_events = done, kept, batches  # kept alive until the next call
+        try:
+            for l in range(self.L):
+                for c, c0 in enumerate(starts):
+                    st = streams[c % 2]
+                    with torch.cuda.stream(st):
+                        if c and l:
+                            st.wait_event(done[c - 1][l - 1])
+                        if l in self.attention:
+                            if c:
+                                st.wait_event(kept[c - 1][l])
+                            self.attention[l].forward_(h[c0:c0 + chunk], batches[c])
+                            kept[c][l].record(st)
+                        self.layer_forward(h[c0:c0 + chunk], l, workspace=spaces[c % 2],
+                                           beside=chunk, **self._chained(l, self.L, chain))
+                        done[c][l].record(st)
+        finally:  # after a refusal too: what is queued there writes the caller's rows
+            cur.wait_stream(self._side)
+            self._done_events = done, kept, batches  # kept alive until the next call
         return h
 
     def _chunk_batches(self, batch, tokens, chunk):
