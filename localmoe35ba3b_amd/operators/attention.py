@@ -61,13 +61,21 @@ def _weight(w, dim, device):
     return w, at
 
 
-def _frequencies(inv_freq, dim, device):
-    """fp32 frequencies on the device, their address (0: no rotation), and how many."""
+def check_frequencies(inv_freq, dim):
+    """The rotated pairs of heads of `dim`, 0 without a rotation; raises where the operators do."""
     if inv_freq is None:
-        return None, 0, 0
+        return 0
     pairs = inv_freq.numel()
     if pairs < 8 or pairs % 8 or 2 * pairs > dim:
         raise ValueError('rotated channels must be a multiple of 16 and fit the head')
+    return pairs
+
+
+def _frequencies(inv_freq, dim, device):
+    """fp32 frequencies on the device, their address (0: no rotation), and how many."""
+    pairs = check_frequencies(inv_freq, dim)
+    if not pairs:
+        return None, 0, 0
     if (inv_freq.dtype is not torch.float32 or inv_freq.get_device() != device
             or not inv_freq.is_contiguous()):
         inv_freq = inv_freq.to(device=device, dtype=torch.float32).contiguous()
@@ -131,6 +139,15 @@ def _batch(device, starts, lengths, table):
         raise ValueError('starts, lengths and the rows of the page table must be contiguous')
     return (starts.data_ptr(), lengths.data_ptr(), table.data_ptr(),
             stride if sequences > 1 else shape[1], shape[1], sequences)
+
+
+def check_batch(rows, k_pages, v_pages, starts, lengths, table):
+    """Raises where append and paged_attention refuse these for new rows of this type and device,
+    for a program that runs several operators and wants to know before the first; returns the
+    cache's (kv_heads, head_dim)."""
+    _, _, heads, _, dim = _cache(k_pages, v_pages, rows.dtype, rows.get_device())
+    _batch(rows.get_device(), starts, lengths, table)
+    return heads, dim
 
 
 def append(k_pages, v_pages, k, v, starts, lengths, table, inv_freq=None, k_weight=None, q=None,

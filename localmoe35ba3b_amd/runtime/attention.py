@@ -47,6 +47,17 @@ class AttentionBlock:
         if (qkv['q'].shape[0] != self.q_width + 2 * self.kv_width
                 or o['q'].shape[1] != q_heads * head_dim or o['q'].shape[0] != qkv['q'].shape[1]):
             raise ValueError('the projections do not match the heads')
+        # what the operators would refuse in every step
+        for bank in (qkv, o):
+            if tuple(bank['scale'].shape) != (bank['q'].shape[0], bank['q'].shape[1] // 128):
+                raise ValueError('the scales do not match their projection')
+        if head_dim not in (64, 128, 256) or kv_heads < 1 or q_heads % kv_heads:
+            raise ValueError('expected heads of 64, 128 or 256, and query heads a multiple of '
+                             'key-value heads')
+        for w, n in ((norm, qkv['q'].shape[1]), (q_norm, head_dim), (k_norm, head_dim)):
+            if w is not None and w.numel() != n:
+                raise ValueError('norm weight does not match its rows')
+        attention.check_frequencies(inv_freq, head_dim)
         self.k_pages = self.v_pages = None
 
     def allocate(self, pages, page_size=64, dtype=torch.bfloat16):
@@ -62,11 +73,30 @@ class AttentionBlock:
         self.v_pages = torch.empty(shape, dtype=dtype, device=device)
         return self
 
-    def forward_(self, h, batch):
-        """h [T, H] bf16, updated in place: h += block(h); the new tokens' keys and values join
-        the cache.  Rows of no sequence stay as they are."""
+    def check(self, h, batch):
+        """Raises for rows h, a batch and a cache that forward_ refuses."""
+        self._check_rows(h, batch)
+        if (not h.is_cuda or h.dtype is not torch.bfloat16
+                or h.shape[1] != self.qkv['q'].shape[1]):
+            raise ValueError('expected CUDA bf16 rows [tokens, hidden]')
+        shape = attention.check_batch(h, self.k_pages, self.v_pages, *batch[:3])
+        if shape != (self.kv_heads, self.head_dim):
+            raise ValueError('the pages do not match the heads')
+
+    def _check_rows(self, h, batch):
+        """Of that, what the operators before the append would not find."""
         if self.k_pages is None:
             raise RuntimeError('allocate() the pages of the attention layers first')
+        if h.ndim != 2:
+            raise ValueError('expected rows [tokens, hidden]')
+        if batch.max_new is not None and batch.max_new < 0:
+            raise ValueError('invalid number of new tokens')
+
+    def forward_(self, h, batch):
+        """h [T, H] bf16, updated in place: h += block(h); the new tokens' keys and values join
+        the cache.  Rows of no sequence stay as they are.  Nothing is written before a call is
+        refused."""
+        self._check_rows(h, batch)
         tokens, dim = h.shape[0], self.head_dim
         x = int8.linear(router.rmsnorm(h, self.norm, self.eps), self.qkv['q'], self.qkv['scale'])
         q, k, v = x.split([self.q_width, self.kv_width, self.kv_width], dim=1)

@@ -262,16 +262,33 @@ class MoEStack:
         attention block run it first, on the sequences of `batch`
         (runtime.attention.Batch)."""
         n = self.L if layers is None else layers
-        self._check_batch(batch, n)
+        if self._check_attention(h, batch, n, h.shape[0]) and workspace is not None and (
+                workspace.numel() < _lib.lib().lm_moe_workspace_bytes(h.shape[0], self.H, self.I,
+                                                                      self.E, self.K)):
+            raise MemoryError('workspace too small for this token count')
         for l in range(n):
             if l in self.attention:
                 self.attention[l].forward_(h, batch)
             self.layer_forward(h, l, workspace=workspace, **self._chained(l, n, chain))
         return h
 
-    def _check_batch(self, batch, layers):
-        if batch is None and any(l < layers for l in self.attention):
+    def _check_attention(self, h, batch, layers, tokens):
+        """Whether the first `layers` layers have attention blocks.  If so, raises here what they
+        or the MoE blocks (on `tokens` rows at a time) refuse: a block writes h and its cache
+        before the layers behind it look at h."""
+        blocks = [b for l, b in self.attention.items() if l < layers]
+        if not blocks:
+            return False
+        if batch is None:
             raise ValueError('layers with attention need the batch of their sequences')
+        if h.dtype != torch.bfloat16 or not h.is_contiguous() or h.shape[-1] != self.H:
+            raise ValueError('expected contiguous bf16 [tokens, 2048] hidden states')
+        if tokens > self.max_tokens:
+            raise MemoryError('token count exceeds the workspace of this stack')
+        self.check_tiles()
+        for b in blocks:
+            b.check(h, batch)
+        return True
 
     def _chained(self, l, n, chain):
         """layer_forward's chain arguments: attention between two layers changes the rows that
@@ -311,12 +328,12 @@ class MoEStack:
             raise ValueError('chunk must be positive')
         if min(chunk, h.shape[0]) > self.max_tokens:  # before anything is queued
             raise MemoryError('token count exceeds the workspace of this stack')
-        self._check_batch(batch, self.L)
+        attends = self._check_attention(h, batch, self.L, min(chunk, h.shape[0]))
         starts = list(range(0, h.shape[0], chunk))
         if not starts:  # no tokens: nothing to queue, no second workspace
             return h
-        batches = self._chunk_batches(batch, h.shape[0], chunk) if self.attention else [None] * len(
-            starts)
+        batches = (self._chunk_batches(batch, h.shape[0], chunk) if attends else
+                   [None] * len(starts))
         if not overlap or len(starts) == 1:
             for c0, part in zip(starts, batches):
                 self.forward(h[c0:c0 + chunk], batch=part)

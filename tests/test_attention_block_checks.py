@@ -85,3 +85,46 @@ def test_allocate():
     assert b.k_pages.shape == b.v_pages.shape == (3, 2, 16, 64)
     assert b.k_pages.dtype == b.v_pages.dtype == torch.bfloat16
     assert block().allocate(2).k_pages.shape == (2, 2, 64, 64)
+
+
+@pytest.mark.parametrize('change,message', [
+    (dict(q_heads=3), 'heads'), (dict(head_dim=32, q_heads=8), 'heads of'),
+    (dict(norm=gpu(H + 1, dtype=F32)), 'norm'), (dict(q_norm=gpu(32, dtype=F32)), 'norm'),
+    (dict(k_norm=gpu(65, dtype=F32)), 'norm'), (dict(inv_freq=gpu(12, dtype=F32)), 'multiple of 16'),
+    (dict(inv_freq=gpu(40, dtype=F32)), 'multiple of 16')])
+def test_blocks_that_could_not_run_are_refused(change, message):
+    """What the operators would refuse in every step."""
+    block(norm=gpu(H, dtype=F32), q_norm=gpu(64, dtype=F32), k_norm=gpu(64, dtype=F32),
+          inv_freq=gpu(32, dtype=F32))
+    with pytest.raises(ValueError, match=message):
+        block(**change)
+
+
+def test_projections_without_their_scales_are_refused():
+    a = block()
+    for name in ('qkv', 'o'):
+        bank = {'q': getattr(a, name)['q'], 'scale': getattr(a, name)['scale'][:, :1]}
+        pair = {'qkv': a.qkv, 'o': a.o, name: bank}
+        with pytest.raises(ValueError, match='scales'):
+            AttentionBlock(pair['qkv'], pair['o'], 4, 2, 64, gated=False)
+
+
+@pytest.mark.parametrize('h', [gpu(1, 5, H), gpu(5, H + 128), gpu(H)])
+def test_block_refuses_other_rows(calls, h):
+    for run in (pages(block()).forward_, pages(block()).check):
+        with pytest.raises(ValueError):
+            run(h, batch())
+    assert 'lm_paged_append' not in calls
+
+
+@pytest.mark.parametrize('change', [dict(max_new=-1), dict(starts=gpu(2, dtype=torch.int64)),
+                                    dict(table=gpu(2, 3, dtype=I32))])
+def test_block_refuses_batches_before_it_appends(calls, change):
+    b = pages(block())
+    with pytest.raises(ValueError):
+        b.forward_(gpu(5, H), batch(**change))
+    assert 'lm_paged_append' not in calls
+    calls.clear()
+    b.forward_(gpu(5, H), batch())
+    assert calls == ['lm_rmsnorm', 'lm_w8a16_linear', 'lm_paged_append', 'lm_paged_attention',
+                     'lm_w8a16_linear']

@@ -201,3 +201,30 @@ def test_stack_without_rows(dev, stack):
     """A step of no token passes through the attention blocks."""
     batch = Batch(ints(dev, 0, 0), ints(dev, 5), ints(dev, [0]), 1)
     assert stack.attention[0].forward_(prompt(dev, 0, 1), batch).shape == (0, H)
+
+
+def test_stack_refuses_before_it_writes(dev, stack):
+    """Calls that one of the layers would refuse leave the rows and every cache as they were."""
+    table, x = ints(dev, [5, 0, 2, 7, 1, 4, 6]), prompt(dev, 70, 9)
+    caches = [t for b in stack.attention.values() for t in (b.k_pages, b.v_pages)]
+    for t in caches:
+        t.normal_()
+    before, h = [t.clone() for t in caches], x.clone()
+    good = Batch(ints(dev, 0, 70), ints(dev, 70), table)
+    late, stack.attention[1] = block(dev, 1), block(dev, 1)  # without pages
+    try:
+        for run in (lambda b: stack.forward(h[:60], batch=b), lambda b: stack.prefill_(h, 32, batch=b),
+                    lambda b: stack.prefill_(h, 32, overlap=False, batch=b)):
+            with pytest.raises(RuntimeError, match='allocate'):
+                run(good)
+            stack.attention[1] = late.allocate(8, 16)
+            with pytest.raises(ValueError, match='int32'):
+                run(good._replace(lengths=good.lengths.long()))
+            stack.attention[1] = block(dev, 1)
+    finally:
+        del stack.attention[1]
+    with pytest.raises(MemoryError, match='token count'):
+        stack.forward(h, batch=good)
+    torch.cuda.synchronize()
+    assert torch.equal(h, x) and all(torch.equal(a, b) for a, b in zip(caches, before))
+    assert stack.prefill_(h, 32, batch=good) is h and not torch.equal(h, x)
