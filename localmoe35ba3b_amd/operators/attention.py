@@ -37,7 +37,9 @@ def _rows(x, what):
         x = x.contiguous()
         if x.data_ptr() % 16:
             x = x.clone()
-        token, head, _ = x.stride()
+        # not x.stride(): torch calls one token or one head contiguous whatever its stride is
+        _, heads, dim = x.shape
+        token, head = heads * dim, dim
     return x, token, head
 
 

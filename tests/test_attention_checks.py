@@ -213,3 +213,24 @@ def test_c_scale_is_finite(scale, monkeypatch):
     monkeypatch.setattr(_lib, 'launch', launch)
     with pytest.raises(ValueError, match='finite'):
         attend(scale=scale)
+
+
+@pytest.mark.parametrize('tokens,heads', [(1, 4), (1, 1), (5, 1), (2, 4)])
+def test_layouts_of_few_rows(calls, tokens, heads):
+    """A row pitch that the library does not take is copied for one token and one head too, where
+    torch calls the rows contiguous whatever their strides are."""
+    pitched = gpu(tokens, heads * 128 + 4)[:, :heads * 128].view(tokens, heads, 128)
+    wide = gpu(tokens, heads, 132)[..., :128]
+    odd = gpu(heads * 128).as_strided((1, heads, 128), (3, 128, 1))
+    for q in (pitched, wide, odd)[:3 if tokens == 1 else 2]:
+        n, h = q.shape[:2]
+        norm(q=q, k=gpu(n, 2, 128), positions=gpu(n, dtype=I64))
+        args = calls.pop()[1]
+        assert args[0] % 16 == 0 and args[1] % 8 == 0 and args[2] % 8 == 0
+        assert args[1] >= 0 and args[3] == h
+        append(q=q, k=gpu(n, 2, 132)[..., :128], v=gpu(n, 2, 128))
+        args = calls.pop()[1]
+        assert all(args[i] % 8 == 0 for i in (1, 2, 5, 6, 8, 9))
+        attend(q=q.expand(n, 4, 128), gate=wide.expand(n, 4, 128))
+        args = calls.pop()[1]
+        assert all(args[i] % 8 == 0 for i in (1, 2, 3)) and args[0] % 16 == 0
