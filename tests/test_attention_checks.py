@@ -233,4 +233,4 @@ def test_layouts_of_few_rows(calls, tokens, heads):
         assert all(args[i] % 8 == 0 for i in (1, 2, 5, 6, 8, 9))
         attend(q=q.expand(n, 4, 128), gate=wide.expand(n, 4, 128))
         args = calls.pop()[1]
-        assert all(args[i] % 8 == 0 for i in (1, 2, 3)) and args[0] % 16 == 0
+        assert all(args[i] % 8 == 0 for i in (1, 2, 21, 22)) and args[0] % 16 == 0
