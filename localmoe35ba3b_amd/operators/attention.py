@@ -116,14 +116,26 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6):
 def _cache(k_pages, v_pages, dtype, device):
     """(pages, page stride, kv_heads, page_size, head_dim) of a cache."""
     shape, strides = k_pages.shape, k_pages.stride()
-    if len(shape) != 4 or v_pages.shape != shape or v_pages.stride() != strides:
+    if len(shape) != 4 or v_pages.shape != shape:
         raise ValueError('Expected key and value pages [pages, kv_heads, page_size, head_dim]')
     _same(k_pages, dtype, device)
     _same(v_pages, dtype, device)
     pages, heads, size, dim = shape
-    if strides[1:] != (size * dim, dim, 1):
-        raise ValueError('the values of a page must be contiguous')
+    if strides[1:] != (size * dim, dim, 1) or v_pages.stride() != strides:
+        # the stride of a dimension of size 1 is of no consequence
+        strides, other = _page_strides(k_pages), _page_strides(v_pages)
+        if strides != other:
+            raise ValueError('key and value pages must lie alike')
+        if strides[1:] != (size * dim, dim, 1):
+            raise ValueError('the values of a page must be contiguous')
     return pages, strides[0] if pages > 1 else heads * size * dim, heads, size, dim
+
+
+def _page_strides(x):
+    """Strides, of dimensions of size 1 those of contiguous pages."""
+    _, heads, size, dim = x.shape
+    plain = heads * size * dim, size * dim, dim, 1
+    return tuple(p if n == 1 else s for n, s, p in zip(x.shape, x.stride(), plain))
 
 
 def _batch(device, starts, lengths, table):

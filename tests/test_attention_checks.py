@@ -234,3 +234,21 @@ def test_layouts_of_few_rows(calls, tokens, heads):
         attend(q=q.expand(n, 4, 128), gate=wide.expand(n, 4, 128))
         args = calls.pop()[1]
         assert all(args[i] % 8 == 0 for i in (1, 2, 21, 22)) and args[0] % 16 == 0
+
+
+def test_pages_whose_single_dimensions_have_other_strides(calls):
+    """One key-value head, one page: their strides are stepped over by nothing."""
+    one = gpu(6, 16, 1, 128).transpose(1, 2)  # [pages, page, heads, D] with a single head
+    assert one.stride()[1] == 128 and one.is_contiguous()
+    for k, v in ((one, one), (one, gpu(6, 1, 16, 128))):
+        append(k_pages=k, v_pages=v, k=gpu(5, 1, 128), v=gpu(5, 1, 128))
+        attend(k_pages=k, v_pages=v)
+        for _, args in (calls.pop(0), calls.pop(0)):
+            assert (6, 16 * 128, 1, 16, 128) in (args[15:20], args[6:11])
+    first, last = gpu(6, 2, 2, 16, 128)[:1, 0], gpu(3, 2, 16, 128)[2:]
+    attend(k_pages=first, v_pages=last)
+    assert calls.pop()[1][6:11] == (1, 2 * 16 * 128, 2, 16, 128)
+    for k, v in ((gpu(6, 1, 16, 128), gpu(6, 2, 1, 16, 128)[:, 0]),  # pages apart by another pitch
+                 (gpu(6, 1, 32, 128)[:, :, ::2], gpu(6, 1, 32, 128)[:, :, ::2])):
+        with pytest.raises(ValueError, match='pages|contiguous'):
+            attend(k_pages=k, v_pages=v)
