@@ -121,6 +121,8 @@ def _cache(k_pages, v_pages, dtype, device):
     _same(k_pages, dtype, device)
     _same(v_pages, dtype, device)
     pages, heads, size, dim = shape
+    if heads < 1:
+        raise ValueError('Expected pages with key-value heads')
     if strides[1:] != (size * dim, dim, 1) or v_pages.stride() != strides:
         # the stride of a dimension of size 1 is of no consequence
         strides, other = _page_strides(k_pages), _page_strides(v_pages)

@@ -252,3 +252,9 @@ def test_pages_whose_single_dimensions_have_other_strides(calls):
                  (gpu(6, 1, 32, 128)[:, :, ::2], gpu(6, 1, 32, 128)[:, :, ::2])):
         with pytest.raises(ValueError, match='pages|contiguous'):
             attend(k_pages=k, v_pages=v)
+
+
+def test_a_cache_without_heads_is_refused(calls):
+    with pytest.raises(ValueError, match='heads'):
+        attend(k_pages=gpu(6, 0, 16, 128), v_pages=gpu(6, 0, 16, 128))
+    assert not calls
