@@ -345,11 +345,11 @@ int lm_qk_norm_rope(const void *q, int64_t q_token_stride, int64_t q_head_stride
  * position p lives in row p % page_size of page table[s * table_stride +
  * p / page_size], table_pages entries a sequence.  A page holds [kv_heads,
  * page_size, head_dim] values, pages lie page_stride elements apart, page_size
- * is a power of two from 16 to 1024.  Rows of no sequence are not appended and
- * are 0 in q_out; a position outside the table is not written.  Page numbers
- * are clamped into [0, pages).  Rows that one call writes lie in different
- * places (its sequences share no page that it writes).  A call of no sequence
- * writes nothing. */
+ * is a power of two from 16 to 1024, table_pages * page_size at most 2^31 -
+ * 4096.  Rows of no sequence are not appended and are 0 in q_out; a position
+ * outside the table is not written.  Page numbers are clamped into [0, pages).
+ * Rows that one call writes lie in different places (its sequences share no
+ * page that it writes).  A call of no sequence writes nothing. */
 int lm_paged_append(const void *k, int64_t k_token_stride, int64_t k_head_stride,
                     const float *k_weight, const void *v, int64_t v_token_stride,
                     int64_t v_head_stride, const void *q, int64_t q_token_stride,

@@ -59,6 +59,10 @@ __device__ __forceinline__ int64_t paged_page(const PagedBatch &b, int s, int p)
 // A launch has fewer than 2^32 threads; the kernels take at most 256 for a token.
 constexpr int64_t kMaxTokens = 1LL << 24;
 
+// Positions are 32 bits in the kernels, which look up to 1024 past the one they are at (the pages
+// of the next steps, a tile's last keys).
+constexpr int64_t kMaxPositions = (1LL << 31) - 4096;
+
 // Host checks of what the entry points of the paged cache share; LM_OK or the status.
 inline int paged_check(int64_t pages, int64_t page_stride, int64_t kv_heads, int64_t page_size,
                        int64_t head_dim, const void *starts, const void *lengths,
@@ -75,8 +79,7 @@ inline int paged_check(int64_t pages, int64_t page_stride, int64_t kv_heads, int
              LM_EINVAL, "invalid pages");
   LM_REQUIRE(tokens >= 0 && tokens < kMaxTokens, LM_EINVAL, "invalid token count");
   LM_REQUIRE(sequences >= 0 && sequences <= 65536, LM_EINVAL, "invalid number of sequences");
-  LM_REQUIRE(table_pages >= 1 && table_pages * page_size < (1LL << 31) &&
-                 table_stride >= 0,
+  LM_REQUIRE(table_pages >= 1 && table_pages <= kMaxPositions / page_size && table_stride >= 0,
              LM_EINVAL, "invalid page table");
   LM_REQUIRE(tokens == 0 || sequences == 0 || (starts && lengths && table), LM_EINVAL,
              "null pointer");

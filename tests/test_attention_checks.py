@@ -258,3 +258,16 @@ def test_a_cache_without_heads_is_refused(calls):
     with pytest.raises(ValueError, match='heads'):
         attend(k_pages=gpu(6, 0, 16, 128), v_pages=gpu(6, 0, 16, 128))
     assert not calls
+
+
+@pytest.mark.parametrize('entry', PAGED)
+@pytest.mark.parametrize('page,table_pages', [(16, (1 << 27) - 1), (64, (1 << 25) - 1), (1024, (1 << 21) - 1),
+                                              (16, 1 << 60), (1024, 1 << 54)])
+def test_c_tables_that_end_at_32_bits(entry, page, table_pages):
+    """Kernels look up to 1024 positions past the one they are at, in 32 bits: a table that ends
+    closer to 2^31 is refused, and so is one whose positions wrap around in 64 bits."""
+    rc, error = rows_call(entry, page=page, table_pages=table_pages, page_stride=2 * page * 128)
+    assert rc == _lib.LM_EINVAL and 'page table' in error
+    rc, error = rows_call(entry, page=page, table_pages=(1 << 31) // page - 4096 // page, tokens=0,
+                          page_stride=2 * page * 128)
+    assert rc == _lib.LM_OK
