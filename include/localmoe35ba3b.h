@@ -368,8 +368,8 @@ int lm_paged_append(const void *k, int64_t k_token_stride, int64_t k_head_stride
  * rounded once; a row that sees no key is 0, rows of no sequence are left as
  * they were.  q_heads is a multiple of kv_heads; out is contiguous [tokens,
  * q_heads, head_dim], may be q or gate itself and overlaps no other operand.
- * scale is finite.  max_new bounds the new tokens of a sequence (tokens is
- * always right); rows of sequences with more may be left unwritten.  workspace
+ * scale * log2(e) is finite.  max_new bounds the new tokens of a sequence (tokens
+ * is always right); rows of sequences with more may be left unwritten.  workspace
  * holds lm_paged_attention_workspace_bytes (max_keys = table_pages * page_size;
  * 0: none is needed), 16-byte aligned; its contents need no initialization, and
  * calls that overlap need one each.  Nothing that a row does not see reaches its

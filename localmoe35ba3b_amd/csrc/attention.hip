@@ -1353,7 +1353,8 @@ extern "C" int lm_paged_attention(const void *q, int64_t q_token_stride, int64_t
   LM_REQUIRE(q_heads >= 1 && q_heads <= 16384 && q_heads % kv_heads == 0, LM_EINVAL,
              "query heads must be a multiple of key-value heads");
   LM_REQUIRE(max_new >= 0, LM_EINVAL, "invalid number of new tokens");
-  LM_REQUIRE(std::isfinite(scale), LM_EINVAL, "the scale must be finite");
+  const float scale2 = fabsf(scale) * 1.4426950408889634f;
+  LM_REQUIRE(std::isfinite(scale2), LM_EINVAL, "the scale must be finite");
   if (tokens == 0 || sequences == 0) return LM_OK;
   LM_REQUIRE(tokens * q_heads < (1LL << 31), LM_EINVAL, "too many rows");
   LM_REQUIRE(q && k_pages && v_pages && out, LM_EINVAL, "null pointer");
@@ -1385,7 +1386,7 @@ extern "C" int lm_paged_attention(const void *q, int64_t q_token_stride, int64_t
              (int)kv_heads};
   a.tokens = (int)tokens, a.q_heads = (int)q_heads, a.group = (int)(q_heads / kv_heads);
   // A scale of 0 as one too small to matter, so that a masked -inf stays one under it.
-  a.scale2 = fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-30f);
+  a.scale2 = fmaxf(scale2, 1e-30f);
   a.flip = scale < 0.0f ? 0x80008000u : 0u;
   float *ws = static_cast<float *>(workspace);
   return dtype == LM_BF16

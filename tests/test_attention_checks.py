@@ -271,3 +271,9 @@ def test_c_tables_that_end_at_32_bits(entry, page, table_pages):
     rc, error = rows_call(entry, page=page, table_pages=(1 << 31) // page - 4096 // page, tokens=0,
                           page_stride=2 * page * 128)
     assert rc == _lib.LM_OK
+
+
+@pytest.mark.parametrize('scale', [2.4e38, -3e38])
+def test_c_scale_whose_exponent_is_finite(scale, monkeypatch):
+    """The kernels work in powers of two: scale * log2(e) has to be a number too."""
+    test_c_scale_is_finite(scale, monkeypatch)
