@@ -36,20 +36,6 @@ __device__ __forceinline__ PagedSequence paged_sequence(const PagedBatch &b, int
           min(max(len, 0), room)};
 }
 
-// The sequence that row t belongs to, or -1: the last s with starts[s] <= t
-// (sequences without new tokens share their start with the next).
-__device__ __forceinline__ int paged_find(const PagedBatch &b, int t) {
-  int lo = 0, hi = b.sequences;  // starts[lo] <= t < starts[hi], if any
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (b.starts[mid] <= t)
-      lo = mid;
-    else
-      hi = mid;
-  }
-  return b.starts[lo] <= t && t < b.starts[lo + 1] ? lo : -1;
-}
-
 // Element offset of position p's page of sequence s.
 __device__ __forceinline__ int64_t paged_page(const PagedBatch &b, int s, int p) {
   const int i = min(p >> b.page_shift, b.table_pages - 1);
