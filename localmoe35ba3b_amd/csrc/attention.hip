@@ -517,8 +517,9 @@ __device__ __forceinline__ RowPlace row_place(const Attention &a, const PagedSeq
   return {q.first + c / a.group, kv * a.group + c % a.group};
 }
 
-// sigmoid(x) by the hardware's exp2 and reciprocal: (|x| + 4) 2^-24 of it at most, as the
-// exponent's rounding shows in a small result.
+// sigmoid(x) by the hardware's exp2 and reciprocal, off by (1.25 |x| + 5) 2^-24 of it at most: half
+// a step of the exponent (1) and the constant log2(e) in fp32 (0.23) count |x| times in e^-x, then
+// exp2 (2), the sum (1) and the reciprocal (2).  Results below 2^-126 may be 0.
 __device__ __forceinline__ float sigmoid_hw(float x) {
   return __builtin_amdgcn_rcpf(1.0f + exp2_hw(x * -1.4426950408889634f));
 }

@@ -554,3 +554,29 @@ def test_attention_fp16_tails_of_small_weights(dev, new, past, sink, dim):
                 slack[t, h] -= (2.0 ** -25 - 2.0 ** -32) * sums[h // 2][seen]
         assert (slack > 0).all()
         U.assert_attention(got, (ref, slack), f'{new} {past} {sink} {dim}')
+
+
+@TYPES
+@pytest.mark.parametrize('new', [1, 40])
+def test_attention_gates_from_far_to_far(dev, new, dtype):
+    """Values of every mantissa under gates to both ends of their range.  Scores of 0 leave the
+    attention exact but for its exponential (2 steps of 2^-24), the division and a product (a step
+    each); the gate adds (1.25 |x| + 5) steps and a product.  Rounding is monotone: a result lies
+    between the roundings of that interval's ends."""
+    gates = [-87.0, -80.0, -60.5, -45.0, -33.25, -17.0, -9.5, -3.0, -1.0, -0.125, 0.0, 0.3, 2.0, 7.0,
+             20.0, 200.0, math.inf, -200.0, -math.inf]
+    heads, dim = len(gates), 128
+    g = torch.tensor(gates).to(dtype)[None, :, None].expand(new, heads, dim)
+    v = (1 + torch.arange(dim) / dim).to(dtype)
+    pages = torch.zeros(3, 1, 16, dim, dtype=dtype)
+    starts, lengths = torch.tensor([0, new], dtype=torch.int32), torch.tensor([new], dtype=torch.int32)
+    table = torch.tensor([[2, 0, 1]], dtype=torch.int32)
+    q = torch.randn(new, heads, dim, generator=seeded(new)).to(dtype)
+    got = A.paged_attention(*to(dev, q, pages, v.expand_as(pages).contiguous(), starts, lengths, table),
+                            gate=to(dev, g)[0]).cpu()
+    x = g.double()
+    want = v.double() * torch.sigmoid(x)
+    slack = torch.where(x.isinf(), 0.0, (1.25 * x.abs() + 10) * 2.0 ** -24)
+    low, high = (want * (1 - slack)).to(dtype), (want * (1 + slack)).to(dtype)
+    assert ((got >= low) & (got <= high)).all()
+    assert torch.equal(got[:, 16], v.expand(new, dim)) and not got[:, 17:].any()
