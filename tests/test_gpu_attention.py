@@ -580,3 +580,25 @@ def test_attention_gates_from_far_to_far(dev, new, dtype):
     low, high = (want * (1 - slack)).to(dtype), (want * (1 + slack)).to(dtype)
     assert ((got >= low) & (got <= high)).all()
     assert torch.equal(got[:, 16], v.expand(new, dim)) and not got[:, 17:].any()
+
+
+def test_one_token_and_one_head_of_odd_pitch(dev):
+    """One token of rows 260 apart, one head, and pages whose single head was transposed into place
+    give what contiguous copies of them give."""
+    gen = seeded(31)
+    rows = rand(gen, 3, 2 * 128 + 4).to(dev)
+    kv = rand(gen, 3, 128 + 4).to(dev)
+    cache = [rand(gen, 9, 16, 1, 128).to(dev).transpose(1, 2) for _ in range(2)]
+    plain = [c.clone(memory_format=torch.contiguous_format).view(-1).view(9, 1, 16, 128) for c in cache]
+    lengths = torch.tensor([100], dtype=torch.int32)
+    table = torch.tensor([[3, 1, 8, 0, 2, 7, 5]], dtype=torch.int32)
+    for count in (1, 3):
+        batch = to(dev, torch.tensor([0, count], dtype=torch.int32), lengths, table)
+        q = rows[:count, :256].view(count, 2, 128)
+        k = kv[:count, :128].view(count, 1, 128)
+        odd = step(cache, q, k, k, q, None, None, None, batch, count)
+        want = step(plain, *(t.clone(memory_format=torch.contiguous_format) for t in (q, k, k, q)),
+                    None, None, None, batch, count)
+        assert torch.equal(odd, want) and all(torch.equal(a, b) for a, b in zip(cache, plain))
+        a, b = A.qk_norm_rope(q, k, None, None, torch.arange(count, device=dev), None)
+        assert torch.equal(a, q) and torch.equal(b, k)

@@ -228,3 +228,30 @@ def test_stack_refuses_before_it_writes(dev, stack):
     torch.cuda.synchronize()
     assert torch.equal(h, x) and all(torch.equal(a, b) for a, b in zip(caches, before))
     assert stack.prefill_(h, 32, batch=good) is h and not torch.equal(h, x)
+
+
+@pytest.mark.parametrize('tokens,chunk', [(60, 32), (90, 32)])
+def test_stack_prefill_graph(dev, stack, tokens, chunk):
+    """A captured prefill of overlapped chunks, replayed with other rows and another length, with
+    eager work in between."""
+    table = ints(dev, [5, 0, 2, 7, 1, 4, 6])
+    ends, lengths = ints(dev, 0, tokens), ints(dev, tokens)
+    batch = Batch(ends, lengths, table)
+    static = prompt(dev, tokens, 1)
+    stack.prefill_(static, chunk, batch=batch)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        stack.prefill_(static, chunk, batch=batch)
+    for step in range(4):
+        x = prompt(dev, tokens, 30 + step)
+        ends[1] = lengths[0] = tokens - 7 * step  # the rows behind are none of the sequence
+        static.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        after = [t.clone() for b in stack.attention.values() for t in (b.k_pages, b.v_pages)]
+        assert torch.equal(static, stack.prefill(x, chunk, overlap=False, batch=batch))
+        torch.cuda.synchronize()
+        eager = [t for b in stack.attention.values() for t in (b.k_pages, b.v_pages)]
+        # as bits: pages that nothing wrote hold whatever was there, NaN among it
+        assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(after, eager))
