@@ -49,6 +49,8 @@ class AttentionBlock:
             raise ValueError('the projections do not match the heads')
         # what the operators would refuse in every step
         for bank in (qkv, o):
+            if bank['q'].shape[1] % 128:
+                raise ValueError('projections have groups of 128')
             if tuple(bank['scale'].shape) != (bank['q'].shape[0], bank['q'].shape[1] // 128):
                 raise ValueError('the scales do not match their projection')
         if head_dim not in (64, 128, 256) or kv_heads < 1 or q_heads % kv_heads:

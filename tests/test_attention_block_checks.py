@@ -128,3 +128,9 @@ def test_block_refuses_batches_before_it_appends(calls, change):
     b.forward_(gpu(5, H), batch())
     assert calls == ['lm_rmsnorm', 'lm_w8a16_linear', 'lm_paged_append', 'lm_paged_attention',
                      'lm_w8a16_linear']
+
+
+def test_projections_that_int8_linear_refuses():
+    """One head of 64 channels leaves the output projection half a group of 128."""
+    with pytest.raises(ValueError, match='128'):
+        block(q_heads=1, kv_heads=1)
