@@ -48,14 +48,14 @@ class AttentionBlock:
                 or o['q'].shape[1] != q_heads * head_dim or o['q'].shape[0] != qkv['q'].shape[1]):
             raise ValueError('the projections do not match the heads')
         # what the operators would refuse in every step
+        if head_dim not in (64, 128, 256) or kv_heads < 1 or q_heads % kv_heads:
+            raise ValueError('expected heads of 64, 128 or 256, and query heads a multiple of '
+                             'key-value heads')
         for bank in (qkv, o):
             if bank['q'].shape[1] % 128:
                 raise ValueError('projections have groups of 128')
             if tuple(bank['scale'].shape) != (bank['q'].shape[0], bank['q'].shape[1] // 128):
                 raise ValueError('the scales do not match their projection')
-        if head_dim not in (64, 128, 256) or kv_heads < 1 or q_heads % kv_heads:
-            raise ValueError('expected heads of 64, 128 or 256, and query heads a multiple of '
-                             'key-value heads')
         for w, n in ((norm, qkv['q'].shape[1]), (q_norm, head_dim), (k_norm, head_dim)):
             if w is not None and w.numel() != n:
                 raise ValueError('norm weight does not match its rows')
