@@ -48,7 +48,7 @@ class AttentionBlock:
                 or o['q'].shape[1] != q_heads * head_dim or o['q'].shape[0] != qkv['q'].shape[1]):
             raise ValueError('the projections do not match the heads')
         # what the operators would refuse in every step
-        if head_dim not in (64, 128, 256) or kv_heads < 1 or q_heads % kv_heads:
+        if head_dim not in (64, 128, 256) or min(q_heads, kv_heads) < 1 or q_heads % kv_heads:
             raise ValueError('expected heads of 64, 128 or 256, and query heads a multiple of '
                              'key-value heads')
         for bank in (qkv, o):

@@ -134,3 +134,9 @@ def test_projections_that_int8_linear_refuses():
     """One head of 64 channels leaves the output projection half a group of 128."""
     with pytest.raises(ValueError, match='128'):
         block(q_heads=1, kv_heads=1)
+
+
+@pytest.mark.parametrize('heads', [dict(q_heads=0), dict(q_heads=2, kv_heads=0)])
+def test_blocks_without_heads_are_refused(heads):
+    with pytest.raises(ValueError, match='heads'):
+        block(**heads)
