@@ -365,9 +365,12 @@ int lm_paged_append(const void *k, int64_t k_token_stride, int64_t k_head_stride
  * the row at position p of its sequence sees the positions up to p,
  *   o = sum_j softmax_j(scale * q . k_j) v_j, times sigmoid(gate) if gate != NULL
  * in fp32 (the weights rounded to dtype for their product with the values),
- * rounded once; a row that sees no key is 0, rows of no sequence are left as
- * they were.  q_heads is a multiple of kv_heads; out is contiguous [tokens,
- * q_heads, head_dim], may be q or gate itself and overlaps no other operand.
+ * rounded once; a row that sees no key, or only scores of -inf, is 0, rows of no
+ * sequence are left as they were.  Scores are fp32: where |scale * q . k| passes
+ * 2^23, steps of theirs are larger than what a softmax tells apart, and the
+ * weights are not defined.  q_heads is a multiple of kv_heads; out is contiguous
+ * [tokens, q_heads, head_dim], may be q or gate itself and overlaps no other
+ * operand.
  * scale * log2(e) is finite.  max_new bounds the new tokens of a sequence (tokens
  * is always right); rows of sequences with more may be left unwritten.  workspace
  * holds lm_paged_attention_workspace_bytes (max_keys = table_pages * page_size;

@@ -15,8 +15,12 @@
 // from the row-major V tile by the LDS transpose read, four keys of one channel a
 // lane.  K and V go from the cache into LDS by direct loads, whole rows at a time,
 // the 16-byte pieces of a row permuted (swizzle) so that neither read meets a bank
-// conflict.  The weights are rounded to the inputs' type for the second product,
-// their sum is of the unrounded ones in fp32; the result is rounded once.
+// conflict.  The weights are rounded to the inputs' type for the second product, as
+// the matrix cores take both operands of one type and a second product for what the
+// rounding leaves would double it; their sum is of the unrounded ones in fp32, and
+// the result is rounded once.  Against 64 bits a result is off by 0.0018 to 0.0023
+// of the norm in bf16 and 0.00026 in fp16; its own rounding alone is 0.0017 and
+// 0.00021 of that.
 //
 //  attention_few_kernel   sequences of at most 16 rows (new tokens x query heads of
 //                         a key-value head): bound by the cache's bytes.  16-column
