@@ -81,7 +81,8 @@ class AttentionBlock:
         if (not h.is_cuda or h.dtype is not torch.bfloat16
                 or h.shape[1] != self.qkv['q'].shape[1]):
             raise ValueError('expected CUDA bf16 rows [tokens, hidden]')
-        shape = attention.check_batch(h, self.k_pages, self.v_pages, *batch[:3])
+        shape = attention.check_batch(h, self.k_pages, self.v_pages, batch.starts, batch.lengths,
+                                      batch.table)
         if shape != (self.kv_heads, self.head_dim):
             raise ValueError('the pages do not match the heads')
 

@@ -175,3 +175,11 @@ def test_step_in_order(step):
     st.forward(gpu(4, H), batch=batch())
     assert [e[1:] for e in log] == [('attention', 0), ('layer', 0), ('layer', 1), ('attention', 2),
                                     ('layer', 2)]
+
+
+def test_batches_are_read_by_name(step):
+    """A program's own batch object serves as before."""
+    import types
+    st, log = step({0: pages(block())})
+    st.forward(gpu(4, H), batch=types.SimpleNamespace(**batch()._asdict()))
+    assert len(log) == 4
