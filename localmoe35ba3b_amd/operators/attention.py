@@ -210,15 +210,16 @@ def paged_attention(q, k_pages, v_pages, starts, lengths, table, scale=None, gat
     """Attention of the new tokens q [T, q_heads, D] over the cache -> [T, q_heads, D].
 
     The token at position p of its sequence sees the positions up to p; a row that sees none,
-    or only scores of -inf, is 0.  Scores are fp32, and defined up to 2^23.  scale
-    defaults to D ** -0.5; gate [T, q_heads, D] multiplies the result by sigmoid(gate).
-    max_new bounds the new tokens of one sequence (default: T); a close bound saves
-    time, and rows of a sequence with more may be left unwritten.  The table's width counts as
-    a sequence's possible length: for one sequence of few new tokens and few keys, a wide one
+    or only scores of -inf, is 0.  Scores are fp32, and defined up to 2^23.  scale defaults to
+    D ** -0.5; gate [T, q_heads, D] multiplies the result by sigmoid(gate).
+    max_new bounds the new tokens of one sequence (default: T); a close bound saves time, and
+    rows of a sequence with more may be left unwritten.  The table's width counts as a
+    sequence's possible length: for one sequence of few new tokens and few keys, a wide one
     costs time and workspace (128 new tokens alone, 16 heads of 256: 39 us with 262144
-    positions, 17 with 128).  out [T, q_heads, D], contiguous, receives the result, and rows of no sequence
-    keep what they hold there; without it they are 0.  It may be q or the gate itself, and
-    shares no memory with them, or with the cache, in another way."""
+    positions, 17 with 128).
+    out [T, q_heads, D], contiguous, receives the result, and rows of no sequence keep what
+    they hold there; without it they are 0.  It may be q or the gate itself, and shares no
+    memory with them, or with the cache, in another way."""
     q, q_token, q_head = _rows(q, 'queries')
     dtype, device, shape = q.dtype, q.get_device(), q.shape
     pages, stride, heads, size, dim = _cache(k_pages, v_pages, dtype, device)
