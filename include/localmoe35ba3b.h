@@ -85,6 +85,21 @@ int lm_w8_tile_rows(const int8_t *q, int64_t experts, int64_t n, int64_t k,
 int lm_act_quant_g128(const void *x, int x_dtype, int8_t *q, float *s,
                       int64_t rows, int64_t k, void *stream);
 
+/* Rows on their way into a W8A8 product, in one pass: h += x (x NULL: h stays as
+ * it is), then the RMS norm of h, quantized as by lm_act_quant_g128 but from
+ * fp32, without a rounding to the rows' type in between:
+ *   m = h * rsqrt(mean h^2 + eps) * (1 + w)              (w NULL: zeros)
+ *   s = max(amax_g |m|, 1e-10) * (1/127), q = rint(m / s)
+ * h and x [rows, n] of `dtype`, h rounded once after the sum; w fp32 [n]; q int8
+ * [rows, n], s fp32 [rows, n/128].  n is a multiple of 128 up to 16384, rows are
+ * fewer than 2^24; h, x and w are 16-byte aligned.  A row with an infinity or NaN
+ * has scales that are not finite.  x may be h itself and overlaps it in no other
+ * way.  No counterpart in the reference as one call (HF:801-815, 866-875 and
+ * w8a8.py:8-22). */
+int lm_norm_quant_g128(void *h, const void *x, const float *w, int8_t *q,
+                       float *s, int64_t rows, int64_t n, float eps, int dtype,
+                       void *stream);
+
 /* Dense W8A16: y[m, n] = sum_k x[m, k] * dtype(q[n, k] * s[n, k/128]),
  * fp32 accumulation, y in the activation dtype.  The size selects
  * the kernel: the HBM streaming GEMV (one or two rows, and up to 8 where the
@@ -337,6 +352,20 @@ int lm_qk_norm_rope(const void *q, int64_t q_token_stride, int64_t q_head_stride
                     int64_t tokens, int64_t head_dim, float eps, int dtype,
                     void *stream);
 
+/* lm_qk_norm_rope with positions of several axes (time, row and column of images
+ * and video): a = positions[axis[i] * position_stride + t] * inv_freq[i].
+ * positions [axes][tokens], position_stride apart (elements, at least tokens where
+ * axes > 1); axis int32 [pairs], clamped into [0, axes) (NULL: all 0); axes 1 to
+ * 64. */
+int lm_qk_norm_rope_axes(const void *q, int64_t q_token_stride, int64_t q_head_stride,
+                         int64_t q_heads, const float *q_weight, void *q_out,
+                         const void *k, int64_t k_token_stride, int64_t k_head_stride,
+                         int64_t k_heads, const float *k_weight, void *k_out,
+                         const int64_t *positions, int64_t position_stride,
+                         int64_t axes, const int32_t *axis, const float *inv_freq,
+                         int64_t pairs, int64_t tokens, int64_t head_dim, float eps,
+                         int dtype, void *stream);
+
 /* Appends keys and values to a paged cache, the keys normed and rotated on the
  * way as in lm_qk_norm_rope, and gives the queries of the same tokens the same
  * treatment (q_heads 0: none).
@@ -360,6 +389,48 @@ int lm_paged_append(const void *k, int64_t k_token_stride, int64_t k_head_stride
                     const int32_t *table, int64_t table_stride, int64_t table_pages,
                     int64_t sequences, const float *inv_freq, int64_t pairs,
                     int64_t tokens, float eps, int dtype, void *stream);
+
+/* lm_paged_append with the angles of lm_qk_norm_rope_axes: positions count for the
+ * rotation only, the place in the cache is that of the batch (positions NULL: as
+ * lm_paged_append; position_stride, axes and axis are then 0, 1 and NULL). */
+int lm_paged_append_axes(const void *k, int64_t k_token_stride, int64_t k_head_stride,
+                         const float *k_weight, const void *v, int64_t v_token_stride,
+                         int64_t v_head_stride, const void *q, int64_t q_token_stride,
+                         int64_t q_head_stride, int64_t q_heads, const float *q_weight,
+                         void *q_out, void *k_pages, void *v_pages, int64_t pages,
+                         int64_t page_stride, int64_t kv_heads, int64_t page_size,
+                         int64_t head_dim, const int32_t *starts, const int32_t *lengths,
+                         const int32_t *table, int64_t table_stride, int64_t table_pages,
+                         int64_t sequences, const int64_t *positions,
+                         int64_t position_stride, int64_t axes, const int32_t *axis,
+                         const float *inv_freq, int64_t pairs, int64_t tokens, float eps,
+                         int dtype, void *stream);
+
+/* lm_paged_append_axes to a cache in 8 bits: pages hold e4m3 values (sign, four
+ * bits of exponent, three of mantissa, no infinities; page_stride is a multiple of
+ * 16), and scales, fp32 [pages][kv_heads][2][page_size / 16] (pages scale_stride
+ * elements apart; keys, then values), a power of two 2^e for each 16 positions of a
+ * head: a value is its e4m3 times that.
+ * A block that begins in this call gets the least e with amax <= 448 * 2^e over the
+ * rows that the call writes to it (e at least -117 in bf16, -15 in fp16).  A block
+ * that goes on keeps its e if that suffices; otherwise e grows, and the rows held
+ * already are rounded again to e4m3 (which changes only values below 2^-6 of the
+ * new scale).  Rows of a block behind its last position keep their bits.  Values
+ * are rounded once, from fp32; sizes beyond four significant bits of `dtype` (61440
+ * in fp16) are held as that, infinities and NaN as NaN. */
+int lm_paged_append_e4m3(const void *k, int64_t k_token_stride, int64_t k_head_stride,
+                         const float *k_weight, const void *v, int64_t v_token_stride,
+                         int64_t v_head_stride, const void *q, int64_t q_token_stride,
+                         int64_t q_head_stride, int64_t q_heads, const float *q_weight,
+                         void *q_out, void *k_pages, void *v_pages, float *scales,
+                         int64_t scale_stride, int64_t pages, int64_t page_stride,
+                         int64_t kv_heads, int64_t page_size, int64_t head_dim,
+                         const int32_t *starts, const int32_t *lengths,
+                         const int32_t *table, int64_t table_stride, int64_t table_pages,
+                         int64_t sequences, const int64_t *positions,
+                         int64_t position_stride, int64_t axes, const int32_t *axis,
+                         const float *inv_freq, int64_t pairs, int64_t tokens, float eps,
+                         int dtype, void *stream);
 
 /* Attention of the new tokens over the cache (the batch of lm_paged_append):
  * the row at position p of its sequence sees the positions up to p,
@@ -392,6 +463,22 @@ int lm_paged_attention(const void *q, int64_t q_token_stride, int64_t q_head_str
                        int64_t gate_token_stride, int64_t gate_head_stride, void *out,
                        void *workspace, int64_t workspace_bytes, int dtype,
                        void *stream);
+
+/* lm_paged_attention over the cache of lm_paged_append_e4m3, whose keys and values
+ * are e4m3 times the power of two of their block (of a scale only the exponent
+ * counts), exact in dtype as they enter the products.  The workspace is as large as
+ * that of lm_paged_attention. */
+int lm_paged_attention_e4m3(const void *q, int64_t q_token_stride, int64_t q_head_stride,
+                            int64_t q_heads, const void *k_pages, const void *v_pages,
+                            const float *scales, int64_t scale_stride, int64_t pages,
+                            int64_t page_stride, int64_t kv_heads, int64_t page_size,
+                            int64_t head_dim, const int32_t *starts,
+                            const int32_t *lengths, const int32_t *table,
+                            int64_t table_stride, int64_t table_pages, int64_t sequences,
+                            int64_t tokens, int64_t max_new, float scale, const void *gate,
+                            int64_t gate_token_stride, int64_t gate_head_stride, void *out,
+                            void *workspace, int64_t workspace_bytes, int dtype,
+                            void *stream);
 
 /* ---------------------------------------------------------------------
  * Fused MoE-FFN block of the synthetic stack (router + 256 routed experts

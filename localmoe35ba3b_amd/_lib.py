@@ -33,6 +33,7 @@ SIGNATURES = {
     'lm_quantize_weight_g128': (I32, [P, P, P, I64, I64, P]),
     'lm_w8_tile_rows': (I32, [P, I64, I64, I64, I64, P, I32, P]),
     'lm_act_quant_g128': (I32, [P, I32, P, P, I64, I64, P]),
+    'lm_norm_quant_g128': (I32, [P, P, P, P, P, I64, I64, F32, I32, P]),
     'lm_w8a16_linear': (I32, [P, P, P, P, I64, I64, I64, I32, I32, P]),
     'lm_w8a16_linear_form': (I32, [I64, I64, I64, P]),
     'lm_w8a16_grouped_gemv': (I32, [P, P, P, I64, I64, I64, I32, I32, I32, P]),
@@ -63,11 +64,22 @@ SIGNATURES = {
     'lm_rmsnorm': (I32, [P, P, P, I64, I64, F32, P]),
     'lm_qk_norm_rope': (I32, [P, I64, I64, I64, P, P, P, I64, I64, I64, P, P, P, P, I64, I64, I64,
                               F32, I32, P]),
+    'lm_qk_norm_rope_axes': (I32, [P, I64, I64, I64, P, P, P, I64, I64, I64, P, P, P, I64, I64, P,
+                                   P, I64, I64, I64, F32, I32, P]),
     'lm_paged_append': (I32, [P, I64, I64, P, P, I64, I64, P, I64, I64, I64, P, P, P, P, I64, I64,
                               I64, I64, I64, P, P, P, I64, I64, I64, P, I64, I64, F32, I32, P]),
+    'lm_paged_append_axes': (I32, [P, I64, I64, P, P, I64, I64, P, I64, I64, I64, P, P, P, P, I64,
+                                   I64, I64, I64, I64, P, P, P, I64, I64, I64, P, I64, I64, P, P,
+                                   I64, I64, F32, I32, P]),
+    'lm_paged_append_e4m3': (I32, [P, I64, I64, P, P, I64, I64, P, I64, I64, I64, P, P, P, P, P,
+                                   I64, I64, I64, I64, I64, I64, P, P, P, I64, I64, I64, P, I64,
+                                   I64, P, P, I64, I64, F32, I32, P]),
     'lm_paged_attention_workspace_bytes': (I64, [I64, I64, I64, I64, I64, I64, I64]),
     'lm_paged_attention': (I32, [P, I64, I64, I64, P, P, I64, I64, I64, I64, I64, P, P, P, I64,
                                  I64, I64, I64, I64, F32, P, I64, I64, P, P, I64, I32, P]),
+    'lm_paged_attention_e4m3': (I32, [P, I64, I64, I64, P, P, P, I64, I64, I64, I64, I64, I64, P, P,
+                                      P, I64, I64, I64, I64, I64, F32, P, I64, I64, P, P, I64, I32,
+                                      P]),
     'lm_moe_workspace_bytes': (I64, [I64, I64, I64, I64, I64]),
     'lm_moe_workspace_init': (I32, [P, I64, P]),
     'lm_moe_workspace_region': (I32, [I64, I32, P, P]),

@@ -5,7 +5,8 @@
 //   y_i = n_i cos a_i - n_{i+h} sin a_i,  y_{i+h} = n_{i+h} cos a_i + n_i sin a_i
 //   a_i = position * inv_freq_i,  i < h;  channels from 2 h on: y = n
 //
-// in fp32, rounded once.  Positions reach hundreds of thousands, where an fp32
+// where a pair's position is that of its axis, if positions have several (time, row, column).
+// In fp32, rounded once.  Positions reach hundreds of thousands, where an fp32
 // angle is off by a hundredth of a turn: the product of a position and an fp32
 // frequency is exact in fp64, and its turns are reduced there before sine and
 // cosine are taken in fp32.
@@ -30,7 +31,10 @@ struct HeadRows {
   uint16_t *q_out, *k_out;    // [tokens][heads][D]; k_out only without a cache
   uint16_t *k_pages, *v_pages;
   const float *q_w, *k_w, *inv_freq;  // null: no norm, no rotation
-  const int64_t *positions;           // without a cache
+  const int64_t *positions;           // [axes][tokens]; null: by the place in the sequence
+  int64_t position_stride;            // between axes
+  const int32_t *axis;                // of each pair; null: the first
+  int axes;
   PagedBatch batch;
   int tokens, q_heads, k_heads;
   int half;  // rotated pairs
@@ -62,13 +66,27 @@ __device__ __forceinline__ void unpack4(uint2 w, float x[4]) {
   x[2] = T::to_f32(w.y & 0xFFFFu), x[3] = T::to_f32(w.y >> 16);
 }
 
+// Sine and cosine of pair i of token t, at position p unless the call gives positions.
+__device__ __forceinline__ void turn(const HeadRows &a, float freq, int i, int t, int p, float *s,
+                                     float *c) {
+  double position = p;
+  if (a.positions) {
+    const int axis = a.axis ? clamp_index32(a.axis[i], a.axes) : 0;
+    position = (double)a.positions[axis * a.position_stride + t];
+  }
+  constexpr double kTurns = 0.15915494309189533577;  // 1 / (2 pi)
+  const double turns = position * (double)freq * kTurns;
+  sincospif(2.0f * (float)(turns - rint(turns)), s, c);
+}
+
+// The rows of token t.
 template <typename T, int LANES, bool PAGED>
-__global__ __launch_bounds__(256) void head_rows_kernel(HeadRows a) {
+__device__ __forceinline__ void token_rows(const HeadRows &a, int t) {
   constexpr int D = LANES * 8, ROWS = 256 / LANES;
   __shared__ __attribute__((aligned(16))) float cosines[kMaxHalf], sines[kMaxHalf];
   __shared__ int64_t place;  // element offset of the token's row of head 0 in the cache; < 0: none
   __shared__ int found, at;  // the token's sequence and position
-  const int t = blockIdx.x, tid = threadIdx.x, lane = tid % LANES, half = a.half;
+  const int tid = threadIdx.x, lane = tid % LANES, half = a.half;
   const int heads = a.q_heads + a.k_heads + (PAGED ? a.k_heads : 0);
   const bool rotated = lane * 8 < 2 * half;
   const int lo = rotated ? lane * 4 : lane * 8, hi = rotated ? half + lane * 4 : lane * 8 + 4;
@@ -87,7 +105,7 @@ __global__ __launch_bounds__(256) void head_rows_kernel(HeadRows a) {
   for (int i = 0; i < kAhead; ++i) raw[i] = load(r0 + i * ROWS);
   const float freq = tid < half ? a.inv_freq[tid] : 0.0f;
 
-  double position;
+  int position = 0;
   int64_t to = 0;
   if constexpr (PAGED) {
     if (tid == 0) found = -1;
@@ -112,14 +130,8 @@ __global__ __launch_bounds__(256) void head_rows_kernel(HeadRows a) {
                                  : paged_page(a.batch, found, p) +
                                        (int64_t)(p & ((1 << a.batch.page_shift) - 1)) * D;
     }
-  } else {
-    position = (double)a.positions[t];
   }
-  if (tid < half) {
-    constexpr double kTurns = 0.15915494309189533577;  // 1 / (2 pi)
-    const double turns = position * (double)freq * kTurns;
-    sincospif(2.0f * (float)(turns - rint(turns)), &sines[tid], &cosines[tid]);
-  }
+  if (tid < half) turn(a, freq, tid, t, position, &sines[tid], &cosines[tid]);
   __syncthreads();
   if constexpr (PAGED) to = place;
 
@@ -181,6 +193,232 @@ __global__ __launch_bounds__(256) void head_rows_kernel(HeadRows a) {
   }
 }
 
+template <typename T, int LANES, bool PAGED>
+__global__ __launch_bounds__(256) void head_rows_kernel(HeadRows a) {
+  token_rows<T, LANES, PAGED>(a, blockIdx.x);
+}
+
+// ------------------------------------------------------------------ a cache in 8 bits
+// A wave takes one side (keys or values) of one head of a block of 16 positions, as far as the call
+// writes them, in registers: norm, rotation, then the block's largest value m and its scale
+//   2^e,  e the least with m <= 448 2^e,
+// not below that of the rows which the block holds already: a row is rounded again only when a later
+// one raises the scale, and as the scale is a power of two, four significant bits stay what they
+// were but for values below 2^-6 of it.  Straight from fp32, so a value is rounded once.
+template <typename T>
+struct Held {  // exponents of scales: the least keeps steps of 2^-9 in T, the largest a value of ..
+  static constexpr int kLeast = __is_same(T, FP16) ? -15 : -117;
+  static constexpr int kMost = __is_same(T, FP16) ? 8 : 120;
+  // .. four significant bits that T holds: 61440 in fp16
+  static constexpr float kLargest = __is_same(T, FP16) ? 61440.0f : 0x1.Ep127f;
+};
+
+struct E4m3Pages {
+  uint8_t *k, *v;
+  float *scales;
+  int64_t scale_stride;
+  int units;      // workgroups of a block: four waves each
+  int64_t blocks;  // workgroups of blocks in all, before those of the queries' tokens
+};
+
+// Positions of sequence s that the call writes.
+struct Written {
+  int first, end;  // positions; first >= end: none
+  int row;         // of `first`
+};
+__device__ __forceinline__ Written written(const HeadRows &a, int s) {
+  const PagedSequence q = paged_sequence(a.batch, s, a.tokens);
+  const int room = a.batch.table_pages << a.batch.page_shift;
+  const int first = max(q.base, 0);
+  return {first, (int)min((int64_t)q.base + q.count, (int64_t)room), q.first + first - q.base};
+}
+__device__ __forceinline__ int block_count(const HeadRows &a, int s) {
+  if (s >= a.batch.sequences) return 0;
+  const Written w = written(a, s);
+  return w.first < w.end ? (w.end - 1) / kScaleKeys - w.first / kScaleKeys + 1 : 0;
+}
+
+// Sequence and place there of the index-th block of all; s < 0: none.  All 256 threads.
+struct BlockPlace {
+  int s, block;
+};
+__device__ BlockPlace find_block(const HeadRows &a, int64_t index) {
+  __shared__ int sums[4];
+  __shared__ BlockPlace found;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  auto scan = [&](int n) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(n, o, 64);
+      if (lane >= o) n += v;
+    }
+    return n;
+  };
+  if (a.batch.sequences <= 64) {  // each wave for itself
+    const int n = block_count(a, lane), sum = scan(n);
+    const uint64_t hit = __ballot(index >= sum - n && index < sum);
+    if (!hit) return {-1, 0};
+    const int at = __builtin_ctzll(hit);
+    return {at, (int)index - __shfl(sum - n, at, 64)};
+  }
+  if (tid == 0) found = {-1, 0};
+  int64_t base = 0;
+  for (int c = 0; c < a.batch.sequences && base <= index; c += 256) {
+    const int n = block_count(a, c + tid), sum = scan(n);
+    __syncthreads();
+    if (lane == 63) sums[wave] = sum;
+    __syncthreads();
+    int64_t before = base + sum - n;
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) before += sums[w];
+      base += sums[w];
+    }
+    if (index >= before && index < before + n) found = {c + tid, (int)(index - before)};
+  }
+  __syncthreads();
+  return found;
+}
+
+// Four values of 8 bits, NaN for what is not finite.
+__device__ __forceinline__ uint32_t to_e4m3(const float x[4], float inverse) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * inverse, x[1] * inverse, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2] * inverse, x[3] * inverse, w, true);
+}
+// Four held values under a scale 1 / `ratio` times as large.
+__device__ __forceinline__ uint32_t rescale_e4m3(uint32_t w, float ratio) {
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+  const float x[4] = {lo[0], lo[1], hi[0], hi[1]};
+  return to_e4m3(x, ratio);
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+template <typename T, int LANES>
+__device__ __forceinline__ void block_rows(const HeadRows &a, const E4m3Pages &p) {
+  constexpr int D = LANES * 8, ROWS = 64 / LANES, PASSES = kScaleKeys / ROWS;
+  __shared__ __attribute__((aligned(16))) float cosines[kScaleKeys][kMaxHalf],
+      sines[kScaleKeys][kMaxHalf];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid % LANES, own = (tid & 63) / LANES;
+  const BlockPlace at = find_block(a, blockIdx.x / p.units);
+  if (at.s < 0) return;
+  const Written w = written(a, at.s);
+  const int block = w.first / kScaleKeys + at.block, p0 = max(block * kScaleKeys, w.first);
+  const int p1 = min((block + 1) * kScaleKeys, w.end);
+  const int before = p0 - block * kScaleKeys, count = p1 - p0;  // rows held already, new ones
+  const int row0 = w.row + p0 - w.first;                        // of the block's first new position
+  const int unit = blockIdx.x % p.units * 4 + wave;             // keys of each head, then values
+  const bool live = unit < 2 * a.k_heads, value = unit >= a.k_heads;
+  const int head = value ? unit - a.k_heads : unit;
+  const int half = value ? 0 : a.half;
+  const bool rotated = lane * 8 < 2 * half;
+  const int lo = rotated ? lane * 4 : lane * 8, hi = rotated ? half + lane * 4 : lane * 8 + 4;
+
+  Row8 raw[PASSES];
+  if (live) {
+    const uint16_t *src = value ? a.v + head * a.v_head : a.k + head * a.k_head;
+    const int64_t stride = value ? a.v_token : a.k_token;
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      const int r = min(max(i * ROWS + own - before, 0), count - 1);
+      const uint16_t *x = src + (row0 + r) * stride;
+      raw[i] = Row8{ldg_u2(x + lo), ldg_u2(x + hi)};
+    }
+  }
+  const int page = paged_number(a.batch, at.s, p0), nb = 1 << (a.batch.page_shift - kScaleShift);
+  const int inside = block & (nb - 1);
+  float *scale = p.scales + page * p.scale_stride + (2 * head + value) * nb + inside;
+  int least = Held<T>::kLeast;
+  if (live && before > 0) {
+    const int held = (int)(__float_as_uint(*scale) >> 23 & 0xFFu) - 127;
+    least = min(max(held, Held<T>::kLeast), Held<T>::kMost);
+  }
+  if (blockIdx.x % p.units * 4 < a.k_heads) {  // keys among the workgroup's
+    for (int i = tid; i < count * a.half; i += 256) {
+      const int r = i / a.half, j = i % a.half;
+      turn(a, a.inv_freq[j], j, row0 + r, p0 + r, &sines[r][j], &cosines[r][j]);
+    }
+    __syncthreads();
+  }
+  if (!live) return;
+
+  float x[PASSES][8];
+  float w0[4] = {}, w1[4] = {};
+  const float *weight = value ? nullptr : a.k_w;
+  if (weight) {
+    *reinterpret_cast<float4 *>(w0) = *reinterpret_cast<const float4 *>(weight + lo);
+    *reinterpret_cast<float4 *>(w1) = *reinterpret_cast<const float4 *>(weight + hi);
+  }
+  float most = 0.0f;
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    float *u = x[i], *v = x[i] + 4;
+    unpack4<T>(raw[i].lo, u);
+    unpack4<T>(raw[i].hi, v);
+    if (weight) {
+      float ss = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss = __builtin_fmaf(u[j], u[j], ss);
+      const float n = 1.0f / sqrtf(lanes_sum<LANES>(ss) * (1.0f / D) + a.eps);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) u[j] *= n * (1.0f + w0[j]), v[j] *= n * (1.0f + w1[j]);
+    }
+    const int r = i * ROWS + own - before;
+    const bool fresh = r >= 0 && r < count;
+    if (rotated) {
+      const int at_row = min(max(r, 0), count - 1);
+      float c[4], s[4];
+      *reinterpret_cast<float4 *>(c) = *reinterpret_cast<const float4 *>(&cosines[at_row][lo]);
+      *reinterpret_cast<float4 *>(s) = *reinterpret_cast<const float4 *>(&sines[at_row][lo]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float y = u[j] * c[j] - v[j] * s[j];
+        v[j] = v[j] * c[j] + u[j] * s[j];
+        u[j] = y;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float size = fabsf(u[j]);  // NaN and infinities are no part of the maximum
+      u[j] = size < INFINITY ? fminf(fmaxf(u[j], -Held<T>::kLargest), Held<T>::kLargest) : NAN;
+      if (fresh && size < INFINITY) most = fmaxf(most, fabsf(u[j]));
+    }
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
+  // 448 = 1.75 * 2^8: one more where the significand is above 1.75
+  const int need = (int)((__float_as_uint(most) + 0x1FFFFFu) >> 23) - 127 - 8;
+  const int e = max(need, least);
+  uint8_t *rows = (value ? p.v : p.k) + page * a.batch.page_stride +
+                  (((int64_t)head << a.batch.page_shift) + inside * kScaleKeys) * D;
+  if (before > 0 && e > least) {
+    const float ratio = power_of_two(max(least - e, -126));
+#pragma unroll 1
+    for (int r = own; r < before; r += ROWS) {
+      uint2 *b = reinterpret_cast<uint2 *>(rows + r * D + lane * 8);
+      const uint2 old = *b;
+      *b = uint2{rescale_e4m3(old.x, ratio), rescale_e4m3(old.y, ratio)};
+    }
+  }
+  const float inverse = power_of_two(-e);
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    const int r = i * ROWS + own;
+    if (r < before || r >= before + count) continue;
+    *reinterpret_cast<uint32_t *>(rows + r * D + lo) = to_e4m3(x[i], inverse);
+    *reinterpret_cast<uint32_t *>(rows + r * D + hi) = to_e4m3(x[i] + 4, inverse);
+  }
+  if ((tid & 63) == 0) *scale = power_of_two(e);
+}
+
+template <typename T, int LANES>
+__global__ __launch_bounds__(256) void append_e4m3_kernel(HeadRows a, E4m3Pages p) {
+  if (blockIdx.x < p.blocks) {
+    block_rows<T, LANES>(a, p);
+  } else {
+    a.k_heads = 0;
+    token_rows<T, LANES, true>(a, (int)(blockIdx.x - p.blocks));
+  }
+}
+
 template <typename T, bool PAGED>
 void launch_rows(const HeadRows &a, int head_dim, hipStream_t st) {
   const unsigned grid = (unsigned)a.tokens;
@@ -210,17 +448,21 @@ int check_rotation(const float *inv_freq, int64_t pairs, int64_t head_dim) {
   return LM_OK;
 }
 
-}  // namespace
-}  // namespace lm
+// Checks of positions and the axes of the pairs; positions may be missing with a cache.
+int check_axes(const int64_t *positions, int64_t position_stride, int64_t axes,
+               const int32_t *axis, int64_t tokens) {
+  LM_REQUIRE(axes >= 1 && axes <= 64, LM_EINVAL, "invalid number of axes");
+  LM_REQUIRE(!axis || positions, LM_EINVAL, "axes need positions");
+  LM_REQUIRE(axes == 1 || position_stride >= tokens, LM_EINVAL, "positions of the axes overlap");
+  return LM_OK;
+}
 
-using namespace lm;
-
-extern "C" int lm_qk_norm_rope(const void *q, int64_t q_token_stride, int64_t q_head_stride,
-                               int64_t q_heads, const float *q_weight, void *q_out, const void *k,
-                               int64_t k_token_stride, int64_t k_head_stride, int64_t k_heads,
-                               const float *k_weight, void *k_out, const int64_t *positions,
-                               const float *inv_freq, int64_t pairs, int64_t tokens,
-                               int64_t head_dim, float eps, int dtype, void *stream) {
+int norm_rope(const void *q, int64_t q_token_stride, int64_t q_head_stride, int64_t q_heads,
+              const float *q_weight, void *q_out, const void *k, int64_t k_token_stride,
+              int64_t k_head_stride, int64_t k_heads, const float *k_weight, void *k_out,
+              const int64_t *positions, int64_t position_stride, int64_t axes, const int32_t *axis,
+              const float *inv_freq, int64_t pairs, int64_t tokens, int64_t head_dim, float eps,
+              int dtype, void *stream) {
   LM_REQUIRE(dtype == LM_BF16 || dtype == LM_FP16, LM_EINVAL, "attention requires FP16/BF16");
   LM_REQUIRE(head_dim == 64 || head_dim == 128 || head_dim == 256, LM_EINVAL,
              "attention supports heads of 64, 128 or 256");
@@ -229,6 +471,7 @@ extern "C" int lm_qk_norm_rope(const void *q, int64_t q_token_stride, int64_t q_
   LM_REQUIRE(tokens >= 0 && tokens < kMaxTokens, LM_EINVAL, "invalid token count");
   if (const int rc = check_rotation(inv_freq, pairs, head_dim)) return rc;
   if (tokens == 0 || q_heads + k_heads == 0) return LM_OK;
+  if (const int rc = check_axes(positions, position_stride, axes, axis, tokens)) return rc;
   if (q_heads)
     if (const int rc = check_rows(q, q_token_stride, q_head_stride, q_weight)) return rc;
   if (k_heads)
@@ -243,7 +486,8 @@ extern "C" int lm_qk_norm_rope(const void *q, int64_t q_token_stride, int64_t q_
   a.k = static_cast<const uint16_t *>(k);
   a.k_token = k_token_stride, a.k_head = k_head_stride, a.k_heads = (int)k_heads;
   a.k_w = k_weight, a.k_out = static_cast<uint16_t *>(k_out);
-  a.positions = positions, a.inv_freq = inv_freq, a.half = (int)pairs;
+  a.positions = positions, a.position_stride = position_stride;
+  a.axis = axis, a.axes = (int)axes, a.inv_freq = inv_freq, a.half = (int)pairs;
   a.tokens = (int)tokens, a.eps = eps;
   if (dtype == LM_BF16)
     launch_rows<BF16, false>(a, (int)head_dim, as_stream(stream));
@@ -252,22 +496,40 @@ extern "C" int lm_qk_norm_rope(const void *q, int64_t q_token_stride, int64_t q_
   return check_launch("head_rows_kernel");
 }
 
-extern "C" int lm_paged_append(const void *k, int64_t k_token_stride, int64_t k_head_stride,
-                               const float *k_weight, const void *v, int64_t v_token_stride,
-                               int64_t v_head_stride, const void *q, int64_t q_token_stride,
-                               int64_t q_head_stride, int64_t q_heads, const float *q_weight,
-                               void *q_out, void *k_pages, void *v_pages, int64_t pages,
-                               int64_t page_stride, int64_t kv_heads, int64_t page_size,
-                               int64_t head_dim, const int32_t *starts, const int32_t *lengths,
-                               const int32_t *table, int64_t table_stride, int64_t table_pages,
-                               int64_t sequences, const float *inv_freq, int64_t pairs,
-                               int64_t tokens, float eps, int dtype, void *stream) {
+template <typename T>
+void launch_e4m3(const HeadRows &a, const E4m3Pages &p, int head_dim, hipStream_t st) {
+  const unsigned grid = (unsigned)(p.blocks + (a.q_heads ? a.tokens : 0));
+  if (head_dim == 256)
+    append_e4m3_kernel<T, 32><<<grid, 256, 0, st>>>(a, p);
+  else if (head_dim == 128)
+    append_e4m3_kernel<T, 16><<<grid, 256, 0, st>>>(a, p);
+  else
+    append_e4m3_kernel<T, 8><<<grid, 256, 0, st>>>(a, p);
+}
+
+// An append to a cache of the rows' type, or of 8 bits (e4m3).
+int paged_append(const void *k, int64_t k_token_stride, int64_t k_head_stride,
+                 const float *k_weight, const void *v, int64_t v_token_stride,
+                 int64_t v_head_stride, const void *q, int64_t q_token_stride,
+                 int64_t q_head_stride, int64_t q_heads, const float *q_weight, void *q_out,
+                 void *k_pages, void *v_pages, bool e4m3, float *scales, int64_t scale_stride,
+                 int64_t pages, int64_t page_stride, int64_t kv_heads, int64_t page_size,
+                 int64_t head_dim, const int32_t *starts, const int32_t *lengths,
+                 const int32_t *table, int64_t table_stride, int64_t table_pages,
+                 int64_t sequences, const int64_t *positions, int64_t position_stride,
+                 int64_t axes, const int32_t *axis, const float *inv_freq, int64_t pairs,
+                 int64_t tokens, float eps, int dtype, void *stream) {
   if (const int rc = paged_check(pages, page_stride, kv_heads, page_size, head_dim, starts, lengths,
                                  table, table_stride, table_pages, sequences, tokens, dtype))
     return rc;
   LM_REQUIRE(q_heads >= 0 && q_heads <= 65536, LM_EINVAL, "invalid number of heads");
   if (const int rc = check_rotation(inv_freq, pairs, head_dim)) return rc;
-  if (tokens == 0 || sequences == 0) return LM_OK;
+  if (const int rc = check_axes(positions, position_stride, axes, axis, tokens)) return rc;
+  const bool empty = tokens == 0 || sequences == 0;
+  if (e4m3)
+    if (const int rc = scales_check(scales, scale_stride, kv_heads, page_size, page_stride, empty))
+      return rc;
+  if (empty) return LM_OK;
   if (const int rc = check_rows(k, k_token_stride, k_head_stride, k_weight)) return rc;
   if (const int rc = check_rows(v, v_token_stride, v_head_stride, nullptr)) return rc;
   if (q_heads) {
@@ -283,14 +545,109 @@ extern "C" int lm_paged_append(const void *k, int64_t k_token_stride, int64_t k_
   a.q = static_cast<const uint16_t *>(q);
   a.q_token = q_token_stride, a.q_head = q_head_stride, a.q_heads = (int)q_heads;
   a.q_w = q_weight, a.q_out = static_cast<uint16_t *>(q_out);
-  a.k_pages = static_cast<uint16_t *>(k_pages), a.v_pages = static_cast<uint16_t *>(v_pages);
   a.batch = {starts, lengths, table, table_stride, (int)sequences, (int)table_pages,
              __builtin_ctzll((unsigned long long)page_size), (int)pages, page_stride,
              (int)kv_heads};
-  a.inv_freq = inv_freq, a.half = (int)pairs, a.tokens = (int)tokens, a.eps = eps;
+  a.positions = positions, a.position_stride = position_stride;
+  a.axis = axis, a.axes = (int)axes, a.inv_freq = inv_freq, a.half = (int)pairs;
+  a.tokens = (int)tokens, a.eps = eps;
+  if (e4m3) {
+    E4m3Pages p = {static_cast<uint8_t *>(k_pages), static_cast<uint8_t *>(v_pages), scales,
+                   scale_stride, (int)((2 * kv_heads + 3) / 4), 0};
+    // n positions of a sequence lie in at most n / 16 + 2 blocks, and in n of them
+    const int64_t most = tokens / kScaleKeys + 2 * sequences;
+    p.blocks = (most < tokens ? most : tokens) * p.units;
+    LM_REQUIRE(p.blocks + tokens < (1LL << 24), LM_EINVAL, "too many rows");
+    if (dtype == LM_BF16)
+      launch_e4m3<BF16>(a, p, (int)head_dim, as_stream(stream));
+    else
+      launch_e4m3<FP16>(a, p, (int)head_dim, as_stream(stream));
+    return check_launch("append_e4m3_kernel");
+  }
+  a.k_pages = static_cast<uint16_t *>(k_pages), a.v_pages = static_cast<uint16_t *>(v_pages);
   if (dtype == LM_BF16)
     launch_rows<BF16, true>(a, (int)head_dim, as_stream(stream));
   else
     launch_rows<FP16, true>(a, (int)head_dim, as_stream(stream));
   return check_launch("head_rows_kernel");
+}
+
+}  // namespace
+}  // namespace lm
+
+using namespace lm;
+
+extern "C" int lm_qk_norm_rope(const void *q, int64_t q_token_stride, int64_t q_head_stride,
+                               int64_t q_heads, const float *q_weight, void *q_out, const void *k,
+                               int64_t k_token_stride, int64_t k_head_stride, int64_t k_heads,
+                               const float *k_weight, void *k_out, const int64_t *positions,
+                               const float *inv_freq, int64_t pairs, int64_t tokens,
+                               int64_t head_dim, float eps, int dtype, void *stream) {
+  return norm_rope(q, q_token_stride, q_head_stride, q_heads, q_weight, q_out, k, k_token_stride,
+                   k_head_stride, k_heads, k_weight, k_out, positions, 0, 1, nullptr, inv_freq,
+                   pairs, tokens, head_dim, eps, dtype, stream);
+}
+
+extern "C" int lm_qk_norm_rope_axes(const void *q, int64_t q_token_stride, int64_t q_head_stride,
+                                    int64_t q_heads, const float *q_weight, void *q_out,
+                                    const void *k, int64_t k_token_stride, int64_t k_head_stride,
+                                    int64_t k_heads, const float *k_weight, void *k_out,
+                                    const int64_t *positions, int64_t position_stride,
+                                    int64_t axes, const int32_t *axis, const float *inv_freq,
+                                    int64_t pairs, int64_t tokens, int64_t head_dim, float eps,
+                                    int dtype, void *stream) {
+  return norm_rope(q, q_token_stride, q_head_stride, q_heads, q_weight, q_out, k, k_token_stride,
+                   k_head_stride, k_heads, k_weight, k_out, positions, position_stride, axes, axis,
+                   inv_freq, pairs, tokens, head_dim, eps, dtype, stream);
+}
+
+extern "C" int lm_paged_append(const void *k, int64_t k_token_stride, int64_t k_head_stride,
+                               const float *k_weight, const void *v, int64_t v_token_stride,
+                               int64_t v_head_stride, const void *q, int64_t q_token_stride,
+                               int64_t q_head_stride, int64_t q_heads, const float *q_weight,
+                               void *q_out, void *k_pages, void *v_pages, int64_t pages,
+                               int64_t page_stride, int64_t kv_heads, int64_t page_size,
+                               int64_t head_dim, const int32_t *starts, const int32_t *lengths,
+                               const int32_t *table, int64_t table_stride, int64_t table_pages,
+                               int64_t sequences, const float *inv_freq, int64_t pairs,
+                               int64_t tokens, float eps, int dtype, void *stream) {
+  return paged_append(k, k_token_stride, k_head_stride, k_weight, v, v_token_stride, v_head_stride,
+                      q, q_token_stride, q_head_stride, q_heads, q_weight, q_out, k_pages, v_pages,
+                      false, nullptr, 0, pages, page_stride, kv_heads, page_size, head_dim, starts,
+                      lengths, table, table_stride, table_pages, sequences, nullptr, 0, 1, nullptr,
+                      inv_freq, pairs, tokens, eps, dtype, stream);
+}
+
+extern "C" int lm_paged_append_axes(
+    const void *k, int64_t k_token_stride, int64_t k_head_stride, const float *k_weight,
+    const void *v, int64_t v_token_stride, int64_t v_head_stride, const void *q,
+    int64_t q_token_stride, int64_t q_head_stride, int64_t q_heads, const float *q_weight,
+    void *q_out, void *k_pages, void *v_pages, int64_t pages, int64_t page_stride,
+    int64_t kv_heads, int64_t page_size, int64_t head_dim, const int32_t *starts,
+    const int32_t *lengths, const int32_t *table, int64_t table_stride, int64_t table_pages,
+    int64_t sequences, const int64_t *positions, int64_t position_stride, int64_t axes,
+    const int32_t *axis, const float *inv_freq, int64_t pairs, int64_t tokens, float eps, int dtype,
+    void *stream) {
+  return paged_append(k, k_token_stride, k_head_stride, k_weight, v, v_token_stride, v_head_stride,
+                      q, q_token_stride, q_head_stride, q_heads, q_weight, q_out, k_pages, v_pages,
+                      false, nullptr, 0, pages, page_stride, kv_heads, page_size, head_dim, starts,
+                      lengths, table, table_stride, table_pages, sequences, positions,
+                      position_stride, axes, axis, inv_freq, pairs, tokens, eps, dtype, stream);
+}
+
+extern "C" int lm_paged_append_e4m3(
+    const void *k, int64_t k_token_stride, int64_t k_head_stride, const float *k_weight,
+    const void *v, int64_t v_token_stride, int64_t v_head_stride, const void *q,
+    int64_t q_token_stride, int64_t q_head_stride, int64_t q_heads, const float *q_weight,
+    void *q_out, void *k_pages, void *v_pages, float *scales, int64_t scale_stride, int64_t pages,
+    int64_t page_stride, int64_t kv_heads, int64_t page_size, int64_t head_dim,
+    const int32_t *starts, const int32_t *lengths, const int32_t *table, int64_t table_stride,
+    int64_t table_pages, int64_t sequences, const int64_t *positions, int64_t position_stride,
+    int64_t axes, const int32_t *axis, const float *inv_freq, int64_t pairs, int64_t tokens,
+    float eps, int dtype, void *stream) {
+  return paged_append(k, k_token_stride, k_head_stride, k_weight, v, v_token_stride, v_head_stride,
+                      q, q_token_stride, q_head_stride, q_heads, q_weight, q_out, k_pages, v_pages,
+                      true, scales, scale_stride, pages, page_stride, kv_heads, page_size, head_dim,
+                      starts, lengths, table, table_stride, table_pages, sequences, positions,
+                      position_stride, axes, axis, inv_freq, pairs, tokens, eps, dtype, stream);
 }

@@ -36,11 +36,19 @@ __device__ __forceinline__ PagedSequence paged_sequence(const PagedBatch &b, int
           min(max(len, 0), room)};
 }
 
-// Element offset of position p's page of sequence s.
-__device__ __forceinline__ int64_t paged_page(const PagedBatch &b, int s, int p) {
+// Position p's page of sequence s, and its element offset.
+__device__ __forceinline__ int paged_number(const PagedBatch &b, int s, int p) {
   const int i = min(p >> b.page_shift, b.table_pages - 1);
-  return clamp_index32(b.table[s * b.table_stride + i], b.pages) * b.page_stride;
+  return clamp_index32(b.table[s * b.table_stride + i], b.pages);
 }
+__device__ __forceinline__ int64_t paged_page(const PagedBatch &b, int s, int p) {
+  return paged_number(b, s, p) * b.page_stride;
+}
+
+// A cache in 8 bits holds e4m3 values (four significant bits, up to 448, no infinities) and a
+// scale, a power of two, for each kScaleKeys positions of a head, keys and values apart.
+struct E4M3 {};
+constexpr int kScaleKeys = 16, kScaleShift = 4;
 
 // A launch has fewer than 2^32 threads; the kernels take at most 256 for a token.
 constexpr int64_t kMaxTokens = 1LL << 24;
@@ -73,5 +81,16 @@ inline int paged_check(int64_t pages, int64_t page_stride, int64_t kv_heads, int
 }
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Of a cache in 8 bits: its scales, and pages whose rows stay 16-byte aligned.
+inline int scales_check(const float *scales, int64_t scale_stride, int64_t kv_heads,
+                        int64_t page_size, int64_t page_stride, bool empty) {
+  LM_REQUIRE(page_stride % 16 == 0, LM_EINVAL, "invalid pages");
+  LM_REQUIRE(scale_stride >= 2 * kv_heads * (page_size / kScaleKeys), LM_EINVAL,
+             "invalid scales of the pages");
+  LM_REQUIRE(empty || (scales && (reinterpret_cast<uintptr_t>(scales) & 3) == 0), LM_EINVAL,
+             "invalid scales of the pages");
+  return LM_OK;
+}
 
 }  // namespace lm

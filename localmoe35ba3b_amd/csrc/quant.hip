@@ -5,6 +5,8 @@
 //  * lm_act_quant_g128: dynamic per-row activation quantization of the W8A8
 //    decode path (w8a8.py:8-22): s = max(amax, 1e-10) * fl32(1/127),
 //    q = rint(x / s) with IEEE division (|x / s| <= 127 by construction).
+//  * lm_norm_quant_g128: rows on their way into a W8A8 product, h += x, their RMS norm and its
+//    quantization in one pass.
 //
 // One 128-element group is handled by 32 lanes holding 4 elements each, so a
 // wave quantizes two groups per iteration with fully coalesced 16-byte loads.
@@ -71,6 +73,102 @@ __global__ __launch_bounds__(256) void act_quant_kernel(const uint16_t *__restri
   }
 }
 
+
+// ------------------------------------------------------------------ norm and quantization
+// h := T(h + x), n = h rsqrt(mean h^2 + eps) (1 + w), s = max(amax |n|, 1e-10) fl(1/127) of each 128,
+// q = rint(n / s): n stays in fp32 until it is quantized.  A row lies in the registers of WAVES
+// waves, eight values a thread and chunk, a group of 128 in 16 lanes; it is read once.  Not finite
+// values leave a scale that is not.
+template <typename T, int WAVES, int CHUNKS, bool ADD>
+__global__ __launch_bounds__(256) void norm_quant_kernel(uint16_t *__restrict__ h,
+                                                         const uint16_t *__restrict__ x,
+                                                         const float *__restrict__ w,
+                                                         int8_t *__restrict__ q,
+                                                         float *__restrict__ s, int64_t rows, int n,
+                                                         float eps) {
+  constexpr int THREADS = WAVES * 64;
+  __shared__ float sums[4];
+  const int tid = threadIdx.x % THREADS;
+  const int64_t row = (int64_t)blockIdx.x * (4 / WAVES) + threadIdx.x / THREADS;
+  if (WAVES == 1 && row >= rows) return;  // with more waves a workgroup has one row
+  const int64_t at = row * n;
+  float v[CHUNKS][8];
+  u32x4 a[CHUNKS], b[CHUNKS];
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int i = min((c * THREADS + tid) * 8, n - 8);  // again the last, where there is no more
+    a[c] = ldg16(h + at + i);
+    if constexpr (ADD) b[c] = ldg16(x + at + i);
+  }
+  float ss = 0.0f;
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int i = (c * THREADS + tid) * 8;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (ADD)
+        a[c][j] = T::pack2(T::to_f32(a[c][j] & 0xFFFFu) + T::to_f32(b[c][j] & 0xFFFFu),
+                           T::to_f32(a[c][j] >> 16) + T::to_f32(b[c][j] >> 16));
+      v[c][2 * j] = T::to_f32(a[c][j] & 0xFFFFu);
+      v[c][2 * j + 1] = T::to_f32(a[c][j] >> 16);
+    }
+    if (i < n) {
+      if constexpr (ADD) *reinterpret_cast<u32x4 *>(h + at + i) = a[c];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss = __builtin_fmaf(v[c][j], v[c][j], ss);
+    }
+  }
+  ss = wave_sum_f32(ss);
+  if constexpr (WAVES > 1) {
+    if ((tid & 63) == 0) sums[tid >> 6] = ss;
+    __syncthreads();
+    ss = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+  }
+  const float scale = 1.0f / sqrtf(ss / (float)n + eps);
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int i = (c * THREADS + tid) * 8;
+    if (i >= n) break;  // 16 lanes at a time
+    uint32_t most = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[c][j] *= scale;
+      if (w) v[c][j] *= 1.0f + w[i + j];
+      most = max(most, __float_as_uint(v[c][j]) & 0x7FFFFFFFu);  // NaN above all
+    }
+    most = max(most, dpp_u32<0xB1>(most));
+    most = max(most, dpp_u32<0x4E>(most));
+    most = max(most, dpp_u32<0x141>(most));
+    most = max(most, dpp_u32<0x140>(most));
+    const float amax = __uint_as_float(max(most, __float_as_uint(1e-10f)));
+    const float group = amax * (1.0f / 127.0f);
+    uint32_t packed[2] = {};
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      packed[j / 4] |= (uint32_t)(uint8_t)(int8_t)(int)fminf(
+                           fmaxf(rintf(v[c][j] / group), -127.0f), 127.0f)
+                       << (8 * (j % 4));
+    *reinterpret_cast<uint2 *>(q + at + i) = uint2{packed[0], packed[1]};
+    if ((tid & 15) == 0) s[(at + i) / 128] = group;
+  }
+}
+
+template <typename T, bool ADD>
+static int launch_norm_quant(void *h, const void *x, const float *w, int8_t *q, float *s,
+                             int64_t rows, int64_t n, float eps, hipStream_t st) {
+  uint16_t *hp = static_cast<uint16_t *>(h);
+  const uint16_t *xp = static_cast<const uint16_t *>(x);
+  const unsigned grid = (unsigned)rows;
+  if (n <= 2048)
+    norm_quant_kernel<T, 4, 1, ADD><<<grid, 256, 0, st>>>(hp, xp, w, q, s, rows, (int)n, eps);
+  else if (n <= 4096)
+    norm_quant_kernel<T, 4, 2, ADD><<<grid, 256, 0, st>>>(hp, xp, w, q, s, rows, (int)n, eps);
+  else if (n <= 8192)
+    norm_quant_kernel<T, 4, 4, ADD><<<grid, 256, 0, st>>>(hp, xp, w, q, s, rows, (int)n, eps);
+  else
+    norm_quant_kernel<T, 4, 8, ADD><<<grid, 256, 0, st>>>(hp, xp, w, q, s, rows, (int)n, eps);
+  return check_launch("norm_quant_kernel");
+}
 
 static unsigned quant_grid(int64_t ngroups) {
   int64_t waves = (ngroups + 1) / 2;
@@ -157,4 +255,25 @@ extern "C" int lm_act_quant_g128(const void *x, int x_dtype, int8_t *q, float *s
   else
     act_quant_kernel<FP16><<<act_quant_grid(ngroups), 256, 0, as_stream(stream)>>>(xp, q, s, ngroups);
   return check_launch("act_quant_kernel");
+}
+
+extern "C" int lm_norm_quant_g128(void *h, const void *x, const float *w, int8_t *q, float *s,
+                                  int64_t rows, int64_t n, float eps, int dtype, void *stream) {
+  LM_REQUIRE(rows >= 0 && rows < (1LL << 24), LM_EINVAL, "invalid number of rows");
+  LM_REQUIRE(n >= 128 && n % 128 == 0 && n <= 16384, LM_EINVAL,
+             "Expected rows of 128 to 16384 values, a multiple of 128");
+  LM_REQUIRE(dtype == LM_BF16 || dtype == LM_FP16, LM_EINVAL,
+             "Expected CUDA rows with K divisible by 128");
+  if (rows == 0) return LM_OK;
+  LM_REQUIRE(h && q && s, LM_EINVAL, "null pointer");
+  LM_REQUIRE(((reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(x) |
+               reinterpret_cast<uintptr_t>(w)) & 15) == 0 &&
+                 (reinterpret_cast<uintptr_t>(q) & 7) == 0,
+             LM_EINVAL, "rows must be 16-byte aligned");
+  hipStream_t st = as_stream(stream);
+  if (dtype == LM_BF16)
+    return x ? launch_norm_quant<BF16, true>(h, x, w, q, s, rows, n, eps, st)
+             : launch_norm_quant<BF16, false>(h, x, w, q, s, rows, n, eps, st);
+  return x ? launch_norm_quant<FP16, true>(h, x, w, q, s, rows, n, eps, st)
+           : launch_norm_quant<FP16, false>(h, x, w, q, s, rows, n, eps, st);
 }

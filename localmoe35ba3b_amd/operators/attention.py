@@ -6,8 +6,10 @@ append            keys (normed and rotated on the way) and values into the cache
                   with the queries of the same tokens in the same pass
 paged_attention   each sequence's new tokens over its cache, causal at its end
 
-A cache is two tensors [pages, kv_heads, page_size, head_dim], keys and values.  A
-batch is three int32 tensors on the GPU, which a program keeps for all layers of a
+A cache is two tensors [pages, kv_heads, page_size, head_dim], keys and values, of the
+rows' type or of 8 bits: torch.float8_e4m3fn with `scales`, fp32 [pages, kv_heads, 2,
+page_size // 16], a power of two for each 16 positions of a head (of keys, then of
+values) by which its values are multiplied.  A batch is three int32 tensors on the GPU, which a program keeps for all layers of a
 step and may rewrite between replays of a captured step:
   starts  [sequences + 1]  the rows of sequence s are starts[s] .. starts[s + 1] - 1
   lengths [sequences]      its positions, the new ones (its last) among them
@@ -25,6 +27,8 @@ import torch
 from .. import _lib
 
 _TYPES = (torch.bfloat16, torch.float16)
+_E4M3 = torch.float8_e4m3fn
+BLOCK = 16  # positions of a head that share a scale in a cache of 8 bits
 
 
 def _rows(x, what):
@@ -45,6 +49,8 @@ def _rows(x, what):
 
 def _same(x, dtype, device):
     if x.dtype is not dtype or x.get_device() != device:
+        if _E4M3 in (x.dtype, dtype) and x.get_device() == device:
+            raise ValueError('pages of 8 bits come with scales, others without')
         raise ValueError('attention tensors must share their type and device')
 
 
@@ -84,13 +90,39 @@ def _frequencies(inv_freq, dim, device):
     return inv_freq, inv_freq.data_ptr(), pairs
 
 
-def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6):
+def _positions(positions, axes, pairs, tokens, device):
+    """The positions and axes of a call (copies of others than int64 and int32), and their C
+    arguments: pointer, stride between axes, axes, each pair's axis."""
+    shape = positions.shape
+    if positions.get_device() != device or not 1 <= len(shape) <= 2 or shape[-1] != tokens:
+        raise ValueError('Expected a CUDA position of every token')
+    if positions.is_floating_point() or positions.is_complex() or positions.dtype is torch.bool:
+        raise ValueError('Expected whole positions')
+    n = shape[0] if len(shape) == 2 else 1
+    if n > 1 and axes is None:
+        raise ValueError('positions of several axes need the axis of every pair')
+    if not 1 <= n <= 64:
+        raise ValueError('Expected 1 to 64 axes of positions')
+    if positions.dtype is not torch.int64 or not positions.is_contiguous():
+        positions = positions.to(torch.int64).contiguous()
+    axis = 0
+    if axes is not None:
+        if axes.numel() != pairs or axes.get_device() != device:
+            raise ValueError('Expected a CUDA axis of every rotated pair')
+        if axes.dtype is not torch.int32 or not axes.is_contiguous():
+            axes = axes.to(torch.int32).contiguous()
+        axis = axes.data_ptr()
+    return positions, axes, (positions.data_ptr(), tokens, n, axis)
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, axes=None):
     """Normed and rotated (q, k), contiguous [tokens, heads, head_dim] each.
 
     q [T, q_heads, D], k [T, k_heads, D] (bf16 or fp16, D = 64, 128 or 256, any token
     and head strides); weights [D] (scale 1 + w) or None for no norm; positions int64
     [T]; inv_freq [R / 2] rotates channels i and i + R / 2 by positions * inv_freq[i]
-    (None: no rotation)."""
+    (None: no rotation).  positions [A, T] have several axes (time, row, column), and axes,
+    int32 [R / 2] on the GPU, says which one rotates pair i (clamped into 0 .. A - 1)."""
     q, q_token, q_head = _rows(q, 'queries')
     k, k_token, k_head = _rows(k, 'keys')
     dtype, device = q.dtype, q.get_device()
@@ -99,17 +131,23 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6):
     k_tokens, k_heads, k_dim = k.shape
     if k_tokens != tokens or k_dim != dim:
         raise ValueError('queries and keys do not match')
-    if positions.get_device() != device or positions.numel() != tokens:
-        raise ValueError('Expected a CUDA position of every token')
-    if positions.dtype is not torch.int64 or not positions.is_contiguous():
-        positions = positions.to(torch.int64).contiguous()
+    inv_freq, freq, pairs = _frequencies(inv_freq, dim, device)
+    several = axes is not None or positions.numel() != tokens
+    if several:
+        positions, axes, places = _positions(positions, axes, pairs, tokens, device)
+    else:
+        if positions.get_device() != device or positions.numel() != tokens:
+            raise ValueError('Expected a CUDA position of every token')
+        if positions.dtype is not torch.int64 or not positions.is_contiguous():
+            positions = positions.to(torch.int64).contiguous()
+        places = positions.data_ptr(),
     q_weight, q_w = _weight(q_weight, dim, device)
     k_weight, k_w = _weight(k_weight, dim, device)
-    inv_freq, freq, pairs = _frequencies(inv_freq, dim, device)
     q_out, k_out = q.new_empty((tokens, q_heads, dim)), k.new_empty((tokens, k_heads, dim))
-    _lib.launch(device, 'lm_qk_norm_rope', q.data_ptr(), q_token, q_head, q_heads, q_w,
-                q_out.data_ptr(), k.data_ptr(), k_token, k_head, k_heads, k_w, k_out.data_ptr(),
-                positions.data_ptr(), freq, pairs, tokens, dim, eps, _lib.dtype_code(dtype))
+    _lib.launch(device, 'lm_qk_norm_rope_axes' if several else 'lm_qk_norm_rope', q.data_ptr(),
+                q_token, q_head, q_heads, q_w, q_out.data_ptr(), k.data_ptr(), k_token, k_head,
+                k_heads, k_w, k_out.data_ptr(), *places, freq, pairs, tokens, dim, eps,
+                _lib.dtype_code(dtype))
     return q_out, k_out
 
 
@@ -140,6 +178,23 @@ def _page_strides(x):
     return tuple(p if n == 1 else s for n, s, p in zip(x.shape, x.stride(), plain))
 
 
+def _scales(scales, k_pages, device):
+    """The C arguments of a cache's scales, () for one of the rows' type."""
+    if scales is None:
+        return ()
+    pages, heads, size, _ = k_pages.shape
+    blocks = size // BLOCK
+    if (scales.dtype is not torch.float32 or scales.get_device() != device
+            or scales.shape != (pages, heads, 2, blocks)):
+        raise ValueError('Expected CUDA fp32 scales [pages, kv_heads, 2, page_size // 16]')
+    stride = scales.stride()
+    if not scales.is_contiguous():  # but for the pages
+        plain = 2 * blocks, blocks, 1
+        if any(n > 1 and a != b for n, a, b in zip(scales.shape[1:], stride[1:], plain)):
+            raise ValueError('the scales of a page must be contiguous')
+    return scales.data_ptr(), stride[0] if pages > 1 else 2 * heads * blocks
+
+
 def _batch(device, starts, lengths, table):
     """The C arguments of a batch: pointers, table stride, table pages, sequences."""
     i32 = torch.int32
@@ -157,19 +212,36 @@ def _batch(device, starts, lengths, table):
             stride if sequences > 1 else shape[1], shape[1], sequences)
 
 
-def check_batch(rows, k_pages, v_pages, starts, lengths, table):
+def check_batch(rows, k_pages, v_pages, starts, lengths, table, scales=None):
     """Raises where append and paged_attention refuse these for new rows of this type and device,
     for a program that runs several operators and wants to know before the first; returns the
     cache's (kv_heads, head_dim)."""
-    _, _, heads, _, dim = _cache(k_pages, v_pages, rows.dtype, rows.get_device())
-    _batch(rows.get_device(), starts, lengths, table)
+    device = rows.get_device()
+    _, _, heads, _, dim = _cache(k_pages, v_pages, rows.dtype if scales is None else _E4M3, device)
+    _scales(scales, k_pages, device)
+    _batch(device, starts, lengths, table)
     return heads, dim
 
 
+def check_positions(positions, axes, pairs, rows):
+    """Raises where append refuses these for rows of which it rotates `pairs` pairs."""
+    if positions is not None:
+        _positions(positions, axes, pairs, rows.shape[0], rows.get_device())
+    elif axes is not None:
+        raise ValueError('axes need positions')
+
+
 def append(k_pages, v_pages, k, v, starts, lengths, table, inv_freq=None, k_weight=None, q=None,
-           q_weight=None, eps=1e-6):
+           q_weight=None, eps=1e-6, positions=None, axes=None, scales=None):
     """Appends k and v [T, kv_heads, D] to the cache, k normed and rotated on the way
-    (k_weight and inv_freq as in qk_norm_rope, by its position in its sequence).
+    (k_weight and inv_freq as in qk_norm_rope, by its position in its sequence, or by
+    positions [T], or [A, T] with axes, which count for the rotation only).
+    With scales, the pages hold 8 bits: each block of 16 positions takes the smallest power
+    of two that brings the values of its rows to 448 at most.  As later calls fill it, the
+    scale only grows; rows held already are then rounded again, which changes those below
+    2^-6 of it alone.  Rows of a block behind a sequence's last keep their bits.  A value is
+    rounded once, from fp32; beyond 61440 in fp16 (0x1.Ep127 in bf16) it is held as that,
+    infinities and NaN as NaN.
     With q [T, q_heads, D], returns the queries normed and rotated for
     paged_attention, 0 in rows of no sequence.  The rows that a call writes must differ:
     no page twice among the new positions of its sequences."""
@@ -177,7 +249,8 @@ def append(k_pages, v_pages, k, v, starts, lengths, table, inv_freq=None, k_weig
     v, v_token, v_head = _rows(v, 'values')
     dtype, device, shape = k.dtype, k.get_device(), k.shape
     _same(v, dtype, device)
-    pages, stride, heads, size, dim = _cache(k_pages, v_pages, dtype, device)
+    pages, stride, heads, size, dim = _cache(k_pages, v_pages, dtype if scales is None else _E4M3,
+                                             device)
     tokens = shape[0]
     if v.shape != shape or shape[1] != heads or shape[2] != dim:
         raise ValueError('keys and values do not match the cache')
@@ -193,10 +266,19 @@ def append(k_pages, v_pages, k, v, starts, lengths, table, inv_freq=None, k_weig
         q_args = (q.data_ptr(), q_token, q_head, q_heads, q_w, q_out.data_ptr())
     k_weight, k_w = _weight(k_weight, dim, device)
     inv_freq, freq, pairs = _frequencies(inv_freq, dim, device)
-    _lib.launch(device, 'lm_paged_append', k.data_ptr(), k_token, k_head, k_w, v.data_ptr(),
-                v_token, v_head, *q_args, k_pages.data_ptr(), v_pages.data_ptr(), pages, stride,
-                heads, size, dim, *_batch(device, starts, lengths, table), freq, pairs, tokens, eps,
-                _lib.dtype_code(dtype))
+    name, places = 'lm_paged_append', ()
+    if scales is not None or positions is not None or axes is not None:
+        name, places = 'lm_paged_append_axes', (0, 0, 1, 0)
+        if positions is not None:
+            positions, axes, places = _positions(positions, axes, pairs, tokens, device)
+        elif axes is not None:
+            raise ValueError('axes need positions')
+        if scales is not None:
+            name = 'lm_paged_append_e4m3'
+    _lib.launch(device, name, k.data_ptr(), k_token, k_head, k_w, v.data_ptr(), v_token, v_head,
+                *q_args, k_pages.data_ptr(), v_pages.data_ptr(), *_scales(scales, k_pages, device),
+                pages, stride, heads, size, dim, *_batch(device, starts, lengths, table), *places,
+                freq, pairs, tokens, eps, _lib.dtype_code(dtype))
     return q_out
 
 
@@ -206,12 +288,13 @@ def _workspace_bytes(*sizes):
 
 
 def paged_attention(q, k_pages, v_pages, starts, lengths, table, scale=None, gate=None,
-                    max_new=None, out=None):
+                    max_new=None, out=None, scales=None):
     """Attention of the new tokens q [T, q_heads, D] over the cache -> [T, q_heads, D].
 
     The token at position p of its sequence sees the positions up to p; a row that sees none,
     or only scores of -inf, is 0.  Scores are fp32, and defined up to 2^23.  scale defaults to
     D ** -0.5; gate [T, q_heads, D] multiplies the result by sigmoid(gate).
+    scales belong to pages of 8 bits; of a scale only the exponent counts.
     max_new bounds the new tokens of one sequence (default: T); a close bound saves time, and
     rows of a sequence with more may be left unwritten.  The table's width counts as a
     sequence's possible length: for one sequence of few new tokens and few keys, a wide one
@@ -222,7 +305,8 @@ def paged_attention(q, k_pages, v_pages, starts, lengths, table, scale=None, gat
     memory with them, or with the cache, in another way."""
     q, q_token, q_head = _rows(q, 'queries')
     dtype, device, shape = q.dtype, q.get_device(), q.shape
-    pages, stride, heads, size, dim = _cache(k_pages, v_pages, dtype, device)
+    pages, stride, heads, size, dim = _cache(k_pages, v_pages, dtype if scales is None else _E4M3,
+                                             device)
     tokens, q_heads, q_dim = shape
     if q_dim != dim or q_heads % heads:
         raise ValueError('queries do not match the cache')
@@ -244,8 +328,8 @@ def paged_attention(q, k_pages, v_pages, starts, lengths, table, scale=None, gat
         max_new = tokens
     need = _workspace_bytes(tokens, batch[5], q_heads, heads, dim, max_new, batch[4] * size)
     workspace = q.new_empty(need // 2) if need > 0 else None
-    _lib.launch(device, 'lm_paged_attention', q.data_ptr(), q_token, q_head, q_heads,
-                k_pages.data_ptr(), v_pages.data_ptr(), pages, stride, heads, size, dim, *batch,
-                tokens, max_new, dim ** -0.5 if scale is None else scale, *gate_args,
+    _lib.launch(device, 'lm_paged_attention' if scales is None else 'lm_paged_attention_e4m3',
+                q.data_ptr(), q_token, q_head, q_heads, k_pages.data_ptr(), v_pages.data_ptr(),
+                *_scales(scales, k_pages, device), pages, stride, heads, size, dim, *batch, tokens, max_new, dim ** -0.5 if scale is None else scale, *gate_args,
                 out.data_ptr(), _lib.ptr(workspace), need, _lib.dtype_code(dtype))
     return out

@@ -2,6 +2,7 @@
 
 quantize          per-row, per-128-group dynamic int8 activation quantization
                   (w8a8.py:8-22): s = max(amax, 1e-10) * fl32(1/127), q = rint(x / s)
+norm_quantize     the residual's addition, the RMS norm and quantize in one pass
 grouped_linear    grouped W8A8 GEMV (w8a8.py:25-48): exact int32 dot per group,
                   acc = acc + (f32(p) * xs) * ws in ascending group order, no FMA
 linear            dense W8A8 linear with optional fused SwiGLU (GEMV up to 8 rows,
@@ -31,6 +32,45 @@ def quantize(x):
     _lib.call('lm_act_quant_g128', x.data_ptr(), _lib.dtype_code(x.dtype), q.data_ptr(),
               s.data_ptr(), rows, k, _lib.stream(x.device))
     return q, s
+
+
+def norm_quantize(h, weight=None, eps=1e-6, add=None):
+    """(q, s) of the normed rows of h, as quantize gives them, for gemm: the RMS norm of
+    router.rmsnorm (scale 1 + weight), quantized straight from fp32.
+
+    h [rows, K] bf16 or fp16, contiguous, K a multiple of 128 up to 16384; weight [K].  With
+    add [rows, K], h += add first, in place, and the rows normed are the sums as h then holds
+    them.  add may be h itself and shares no memory with it in another way.  Rows with
+    infinities or NaN get scales that are not finite."""
+    if not h.is_cuda or h.ndim != 2 or h.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError('Expected CUDA rows with K divisible by 128')
+    rows, k = h.shape
+    if k % 128 or not 128 <= k <= 16384:
+        raise ValueError('Expected rows of 128 to 16384 values, a multiple of 128')
+    device = h.get_device()
+    if add is not None:
+        if not h.is_contiguous() or h.data_ptr() % 16:
+            raise ValueError('Expected contiguous, 16-byte aligned rows to add to')
+        if add.shape != h.shape or add.dtype is not h.dtype or add.get_device() != device:
+            raise ValueError('the rows to add do not match')
+        add = _aligned(add)
+    else:
+        h = _aligned(h)
+    if weight is not None:
+        if weight.numel() != k:
+            raise ValueError('norm weight does not match the rows')
+        weight = _aligned(weight.to(device=h.device, dtype=torch.float32))
+    q = h.new_empty((rows, k), dtype=torch.int8)
+    s = h.new_empty((rows, k // 128), dtype=torch.float32)
+    _lib.launch(device, 'lm_norm_quant_g128', h.data_ptr(), _lib.ptr(add), _lib.ptr(weight),
+                q.data_ptr(), s.data_ptr(), rows, k, eps, _lib.dtype_code(h.dtype))
+    return q, s
+
+
+def _aligned(x):
+    """x contiguous and 16-byte aligned, a copy where it is not."""
+    x = x.contiguous()
+    return x.clone() if x.data_ptr() % 16 else x
 
 
 def _check_rows(x):
