@@ -91,8 +91,8 @@ def _frequencies(inv_freq, dim, device):
 
 
 def _positions(positions, axes, pairs, tokens, device):
-    """The positions and axes of a call (copies of others than int64 and int32), and their C
-    arguments: pointer, stride between axes, axes, each pair's axis."""
+    """The positions and axes of a call (copies of others than int64 and int32, and of tokens apart),
+    and their C arguments: pointer, stride between axes, axes, each pair's axis."""
     shape = positions.shape
     if positions.get_device() != device or not 1 <= len(shape) <= 2 or shape[-1] != tokens:
         raise ValueError('Expected a CUDA position of every token')
@@ -103,8 +103,12 @@ def _positions(positions, axes, pairs, tokens, device):
         raise ValueError('positions of several axes need the axis of every pair')
     if not 1 <= n <= 64:
         raise ValueError('Expected 1 to 64 axes of positions')
-    if positions.dtype is not torch.int64 or not positions.is_contiguous():
-        positions = positions.to(torch.int64).contiguous()
+    if positions.dtype is not torch.int64:
+        positions = positions.to(torch.int64)
+    strides = positions.stride()  # axes apart by any pitch, as in a part of a prompt's
+    if tokens > 1 and strides[-1] != 1 or n > 1 and strides[0] < tokens:
+        positions = positions.contiguous()
+        strides = positions.stride()
     axis = 0
     if axes is not None:
         if axes.numel() != pairs or axes.get_device() != device:
@@ -112,7 +116,7 @@ def _positions(positions, axes, pairs, tokens, device):
         if axes.dtype is not torch.int32 or not axes.is_contiguous():
             axes = axes.to(torch.int32).contiguous()
         axis = axes.data_ptr()
-    return positions, axes, (positions.data_ptr(), tokens, n, axis)
+    return positions, axes, (positions.data_ptr(), strides[0] if n > 1 else tokens, n, axis)
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, axes=None):

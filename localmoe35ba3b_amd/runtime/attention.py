@@ -3,8 +3,8 @@ layer's MoE block:
 
   h += o( attention( rotate(norm(q)), cache ) * sigmoid(gate) ),  [q, gate, k, v] = qkv(rmsnorm(h))
 
-with int8 projections (operators/int8.linear), the norms, rotation and append in one launch
-and paged attention (operators/attention).  Rows, heads and weights are laid out as the
+with int8 projections (operators/int8.linear, or W8A8: w8a8.norm_quantize and w8a8.gemm), the
+norms, rotation and append in one launch and paged attention (operators/attention).  Rows, heads and weights are laid out as the
 Transformers module has them (HF:627-735): a head's query and gate side by side, norm
 weights as 1 + w, the first channels of a head rotated in two halves.  The reference runs
 the Transformers module itself; its cache is a contiguous one per request
@@ -15,17 +15,19 @@ from typing import NamedTuple
 import torch
 
 from .. import router
-from ..operators import attention, int8
+from ..operators import attention, int8, w8a8
 
 
 class Batch(NamedTuple):
     """What a step's attention works on, the same for every layer: starts [sequences + 1],
     lengths [sequences] and page table [sequences, n], int32 on the GPU (operators/attention),
-    and the most new tokens of a sequence (None: not known)."""
+    the most new tokens of a sequence (None: not known), and the positions that rotate the rows, int64
+    [T] or [axes, T] on the GPU (None: their places in their sequences)."""
     starts: torch.Tensor
     lengths: torch.Tensor
     table: torch.Tensor
     max_new: int | None = None
+    positions: torch.Tensor | None = None
 
 
 class AttentionBlock:
@@ -34,14 +36,17 @@ class AttentionBlock:
     qkv and o are {'q': int8 [N, K], 'scale': fp32 [N, K / 128]} as quantize_g128 and
     Artifact.quantized give them; the rows of qkv are each head's query and, if gated, its
     gate, then the keys, then the values.  norm [H], q_norm and k_norm [head_dim] are RMSNorm
-    weights w of (1 + w), None for zeros (norm) or no norm (q_norm, k_norm)."""
+    weights w of (1 + w), None for zeros (norm) or no norm (q_norm, k_norm).  axes, int32 [pairs] on
+    the GPU, says by which axis of the batch's positions each pair is rotated.  With w8a8 the
+    projections take their rows in 8 bits too."""
 
     def __init__(self, qkv, o, q_heads, kv_heads, head_dim, norm=None, q_norm=None, k_norm=None,
-                 inv_freq=None, gated=True, eps=1e-6):
+                 inv_freq=None, gated=True, eps=1e-6, axes=None, w8a8=False):
         self.qkv, self.o = qkv, o
         self.q_heads, self.kv_heads, self.head_dim = q_heads, kv_heads, head_dim
         self.norm, self.q_norm, self.k_norm = norm, q_norm, k_norm
         self.inv_freq, self.gated, self.eps = inv_freq, gated, eps
+        self.axes, self.w8a8 = axes, w8a8
         self.q_width = q_heads * head_dim * (2 if gated else 1)
         self.kv_width = kv_heads * head_dim
         if (qkv['q'].shape[0] != self.q_width + 2 * self.kv_width
@@ -59,13 +64,17 @@ class AttentionBlock:
         for w, n in ((norm, qkv['q'].shape[1]), (q_norm, head_dim), (k_norm, head_dim)):
             if w is not None and w.numel() != n:
                 raise ValueError('norm weight does not match its rows')
-        attention.check_frequencies(inv_freq, head_dim)
-        self.k_pages = self.v_pages = None
+        self.pairs = attention.check_frequencies(inv_freq, head_dim)
+        if axes is not None and axes.numel() != self.pairs:
+            raise ValueError('Expected an axis of every rotated pair')
+        if w8a8 and qkv['q'].shape[1] > 16384:
+            raise ValueError('W8A8 projections take rows of at most 16384 values')
+        self.k_pages = self.v_pages = self.scales = None
 
     def allocate(self, pages, page_size=64, dtype=torch.bfloat16):
         """An empty cache of `pages` pages for this layer, of bf16 like the rows that forward_
-        takes."""
-        if dtype is not torch.bfloat16:
+        takes, or of 8 bits (torch.float8_e4m3fn) with its scales."""
+        if dtype not in (torch.bfloat16, torch.float8_e4m3fn):
             raise ValueError('the block appends bf16 keys and values')
         if not 16 <= page_size <= 1024 or page_size & (page_size - 1):
             raise ValueError('page size must be a power of two from 16 to 1024')
@@ -73,6 +82,10 @@ class AttentionBlock:
         device = self.qkv['q'].device
         self.k_pages = torch.empty(shape, dtype=dtype, device=device)
         self.v_pages = torch.empty(shape, dtype=dtype, device=device)
+        self.scales = None
+        if dtype is torch.float8_e4m3fn:
+            self.scales = torch.zeros((pages, self.kv_heads, 2, page_size // attention.BLOCK),
+                                      dtype=torch.float32, device=device)
         return self
 
     def check(self, h, batch):
@@ -82,7 +95,8 @@ class AttentionBlock:
                 or h.shape[1] != self.qkv['q'].shape[1]):
             raise ValueError('expected CUDA bf16 rows [tokens, hidden]')
         shape = attention.check_batch(h, self.k_pages, self.v_pages, batch.starts, batch.lengths,
-                                      batch.table)
+                                      batch.table, self.scales)
+        attention.check_positions(batch.positions, self.axes, self.pairs, h)
         if shape != (self.kv_heads, self.head_dim):
             raise ValueError('the pages do not match the heads')
 
@@ -101,7 +115,12 @@ class AttentionBlock:
         refused."""
         self._check_rows(h, batch)
         tokens, dim = h.shape[0], self.head_dim
-        x = int8.linear(router.rmsnorm(h, self.norm, self.eps), self.qkv['q'], self.qkv['scale'])
+        if self.w8a8:
+            x = w8a8.gemm(*w8a8.norm_quantize(h, self.norm, self.eps), self.qkv['q'],
+                          self.qkv['scale'])
+        else:
+            x = int8.linear(router.rmsnorm(h, self.norm, self.eps), self.qkv['q'],
+                            self.qkv['scale'])
         q, k, v = x.split([self.q_width, self.kv_width, self.kv_width], dim=1)
         q, gate = q.view(tokens, self.q_heads, self.q_width // self.q_heads), None
         if self.gated:
@@ -109,8 +128,10 @@ class AttentionBlock:
         k, v = (t.view(tokens, self.kv_heads, dim) for t in (k, v))
         place = batch.starts, batch.lengths, batch.table
         q = attention.append(self.k_pages, self.v_pages, k, v, *place, inv_freq=self.inv_freq,
-                             k_weight=self.k_norm, q=q, q_weight=self.q_norm, eps=self.eps)
+                             k_weight=self.k_norm, q=q, q_weight=self.q_norm, eps=self.eps,
+                             positions=batch.positions, axes=self.axes, scales=self.scales)
         o = attention.paged_attention(q, self.k_pages, self.v_pages, *place, gate=gate,
-                                      max_new=batch.max_new)
-        h += int8.linear(o.view(tokens, self.q_heads * dim), self.o['q'], self.o['scale'])
+                                      max_new=batch.max_new, scales=self.scales)
+        o = o.view(tokens, self.q_heads * dim)
+        h += (w8a8 if self.w8a8 else int8).linear(o, self.o['q'], self.o['scale'])
         return h

@@ -380,7 +380,9 @@ class MoEStack:
         for c0 in range(0, tokens, chunk):
             n = min(chunk, tokens - c0)
             later = (batch.starts[1:] - (c0 + n)).clamp(min=0)
-            out.append(Batch((batch.starts - c0).clamp(0, n), batch.lengths - later, batch.table, n))
+            at = None if batch.positions is None else batch.positions[..., c0:c0 + n]
+            out.append(Batch((batch.starts - c0).clamp(0, n), batch.lengths - later, batch.table, n,
+                             at))
         return out
 
     # ------------------------------------------------------------------ oracle views
