@@ -92,13 +92,17 @@ __global__ __launch_bounds__(256) void norm_quant_kernel(uint16_t *__restrict__ 
   const int64_t row = (int64_t)blockIdx.x * (4 / WAVES) + threadIdx.x / THREADS;
   if (WAVES == 1 && row >= rows) return;  // with more waves a workgroup has one row
   const int64_t at = row * n;
-  float v[CHUNKS][8];
+  float v[CHUNKS][8], g[CHUNKS][8];
   u32x4 a[CHUNKS], b[CHUNKS];
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
     const int i = min((c * THREADS + tid) * 8, n - 8);  // again the last, where there is no more
     a[c] = ldg16(h + at + i);
     if constexpr (ADD) b[c] = ldg16(x + at + i);
+    if (w) {
+      *reinterpret_cast<f32x4 *>(g[c]) = *reinterpret_cast<const f32x4 *>(w + i);
+      *reinterpret_cast<f32x4 *>(g[c] + 4) = *reinterpret_cast<const f32x4 *>(w + i + 4);
+    }
   }
   float ss = 0.0f;
 #pragma unroll
@@ -129,26 +133,30 @@ __global__ __launch_bounds__(256) void norm_quant_kernel(uint16_t *__restrict__ 
   for (int c = 0; c < CHUNKS; ++c) {
     const int i = (c * THREADS + tid) * 8;
     if (i >= n) break;  // 16 lanes at a time
-    uint32_t most = 0;
+    float most = 0.0f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       v[c][j] *= scale;
-      if (w) v[c][j] *= 1.0f + w[i + j];
-      most = max(most, __float_as_uint(v[c][j]) & 0x7FFFFFFFu);  // NaN above all
+      if (w) v[c][j] *= 1.0f + g[c][j];
+      most = __builtin_elementwise_maximum(most, fabsf(v[c][j]));  // NaN above all
     }
-    most = max(most, dpp_u32<0xB1>(most));
-    most = max(most, dpp_u32<0x4E>(most));
-    most = max(most, dpp_u32<0x141>(most));
-    most = max(most, dpp_u32<0x140>(most));
-    const float amax = __uint_as_float(max(most, __float_as_uint(1e-10f)));
-    const float group = amax * (1.0f / 127.0f);
-    uint32_t packed[2] = {};
+    uint32_t bits = __float_as_uint(most);
+    bits = max(bits, dpp_u32<0xB1>(bits));
+    bits = max(bits, dpp_u32<0x4E>(bits));
+    bits = max(bits, dpp_u32<0x141>(bits));
+    bits = max(bits, dpp_u32<0x140>(bits));
+    const float amax = __uint_as_float(max(bits, __float_as_uint(1e-10f)));
+    const float group = amax * (1.0f / 127.0f), inverse = 1.0f / group;
+    // The quotient, at most 127 and half a step, plus 1.5 * 2^23 is rint of it in the low byte.
+    uint32_t b[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      packed[j / 4] |= (uint32_t)(uint8_t)(int8_t)(int)fminf(
-                           fmaxf(rintf(v[c][j] / group), -127.0f), 127.0f)
-                       << (8 * (j % 4));
-    *reinterpret_cast<uint2 *>(q + at + i) = uint2{packed[0], packed[1]};
+      b[j] = __float_as_uint(quant_div(v[c][j], group, inverse) + 12582912.0f);
+    auto bytes = [&](int j) {
+      return __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[j + 3], b[j + 2], 0x0C0C0400u),
+                                   __builtin_amdgcn_perm(b[j + 1], b[j], 0x0C0C0400u), 0x05040100u);
+    };
+    *reinterpret_cast<uint2 *>(q + at + i) = uint2{bytes(0), bytes(4)};
     if ((tid & 15) == 0) s[(at + i) / 128] = group;
   }
 }
@@ -159,7 +167,10 @@ static int launch_norm_quant(void *h, const void *x, const float *w, int8_t *q, 
   uint16_t *hp = static_cast<uint16_t *>(h);
   const uint16_t *xp = static_cast<const uint16_t *>(x);
   const unsigned grid = (unsigned)rows;
-  if (n <= 2048)
+  if (n <= 512)  // a wave a row
+    norm_quant_kernel<T, 1, 1, ADD><<<(grid + 3) / 4, 256, 0, st>>>(hp, xp, w, q, s, rows, (int)n,
+                                                                     eps);
+  else if (n <= 2048)
     norm_quant_kernel<T, 4, 1, ADD><<<grid, 256, 0, st>>>(hp, xp, w, q, s, rows, (int)n, eps);
   else if (n <= 4096)
     norm_quant_kernel<T, 4, 2, ADD><<<grid, 256, 0, st>>>(hp, xp, w, q, s, rows, (int)n, eps);

@@ -59,7 +59,9 @@ def norm_quantize(h, weight=None, eps=1e-6, add=None):
     if weight is not None:
         if weight.numel() != k:
             raise ValueError('norm weight does not match the rows')
-        weight = _aligned(weight.to(device=h.device, dtype=torch.float32))
+        if weight.dtype is not torch.float32 or weight.get_device() != device:
+            weight = weight.to(device=h.device, dtype=torch.float32)
+        weight = _aligned(weight)
     q = h.new_empty((rows, k), dtype=torch.int8)
     s = h.new_empty((rows, k // 128), dtype=torch.float32)
     _lib.launch(device, 'lm_norm_quant_g128', h.data_ptr(), _lib.ptr(add), _lib.ptr(weight),
@@ -69,7 +71,8 @@ def norm_quantize(h, weight=None, eps=1e-6, add=None):
 
 def _aligned(x):
     """x contiguous and 16-byte aligned, a copy where it is not."""
-    x = x.contiguous()
+    if not x.is_contiguous():
+        x = x.contiguous()
     return x.clone() if x.data_ptr() % 16 else x
 
 
