@@ -199,8 +199,9 @@ __global__ __launch_bounds__(256) void head_rows_kernel(HeadRows a) {
 }
 
 // ------------------------------------------------------------------ a cache in 8 bits
-// A wave takes one side (keys or values) of one head of a block of 16 positions, as far as the call
-// writes them, in registers: norm, rotation, then the block's largest value m and its scale
+// Four waves (two for heads of 64) take one side (keys or values) of one head of a block of 16
+// positions, as far as the call writes them, in registers: norm, rotation, then the block's largest
+// value m and its scale
 //   2^e,  e the least with m <= 448 2^e,
 // not below that of the rows which the block holds already: a row is rounded again only when a later
 // one raises the scale, and as the scale is a power of two, four significant bits stay what they
@@ -217,8 +218,8 @@ struct E4m3Pages {
   uint8_t *k, *v;
   float *scales;
   int64_t scale_stride;
-  int units;      // workgroups of a block: four waves each
-  int64_t blocks;  // workgroups of blocks in all, before those of the queries' tokens
+  int shares;  // workgroups of a block, which share its heads' sides
+  int blocks;  // workgroups of blocks in all, before those of the queries' tokens
 };
 
 // Positions of sequence s that the call writes.
@@ -293,129 +294,141 @@ __device__ __forceinline__ uint32_t rescale_e4m3(uint32_t w, float ratio) {
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 template <typename T, int LANES>
-__device__ __forceinline__ void block_rows(const HeadRows &a, const E4m3Pages &p) {
-  constexpr int D = LANES * 8, ROWS = 64 / LANES, PASSES = kScaleKeys / ROWS;
+__device__ __forceinline__ void block_rows(const HeadRows &a, const E4m3Pages &p, int index) {
+  constexpr int D = LANES * 8, ROWS = 64 / LANES;  // rows of a wave at a time
+  constexpr int WAVES = LANES == 8 ? 2 : 4, UNITS = 4 / WAVES;  // of a side, sides at a time
+  constexpr int PASSES = kScaleKeys / WAVES / ROWS;
   __shared__ __attribute__((aligned(16))) float cosines[kScaleKeys][kMaxHalf],
       sines[kScaleKeys][kMaxHalf];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid % LANES, own = (tid & 63) / LANES;
-  const BlockPlace at = find_block(a, blockIdx.x / p.units);
+  __shared__ int largest[2][4];  // exponents, of the sides in turn
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid % LANES;
+  const int row = wave % WAVES * (PASSES * ROWS) + (tid & 63) / LANES;  // of the block, first pass
+  const BlockPlace at = find_block(a, index / p.shares);
   if (at.s < 0) return;
   const Written w = written(a, at.s);
   const int block = w.first / kScaleKeys + at.block, p0 = max(block * kScaleKeys, w.first);
   const int p1 = min((block + 1) * kScaleKeys, w.end);
   const int before = p0 - block * kScaleKeys, count = p1 - p0;  // rows held already, new ones
   const int row0 = w.row + p0 - w.first;                        // of the block's first new position
-  const int unit = blockIdx.x % p.units * 4 + wave;             // keys of each head, then values
-  const bool live = unit < 2 * a.k_heads, value = unit >= a.k_heads;
-  const int head = value ? unit - a.k_heads : unit;
-  const int half = value ? 0 : a.half;
-  const bool rotated = lane * 8 < 2 * half;
-  const int lo = rotated ? lane * 4 : lane * 8, hi = rotated ? half + lane * 4 : lane * 8 + 4;
-
-  Row8 raw[PASSES];
-  if (live) {
-    const uint16_t *src = value ? a.v + head * a.v_head : a.k + head * a.k_head;
-    const int64_t stride = value ? a.v_token : a.k_token;
+  const int page = paged_number(a.batch, at.s, p0), nb = 1 << (a.batch.page_shift - kScaleShift);
+  const int inside = block & (nb - 1), share = index % p.shares;
+  struct Side {  // of a head, and how a lane's channels lie there
+    int head, lo, hi;
+    bool value, rotated;
+  };
+  auto side = [&](int first) {
+    const int unit = min(first + wave / WAVES, 2 * a.k_heads - 1);  // the last one twice alike
+    const bool value = unit >= a.k_heads, rotated = !value && lane * 8 < 2 * a.half;
+    return Side{value ? unit - a.k_heads : unit, rotated ? lane * 4 : lane * 8,
+                rotated ? a.half + lane * 4 : lane * 8 + 4, value, rotated};
+  };
+  auto load = [&](const Side &d, Row8 (&raw)[PASSES]) {
+    const uint16_t *src = d.value ? a.v + d.head * a.v_head : a.k + d.head * a.k_head;
+    const int64_t stride = d.value ? a.v_token : a.k_token;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
-      const int r = min(max(i * ROWS + own - before, 0), count - 1);
+      const int r = min(max(row + i * ROWS - before, 0), count - 1);
       const uint16_t *x = src + (row0 + r) * stride;
-      raw[i] = Row8{ldg_u2(x + lo), ldg_u2(x + hi)};
+      raw[i] = Row8{ldg_u2(x + d.lo), ldg_u2(x + d.hi)};
     }
-  }
-  const int page = paged_number(a.batch, at.s, p0), nb = 1 << (a.batch.page_shift - kScaleShift);
-  const int inside = block & (nb - 1);
-  float *scale = p.scales + page * p.scale_stride + (2 * head + value) * nb + inside;
-  int least = Held<T>::kLeast;
-  if (live && before > 0) {
-    const int held = (int)(__float_as_uint(*scale) >> 23 & 0xFFu) - 127;
-    least = min(max(held, Held<T>::kLeast), Held<T>::kMost);
-  }
-  if (blockIdx.x % p.units * 4 < a.k_heads) {  // keys among the workgroup's
+  };
+  const int step = p.shares * UNITS;
+  if (share * UNITS < a.k_heads) {  // keys among the workgroup's, which come first
     for (int i = tid; i < count * a.half; i += 256) {
       const int r = i / a.half, j = i % a.half;
       turn(a, a.inv_freq[j], j, row0 + r, p0 + r, &sines[r][j], &cosines[r][j]);
     }
     __syncthreads();
   }
-  if (!live) return;
-
-  float x[PASSES][8];
-  float w0[4] = {}, w1[4] = {};
-  const float *weight = value ? nullptr : a.k_w;
-  if (weight) {
-    *reinterpret_cast<float4 *>(w0) = *reinterpret_cast<const float4 *>(weight + lo);
-    *reinterpret_cast<float4 *>(w1) = *reinterpret_cast<const float4 *>(weight + hi);
-  }
-  float most = 0.0f;
-#pragma unroll
-  for (int i = 0; i < PASSES; ++i) {
-    float *u = x[i], *v = x[i] + 4;
-    unpack4<T>(raw[i].lo, u);
-    unpack4<T>(raw[i].hi, v);
-    if (weight) {
-      float ss = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) ss = __builtin_fmaf(u[j], u[j], ss);
-      const float n = 1.0f / sqrtf(lanes_sum<LANES>(ss) * (1.0f / D) + a.eps);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) u[j] *= n * (1.0f + w0[j]), v[j] *= n * (1.0f + w1[j]);
+  for (int first = share * UNITS, odd = 0; first < 2 * a.k_heads; first += step, odd ^= 1) {
+    const Side d = side(first);
+    const int head = d.head, lo = d.lo, hi = d.hi;
+    const bool value = d.value, rotated = d.rotated;
+    Row8 raw[PASSES];
+    load(d, raw);
+    float *scale = p.scales + page * p.scale_stride + (2 * head + value) * nb + inside;
+    int least = Held<T>::kLeast;
+    if (before > 0) {
+      const int held = (int)(__float_as_uint(*scale) >> 23 & 0xFFu) - 127;
+      least = min(max(held, Held<T>::kLeast), Held<T>::kMost);
     }
-    const int r = i * ROWS + own - before;
-    const bool fresh = r >= 0 && r < count;
-    if (rotated) {
-      const int at_row = min(max(r, 0), count - 1);
-      float c[4], s[4];
-      *reinterpret_cast<float4 *>(c) = *reinterpret_cast<const float4 *>(&cosines[at_row][lo]);
-      *reinterpret_cast<float4 *>(s) = *reinterpret_cast<const float4 *>(&sines[at_row][lo]);
+    const float *weight = value ? nullptr : a.k_w;
+    float w0[4] = {}, w1[4] = {};
+    if (weight) {
+      *reinterpret_cast<float4 *>(w0) = *reinterpret_cast<const float4 *>(weight + lo);
+      *reinterpret_cast<float4 *>(w1) = *reinterpret_cast<const float4 *>(weight + hi);
+    }
+
+    float x[PASSES][8], most = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float y = u[j] * c[j] - v[j] * s[j];
-        v[j] = v[j] * c[j] + u[j] * s[j];
-        u[j] = y;
+    for (int i = 0; i < PASSES; ++i) {
+      float *u = x[i], *v = x[i] + 4;
+      unpack4<T>(raw[i].lo, u);
+      unpack4<T>(raw[i].hi, v);
+      if (weight) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss = __builtin_fmaf(u[j], u[j], ss);
+        const float n = 1.0f / sqrtf(lanes_sum<LANES>(ss) * (1.0f / D) + a.eps);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[j] *= n * (1.0f + w0[j]), v[j] *= n * (1.0f + w1[j]);
+      }
+      const int r = row + i * ROWS - before;
+      if (rotated) {
+        const int of = min(max(r, 0), count - 1);
+        float c[4], s[4];
+        *reinterpret_cast<float4 *>(c) = *reinterpret_cast<const float4 *>(&cosines[of][lo]);
+        *reinterpret_cast<float4 *>(s) = *reinterpret_cast<const float4 *>(&sines[of][lo]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float y = u[j] * c[j] - v[j] * s[j];
+          v[j] = v[j] * c[j] + u[j] * s[j];
+          u[j] = y;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float size = fabsf(u[j]);  // NaN and infinities are no part of the maximum
+        u[j] = size < INFINITY ? fminf(fmaxf(u[j], -Held<T>::kLargest), Held<T>::kLargest) : NAN;
+        if (r >= 0 && r < count && size < INFINITY) most = fmaxf(most, fabsf(u[j]));
       }
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float size = fabsf(u[j]);  // NaN and infinities are no part of the maximum
-      u[j] = size < INFINITY ? fminf(fmaxf(u[j], -Held<T>::kLargest), Held<T>::kLargest) : NAN;
-      if (fresh && size < INFINITY) most = fmaxf(most, fabsf(u[j]));
-    }
-  }
+    for (int o = 32; o >= 1; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
+    // 448 = 1.75 * 2^8: one more where the significand is above 1.75
+    int e = max((int)((__float_as_uint(most) + 0x1FFFFFu) >> 23) - 127 - 8, least);
+    if ((tid & 63) == 0) largest[odd][wave] = e;
+    __syncthreads();  // every wave has read the scale
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
-  // 448 = 1.75 * 2^8: one more where the significand is above 1.75
-  const int need = (int)((__float_as_uint(most) + 0x1FFFFFu) >> 23) - 127 - 8;
-  const int e = max(need, least);
-  uint8_t *rows = (value ? p.v : p.k) + page * a.batch.page_stride +
-                  (((int64_t)head << a.batch.page_shift) + inside * kScaleKeys) * D;
-  if (before > 0 && e > least) {
-    const float ratio = power_of_two(max(least - e, -126));
-#pragma unroll 1
-    for (int r = own; r < before; r += ROWS) {
-      uint2 *b = reinterpret_cast<uint2 *>(rows + r * D + lane * 8);
-      const uint2 old = *b;
-      *b = uint2{rescale_e4m3(old.x, ratio), rescale_e4m3(old.y, ratio)};
-    }
-  }
-  const float inverse = power_of_two(-e);
+    for (int i = 0; i < WAVES; ++i) e = max(e, largest[odd][wave / WAVES * WAVES + i]);
+    uint8_t *rows = (value ? p.v : p.k) + page * a.batch.page_stride +
+                    (((int64_t)head << a.batch.page_shift) + inside * kScaleKeys) * D;
+    const float inverse = power_of_two(-e), ratio = power_of_two(max(least - e, -126));
 #pragma unroll
-  for (int i = 0; i < PASSES; ++i) {
-    const int r = i * ROWS + own;
-    if (r < before || r >= before + count) continue;
-    *reinterpret_cast<uint32_t *>(rows + r * D + lo) = to_e4m3(x[i], inverse);
-    *reinterpret_cast<uint32_t *>(rows + r * D + hi) = to_e4m3(x[i] + 4, inverse);
+    for (int i = 0; i < PASSES; ++i) {
+      const int r = row + i * ROWS;
+      if (r < before) {
+        if (e > least) {
+          uint2 *b = reinterpret_cast<uint2 *>(rows + r * D + lane * 8);
+          const uint2 old = *b;
+          *b = uint2{rescale_e4m3(old.x, ratio), rescale_e4m3(old.y, ratio)};
+        }
+      } else if (r < before + count) {
+        *reinterpret_cast<uint32_t *>(rows + r * D + lo) = to_e4m3(x[i], inverse);
+        *reinterpret_cast<uint32_t *>(rows + r * D + hi) = to_e4m3(x[i] + 4, inverse);
+      }
+    }
+    if (tid % (WAVES * 64) == 0) *scale = power_of_two(e);
   }
-  if ((tid & 63) == 0) *scale = power_of_two(e);
 }
 
 template <typename T, int LANES>
 __global__ __launch_bounds__(256) void append_e4m3_kernel(HeadRows a, E4m3Pages p) {
   if (blockIdx.x < p.blocks) {
-    block_rows<T, LANES>(a, p);
+    block_rows<T, LANES>(a, p, blockIdx.x);
   } else {
     a.k_heads = 0;
-    token_rows<T, LANES, true>(a, (int)(blockIdx.x - p.blocks));
+    token_rows<T, LANES, true>(a, blockIdx.x - p.blocks);
   }
 }
 
@@ -553,11 +566,16 @@ int paged_append(const void *k, int64_t k_token_stride, int64_t k_head_stride,
   a.tokens = (int)tokens, a.eps = eps;
   if (e4m3) {
     E4m3Pages p = {static_cast<uint8_t *>(k_pages), static_cast<uint8_t *>(v_pages), scales,
-                   scale_stride, (int)((2 * kv_heads + 3) / 4), 0};
+                   scale_stride, 1, 0};
     // n positions of a sequence lie in at most n / 16 + 2 blocks, and in n of them
-    const int64_t most = tokens / kScaleKeys + 2 * sequences;
-    p.blocks = (most < tokens ? most : tokens) * p.units;
-    LM_REQUIRE(p.blocks + tokens < (1LL << 24), LM_EINVAL, "too many rows");
+    const int64_t bound = tokens / kScaleKeys + 2 * sequences, most = bound < tokens ? bound : tokens;
+    // Four workgroups a CU, if the sides are that many: with half or twice as many, 9 sequences of 30
+    // to 900 tokens (32 + 8 heads of 128) took 19.5 and 21.5 us instead of 19.3, 4 of 700 (16 + 16
+    // heads of 64) 16.5 and 14.5 instead of 13.1.
+    const int64_t sides = head_dim == 64 ? kv_heads : 2 * kv_heads, some = 1024 / most;
+    p.shares = (int)(some < 1 ? 1 : some < sides ? some : sides);
+    LM_REQUIRE(most * p.shares + tokens < (1LL << 24), LM_EINVAL, "too many rows");
+    p.blocks = (int)(most * p.shares);
     if (dtype == LM_BF16)
       launch_e4m3<BF16>(a, p, (int)head_dim, as_stream(stream));
     else
