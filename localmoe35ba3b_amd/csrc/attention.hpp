@@ -330,6 +330,22 @@ struct Pair {
   }
 };
 
+// Of 8-bit values NaN (0x7F and 0xFF) are the only ones, see scale_exponent: bit 7 of each byte that
+// is one.
+__device__ __forceinline__ uint32_t odd_bytes(uint32_t v) {
+  return ((v & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+}
+// v without them; `any`: there were some, in the wave.
+__device__ __forceinline__ u32x2 finite_bytes(u32x2 v, bool &any) {
+  const u32x2 s = {odd_bytes(v[0]), odd_bytes(v[1])};
+  if (__builtin_expect(__any((s[0] | s[1]) != 0), 0)) {
+    any = true;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) v[i] &= ~(s[i] | (s[i] - (s[i] >> 7)));
+  }
+  return v;
+}
+
 // Eight values of 8 bits (the type's own conversions, exact: four significant bits times a power of
 // two that keeps them normal, or whole steps of fp16's smallest).  The scale's exponent counts.
 __device__ __forceinline__ u32x4 from_e4m3(BF16, u32x2 w, float lo, float hi) {
@@ -354,11 +370,18 @@ __device__ __forceinline__ int64_t scale_place(const Attention &a, int page, int
   return page * a.scale_stride + 2 * kv * blocks + ((p >> kScaleShift) & (blocks - 1));
 }
 
-// Exponents of a block's two scales: of keys in the low byte, of values in the next.
+// Exponents of a block's two scales: of keys in the low byte, of values in the next.  None is
+// beyond what T holds the values with, whatever lies in the scales of pages that nobody uses: then
+// only NaN among the 8-bit values are not finite.
+template <typename T>
+__device__ __forceinline__ uint32_t scale_exponent(float s) {
+  return min(__float_as_uint(s) >> 23 & 0xFFu, (uint32_t)(127 + kScaleMost<T>));
+}
+template <typename T>
 __device__ __forceinline__ uint32_t load_exponents(const Attention &a, int page, int kv, int p) {
   const float *scale = a.scales + scale_place(a, page, kv, p);
   const float k = scale[0], v = scale[1 << (a.batch.page_shift - kScaleShift)];
-  return (__float_as_uint(k) >> 23 & 0xFFu) | (__float_as_uint(v) >> 15 & 0xFF00u);
+  return scale_exponent<T>(k) | scale_exponent<T>(v) << 8;
 }
 __device__ __forceinline__ float key_scale(uint32_t e) { return __uint_as_float((e & 0xFFu) << 23); }
 __device__ __forceinline__ float value_scale(uint32_t e) {
@@ -376,7 +399,7 @@ struct ValueRow {
     row = static_cast<const typename Cache<C>::Elem *>(a.v_pages) + page * a.batch.page_stride +
           head + (int64_t)(k & ((1 << a.batch.page_shift) - 1)) * D;
     if constexpr (Cache<C>::kScaled)
-      scale = a.scales[scale_place(a, page, kv, k) + (1 << (a.batch.page_shift - kScaleShift))];
+      scale = value_scale(load_exponents<T>(a, page, kv, k));
   }
   // those among the four channels from d, 0 for others
   __device__ __forceinline__ f32x4 odd_parts(int d) const {
@@ -407,11 +430,9 @@ constexpr int kBlockKeys = 4 * Cache<C>::kFewKeys;
 __device__ __forceinline__ bool few_rows(const PagedSequence &q, int group) {
   return q.count > 0 && q.count <= kFewRows / group;
 }
-// Blocks of sequence s: 0 of one that is not the few-row kernel's, at least 1 of others.
+// Blocks of a sequence: 0 of one that is not the few-row kernel's, at least 1 of others.
 template <typename C>
-__device__ __forceinline__ int few_blocks(const Attention &a, int s) {
-  if (s >= a.batch.sequences) return 0;
-  const PagedSequence q = paged_sequence(a.batch, s, a.tokens);
+__device__ __forceinline__ int few_blocks(const Attention &a, const PagedSequence &q) {
   return few_rows(q, a.group) ? max((q.length + kBlockKeys<C> - 1) / kBlockKeys<C>, 1) : 0;
 }
 
@@ -430,19 +451,20 @@ struct Find {
 
 // The spans, and the sequence that holds the first block of span `index`.  All 256 threads;
 // scratch (8 words of LDS) and found are free again afterwards.
+// `mine`: the lane's sequence, of up to 64 (of the lanes behind them, none).
 template <typename C>
-__device__ Spans find_span(const Attention &a, int index, int64_t *scratch, Find *found, Find &got) {
+__device__ Spans find_span(const Attention &a, int index, int64_t *scratch, Find *found, Find &got,
+                           PagedSequence &mine) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, S = a.batch.sequences;
   Spans sp;
   got = {0, -1};
+  auto blocks = [&](int s) {
+    return s < S ? few_blocks<C>(a, paged_sequences(a.batch, s, a.tokens)) : 0;
+  };
   if (S <= 64) {  // every wave by itself: a sequence a lane
-    const uint32_t n = few_blocks<C>(a, lane);  // 64 of at most 2^25
-    uint32_t sum = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint32_t v = __shfl_up(sum, o, 64);
-      if (lane >= o) sum += v;
-    }
+    mine = paged_sequences(a.batch, min(lane, S - 1), a.tokens);
+    const uint32_t n = lane < S ? few_blocks<C>(a, mine) : 0;  // 64 of at most 2^25
+    const uint32_t sum = wave_scan(n);
     sp.blocks = (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
     sp.spans = (int)min((int64_t)a.shares, sp.blocks);
     if (index < sp.spans) {
@@ -453,9 +475,9 @@ __device__ Spans find_span(const Attention &a, int index, int64_t *scratch, Find
     return sp;
   }
   if (tid == 0) found->s = -1;
-  const int mine = few_blocks<C>(a, tid);
-  int64_t all = mine;
-  for (int s = tid + 256; s < S; s += 256) all += few_blocks<C>(a, s);
+  const int own = blocks(tid);
+  int64_t all = own;
+  for (int s = tid + 256; s < S; s += 256) all += blocks(s);
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) all += __shfl_xor(all, o, 64);
   if (lane == 0) scratch[wave] = all;
@@ -466,13 +488,8 @@ __device__ Spans find_span(const Attention &a, int index, int64_t *scratch, Find
     const int64_t want = sp.start(index);
     int64_t base = 0;  // blocks before this group of 256 sequences
     for (int c = 0; c < S && base <= want; c += 256) {
-      const int n = c == 0 ? mine : few_blocks<C>(a, c + tid);
-      int64_t sum = n;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int64_t v = __shfl_up(sum, o, 64);
-        if (lane >= o) sum += v;
-      }
+      const int n = c == 0 ? own : blocks(c + tid);
+      const int64_t sum = (int64_t)wave_scan((uint64_t)n);
       __syncthreads();
       if (lane == 63) scratch[4 + wave] = sum;
       __syncthreads();
@@ -634,7 +651,6 @@ __device__ __forceinline__ void few_values(const LDS char *vt,
                                            const FewWeights<Cache<C>::kFewKeys> &p,
                                            const FewScales<C> &scales, bool mixed,
                                            FewState<D> &st, int lane) {
-  uint32_t any = 0;
   if constexpr (Cache<C>::kScaled) {
     constexpr int N = D == 64 ? 4 : 8;
     const u32x4 w = {p.w[0], p.w[1], p.w[2], p.w[3]};
@@ -643,17 +659,20 @@ __device__ __forceinline__ void few_values(const LDS char *vt,
     for (int i0 = 0; i0 < D / 16; i0 += N) {
       u32x2 v[N];
       few_operands8<D, N>(vt, i0, v, lane);
+      if (mixed) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        u32x4 x = from_e4m3(T{}, v[i], lo, hi);
-        if (mixed)
+        for (int i = 0; i < N; ++i) {
+          const u32x2 x = finite_bytes(v[i], st.odd);
+          st.o[i0 + i] = mfma16(T{}, from_e4m3(T{}, x, lo, hi), w, st.o[i0 + i]);
+        }
+      } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[j] = Pair<T>::finite(x[j], any);
-        st.o[i0 + i] = mfma16(T{}, x, w, st.o[i0 + i]);
+        for (int i = 0; i < N; ++i)
+          st.o[i0 + i] = mfma16(T{}, from_e4m3(T{}, v[i], lo, hi), w, st.o[i0 + i]);
       }
     }
-    if (mixed) st.odd |= __any(any != 0);
   } else {
+    uint32_t any = 0;
     u32x2 v[D / 16];
     few_operands<D>(vt, v, lane);
     const u32x2 w = {p.w[0], p.w[1]};
@@ -681,18 +700,25 @@ struct FewKeys {
   static constexpr int kUnits = Cache<C>::kFewKeys / 16, kSteps = 64 / kUnits;
 };
 
+// The lane's key among those of the steps from `from` on, its entry of the page table, and what
+// that gives: the page, and of 8 bits the scales.
 template <typename C>
-__device__ __forceinline__ void few_pages(const Attention &a, FewKeys<C> &f, int from, int kv,
-                                          int lane) {
+__device__ __forceinline__ int few_key(const FewKeys<C> &f, int from, int lane) {
   constexpr int U = FewKeys<C>::kUnits;
   const int step = f.first + min(from + lane / U, max(f.steps - 1, 0)) * f.stride;
-  const int key = step * Cache<C>::kFewKeys + lane % U * 16;
-  f.page_of = clamp_index32(f.table[min(key >> f.shift, f.entries - 1)], f.pages);
+  return step * Cache<C>::kFewKeys + lane % U * 16;
+}
+template <typename C>
+__device__ __forceinline__ int few_entry(const FewKeys<C> &f, int from, int lane) {
+  return f.table[min(few_key(f, from, lane) >> f.shift, f.entries - 1)];
+}
+template <typename T, typename C>
+__device__ __forceinline__ void few_pages(const Attention &a, FewKeys<C> &f, int entry, int from,
+                                          int kv, int lane) {
+  f.page_of = clamp_index32(entry, f.pages);
   settle(f.page_of);
-  if constexpr (Cache<C>::kScaled) {
-    f.exponents = load_exponents(a, f.page_of, kv, key);
-    settle(f.exponents);
-  }
+  if constexpr (Cache<C>::kScaled)
+    f.exponents = load_exponents<T>(a, f.page_of, kv, few_key(f, from, lane));
 }
 
 // Loads step i's rows of one side (a step past the end: again the last, never used).
@@ -792,17 +818,13 @@ __device__ __forceinline__ int64_t part_row(const Attention &a, int span, bool l
 // Blocks b0 .. b1 - 1 of sequence s at key-value head kv; `part`: its row among the parts, or
 // negative where these are all of its blocks.
 template <typename T, int D, typename C>
-__device__ __forceinline__ void few_part(const Attention &a, int s, int kv, int b0, int b1,
-                                         int64_t part, char *lds) {
+__device__ __forceinline__ void few_part(const Attention &a, const PagedSequence &seq, int s, int kv,
+                                         int b0, int b1, int64_t part, char *lds) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const PagedSequence seq = paged_sequence(a.batch, s, a.tokens);
   const int rows = seq.count * a.group;
   const int col = min(lane & 15, rows - 1), g = lane >> 4;
   const RowPlace at = row_place(a, seq, kv, col);
   u32x4 q[D / 32];
-  const uint16_t *qr = a.q + (int64_t)at.token * a.q_token + (int64_t)at.head * a.q_head;
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) q[i] = ldg16(qr + few_channel<C>(i, g)) ^ a.flip;
 
   using Elem = typename Cache<C>::Elem;
   constexpr int KEYS = Cache<C>::kFewKeys;
@@ -821,9 +843,15 @@ __device__ __forceinline__ void few_part(const Attention &a, int s, int kv, int 
 
   FewState<D> st;
   if (f.steps > 0) {
-    few_pages(a, f, 0, kv, lane);
+    // The pages' and the queries' loads go out together, the rows' behind the pages', and only then
+    // are the others waited for.
+    int entry = few_entry(f, 0, lane);
+    const uint16_t *qr = a.q + (int64_t)at.token * a.q_token + (int64_t)at.head * a.q_head;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) settle(q[i]);
+    for (int i = 0; i < D / 32; ++i) q[i] = ldg16(qr + few_channel<C>(i, g));
+    __builtin_amdgcn_sched_barrier(0);
+    settle(entry);
+    few_pages<T>(a, f, entry, 0, kv, lane);
     LDS char *ring = (LDS char *)lds + wave * few_ring<D>();
     constexpr int TILE = KEYS * D * Cache<C>::kBytes, STEPS = few_steps<D>();
     static_assert(TILE * 2 * STEPS == few_ring<D>(), "a ring holds its steps");
@@ -835,10 +863,18 @@ __device__ __forceinline__ void few_part(const Attention &a, int s, int kv, int 
       asm volatile("" ::: "memory");
     }
 #pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      settle(q[i]);
+      q[i] ^= a.flip;
+    }
+    if constexpr (Cache<C>::kScaled) settle(f.exponents);
+#pragma unroll
     for (int j = 0; j < STEPS; ++j) scales[j] = few_step_scales(f, j);
     for (int i = 0; i < f.steps; ++i) {
-      // that step is loaded next
-      if (((i + STEPS) & (FewKeys<C>::kSteps - 1)) == 0) few_pages(a, f, i + STEPS, kv, lane);
+      if (((i + STEPS) & (FewKeys<C>::kSteps - 1)) == 0) {  // that step is loaded next
+        few_pages<T>(a, f, few_entry(f, i + STEPS, lane), i + STEPS, kv, lane);
+        if constexpr (Cache<C>::kScaled) settle(f.exponents);
+      }
       const FewScales<C> now = scales[0];
 #pragma unroll
       for (int j = 1; j < STEPS; ++j) scales[j - 1] = scales[j];
@@ -903,7 +939,8 @@ __global__ __launch_bounds__(256, Cache<C>::kScaled ? 2 : 1) void attention_few_
   int64_t *scratch = reinterpret_cast<int64_t *>(lds);
   const int kv = blockIdx.x % a.batch.kv_heads, span = blockIdx.x / a.batch.kv_heads;
   Find at;
-  const Spans sp = find_span<C>(a, span, scratch, reinterpret_cast<Find *>(scratch + 8), at);
+  PagedSequence mine;
+  const Spans sp = find_span<C>(a, span, scratch, reinterpret_cast<Find *>(scratch + 8), at, mine);
   if (at.s < 0) return;
   int64_t block = sp.start(span);
   const int64_t end = sp.start(span + 1);
@@ -911,13 +948,14 @@ __global__ __launch_bounds__(256, Cache<C>::kScaled ? 2 : 1) void attention_few_
   int done = __builtin_amdgcn_readfirstlane((int)(block - at.first));  // blocks of s before
   bool later = false;
   for (; block < end && s < a.batch.sequences; ++s, done = 0) {
-    const int all = __builtin_amdgcn_readfirstlane(few_blocks<C>(a, s));
+    const PagedSequence seq = sequence_at(a.batch, s, mine, a.tokens);
+    const int all = few_blocks<C>(a, seq);
     const int take = __builtin_amdgcn_readfirstlane((int)min((int64_t)(all - done), end - block));
     if (take <= 0) continue;
     if (done == 0 && threadIdx.x == 0)  // where its parts are, for the kernel that joins them
       a.parts[s * a.batch.kv_heads + kv] = {span, later, sp.of(block + all - 1) - span + 1};
-    few_part<T, D, C>(a, s, kv, done, done + take, take == all ? -1 : part_row(a, span, later, kv),
-                   lds);
+    few_part<T, D, C>(a, seq, s, kv, done, done + take,
+                      take == all ? -1 : part_row(a, span, later, kv), lds);
     block += take;
     later = true;
   }
@@ -1014,10 +1052,8 @@ struct TileForm {
   static constexpr int kBytes = kKeys * D * Cache<C>::kBytes;  // of one side
 };
 
-// Tiles of the rows of sequence s, unless the few-row kernel takes them.
-__device__ __forceinline__ int tile_count(const Attention &a, int s) {
-  if (s >= a.batch.sequences) return 0;
-  const PagedSequence q = paged_sequence(a.batch, s, a.tokens);
+// Tiles of the rows of a sequence, unless the few-row kernel takes them.
+__device__ __forceinline__ int tile_count(const Attention &a, const PagedSequence &q) {
   if (a.few && few_rows(q, a.group)) return 0;
   return (int)(((int64_t)q.count * a.group + kTileRows - 1) / kTileRows);
 }
@@ -1028,18 +1064,17 @@ __device__ __forceinline__ int tile_keys(const PagedSequence &q, int group, int 
   return max(min(q.base + last / group + 1, q.length), 0);
 }
 
-// Keys of n tiles of sequence s together (their mean is that of the first and the last).
-__device__ __forceinline__ int64_t all_keys(const Attention &a, int s, int n) {
+// Keys of n tiles of a sequence together (their mean is that of the first and the last).
+__device__ __forceinline__ uint64_t all_keys(const Attention &a, const PagedSequence &q, int n) {
   if (n == 0) return 0;
-  const PagedSequence q = paged_sequence(a.batch, s, a.tokens);
-  return ((int64_t)tile_keys(q, a.group, 0) + tile_keys(q, a.group, n - 1)) * n / 2;
+  return ((uint64_t)tile_keys(q, a.group, 0) + tile_keys(q, a.group, n - 1)) * n / 2;
 }
 
 struct TilePlace {
   int s, tile;   // s < 0: none
   // where tiles are split each in its own way: all tiles of the call, and their keys
   int tiles;
-  int64_t keys;
+  uint64_t keys;
 };
 
 // Parts of a tile that sees `keys` keys, where sequences differ: about equal parts, as many as
@@ -1050,51 +1085,36 @@ struct TilePlace {
 // 30 % more in one case or another.
 __device__ __forceinline__ int tile_parts(const Attention &a, const TilePlace &place, int keys) {
   const int rounds = (int)((float)place.tiles * 1.5f / (float)a.room) + 1;
-  const float all = (float)max(place.keys, (int64_t)1);
+  const float all = (float)max(place.keys, (uint64_t)1);
   const float n = (float)keys * (float)(rounds * a.room - place.tiles) / all + 0.5f;
   return max(min(min((int)fminf(n, 65536.0f), a.splits), keys / 256), 1);
 }
 
-// The index-th tile; the tile with the most keys of a sequence comes first.
+// The index-th tile, and its sequence; the tile with the most keys of a sequence comes first.
 // All THREADS threads; scratch (a word and a long word a wave) and found are free again
 // afterwards.
 template <int THREADS>
-__device__ TilePlace find_tile(const Attention &a, int index, int *scratch, int64_t *sums,
-                               TilePlace *found) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+__device__ TilePlace find_tile(const Attention &a, int index, int *scratch, uint64_t *sums,
+                               TilePlace *found, PagedSequence &seq) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, S = a.batch.sequences;
   const bool split = a.room > 0;
-  if (a.batch.sequences == 1) {
-    const int n = tile_count(a, 0);
-    return {index < n ? 0 : -1, n - 1 - index, 0, 0};
-  }
-  auto scan = [&](int &sum, int64_t &keys) {  // counts up to the lane's, keys of all lanes
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int v = __shfl_up(sum, o, 64);
-      if (lane >= o) sum += v;
-    }
-    if (split)
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) keys += __shfl_xor(keys, o, 64);
-  };
-  if (a.batch.sequences <= 64) {  // each wave for itself
-    const int n = tile_count(a, lane);
-    int sum = n;
-    int64_t keys = split ? all_keys(a, lane, n) : 0;
-    scan(sum, keys);
+  if (S <= 64) {  // each wave for itself
+    const PagedSequence mine = paged_sequences(a.batch, min(lane, S - 1), a.tokens);
+    const int n = lane < S ? tile_count(a, mine) : 0, sum = (int)wave_scan((uint32_t)n);
     const uint64_t hit = __ballot(index >= sum - n && index < sum);
     if (!hit) return {-1, 0, 0, 0};
     const int at = __builtin_ctzll(hit);
-    return {at, __shfl(sum, at, 64) - 1 - index, __shfl(sum, 63, 64), keys};
+    seq = sequence_at(a.batch, at, mine, a.tokens);
+    return {at, __builtin_amdgcn_readlane(sum, at) - 1 - index, __builtin_amdgcn_readlane(sum, 63),
+            split ? wave_total(all_keys(a, mine, n)) : 0};
   }
   if (tid == 0) found->s = -1;
   int base = 0;
-  int64_t all = 0;
-  for (int c = 0; c < a.batch.sequences; c += THREADS) {
-    const int n = tile_count(a, c + tid);
-    int sum = n;
-    int64_t keys = split ? all_keys(a, c + tid, n) : 0;
-    scan(sum, keys);
+  uint64_t all = 0;
+  for (int c = 0; c < S; c += THREADS) {
+    const PagedSequence mine = paged_sequences(a.batch, min(c + tid, S - 1), a.tokens);
+    const int n = c + tid < S ? tile_count(a, mine) : 0, sum = (int)wave_scan((uint32_t)n);
+    const uint64_t keys = split ? wave_total(all_keys(a, mine, n)) : 0;
     __syncthreads();
     if (lane == 63) scratch[wave] = sum, sums[wave] = keys;
     __syncthreads();
@@ -1111,6 +1131,7 @@ __device__ TilePlace find_tile(const Attention &a, int index, int *scratch, int6
   TilePlace got = *found;
   got.tiles = base, got.keys = all;
   __syncthreads();
+  if (got.s >= 0) seq = sequence_at(a.batch, got.s, {}, a.tokens);
   return got;
 }
 
@@ -1135,17 +1156,21 @@ struct TilePages {
                        // on, until the tile there is next (its rows are loaded a tile earlier)
 };
 
+// The lane's entry of the page table for the keys from `key` on, and what that gives: the page, and
+// of 8 bits the scales.
 template <typename C>
-__device__ __forceinline__ void tile_pages(const Attention &a, TilePages<C> &f, int key, int kv,
-                                           int lane) {
+__device__ __forceinline__ int tile_entry(const TilePages<C> &f, int key, int lane) {
+  return f.table[min((key + lane * 16) >> f.shift, f.entries - 1)];
+}
+template <typename T, typename C>
+__device__ __forceinline__ void tile_pages(const Attention &a, TilePages<C> &f, int entry, int key,
+                                           int kv, int lane) {
   f.from = key;
-  const int at = key + lane * 16;
-  f.page_of = clamp_index32(f.table[min(at >> f.shift, f.entries - 1)], f.pages);
+  f.page_of = clamp_index32(entry, f.pages);
   settle(f.page_of);
-  if constexpr (Cache<C>::kScaled) {
-    f.exponents = (f.exponents & 0xFFFFu) | load_exponents(a, f.page_of, kv, at) << 16;
-    settle(f.exponents);
-  }
+  if constexpr (Cache<C>::kScaled)
+    f.exponents = (f.exponents & 0xFFFFu) |
+                  load_exponents<T>(a, f.page_of, kv, key + lane * 16) << 16;
 }
 
 // The transpose reads of 8-bit values touch other rows together than those of 16 bits.
@@ -1153,11 +1178,14 @@ template <typename C>
 constexpr Swizzle kTileValues = Cache<C>::kScaled ? kOctets : kQuads;
 
 // Loads a tile of keys and values from `key` on into LDS: ROWS rows of each a wave.
-template <int D, int ROWS, typename C>
+template <typename T, int D, int ROWS, typename C>
 __device__ __forceinline__ void tile_load(const Attention &a, TilePages<C> &f, int key,
                                           LDS char *kt, LDS char *vt, int kv, int wave, int lane) {
   constexpr int B = D * Cache<C>::kBytes;
-  if (key - f.from >= 1024) tile_pages(a, f, key, kv, lane);
+  if (key - f.from >= 1024) {
+    tile_pages<T>(a, f, tile_entry(f, key, lane), key, kv, lane);
+    if constexpr (Cache<C>::kScaled) settle(f.exponents);
+  }
 #pragma unroll
   for (int r = 0; r < ROWS; r += 16) {  // of one page each
     constexpr int N = ROWS < 16 ? ROWS : 16;
@@ -1251,15 +1279,11 @@ __device__ __forceinline__ void tile_values(E4M3, const LDS char *vt, const u32x
     return read_transposed8b<D, kOctets>(vt, base, u % 2 * 16, u / 2 * 2);
   };
   if constexpr (MIXED) {
-    uint32_t any = 0;
 #pragma unroll
     for (int u = 0; u < D / 16; ++u) {
-      u32x4 v = from_e4m3(T{}, read(u), scale[u % 2], scale[u % 2]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = Pair<T>::finite(v[j], any);
-      st.o[u / 2] = mfma32(T{}, v, p[u % 2], st.o[u / 2]);
+      const u32x2 v = finite_bytes(read(u), st.odd);
+      st.o[u / 2] = mfma32(T{}, from_e4m3(T{}, v, scale[u % 2], scale[u % 2]), p[u % 2], st.o[u / 2]);
     }
-    st.odd |= __any(any != 0);
     return;
   }
   __builtin_amdgcn_s_setprio(1);
@@ -1402,16 +1426,19 @@ __global__ __launch_bounds__((TileForm<D, C>::kWaves * 64), 2) void attention_ti
   // One array: with several, the compiler waits for all direct loads at each LDS read.
   __shared__ __attribute__((aligned(16))) char lds[tile_lds<D, C>()];
   int *scratch = reinterpret_cast<int *>(lds);
-  int64_t *key_sums = reinterpret_cast<int64_t *>(scratch + 8);
+  uint64_t *key_sums = reinterpret_cast<uint64_t *>(scratch + 8);
   TilePlace *found = reinterpret_cast<TilePlace *>(key_sums + 8);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int set = wave & 3, group = wave >> 2;
-  const int kv = blockIdx.x % a.batch.kv_heads, split = blockIdx.y;
+  // Where tiles have parts of their own count, a tile's parts lie next to each other: those that
+  // there are begin among those that there are not, and none of them last.
+  const int kv = blockIdx.x % a.batch.kv_heads, index = blockIdx.x / a.batch.kv_heads;
+  const int split = a.room ? index % a.splits : (int)blockIdx.y;
+  PagedSequence seq;
   const TilePlace place =
-      find_tile<WAVES * 64>(a, blockIdx.x / a.batch.kv_heads, scratch, key_sums, found);
+      find_tile<WAVES * 64>(a, a.room ? index / a.splits : index, scratch, key_sums, found, seq);
   const int s = __builtin_amdgcn_readfirstlane(place.s);
   if (s < 0) return;
-  const PagedSequence seq = paged_sequence(a.batch, s, a.tokens);
   const int tile = __builtin_amdgcn_readfirstlane(place.tile);
   const int rows = seq.count * a.group, c0 = tile * kTileRows;
   const int c = c0 + set * 32 + (lane & 31);
@@ -1437,12 +1464,21 @@ __global__ __launch_bounds__((TileForm<D, C>::kWaves * 64), 2) void attention_ti
     f.k = static_cast<const Elem *>(a.k_pages) + head;
     f.v = static_cast<const Elem *>(a.v_pages) + head, f.shift = a.batch.page_shift;
     f.pages = a.batch.pages, f.entries = a.batch.table_pages, f.exponents = 0;
-    tile_pages(a, f, key0, kv, lane);
-    tile_load<D, ROWS>(a, f, key0, base, base + TILE, kv, wave, lane);
+    // The pages' and the queries' loads go out together, the rows' behind the pages', and only then
+    // are the others waited for.
+    int entry = tile_entry(f, key0, lane);
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) q[i] = ldg16(qr + tile_channel<C>(i, lane >> 5)) ^ a.flip;
+    for (int i = 0; i < D / 16; ++i) q[i] = ldg16(qr + tile_channel<C>(i, lane >> 5));
+    __builtin_amdgcn_sched_barrier(0);
+    settle(entry);
+    tile_pages<T>(a, f, entry, key0, kv, lane);
+    tile_load<T, D, ROWS>(a, f, key0, base, base + TILE, kv, wave, lane);
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) settle(q[i]);
+    for (int i = 0; i < D / 16; ++i) {
+      settle(q[i]);
+      q[i] ^= a.flip;
+    }
+    if constexpr (Cache<C>::kScaled) settle(f.exponents);
     wait_loads<0>();
     __syncthreads();
     // A tile, the next one's loads started before it into the other half.
@@ -1452,7 +1488,7 @@ __global__ __launch_bounds__((TileForm<D, C>::kWaves * 64), 2) void attention_ti
       LDS char *cur = base + half * 2 * TILE, *next = base + (half ^ 1) * 2 * TILE;
       tile_advance(f, key);
       if (key + KEYS < key1)
-        tile_load<D, ROWS>(a, f, key + KEYS, next, next + TILE, kv, wave, lane);
+        tile_load<T, D, ROWS>(a, f, key + KEYS, next, next + TILE, kv, wave, lane);
       if (!idle)
 #pragma unroll
         for (int i = 0; i < F::kSteps; ++i) {
@@ -1467,7 +1503,7 @@ __global__ __launch_bounds__((TileForm<D, C>::kWaves * 64), 2) void attention_ti
       LDS char *cur = base + half * 2 * TILE, *next = base + (half ^ 1) * 2 * TILE;
       tile_advance(f, key);
       if (key + KEYS < key1)
-        tile_load<D, ROWS>(a, f, key + KEYS, next, next + TILE, kv, wave, lane);
+        tile_load<T, D, ROWS>(a, f, key + KEYS, next, next + TILE, kv, wave, lane);
       if (!idle)
 #pragma unroll
         for (int i = 0; i < F::kSteps; ++i) {
@@ -1694,13 +1730,16 @@ int launch_attention(const AttentionPlan &p, Attention a, float *workspace, hipS
   if (p.few) {
     attention_few_kernel<T, D, C><<<(unsigned)p.few_grid, 256, 0, st>>>(a);
     if (const int rc = check_launch("attention_few_kernel")) return rc;
-    // Where there are few sequences, their rows and channels fill the chip.
-    const int64_t units = kFewRows / a.group * a.group * (D / 64), some = 4096 / p.parts;
+    // Where there are few sequences, their rows and channels fill the chip.  Against four times as
+    // many workgroups at most, 24 sequences with 2 to 9 rows took 24.4 instead of 25.7 us and 12 of up
+    // to 700 new tokens 48.0 instead of 49.0; half as many took 53.7 there.
+    const int64_t units = kFewRows / a.group * a.group * (D / 64), some = 1024 / p.parts;
     ys = some < 1 ? 1 : some < units ? some : units;
   }
   const int chunks = (a.q_heads * (D / 4) + 255) / 256;
   if (p.tile) {
-    const dim3 grid((unsigned)(p.tiles * a.batch.kv_heads), (unsigned)p.splits);
+    const int64_t all = p.tiles * a.batch.kv_heads;
+    const dim3 grid((unsigned)(p.room ? all * p.splits : all), (unsigned)(p.room ? 1 : p.splits));
     attention_tile_kernel<T, D, C><<<grid, TileForm<D, C>::kWaves * 64, 0, st>>>(a);
     if (const int rc = check_launch("attention_tile_kernel")) return rc;
     if (p.splits > 1) tile = (int64_t)a.tokens * chunks;

@@ -79,13 +79,38 @@ __device__ __forceinline__ void turn(const HeadRows &a, float freq, int i, int t
   sincospif(2.0f * (float)(turns - rint(turns)), s, c);
 }
 
+// The sequence of row t, negative for none, and its position there.  All 256 threads; of up to 64
+// sequences each wave looks by itself.
+struct TokenPlace {
+  int s, position;
+};
+__device__ __forceinline__ TokenPlace find_token(const HeadRows &a, int t) {
+  __shared__ int found, at;
+  const int tid = threadIdx.x, S = a.batch.sequences;
+  if (S <= 64) {
+    const int k = min(tid & 63, S - 1);
+    int first = a.batch.starts[k], end = a.batch.starts[k + 1], n = a.batch.lengths[k];
+    asm volatile("" : "+v"(first), "+v"(end), "+v"(n));  // looked up together
+    const uint64_t hit = __ballot(first <= t && t < end);
+    if (!hit) return {-1, 0};
+    const int s = min((int)__builtin_ctzll(hit), S - 1);
+    return {s, __builtin_amdgcn_readlane(n - (end - first) + (t - first), s)};
+  }
+  if (tid == 0) found = -1;
+  __syncthreads();
+  for (int s = tid; s < S; s += 256) {
+    const int first = a.batch.starts[s], end = a.batch.starts[s + 1], n = a.batch.lengths[s];
+    if (first <= t && t < end) found = s, at = n - (end - first) + (t - first);
+  }
+  __syncthreads();
+  return {found, at};
+}
+
 // The rows of token t.
 template <typename T, int LANES, bool PAGED>
 __device__ __forceinline__ void token_rows(const HeadRows &a, int t) {
   constexpr int D = LANES * 8, ROWS = 256 / LANES;
   __shared__ __attribute__((aligned(16))) float cosines[kMaxHalf], sines[kMaxHalf];
-  __shared__ int64_t place;  // element offset of the token's row of head 0 in the cache; < 0: none
-  __shared__ int found, at;  // the token's sequence and position
   const int tid = threadIdx.x, lane = tid % LANES, half = a.half;
   const int heads = a.q_heads + a.k_heads + (PAGED ? a.k_heads : 0);
   const bool rotated = lane * 8 < 2 * half;
@@ -108,32 +133,25 @@ __device__ __forceinline__ void token_rows(const HeadRows &a, int t) {
   int position = 0;
   int64_t to = 0;
   if constexpr (PAGED) {
-    if (tid == 0) found = -1;
-    __syncthreads();
-    for (int s = tid; s < a.batch.sequences; s += 256) {
-      const int first = a.batch.starts[s], end = a.batch.starts[s + 1], n = a.batch.lengths[s];
-      if (first <= t && t < end) found = s, at = n - (end - first) + (t - first);
-    }
-    __syncthreads();
-    if (found < 0) {  // a row of no sequence
+    const TokenPlace of = find_token(a, t);
+    if (of.s < 0) {  // a row of no sequence
       for (int r = r0; r < a.q_heads; r += ROWS) {
         uint16_t *dst = a.q_out + ((int64_t)t * a.q_heads + r) * D;
         *reinterpret_cast<uint2 *>(dst + lo) = *reinterpret_cast<uint2 *>(dst + hi) = uint2{0, 0};
       }
       return;
     }
-    const int p = at;
-    position = p;
-    if (tid == 255) {
+    position = of.position;
+    if (a.k_heads) {  // offset of the token's row of head 0 in the cache; negative: none
       const int64_t room = (int64_t)a.batch.table_pages << a.batch.page_shift;
-      place = p < 0 || p >= room ? -1
-                                 : paged_page(a.batch, found, p) +
-                                       (int64_t)(p & ((1 << a.batch.page_shift) - 1)) * D;
+      to = position < 0 || position >= room
+               ? -1
+               : paged_page(a.batch, of.s, position) +
+                     (int64_t)(position & ((1 << a.batch.page_shift) - 1)) * D;
     }
   }
   if (tid < half) turn(a, freq, tid, t, position, &sines[tid], &cosines[tid]);
   __syncthreads();
-  if constexpr (PAGED) to = place;
 
   float c[4], s[4];
   if (rotated) {
@@ -206,14 +224,6 @@ __global__ __launch_bounds__(256) void head_rows_kernel(HeadRows a) {
 // not below that of the rows which the block holds already: a row is rounded again only when a later
 // one raises the scale, and as the scale is a power of two, four significant bits stay what they
 // were but for values below 2^-6 of it.  Straight from fp32, so a value is rounded once.
-template <typename T>
-struct Held {  // exponents of scales: the least keeps steps of 2^-9 in T, the largest a value of ..
-  static constexpr int kLeast = __is_same(T, FP16) ? -15 : -117;
-  static constexpr int kMost = __is_same(T, FP16) ? 8 : 120;
-  // .. four significant bits that T holds: 61440 in fp16
-  static constexpr float kLargest = __is_same(T, FP16) ? 61440.0f : 0x1.Ep127f;
-};
-
 struct E4m3Pages {
   uint8_t *k, *v;
   float *scales;
@@ -347,10 +357,10 @@ __device__ __forceinline__ void block_rows(const HeadRows &a, const E4m3Pages &p
     Row8 raw[PASSES];
     load(d, raw);
     float *scale = p.scales + page * p.scale_stride + (2 * head + value) * nb + inside;
-    int least = Held<T>::kLeast;
+    int least = kScaleLeast<T>;
     if (before > 0) {
       const int held = (int)(__float_as_uint(*scale) >> 23 & 0xFFu) - 127;
-      least = min(max(held, Held<T>::kLeast), Held<T>::kMost);
+      least = min(max(held, kScaleLeast<T>), kScaleMost<T>);
     }
     const float *weight = value ? nullptr : a.k_w;
     float w0[4] = {}, w1[4] = {};
@@ -389,7 +399,7 @@ __device__ __forceinline__ void block_rows(const HeadRows &a, const E4m3Pages &p
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float size = fabsf(u[j]);  // NaN and infinities are no part of the maximum
-        u[j] = size < INFINITY ? fminf(fmaxf(u[j], -Held<T>::kLargest), Held<T>::kLargest) : NAN;
+        u[j] = size < INFINITY ? fminf(fmaxf(u[j], -kHeldMost<T>), kHeldMost<T>) : NAN;
         if (r >= 0 && r < count && size < INFINITY) most = fmaxf(most, fabsf(u[j]));
       }
     }

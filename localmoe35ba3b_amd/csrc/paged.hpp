@@ -28,12 +28,60 @@ struct PagedSequence {
   int first, count, base, length;
 };
 
-__device__ __forceinline__ PagedSequence paged_sequence(const PagedBatch &b, int s, int tokens) {
-  const int lo = b.starts[s], hi = b.starts[s + 1], len = b.lengths[s];
+__device__ __forceinline__ PagedSequence paged_sequence(const PagedBatch &b, int lo, int hi, int len,
+                                                       int tokens) {
   const int room = b.table_pages << b.page_shift;
   const int first = min(max(lo, 0), tokens);
   return {first, max(min(hi, tokens) - first, 0), len - (hi - lo) + (first - lo),
           min(max(len, 0), room)};
+}
+
+__device__ __forceinline__ PagedSequence paged_sequence(const PagedBatch &b, int s, int tokens) {
+  return paged_sequence(b, b.starts[s], b.starts[s + 1], b.lengths[s], tokens);
+}
+// Sums over the lanes up to each of a wave (whole numbers), without the LDS round trips of shuffles:
+// within 16 lanes, then over the 16s and the halves before.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t lanes_before(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t lanes_before(uint64_t v) {
+  return (uint64_t)lanes_before<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 |
+         lanes_before<CTRL, ROWS>((uint32_t)v);
+}
+template <typename U>
+__device__ __forceinline__ U wave_scan(U v) {
+  v += lanes_before<0x111, 0xF>(v);
+  v += lanes_before<0x112, 0xF>(v);
+  v += lanes_before<0x114, 0xF>(v);
+  v += lanes_before<0x118, 0xF>(v);
+  v += lanes_before<0x142, 0xA>(v);  // lane 15 of the 16 before
+  v += lanes_before<0x143, 0xC>(v);  // lane 31
+  return v;
+}
+__device__ __forceinline__ uint64_t wave_total(uint64_t v) {
+  const uint64_t s = wave_scan(v);
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(s >> 32), 63) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)s, 63);
+}
+
+// The sequence of each lane, looked up in one round of loads: left to itself, the compiler looks for
+// the length only where the starts leave new tokens.
+__device__ __forceinline__ PagedSequence paged_sequences(const PagedBatch &b, int s, int tokens) {
+  int lo = b.starts[s], hi = b.starts[s + 1], len = b.lengths[s];
+  asm volatile("" : "+v"(lo), "+v"(hi), "+v"(len));
+  return paged_sequence(b, lo, hi, len, tokens);
+}
+// Sequence s, the same for every lane: of up to 64 from the lane that has it.
+__device__ __forceinline__ PagedSequence sequence_at(const PagedBatch &b, int s,
+                                                     const PagedSequence &mine, int tokens) {
+  if (b.sequences <= 64)
+    return {__builtin_amdgcn_readlane(mine.first, s), __builtin_amdgcn_readlane(mine.count, s),
+            __builtin_amdgcn_readlane(mine.base, s), __builtin_amdgcn_readlane(mine.length, s)};
+  const PagedSequence q = paged_sequences(b, s, tokens);
+  return {__builtin_amdgcn_readfirstlane(q.first), __builtin_amdgcn_readfirstlane(q.count),
+          __builtin_amdgcn_readfirstlane(q.base), __builtin_amdgcn_readfirstlane(q.length)};
 }
 
 // Position p's page of sequence s, and its element offset.
@@ -49,6 +97,14 @@ __device__ __forceinline__ int64_t paged_page(const PagedBatch &b, int s, int p)
 // scale, a power of two, for each kScaleKeys positions of a head, keys and values apart.
 struct E4M3 {};
 constexpr int kScaleKeys = 16, kScaleShift = 4;
+// Exponents of scales for rows of type T: the least keeps steps of 2^-9 of a scale in T, the largest
+// a value of four significant bits that T holds, kHeldMost (61440 in fp16).
+template <typename T>
+constexpr int kScaleLeast = __is_same(T, FP16) ? -15 : -117;
+template <typename T>
+constexpr int kScaleMost = __is_same(T, FP16) ? 8 : 120;
+template <typename T>
+constexpr float kHeldMost = __is_same(T, FP16) ? 61440.0f : 0x1.Ep127f;
 
 // A launch has fewer than 2^32 threads; the kernels take at most 256 for a token.
 constexpr int64_t kMaxTokens = 1LL << 24;
