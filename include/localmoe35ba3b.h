@@ -465,9 +465,10 @@ int lm_paged_attention(const void *q, int64_t q_token_stride, int64_t q_head_str
                        void *stream);
 
 /* lm_paged_attention over the cache of lm_paged_append_e4m3, whose keys and values
- * are e4m3 times the power of two of their block (of a scale only the exponent
- * counts), exact in dtype as they enter the products.  The workspace is as large as
- * that of lm_paged_attention. */
+ * are e4m3 times the power of two of their block, exact in dtype as they enter the
+ * products.  Of a scale only the exponent counts, and one beyond 120 in bf16 or 8 in
+ * fp16, the largest that the append makes, counts as that.  The workspace is as
+ * large as that of lm_paged_attention. */
 int lm_paged_attention_e4m3(const void *q, int64_t q_token_stride, int64_t q_head_stride,
                             int64_t q_heads, const void *k_pages, const void *v_pages,
                             const float *scales, int64_t scale_stride, int64_t pages,

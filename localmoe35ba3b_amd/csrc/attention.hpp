@@ -330,14 +330,17 @@ struct Pair {
   }
 };
 
-// Of 8-bit values NaN (0x7F and 0xFF) are the only ones, see scale_exponent: bit 7 of each byte that
-// is one.
-__device__ __forceinline__ uint32_t odd_bytes(uint32_t v) {
-  return ((v & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+// Of 8-bit values NaN (0x7F and 0xFF), and under the largest scale, of which no larger is looked up
+// (scale_exponent), those from 256 on (0x78): bit 7 of each byte that is one.
+template <typename T>
+__device__ __forceinline__ uint32_t odd_bytes(uint32_t v, float scale) {
+  const bool largest = __float_as_uint(scale) >> 23 == 127 + kScaleMost<T>;
+  return ((v & 0x7F7F7F7Fu) + (largest ? 0x08080808u : 0x01010101u)) & 0x80808080u;
 }
 // v without them; `any`: there were some, in the wave.
-__device__ __forceinline__ u32x2 finite_bytes(u32x2 v, bool &any) {
-  const u32x2 s = {odd_bytes(v[0]), odd_bytes(v[1])};
+template <typename T>
+__device__ __forceinline__ u32x2 finite_bytes(u32x2 v, float lo, float hi, bool &any) {
+  const u32x2 s = {odd_bytes<T>(v[0], lo), odd_bytes<T>(v[1], hi)};
   if (__builtin_expect(__any((s[0] | s[1]) != 0), 0)) {
     any = true;
 #pragma unroll
@@ -371,8 +374,7 @@ __device__ __forceinline__ int64_t scale_place(const Attention &a, int page, int
 }
 
 // Exponents of a block's two scales: of keys in the low byte, of values in the next.  None is
-// beyond what T holds the values with, whatever lies in the scales of pages that nobody uses: then
-// only NaN among the 8-bit values are not finite.
+// beyond those of the append, whatever lies in the scales of pages that nobody uses.
 template <typename T>
 __device__ __forceinline__ uint32_t scale_exponent(float s) {
   return min(__float_as_uint(s) >> 23 & 0xFFu, (uint32_t)(127 + kScaleMost<T>));
@@ -662,7 +664,7 @@ __device__ __forceinline__ void few_values(const LDS char *vt,
       if (mixed) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          const u32x2 x = finite_bytes(v[i], st.odd);
+          const u32x2 x = finite_bytes<T>(v[i], lo, hi, st.odd);
           st.o[i0 + i] = mfma16(T{}, from_e4m3(T{}, x, lo, hi), w, st.o[i0 + i]);
         }
       } else {
@@ -1281,8 +1283,9 @@ __device__ __forceinline__ void tile_values(E4M3, const LDS char *vt, const u32x
   if constexpr (MIXED) {
 #pragma unroll
     for (int u = 0; u < D / 16; ++u) {
-      const u32x2 v = finite_bytes(read(u), st.odd);
-      st.o[u / 2] = mfma32(T{}, from_e4m3(T{}, v, scale[u % 2], scale[u % 2]), p[u % 2], st.o[u / 2]);
+      const float own = scale[u % 2];
+      const u32x2 v = finite_bytes<T>(read(u), own, own, st.odd);
+      st.o[u / 2] = mfma32(T{}, from_e4m3(T{}, v, own, own), p[u % 2], st.o[u / 2]);
     }
     return;
   }

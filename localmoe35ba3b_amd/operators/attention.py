@@ -9,7 +9,8 @@ paged_attention   each sequence's new tokens over its cache, causal at its end
 A cache is two tensors [pages, kv_heads, page_size, head_dim], keys and values, of the
 rows' type or of 8 bits: torch.float8_e4m3fn with `scales`, fp32 [pages, kv_heads, 2,
 page_size // 16], a power of two for each 16 positions of a head (of keys, then of
-values) by which its values are multiplied.  A batch is three int32 tensors on the GPU, which a program keeps for all layers of a
+values) by which its values are multiplied; a page that is copied takes its scales along.
+A batch is three int32 tensors on the GPU, which a program keeps for all layers of a
 step and may rewrite between replays of a captured step:
   starts  [sequences + 1]  the rows of sequence s are starts[s] .. starts[s + 1] - 1
   lengths [sequences]      its positions, the new ones (its last) among them
@@ -298,7 +299,8 @@ def paged_attention(q, k_pages, v_pages, starts, lengths, table, scale=None, gat
     The token at position p of its sequence sees the positions up to p; a row that sees none,
     or only scores of -inf, is 0.  Scores are fp32, and defined up to 2^23.  scale defaults to
     D ** -0.5; gate [T, q_heads, D] multiplies the result by sigmoid(gate).
-    scales belong to pages of 8 bits; of a scale only the exponent counts.
+    scales belong to pages of 8 bits; of a scale only the exponent counts, and one beyond 120
+    in bf16 or 8 in fp16 counts as that.
     max_new bounds the new tokens of one sequence (default: T); a close bound saves time, and
     rows of a sequence with more may be left unwritten.  The table's width counts as a
     sequence's possible length: for one sequence of few new tokens and few keys, a wide one

@@ -368,6 +368,38 @@ def test_attention_every_code_and_scale(dev, new, dtype):
     U.assert_attention(got, U.attention(q, *kv, starts, lengths, table), 'codes')
 
 
+@TYPES
+@pytest.mark.parametrize('dim', [64, 128, 256])
+@pytest.mark.parametrize('new', [1, 40])
+def test_attention_values_beyond_the_type_that_no_row_sees(dev, new, dim, dtype):
+    """Under the largest scale the upper 8-bit values are infinities of the type: behind a sequence's
+    end they reach no row, and before it only those that see them."""
+    gen = seeded(dim)
+    lens = [(new, 85), (new, 70)]
+    starts, lengths, table, pages = U.batch(lens, 16)
+    q = rand(gen, 2 * new, 4, dim, dtype=dtype)
+    kp, vp, scales = C.random_cache(gen, pages, 2, 16, dim, dtype)
+    last = [int(table[s, n // 16]) for s, (_, n) in enumerate(lens)]  # blocks that rows go on in
+    scales[last, :, 1] = 2.0 ** (120 if dtype == BF16 else 8)
+    vb = vp.view(torch.uint8)
+    for at, (_, n) in zip(last, lens):
+        vb[at] = torch.randint(0, 2, vb[at].shape, generator=gen).to(torch.uint8)  # tiny, seen
+        vb[at, :, n % 16:] = torch.randint(0x78, 0x7F, vb[at, :, n % 16:].shape, generator=gen).to(torch.uint8)
+    k64, v64 = C.held(kp, vp, scales, dtype)
+    for at, (_, n) in zip(last, lens):
+        assert v64[at, :, n % 16:].isinf().all()
+    got = A.paged_attention(*to(dev, q, kp, vp, starts, lengths, table), scales=scales.to(dev)).cpu()
+    want = U.attention(q, k64, v64, starts, lengths, table)
+    U.assert_attention(got, want, 'behind the end')
+    at, bad = last[0], 85 - max(1, new // 2)  # a position of sequence 0 that its last rows see
+    if bad // 16 == 85 // 16:
+        vb[at, 0, bad % 16, 3] = 0x78
+        got = A.paged_attention(*to(dev, q, kp, vp, starts, lengths, table), scales=scales.to(dev)).cpu()
+        assert got[new - (85 - bad):new, :2, 3].isinf().all()
+        got[new - (85 - bad):new, :2, 3] = want[0][new - (85 - bad):new, :2, 3].to(dtype)
+        U.assert_attention(got, want, 'rows before it')
+
+
 def test_attention_malformed_batches_stay_in_bounds(dev):
     """Page numbers, lengths and starts out of range, for both operators: some result, no access
     outside."""
