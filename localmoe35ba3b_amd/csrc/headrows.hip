@@ -396,11 +396,22 @@ __device__ __forceinline__ void block_rows(const HeadRows &a, const E4m3Pages &p
           u[j] = y;
         }
       }
+      float top = 0.0f;  // fmaxf passes over NaN
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float size = fabsf(u[j]);  // NaN and infinities are no part of the maximum
-        u[j] = size < INFINITY ? fminf(fmaxf(u[j], -kHeldMost<T>), kHeldMost<T>) : NAN;
-        if (r >= 0 && r < count && size < INFINITY) most = fmaxf(most, fabsf(u[j]));
+      for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(u[j]));
+      if (r >= 0 && r < count) most = fmaxf(most, top);
+    }
+    if (__builtin_expect(__any(most > kHeldMost<T>), 0)) {  // and over infinities
+      most = 0.0f;
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i) {
+        const int r = row + i * ROWS - before;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float size = fabsf(x[i][j]);
+          x[i][j] = size < INFINITY ? fminf(fmaxf(x[i][j], -kHeldMost<T>), kHeldMost<T>) : NAN;
+          if (r >= 0 && r < count && size < INFINITY) most = fmaxf(most, fabsf(x[i][j]));
+        }
       }
     }
 #pragma unroll
