@@ -232,50 +232,43 @@ struct E4m3Pages {
   int blocks;  // workgroups of blocks in all, before those of the queries' tokens
 };
 
-// Positions of sequence s that the call writes.
+// Positions of a sequence that the call writes.
 struct Written {
   int first, end;  // positions; first >= end: none
   int row;         // of `first`
 };
-__device__ __forceinline__ Written written(const HeadRows &a, int s) {
-  const PagedSequence q = paged_sequence(a.batch, s, a.tokens);
+__device__ __forceinline__ Written written(const HeadRows &a, const PagedSequence &q) {
   const int room = a.batch.table_pages << a.batch.page_shift;
   const int first = max(q.base, 0);
   return {first, (int)min((int64_t)q.base + q.count, (int64_t)room), q.first + first - q.base};
 }
-__device__ __forceinline__ int block_count(const HeadRows &a, int s) {
-  if (s >= a.batch.sequences) return 0;
-  const Written w = written(a, s);
+__device__ __forceinline__ int block_count(const HeadRows &a, const PagedSequence &q) {
+  const Written w = written(a, q);
   return w.first < w.end ? (w.end - 1) / kScaleKeys - w.first / kScaleKeys + 1 : 0;
 }
 
-// Sequence and place there of the index-th block of all; s < 0: none.  All 256 threads.
+// Sequence of the index-th block of all, and the block's place there; s < 0: none.  All 256 threads.
 struct BlockPlace {
   int s, block;
 };
-__device__ BlockPlace find_block(const HeadRows &a, int64_t index) {
+__device__ BlockPlace find_block(const HeadRows &a, int index, PagedSequence &seq) {
   __shared__ int sums[4];
   __shared__ BlockPlace found;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  auto scan = [&](int n) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int v = __shfl_up(n, o, 64);
-      if (lane >= o) n += v;
-    }
-    return n;
-  };
-  if (a.batch.sequences <= 64) {  // each wave for itself
-    const int n = block_count(a, lane), sum = scan(n);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, S = a.batch.sequences;
+  if (S <= 64) {  // each wave for itself
+    const PagedSequence mine = paged_sequences(a.batch, min(lane, S - 1), a.tokens);
+    const int n = lane < S ? block_count(a, mine) : 0, sum = (int)wave_scan((uint32_t)n);
     const uint64_t hit = __ballot(index >= sum - n && index < sum);
     if (!hit) return {-1, 0};
     const int at = __builtin_ctzll(hit);
-    return {at, (int)index - __shfl(sum - n, at, 64)};
+    seq = sequence_at(a.batch, at, mine, a.tokens);
+    return {at, index - __builtin_amdgcn_readlane(sum - n, at)};
   }
   if (tid == 0) found = {-1, 0};
   int64_t base = 0;
-  for (int c = 0; c < a.batch.sequences && base <= index; c += 256) {
-    const int n = block_count(a, c + tid), sum = scan(n);
+  for (int c = 0; c < S && base <= index; c += 256) {
+    const PagedSequence mine = paged_sequences(a.batch, min(c + tid, S - 1), a.tokens);
+    const int n = c + tid < S ? block_count(a, mine) : 0, sum = (int)wave_scan((uint32_t)n);
     __syncthreads();
     if (lane == 63) sums[wave] = sum;
     __syncthreads();
@@ -287,6 +280,7 @@ __device__ BlockPlace find_block(const HeadRows &a, int64_t index) {
     if (index >= before && index < before + n) found = {c + tid, (int)(index - before)};
   }
   __syncthreads();
+  if (found.s >= 0) seq = sequence_at(a.batch, found.s, {}, a.tokens);
   return found;
 }
 
@@ -313,9 +307,10 @@ __device__ __forceinline__ void block_rows(const HeadRows &a, const E4m3Pages &p
   __shared__ int largest[2][4];  // exponents, of the sides in turn
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid % LANES;
   const int row = wave % WAVES * (PASSES * ROWS) + (tid & 63) / LANES;  // of the block, first pass
-  const BlockPlace at = find_block(a, index / p.shares);
+  PagedSequence seq;
+  const BlockPlace at = find_block(a, index / p.shares, seq);
   if (at.s < 0) return;
-  const Written w = written(a, at.s);
+  const Written w = written(a, seq);
   const int block = w.first / kScaleKeys + at.block, p0 = max(block * kScaleKeys, w.first);
   const int p1 = min((block + 1) * kScaleKeys, w.end);
   const int before = p0 - block * kScaleKeys, count = p1 - p0;  // rows held already, new ones
