@@ -18,8 +18,8 @@
 // the longest chain of a small call.
 //
 // Bound by the rows' bytes where there are many, by that chain where there are few.  18 heads
-// of 256: 4096 tokens 16 us (75.5 MB, 4.7 TB/s), one token 3 us; 64 tokens into a cache 5 us;
-// 3310 tokens into a cache (48 heads of 128) 18 us (81 MB, 4.6 TB/s).
+// of 256: 4096 tokens 16 us (75.5 MB, 4.7 TB/s), one token 3 us, of three axes too; 64 tokens
+// into a cache 4 us; 3310 tokens into a cache (48 heads of 128) 18 us (81 MB, 4.5 TB/s).
 #include "paged.hpp"
 
 namespace lm {
@@ -224,6 +224,14 @@ __global__ __launch_bounds__(256) void head_rows_kernel(HeadRows a) {
 // not below that of the rows which the block holds already: a row is rounded again only when a later
 // one raises the scale, and as the scale is a power of two, four significant bits stay what they
 // were but for values below 2^-6 of it.  Straight from fp32, so a value is rounded once.
+// (int8 under such scales would be rounded again in every row whenever one grows.)
+//
+// Blocks come first, as their chain is the longest: lengths, then page and rows, then the exchange
+// of the largest value; the queries' rows go as without a cache, a workgroup a token.  20 heads of
+// 256 (16 of them queries'): 64 tokens 4.9 us, 4096 tokens 20 us (79.7 MB, 4.0 TB/s), 16000 65 us
+// (4.8 TB/s); 3310 tokens, 48 heads of 128, 18 us (74.6 MB, 4.1 TB/s).  The next side's rows
+// requested before the one at hand cost registers and gained nothing; the blocks' workgroups spread
+// among the queries' were slower.
 struct E4m3Pages {
   uint8_t *k, *v;
   float *scales;
