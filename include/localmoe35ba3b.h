@@ -93,7 +93,7 @@ int lm_act_quant_g128(const void *x, int x_dtype, int8_t *q, float *s,
  * h and x [rows, n] of `dtype`, h rounded once after the sum; w fp32 [n]; q int8
  * [rows, n], s fp32 [rows, n/128].  n is a multiple of 128 up to 16384, rows are
  * fewer than 2^24; h, x and w are 16-byte aligned.  A row with an infinity or NaN
- * has scales that are not finite.  x may be h itself and overlaps it in no other
+ * has a scale that is not finite.  x may be h itself and overlaps it in no other
  * way.  No counterpart in the reference as one call (HF:801-815, 866-875 and
  * w8a8.py:8-22). */
 int lm_norm_quant_g128(void *h, const void *x, const float *w, int8_t *q,

@@ -92,8 +92,8 @@ def _frequencies(inv_freq, dim, device):
 
 
 def _positions(positions, axes, pairs, tokens, device):
-    """The positions and axes of a call (copies of others than int64 and int32, and of tokens apart),
-    and their C arguments: pointer, stride between axes, axes, each pair's axis."""
+    """The positions and axes of a call (copies of others than int64 and int32, and of tokens
+    apart), and their C arguments: pointer, stride between axes, axes, each pair's axis."""
     shape = positions.shape
     if positions.get_device() != device or not 1 <= len(shape) <= 2 or shape[-1] != tokens:
         raise ValueError('Expected a CUDA position of every token')
@@ -244,7 +244,8 @@ def append(k_pages, v_pages, k, v, starts, lengths, table, inv_freq=None, k_weig
     With scales, the pages hold 8 bits: each block of 16 positions takes the smallest power
     of two that brings the values of its rows to 448 at most.  As later calls fill it, the
     scale only grows; rows held already are then rounded again, which changes those below
-    2^-6 of it alone.  Rows of a block behind a sequence's last keep their bits.  A value is
+    2^-6 of it alone.  Rows of a block behind a sequence's last keep their bits, and where
+    positions are taken back inside a block, it keeps the scale that they needed.  A value is
     rounded once, from fp32; beyond 61440 in fp16 (0x1.Ep127 in bf16) it is held as that,
     infinities and NaN as NaN.
     With q [T, q_heads, D], returns the queries normed and rotated for
@@ -336,6 +337,7 @@ def paged_attention(q, k_pages, v_pages, starts, lengths, table, scale=None, gat
     workspace = q.new_empty(need // 2) if need > 0 else None
     _lib.launch(device, 'lm_paged_attention' if scales is None else 'lm_paged_attention_e4m3',
                 q.data_ptr(), q_token, q_head, q_heads, k_pages.data_ptr(), v_pages.data_ptr(),
-                *_scales(scales, k_pages, device), pages, stride, heads, size, dim, *batch, tokens, max_new, dim ** -0.5 if scale is None else scale, *gate_args,
-                out.data_ptr(), _lib.ptr(workspace), need, _lib.dtype_code(dtype))
+                *_scales(scales, k_pages, device), pages, stride, heads, size, dim, *batch, tokens,
+                max_new, dim ** -0.5 if scale is None else scale, *gate_args, out.data_ptr(),
+                _lib.ptr(workspace), need, _lib.dtype_code(dtype))
     return out

@@ -40,8 +40,8 @@ def norm_quantize(h, weight=None, eps=1e-6, add=None):
 
     h [rows, K] bf16 or fp16, contiguous, K a multiple of 128 up to 16384; weight [K].  With
     add [rows, K], h += add first, in place, and the rows normed are the sums as h then holds
-    them.  add may be h itself and shares no memory with it in another way.  Rows with
-    infinities or NaN get scales that are not finite."""
+    them.  add may be h itself and shares no memory with it in another way.  A row with
+    infinities or NaN gets a scale that is not finite."""
     if not h.is_cuda or h.ndim != 2 or h.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError('Expected CUDA rows with K divisible by 128')
     rows, k = h.shape

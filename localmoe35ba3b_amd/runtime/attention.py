@@ -3,9 +3,10 @@ layer's MoE block:
 
   h += o( attention( rotate(norm(q)), cache ) * sigmoid(gate) ),  [q, gate, k, v] = qkv(rmsnorm(h))
 
-with int8 projections (operators/int8.linear, or W8A8: w8a8.norm_quantize and w8a8.gemm), the
-norms, rotation and append in one launch and paged attention (operators/attention).  Rows, heads and weights are laid out as the
-Transformers module has them (HF:627-735): a head's query and gate side by side, norm
+with int8 projections (operators/int8.linear, or W8A8: w8a8.norm_quantize and w8a8.gemm before
+the attention, w8a8.linear behind it), the norms, rotation and append in one launch and paged
+attention (operators/attention).  Rows, heads and weights are laid out as the Transformers module
+has them (HF:627-735): a head's query and gate side by side, norm
 weights as 1 + w, the first channels of a head rotated in two halves.  The reference runs
 the Transformers module itself; its cache is a contiguous one per request
 (generation.py:32).
@@ -21,8 +22,8 @@ from ..operators import attention, int8, w8a8
 class Batch(NamedTuple):
     """What a step's attention works on, the same for every layer: starts [sequences + 1],
     lengths [sequences] and page table [sequences, n], int32 on the GPU (operators/attention),
-    the most new tokens of a sequence (None: not known), and the positions that rotate the rows, int64
-    [T] or [axes, T] on the GPU (None: their places in their sequences)."""
+    the most new tokens of a sequence (None: not known), and the positions that rotate the rows,
+    int64 [T] or [axes, T] on the GPU (None: their places in their sequences)."""
     starts: torch.Tensor
     lengths: torch.Tensor
     table: torch.Tensor

@@ -166,8 +166,8 @@ C_REFUSED = [
     (EIGHT, dict(page=8), 'page size'), (EIGHT, dict(table_pages=1 << 27), 'page table'),
     (EIGHT, dict(k_pages=4104), 'aligned'), (EIGHT, dict(starts=None), 'null'),
     (('append8',), dict(v=None), 'aligned'), (('append8',), dict(q_out=None), 'aligned'),
-    (('append8',), dict(k_heads=1024, k_token=1 << 17, page_stride=1 << 21, scale_stride=2048,
-                        tokens=1 << 20, position_stride=1 << 20), 'too many rows'),
+    # a workgroup for each token and each block: 2^24 are refused, whatever the heads
+    (('append8',), dict(tokens=(1 << 24) - 1, position_stride=1 << 24), 'too many rows'),
     (('attend8',), dict(q_heads=5), 'multiple'), (('attend8',), dict(out=4104), 'aligned'),
     (('attend8',), dict(ws=None), 'workspace'), (('attend8',), dict(ws=4104), 'workspace'),
     (('quant',), dict(n=100), 'multiple of 128'), (('quant',), dict(n=0), 'multiple of 128'),

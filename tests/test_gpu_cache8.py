@@ -191,6 +191,23 @@ def test_append_many_sequences(dev, sequences):
     run_append(dev, [first, [(s, 1) for s in range(sequences)]], 16, 1, 64, BF16, seed=sequences)
 
 
+@TYPES
+def test_append_after_positions_are_taken_back(dev, dtype):
+    """A draft whose last tokens are dropped: the block keeps its scale, and the dropped rows' bits
+    where no new row comes; from the block's begin on, the scale is the new rows'."""
+    gen = seeded(5)
+    kp, vp, scales = to(dev, *C.random_cache(gen, 3, 2, 16, 64, dtype))
+    want, scale64 = C.held(kp, vp, scales)[1], scales[:, :, 1].cpu().double()
+    table = [2, 0]
+    for base, n, size in ((0, 30, 1.0), (30, 2, 900.0), (20, 3, 1.0), (16, 5, 0.25), (3, 1, 40.0)):
+        v = rand(gen, n, 2, 64, dtype=dtype) * size
+        A.append(kp, vp, *to(dev, v, v, ints(0, n), ints(base + n), ints(*table).view(1, 2)),
+                 scales=scales)
+        C.append(want, scale64, v.double(), base, table, 16, dtype)
+        assert torch.equal(C.held(kp, vp, scales)[1], want), (base, n)
+        assert torch.equal(scales[:, :, 1].cpu().double(), scale64), (base, n)
+
+
 def test_append_outside_the_table(dev):
     """Positions before 0 or behind the table's pages, and page numbers out of range; rows of no
     sequence leave the cache as it is."""
