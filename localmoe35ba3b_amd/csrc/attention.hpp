@@ -1088,8 +1088,12 @@ __device__ __forceinline__ uint64_t all_keys(const Attention &a, const PagedSequ
 }
 
 struct TilePlace {
-  int s, tile;   // s < 0: none
-  // where tiles are split each in its own way: all tiles of the call, and their keys
+  int s, tile;        // s < 0: none
+  int split, splits;  // which part of its keys, of how many
+};
+
+// All tiles of a call, and their keys.
+struct TileTotals {
   int tiles;
   uint64_t keys;
 };
@@ -1100,53 +1104,92 @@ struct TilePlace {
 // up to 700 new tokens took 52 us instead of 61 (heads of 128) and 61 instead of 77 (256), 24 of
 // 8 to 24 tokens 46 instead of 55; parts of 128 or 512 keys and fewer or more rounds took up to
 // 30 % more in one case or another.
-__device__ __forceinline__ int tile_parts(const Attention &a, const TilePlace &place, int keys) {
-  const int rounds = (int)((float)place.tiles * 1.5f / (float)a.room) + 1;
-  const float all = (float)max(place.keys, (uint64_t)1);
-  const float n = (float)keys * (float)(rounds * a.room - place.tiles) / all + 0.5f;
+__device__ __forceinline__ int tile_parts(const Attention &a, const TileTotals &total, int keys) {
+  const int rounds = (int)((float)total.tiles * 1.5f / (float)a.room) + 1;
+  const float all = (float)max(total.keys, (uint64_t)1);
+  const float n = (float)keys * (float)(rounds * a.room - total.tiles) / all + 0.5f;
   return max(min(min((int)fminf(n, 65536.0f), a.splits), keys / 256), 1);
 }
+// A sequence's tiles have as many places each in the grid as its last one, which sees the most keys,
+// has parts, so that few places are empty.  Workgroups go to the chip's dies and CUs in turn, and
+// with `splits` places for every tile those of the parts that there are came round to the same
+// CUs: 2048 new tokens beside 8 of one (heads of 128) took 141 us instead of 95, behind 8192 keys
+// beside 32 (256) 1022 instead of 377.  A grid of all first parts, then all second ones, has the
+// empty places before work: 12 sequences of up to 700 new tokens 50 us instead of 45.
+__device__ __forceinline__ int tile_places(const Attention &a, const TileTotals &total,
+                                           const PagedSequence &q, int n) {
+  return n > 0 ? tile_parts(a, total, tile_keys(q, a.group, n - 1)) : 1;
+}
+// Place `at` of a sequence's n tiles with `places` each; a tile's first part is at another one in
+// each, for the same reason.
+__device__ __forceinline__ TilePlace tile_place(const Attention &a, const TileTotals &total, int s,
+                                                const PagedSequence &q, int n, int places, int at) {
+  const int t = at / places, tile = n - 1 - t;
+  return {s, tile, (at % places + t + (t >> 2) + (t >> 4)) % places,
+          tile_parts(a, total, tile_keys(q, a.group, tile))};
+}
 
-// The index-th tile, and its sequence; the tile with the most keys of a sequence comes first.
-// All THREADS threads; scratch (a word and a long word a wave) and found are free again
+// The index-th tile, or place of one, and its sequence; the tile with the most keys of a sequence
+// comes first.  `split`: the part, where all tiles have a.splits.  All THREADS threads; scratch (a word and a long word a wave) and found are free again
 // afterwards.
 template <int THREADS>
-__device__ TilePlace find_tile(const Attention &a, int index, int *scratch, uint64_t *sums,
-                               TilePlace *found, PagedSequence &seq) {
+__device__ TilePlace find_tile(const Attention &a, int index, int split, int *scratch,
+                               uint64_t *sums, TilePlace *found, PagedSequence &seq) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, S = a.batch.sequences;
-  const bool split = a.room > 0;
+  const bool places = a.room > 0;
   if (S <= 64) {  // each wave for itself
     const PagedSequence mine = paged_sequences(a.batch, min(lane, S - 1), a.tokens);
-    const int n = lane < S ? tile_count(a, mine) : 0, sum = (int)wave_scan((uint32_t)n);
-    const uint64_t hit = __ballot(index >= sum - n && index < sum);
+    const int n = lane < S ? tile_count(a, mine) : 0;
+    TileTotals total = {};
+    int m = 1;
+    if (places) {
+      total = {(int)wave_total((uint64_t)n), wave_total(all_keys(a, mine, n))};
+      m = tile_places(a, total, mine, n);
+    }
+    const int sum = (int)wave_scan((uint32_t)(n * m));
+    const uint64_t hit = __ballot(index >= sum - n * m && index < sum);
     if (!hit) return {-1, 0, 0, 0};
-    const int at = __builtin_ctzll(hit);
+    const int at = __builtin_ctzll(hit), before = __builtin_amdgcn_readlane(sum - n * m, at);
+    const int tiles = __builtin_amdgcn_readlane(n, at);
     seq = sequence_at(a.batch, at, mine, a.tokens);
-    return {at, __builtin_amdgcn_readlane(sum, at) - 1 - index, __builtin_amdgcn_readlane(sum, 63),
-            split ? wave_total(all_keys(a, mine, n)) : 0};
+    if (!places) return {at, tiles - 1 - (index - before), split, a.splits};
+    return tile_place(a, total, at, seq, tiles, __builtin_amdgcn_readlane(m, at), index - before);
   }
   if (tid == 0) found->s = -1;
-  int base = 0;
-  uint64_t all = 0;
-  for (int c = 0; c < S; c += THREADS) {
-    const PagedSequence mine = paged_sequences(a.batch, min(c + tid, S - 1), a.tokens);
-    const int n = c + tid < S ? tile_count(a, mine) : 0, sum = (int)wave_scan((uint32_t)n);
-    const uint64_t keys = split ? wave_total(all_keys(a, mine, n)) : 0;
+  TileTotals total = {};
+  if (places) {
+    for (int c = tid; c < S; c += THREADS) {
+      const PagedSequence mine = paged_sequences(a.batch, c, a.tokens);
+      const int n = tile_count(a, mine);
+      total.tiles += n, total.keys += all_keys(a, mine, n);
+    }
+    total.tiles = (int)wave_total((uint64_t)total.tiles), total.keys = wave_total(total.keys);
+    if (lane == 0) scratch[wave] = total.tiles, sums[wave] = total.keys;
     __syncthreads();
-    if (lane == 63) scratch[wave] = sum, sums[wave] = keys;
+    total = {};
+    for (int w = 0; w < THREADS / 64; ++w) total.tiles += scratch[w], total.keys += sums[w];
+  }
+  int base = 0;
+  for (int c = 0; c < S && base <= index; c += THREADS) {
+    const PagedSequence mine = paged_sequences(a.batch, min(c + tid, S - 1), a.tokens);
+    const int n = c + tid < S ? tile_count(a, mine) : 0;
+    const int m = places ? tile_places(a, total, mine, n) : 1;
+    const int sum = (int)wave_scan((uint32_t)(n * m));
+    __syncthreads();
+    if (lane == 63) scratch[wave] = sum;
     __syncthreads();
     int before = base;
     for (int w = 0; w < THREADS / 64; ++w) {
       if (w < wave) before += scratch[w];
-      base += scratch[w], all += sums[w];
+      base += scratch[w];
     }
-    before += sum - n;
-    if (index >= before && index < before + n) *found = {c + tid, n - 1 - (index - before), 0, 0};
-    if (base > index && !split) break;  // the same for every thread
+    before += sum - n * m;
+    if (index >= before && index < before + n * m)
+      *found = places ? tile_place(a, total, c + tid, mine, n, m, index - before)
+                      : TilePlace{c + tid, n - 1 - (index - before), split, a.splits};
   }
   __syncthreads();
-  TilePlace got = *found;
-  got.tiles = base, got.keys = all;
+  const TilePlace got = *found;
   __syncthreads();
   if (got.s >= 0) seq = sequence_at(a.batch, got.s, {}, a.tokens);
   return got;
@@ -1448,13 +1491,10 @@ __global__ __launch_bounds__((TileForm<D, C>::kWaves * 64), 2) void attention_ti
   TilePlace *found = reinterpret_cast<TilePlace *>(key_sums + 8);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int set = wave & 3, group = wave >> 2;
-  // Where tiles have parts of their own count, a tile's parts lie next to each other: those that
-  // there are begin among those that there are not, and none of them last.
   const int kv = blockIdx.x % a.batch.kv_heads, index = blockIdx.x / a.batch.kv_heads;
-  const int split = a.room ? index % a.splits : (int)blockIdx.y;
   PagedSequence seq;
   const TilePlace place =
-      find_tile<WAVES * 64>(a, a.room ? index / a.splits : index, scratch, key_sums, found, seq);
+      find_tile<WAVES * 64>(a, index, blockIdx.y, scratch, key_sums, found, seq);
   const int s = __builtin_amdgcn_readfirstlane(place.s);
   if (s < 0) return;
   const int tile = __builtin_amdgcn_readfirstlane(place.tile);
@@ -1466,7 +1506,8 @@ __global__ __launch_bounds__((TileForm<D, C>::kWaves * 64), 2) void attention_ti
   const int all_see = min(seq.base + c0 / a.group + 1, seq.length);  // seen by every row
   // keys that the tile's last row sees, and this part of them
   const int keys = tile_keys(seq, a.group, tile), tiles = (keys + KEYS - 1) / KEYS;
-  const int splits = __builtin_amdgcn_readfirstlane(a.room ? tile_parts(a, place, keys) : a.splits);
+  const int split = __builtin_amdgcn_readfirstlane(place.split);
+  const int splits = __builtin_amdgcn_readfirstlane(place.splits);
   if (split >= splits) return;
   const int key0 = (int)((int64_t)tiles * split / splits) * KEYS;
   const int key1 = min((int)((int64_t)tiles * (split + 1) / splits) * KEYS, keys);
@@ -1748,10 +1789,11 @@ int launch_attention(const AttentionPlan &p, Attention a, float *workspace, hipS
   if (p.few) {
     attention_few_kernel<T, D, C><<<(unsigned)p.few_grid, 256, 0, st>>>(a);
     if (const int rc = check_launch("attention_few_kernel")) return rc;
-    // Where there are few sequences, their rows and channels fill the chip.  Against four times as
-    // many workgroups at most, 24 sequences with 2 to 9 rows took 24.4 instead of 25.7 us and 12 of up
-    // to 700 new tokens 48.0 instead of 49.0; half as many took 53.7 there.
-    const int64_t units = kFewRows / a.group * a.group * (D / 64), some = 1024 / p.parts;
+    // Where there are few sequences, their rows and channels fill the chip.  Against twice as many
+    // workgroups at most, 24 sequences with 2 to 9 rows took 24.1 instead of 25.2 us and 16 of up to
+    // 300 new tokens 34.3 instead of 35.6; with half as many, 24 of 2 to 24 (heads of 256), of which
+    // three are split in many parts, took 69.0 instead of 63.5.
+    const int64_t units = kFewRows / a.group * a.group * (D / 64), some = 2048 / p.parts;
     ys = some < 1 ? 1 : some < units ? some : units;
   }
   const int chunks = (a.q_heads * (D / 4) + 255) / 256;
