@@ -45,6 +45,8 @@
 //                         behind 8192 keys: 293 to 302 us in a long run of calls,
 //                         1024 to 1054 TFLOP/s (1371 for a large library product);
 //                         without a history 64 us.
+//  attention_both_kernel  the two in one launch, for calls that may have both and heads
+//                         of 64 or 128.
 //  attention_combine_kernel  joins the parts of split keys, 4 to 12 us: the partial
 //                         sums are fp32, written and read once.
 //
@@ -466,12 +468,18 @@ struct Find {
   int s;          // < 0: none
 };
 
+// The lane's sequence, of up to 64; of more, none.
+__device__ __forceinline__ PagedSequence lane_sequence(const Attention &a) {
+  const int S = a.batch.sequences;
+  return S <= 64 ? paged_sequences(a.batch, min((int)threadIdx.x & 63, S - 1), a.tokens)
+                 : PagedSequence{};
+}
+
 // The spans, and the sequence that holds the first block of span `index`.  All 256 threads;
 // scratch (8 words of LDS) and found are free again afterwards.
-// `mine`: the lane's sequence, of up to 64 (of the lanes behind them, none).
 template <typename C>
-__device__ Spans find_span(const Attention &a, int index, int64_t *scratch, Find *found, Find &got,
-                           PagedSequence &mine) {
+__device__ Spans find_span(const Attention &a, int index, const PagedSequence &mine,
+                           int64_t *scratch, Find *found, Find &got) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, S = a.batch.sequences;
   Spans sp;
   got = {0, -1};
@@ -479,7 +487,6 @@ __device__ Spans find_span(const Attention &a, int index, int64_t *scratch, Find
     return s < S ? few_blocks<C>(a, paged_sequences(a.batch, s, a.tokens)) : 0;
   };
   if (S <= 64) {  // every wave by itself: a sequence a lane
-    mine = paged_sequences(a.batch, min(lane, S - 1), a.tokens);
     const uint32_t n = lane < S ? few_blocks<C>(a, mine) : 0;  // 64 of at most 2^25
     const uint32_t sum = wave_scan(n);
     sp.blocks = (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
@@ -533,13 +540,14 @@ constexpr int kFewWaves = 4;
 // 23.5.  Four workgroups, or three with 48 KB, took 1 to 5 % more than three with 32.
 template <int D>
 constexpr int few_steps() { return D == 256 ? 1 : 2; }
-template <int D>
-constexpr int few_ring() { return few_steps<D>() * 2 * 16 * D * 2; }
+template <int D, int STEPS = few_steps<D>()>
+constexpr int few_ring() { return STEPS * 2 * 16 * D * 2; }
 template <int D>
 constexpr int few_merge() { return kFewWaves * (kFewRows * (D + 4) + 2 * kFewRows) * 4; }
-template <int D>
+template <int D, int STEPS = few_steps<D>()>
 constexpr int few_lds() {
-  return kFewWaves * few_ring<D>() > few_merge<D>() ? kFewWaves * few_ring<D>() : few_merge<D>();
+  return kFewWaves * few_ring<D, STEPS>() > few_merge<D>() ? kFewWaves * few_ring<D, STEPS>()
+                                                           : few_merge<D>();
 }
 
 // The running state of a wave's 16 columns (column lane & 15 in each 16 lanes).
@@ -769,14 +777,14 @@ __device__ __forceinline__ FewScales<C> few_step_scales(const FewKeys<C> &f, int
       s.exponents[u] = __builtin_amdgcn_readlane(f.exponents, (i * FewKeys<C>::kUnits + u) & 63);
   return s;
 }
-template <typename T, int D, typename C>
+template <typename T, int D, typename C, int STEPS>
 __device__ __forceinline__ void few_step(LDS char *ring, const FewKeys<C> &f,
                                          const FewScales<C> &scales, const u32x4 (&q)[D / 32],
                                          int i, int limit, int all_see, float scale2,
                                          FewState<D> &st, int lane) {
   constexpr int KEYS = Cache<C>::kFewKeys;
   constexpr int TILE = KEYS * D * Cache<C>::kBytes, N = TILE / 1024;  // bytes, loads of one side
-  constexpr int STEPS = few_steps<D>(), OUT = (2 * STEPS - 1) * N;
+  constexpr int OUT = (2 * STEPS - 1) * N;
   LDS char *k = ring + i % STEPS * 2 * TILE, *v = k + TILE;
   const int key = (f.first + i * f.stride) * KEYS;
   wait_loads<OUT>();
@@ -834,7 +842,7 @@ __device__ __forceinline__ int64_t part_row(const Attention &a, int span, bool l
 
 // Blocks b0 .. b1 - 1 of sequence s at key-value head kv; `part`: its row among the parts, or
 // negative where these are all of its blocks.
-template <typename T, int D, typename C>
+template <typename T, int D, typename C, int STEPS>
 __device__ __forceinline__ void few_part(const Attention &a, const PagedSequence &seq, int s, int kv,
                                          int b0, int b1, int64_t part, char *lds) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -869,9 +877,9 @@ __device__ __forceinline__ void few_part(const Attention &a, const PagedSequence
     __builtin_amdgcn_sched_barrier(0);
     settle(entry);
     few_pages<T>(a, f, entry, 0, kv, lane);
-    LDS char *ring = (LDS char *)lds + wave * few_ring<D>();
-    constexpr int TILE = KEYS * D * Cache<C>::kBytes, STEPS = few_steps<D>();
-    static_assert(TILE * 2 * STEPS == few_ring<D>(), "a ring holds its steps");
+    LDS char *ring = (LDS char *)lds + wave * few_ring<D, STEPS>();
+    constexpr int TILE = KEYS * D * Cache<C>::kBytes;
+    static_assert(TILE * 2 * STEPS == few_ring<D, STEPS>(), "a ring holds its steps");
     FewScales<C> scales[STEPS];
     for (int j = 0; j < STEPS; ++j) {  // in this order: the waits count what was issued later
       few_load<D, C, kRows>(f, f.k, j, ring + 2 * j * TILE, lane);
@@ -896,7 +904,7 @@ __device__ __forceinline__ void few_part(const Attention &a, const PagedSequence
 #pragma unroll
       for (int j = 1; j < STEPS; ++j) scales[j - 1] = scales[j];
       scales[STEPS - 1] = few_step_scales(f, i + STEPS);
-      few_step<T, D, C>(ring, f, now, q, i, limit, all_see, a.scale2, st, lane);
+      few_step<T, D, C, STEPS>(ring, f, now, q, i, limit, all_see, a.scale2, st, lane);
     }
     wait_loads<0>();  // the last refills, before the ring is used otherwise
     if (__builtin_expect(st.odd, 0)) {
@@ -949,15 +957,14 @@ __device__ __forceinline__ void few_part(const Attention &a, const PagedSequence
   __syncthreads();  // before the ring is used again
 }
 
-template <typename T, int D, typename C>
-__global__ __launch_bounds__(256, Cache<C>::kScaled ? 2 : 1) void attention_few_kernel(Attention a) {
-  // One array: with several, the compiler waits for all direct loads at each LDS read.
-  __shared__ __attribute__((aligned(16))) char lds[few_lds<D>()];
+// Workgroup `index` of those of few rows.
+template <typename T, int D, typename C, int STEPS>
+__device__ __forceinline__ void few_span(const Attention &a, int index, const PagedSequence &mine,
+                                         char *lds) {
   int64_t *scratch = reinterpret_cast<int64_t *>(lds);
-  const int kv = blockIdx.x % a.batch.kv_heads, span = blockIdx.x / a.batch.kv_heads;
+  const int kv = index % a.batch.kv_heads, span = index / a.batch.kv_heads;
   Find at;
-  PagedSequence mine;
-  const Spans sp = find_span<C>(a, span, scratch, reinterpret_cast<Find *>(scratch + 8), at, mine);
+  const Spans sp = find_span<C>(a, span, mine, scratch, reinterpret_cast<Find *>(scratch + 8), at);
   if (at.s < 0) return;
   int64_t block = sp.start(span);
   const int64_t end = sp.start(span + 1);
@@ -971,11 +978,18 @@ __global__ __launch_bounds__(256, Cache<C>::kScaled ? 2 : 1) void attention_few_
     if (take <= 0) continue;
     if (done == 0 && threadIdx.x == 0)  // where its parts are, for the kernel that joins them
       a.parts[s * a.batch.kv_heads + kv] = {span, later, sp.of(block + all - 1) - span + 1};
-    few_part<T, D, C>(a, seq, s, kv, done, done + take,
+    few_part<T, D, C, STEPS>(a, seq, s, kv, done, done + take,
                       take == all ? -1 : part_row(a, span, later, kv), lds);
     block += take;
     later = true;
   }
+}
+
+template <typename T, int D, typename C>
+__global__ __launch_bounds__(256, Cache<C>::kScaled ? 2 : 1) void attention_few_kernel(Attention a) {
+  // One array: with several, the compiler waits for all direct loads at each LDS read.
+  __shared__ __attribute__((aligned(16))) char lds[few_lds<D>()];
+  few_span<T, D, C, few_steps<D>()>(a, blockIdx.x, lane_sequence(a), lds);
 }
 
 // The sum of parts of a row: a thread's four channels, under the largest maximum so far.
@@ -1130,15 +1144,15 @@ __device__ __forceinline__ TilePlace tile_place(const Attention &a, const TileTo
 }
 
 // The index-th tile, or place of one, and its sequence; the tile with the most keys of a sequence
-// comes first.  `split`: the part, where all tiles have a.splits.  All THREADS threads; scratch (a word and a long word a wave) and found are free again
-// afterwards.
+// comes first.  `split`: the part, where all tiles have a.splits.  All THREADS threads; scratch (a
+// word and a long word a wave) and found are free again afterwards.
 template <int THREADS>
-__device__ TilePlace find_tile(const Attention &a, int index, int split, int *scratch,
-                               uint64_t *sums, TilePlace *found, PagedSequence &seq) {
+__device__ TilePlace find_tile(const Attention &a, int index, int split, const PagedSequence &mine,
+                               int *scratch, uint64_t *sums, TilePlace *found,
+                               PagedSequence &seq) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, S = a.batch.sequences;
   const bool places = a.room > 0;
   if (S <= 64) {  // each wave for itself
-    const PagedSequence mine = paged_sequences(a.batch, min(lane, S - 1), a.tokens);
     const int n = lane < S ? tile_count(a, mine) : 0;
     TileTotals total = {};
     int m = 1;
@@ -1159,9 +1173,9 @@ __device__ TilePlace find_tile(const Attention &a, int index, int split, int *sc
   TileTotals total = {};
   if (places) {
     for (int c = tid; c < S; c += THREADS) {
-      const PagedSequence mine = paged_sequences(a.batch, c, a.tokens);
-      const int n = tile_count(a, mine);
-      total.tiles += n, total.keys += all_keys(a, mine, n);
+      const PagedSequence q = paged_sequences(a.batch, c, a.tokens);
+      const int n = tile_count(a, q);
+      total.tiles += n, total.keys += all_keys(a, q, n);
     }
     total.tiles = (int)wave_total((uint64_t)total.tiles), total.keys = wave_total(total.keys);
     if (lane == 0) scratch[wave] = total.tiles, sums[wave] = total.keys;
@@ -1171,9 +1185,9 @@ __device__ TilePlace find_tile(const Attention &a, int index, int split, int *sc
   }
   int base = 0;
   for (int c = 0; c < S && base <= index; c += THREADS) {
-    const PagedSequence mine = paged_sequences(a.batch, min(c + tid, S - 1), a.tokens);
-    const int n = c + tid < S ? tile_count(a, mine) : 0;
-    const int m = places ? tile_places(a, total, mine, n) : 1;
+    const PagedSequence q = paged_sequences(a.batch, min(c + tid, S - 1), a.tokens);
+    const int n = c + tid < S ? tile_count(a, q) : 0;
+    const int m = places ? tile_places(a, total, q, n) : 1;
     const int sum = (int)wave_scan((uint32_t)(n * m));
     __syncthreads();
     if (lane == 63) scratch[wave] = sum;
@@ -1185,7 +1199,7 @@ __device__ TilePlace find_tile(const Attention &a, int index, int split, int *sc
     }
     before += sum - n * m;
     if (index >= before && index < before + n * m)
-      *found = places ? tile_place(a, total, c + tid, mine, n, m, index - before)
+      *found = places ? tile_place(a, total, c + tid, q, n, m, index - before)
                       : TilePlace{c + tid, n - 1 - (index - before), split, a.splits};
   }
   __syncthreads();
@@ -1476,25 +1490,24 @@ constexpr int tile_lds() {
   return out > ring ? out : ring;
 }
 
+// Workgroup (x, y) of those of tiles; y: the part, where all tiles have a.splits.
 template <typename T, int D, typename C>
-__global__ __launch_bounds__((TileForm<D, C>::kWaves * 64), 2) void attention_tile_kernel(
-    Attention a) {
+__device__ __forceinline__ void tile_rows(const Attention &a, int x, int y,
+                                          const PagedSequence &mine, char *lds) {
   using F = TileForm<D, C>;
   using Elem = typename Cache<C>::Elem;
   constexpr int WAVES = F::kWaves, KEYS = F::kKeys, ROWS = KEYS / WAVES;
   constexpr int GROUPS = F::kGroups, TILE = F::kBytes, B = D * Cache<C>::kBytes;
   static_assert(GROUPS == 1 || GROUPS == 2, "two groups are joined");
-  // One array: with several, the compiler waits for all direct loads at each LDS read.
-  __shared__ __attribute__((aligned(16))) char lds[tile_lds<D, C>()];
   int *scratch = reinterpret_cast<int *>(lds);
   uint64_t *key_sums = reinterpret_cast<uint64_t *>(scratch + 8);
   TilePlace *found = reinterpret_cast<TilePlace *>(key_sums + 8);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int set = wave & 3, group = wave >> 2;
-  const int kv = blockIdx.x % a.batch.kv_heads, index = blockIdx.x / a.batch.kv_heads;
+  const int kv = x % a.batch.kv_heads, index = x / a.batch.kv_heads;
   PagedSequence seq;
   const TilePlace place =
-      find_tile<WAVES * 64>(a, index, blockIdx.y, scratch, key_sums, found, seq);
+      find_tile<WAVES * 64>(a, index, y, mine, scratch, key_sums, found, seq);
   const int s = __builtin_amdgcn_readfirstlane(place.s);
   if (s < 0) return;
   const int tile = __builtin_amdgcn_readfirstlane(place.tile);
@@ -1678,6 +1691,90 @@ __global__ __launch_bounds__((TileForm<D, C>::kWaves * 64), 2) void attention_ti
   }
 }
 
+template <typename T, int D, typename C>
+__global__ __launch_bounds__((TileForm<D, C>::kWaves * 64), 2) void attention_tile_kernel(
+    Attention a) {
+  // One array: with several, the compiler waits for all direct loads at each LDS read.
+  __shared__ __attribute__((aligned(16))) char lds[tile_lds<D, C>()];
+  tile_rows<T, D, C>(a, blockIdx.x, blockIdx.y, lane_sequence(a), lds);
+}
+
+// ------------------------------------------------------------------ both in one launch
+// Spans of few rows and places of tiles of a call, for a key-value head.  All 256 threads; sums is
+// free again afterwards.
+struct Counts {
+  int spans;
+  int64_t places;
+};
+template <typename C>
+__device__ Counts count_both(const Attention &a, const PagedSequence &mine, uint64_t *sums) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, S = a.batch.sequences;
+  TileTotals total = {};
+  if (S <= 64) {  // each wave for itself
+    const int n = lane < S ? tile_count(a, mine) : 0;
+    const uint64_t blocks = wave_total((uint64_t)(lane < S ? few_blocks<C>(a, mine) : 0));
+    if (a.room) total = {(int)wave_total((uint64_t)n), wave_total(all_keys(a, mine, n))};
+    const int m = a.room ? tile_places(a, total, mine, n) : 1;
+    return {(int)min((uint64_t)a.shares, blocks), (int64_t)wave_total((uint64_t)n * m)};
+  }
+  auto all = [&](uint64_t v) {
+    v = wave_total(v);
+    __syncthreads();
+    if (lane == 0) sums[wave] = v;
+    __syncthreads();
+    return sums[0] + sums[1] + sums[2] + sums[3];
+  };
+  uint64_t blocks = 0, tiles = 0, keys = 0, places = 0;
+  for (int c = tid; c < S; c += 256) {
+    const PagedSequence q = paged_sequences(a.batch, c, a.tokens);
+    const int n = tile_count(a, q);
+    blocks += few_blocks<C>(a, q), tiles += n, keys += all_keys(a, q, n);
+  }
+  blocks = all(blocks), places = tiles = all(tiles);
+  if (a.room) {
+    total = {(int)tiles, all(keys)};
+    places = 0;
+    for (int c = tid; c < S; c += 256) {
+      const PagedSequence q = paged_sequences(a.batch, c, a.tokens);
+      const int n = tile_count(a, q);
+      places += (uint64_t)n * tile_places(a, total, q, n);
+    }
+    places = all(places);
+  }
+  __syncthreads();
+  return {(int)min((uint64_t)a.shares, blocks), (int64_t)places};
+}
+
+// Workgroups of tiles and of few rows, kTurn of each in turn while there are both: the first bound
+// by the matrix cores and a chain of steps, the others by the cache's bytes.  Against a launch each,
+// 12 sequences of up to 700 new tokens (heads of 128) take 39 us instead of 45, 2048 tokens behind
+// 8192 keys beside 32 of one 263 instead of 310 (64) and 380 instead of 463 (128), 24 of 2 to 24
+// 41 instead of 51 (64).  All of one kind first was better for some and 10 % worse than two
+// launches for others, as were places for the most that a call can have of each: those without
+// work then come before some with it.  Heads of 128 have a ring of one step here, so that three
+// workgroups still share a CU.  Heads of 256 have two launches: their tiles' workgroups have eight
+// waves.
+constexpr int kTurn = 256;
+
+template <typename T, int D, typename C>
+__global__ __launch_bounds__(256, D == 64 ? 4 : 3) void attention_both_kernel(Attention a) {
+  constexpr int STEPS = D == 64 ? 2 : 1, FEW = few_lds<D, STEPS>(), TILE = tile_lds<D, C>();
+  // One array: with several, the compiler waits for all direct loads at each LDS read.
+  __shared__ __attribute__((aligned(16))) char lds[FEW > TILE ? FEW : TILE];
+  const PagedSequence mine = lane_sequence(a);
+  const Counts n = count_both<C>(a, mine, reinterpret_cast<uint64_t *>(lds));
+  const int few = n.spans * a.batch.kv_heads;
+  const int64_t tiles = n.places * a.batch.kv_heads;
+  const int turns = (int)min((int64_t)(few + kTurn - 1) / kTurn, (tiles + kTurn - 1) / kTurn);
+  const int turn = blockIdx.x / kTurn, at = blockIdx.x % kTurn;
+  const int index = (turn < 2 * turns ? turn / 2 : turn - turns) * kTurn + at;
+  if (turn < 2 * turns ? turn % 2 == 0 : tiles > few) {
+    if (index < tiles) tile_rows<T, D, C>(a, index, 0, mine, lds);
+  } else {
+    if (index < few) few_span<T, D, C, STEPS>(a, index, mine, lds);
+  }
+}
+
 // Rows of sequences in tiles, where their keys were split: D / 4 threads a row, `chunks`
 // workgroups a token.
 template <typename T, int D>
@@ -1786,9 +1883,12 @@ int launch_attention(const AttentionPlan &p, Attention a, float *workspace, hipS
   a.row_parts = reinterpret_cast<int *>(a.parts + p.parts);
   a.shares = (int)p.shares, a.splits = (int)p.splits, a.room = (int)p.room;
   int64_t ys = 0, tile = 0;  // workgroups that join parts: ys for each of p.parts, and tile
+  const bool both = D < 256 && p.few && p.tile;
   if (p.few) {
-    attention_few_kernel<T, D, C><<<(unsigned)p.few_grid, 256, 0, st>>>(a);
-    if (const int rc = check_launch("attention_few_kernel")) return rc;
+    if (!both) {
+      attention_few_kernel<T, D, C><<<(unsigned)p.few_grid, 256, 0, st>>>(a);
+      if (const int rc = check_launch("attention_few_kernel")) return rc;
+    }
     // Where there are few sequences, their rows and channels fill the chip.  Against twice as many
     // workgroups at most, 24 sequences with 2 to 9 rows took 24.1 instead of 25.2 us and 16 of up to
     // 300 new tokens 34.3 instead of 35.6; with half as many, 24 of 2 to 24 (heads of 256), of which
@@ -1800,8 +1900,14 @@ int launch_attention(const AttentionPlan &p, Attention a, float *workspace, hipS
   if (p.tile) {
     const int64_t all = p.tiles * a.batch.kv_heads;
     const dim3 grid((unsigned)(p.room ? all * p.splits : all), (unsigned)(p.room ? 1 : p.splits));
-    attention_tile_kernel<T, D, C><<<grid, TileForm<D, C>::kWaves * 64, 0, st>>>(a);
-    if (const int rc = check_launch("attention_tile_kernel")) return rc;
+    if (!both) {
+      attention_tile_kernel<T, D, C><<<grid, TileForm<D, C>::kWaves * 64, 0, st>>>(a);
+      if (const int rc = check_launch("attention_tile_kernel")) return rc;
+    } else if constexpr (D < 256) {  // of several sequences, whose parts have no dimension of the grid
+      const int64_t turns = (grid.x + kTurn - 1) / kTurn + (p.few_grid + kTurn - 1) / kTurn;
+      attention_both_kernel<T, D, C><<<(unsigned)(turns * kTurn), 256, 0, st>>>(a);
+      if (const int rc = check_launch("attention_both_kernel")) return rc;
+    }
     if (p.splits > 1) tile = (int64_t)a.tokens * chunks;
   }
   const int64_t all = p.parts * ys + tile;

@@ -10,6 +10,7 @@ from tests import attention_util as U
 from tests import cache8_util as C
 from tests.conftest import seeded
 from tests.test_gpu_attention import CHUNKS, DECODE, rand, to
+from tests.test_gpu_attention import attend as attend16
 
 pytestmark = pytest.mark.gpu
 
@@ -314,6 +315,22 @@ def test_attention_many_sequences(dev, sequences, chunks):
     lens = [(new, max(n, new - 1)) for new, n in lens]
     attend(dev, lens, 16, 4, 2, 64, BF16, gate=chunks, pad=2, seed=sequences,
            max_new=max(n for n, _ in lens))
+
+
+@pytest.mark.parametrize('dim', [64, 128, 256])
+@pytest.mark.parametrize('sequences,tokens,prompts', [(9, 3, 3), (40, 30, 0), (40, 0, 11), (70, 30, 9),
+                                                      (300, 90, 5)])
+def test_attention_tokens_beside_prompts(dev, sequences, tokens, prompts, dim):
+    """Single tokens and prompts of one call, behind many keys and none, among sequences that have no
+    new token; also where a call could have both and has one kind alone."""
+    gen = torch.Generator().manual_seed(sequences)
+    kind = torch.randperm(sequences, generator=gen).tolist()
+    lens = []
+    for i in kind:
+        new = 1 if i < tokens else 20 + i * 37 % 150 if i < tokens + prompts else 0
+        lens.append((new, new + i * 131 % (1200 if sequences < 100 else 300)))
+    for call in (attend, attend16):
+        call(dev, lens, 16, 8, 2, dim, BF16, gate=True, pad=2, seed=dim)
 
 
 @pytest.mark.parametrize('new,heads,keys,dim', [(2, 128, 36000, 64), (2, 128, 20000, 128),
