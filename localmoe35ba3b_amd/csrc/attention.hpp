@@ -45,8 +45,8 @@
 //                         behind 8192 keys: 293 to 302 us in a long run of calls,
 //                         1024 to 1054 TFLOP/s (1371 for a large library product);
 //                         without a history 64 us.
-//  attention_both_kernel  the two in one launch, for calls that may have both and heads
-//                         of 64 or 128.
+//  attention_both_kernel  the two in one launch, for calls that may have both (not with
+//                         heads of 256 in 16 bits).
 //  attention_combine_kernel  joins the parts of split keys, 4 to 12 us: the partial
 //                         sums are fp32, written and read once.
 //
@@ -442,17 +442,17 @@ struct ValueRow {
 // work for each, whatever the lengths.  Every workgroup works the cuts out from the lengths,
 // so the host needs to know none of them and a captured call follows them.  Blocks of 8-bit keys
 // are twice as long, as a wave's steps are.
-template <typename C>
-constexpr int kBlockKeys = 4 * Cache<C>::kFewKeys;
+template <typename C, int W>
+constexpr int kBlockKeys = W * Cache<C>::kFewKeys;
 
 // count > 0 of a sequence whose rows fit the few-row kernel
 __device__ __forceinline__ bool few_rows(const PagedSequence &q, int group) {
   return q.count > 0 && q.count <= kFewRows / group;
 }
 // Blocks of a sequence: 0 of one that is not the few-row kernel's, at least 1 of others.
-template <typename C>
+template <typename C, int W>
 __device__ __forceinline__ int few_blocks(const Attention &a, const PagedSequence &q) {
-  return few_rows(q, a.group) ? max((q.length + kBlockKeys<C> - 1) / kBlockKeys<C>, 1) : 0;
+  return few_rows(q, a.group) ? max((q.length + kBlockKeys<C, W> - 1) / kBlockKeys<C, W>, 1) : 0;
 }
 
 struct Spans {
@@ -475,19 +475,19 @@ __device__ __forceinline__ PagedSequence lane_sequence(const Attention &a) {
                  : PagedSequence{};
 }
 
-// The spans, and the sequence that holds the first block of span `index`.  All 256 threads;
-// scratch (8 words of LDS) and found are free again afterwards.
-template <typename C>
+// The spans, and the sequence that holds the first block of span `index`.  All threads of
+// the W waves; scratch (2 W words of LDS) and found are free again afterwards.
+template <typename C, int W>
 __device__ Spans find_span(const Attention &a, int index, const PagedSequence &mine,
                            int64_t *scratch, Find *found, Find &got) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, S = a.batch.sequences;
   Spans sp;
   got = {0, -1};
   auto blocks = [&](int s) {
-    return s < S ? few_blocks<C>(a, paged_sequences(a.batch, s, a.tokens)) : 0;
+    return s < S ? few_blocks<C, W>(a, paged_sequences(a.batch, s, a.tokens)) : 0;
   };
   if (S <= 64) {  // every wave by itself: a sequence a lane
-    const uint32_t n = lane < S ? few_blocks<C>(a, mine) : 0;  // 64 of at most 2^25
+    const uint32_t n = lane < S ? few_blocks<C, W>(a, mine) : 0;  // 64 of at most 2^25
     const uint32_t sum = wave_scan(n);
     sp.blocks = (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
     sp.spans = (int)min((int64_t)a.shares, sp.blocks);
@@ -501,26 +501,27 @@ __device__ Spans find_span(const Attention &a, int index, const PagedSequence &m
   if (tid == 0) found->s = -1;
   const int own = blocks(tid);
   int64_t all = own;
-  for (int s = tid + 256; s < S; s += 256) all += blocks(s);
+  for (int s = tid + W * 64; s < S; s += W * 64) all += blocks(s);
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) all += __shfl_xor(all, o, 64);
   if (lane == 0) scratch[wave] = all;
   __syncthreads();
-  sp.blocks = scratch[0] + scratch[1] + scratch[2] + scratch[3];
+  sp.blocks = 0;
+  for (int w = 0; w < W; ++w) sp.blocks += scratch[w];
   sp.spans = (int)min((int64_t)a.shares, sp.blocks);
   if (index < sp.spans) {
     const int64_t want = sp.start(index);
-    int64_t base = 0;  // blocks before this group of 256 sequences
-    for (int c = 0; c < S && base <= want; c += 256) {
+    int64_t base = 0;  // blocks before this group of sequences
+    for (int c = 0; c < S && base <= want; c += W * 64) {
       const int n = c == 0 ? own : blocks(c + tid);
       const int64_t sum = (int64_t)wave_scan((uint64_t)n);
       __syncthreads();
-      if (lane == 63) scratch[4 + wave] = sum;
+      if (lane == 63) scratch[W + wave] = sum;
       __syncthreads();
       int64_t before = base + sum - n;
-      for (int w = 0; w < 4; ++w) {
-        if (w < wave) before += scratch[4 + w];
-        base += scratch[4 + w];
+      for (int w = 0; w < W; ++w) {
+        if (w < wave) before += scratch[W + w];
+        base += scratch[W + w];
       }
       if (n > 0 && want >= before && want < before + n) *found = {before, c + tid};
     }
@@ -532,7 +533,7 @@ __device__ Spans find_span(const Attention &a, int index, const PagedSequence &m
 }
 
 // ------------------------------------------------------------------ few rows
-constexpr int kFewWaves = 4;
+constexpr int kFewWaves = 4;  // W, but for attention_both_kernel with heads of 256
 
 // Steps of 16 keys in a wave's ring: 64 KB for a workgroup, two of which share a CU, or 32 KB
 // with heads of 64, of which three do: of 24 sequences of 300 to 5000 keys 33 instead of 37 us,
@@ -542,12 +543,11 @@ template <int D>
 constexpr int few_steps() { return D == 256 ? 1 : 2; }
 template <int D, int STEPS = few_steps<D>()>
 constexpr int few_ring() { return STEPS * 2 * 16 * D * 2; }
-template <int D>
-constexpr int few_merge() { return kFewWaves * (kFewRows * (D + 4) + 2 * kFewRows) * 4; }
-template <int D, int STEPS = few_steps<D>()>
+template <int D, int W>
+constexpr int few_merge() { return W * (kFewRows * (D + 4) + 2 * kFewRows) * 4; }
+template <int D, int STEPS = few_steps<D>(), int W = kFewWaves>
 constexpr int few_lds() {
-  return kFewWaves * few_ring<D, STEPS>() > few_merge<D>() ? kFewWaves * few_ring<D, STEPS>()
-                                                           : few_merge<D>();
+  return W * few_ring<D, STEPS>() > few_merge<D, W>() ? W * few_ring<D, STEPS>() : few_merge<D, W>();
 }
 
 // The running state of a wave's 16 columns (column lane & 15 in each 16 lanes).
@@ -842,7 +842,7 @@ __device__ __forceinline__ int64_t part_row(const Attention &a, int span, bool l
 
 // Blocks b0 .. b1 - 1 of sequence s at key-value head kv; `part`: its row among the parts, or
 // negative where these are all of its blocks.
-template <typename T, int D, typename C, int STEPS>
+template <typename T, int D, typename C, int STEPS, int W>
 __device__ __forceinline__ void few_part(const Attention &a, const PagedSequence &seq, int s, int kv,
                                          int b0, int b1, int64_t part, char *lds) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -860,9 +860,9 @@ __device__ __forceinline__ void few_part(const Attention &a, const PagedSequence
   f.table = a.batch.table + s * a.batch.table_stride;
   f.page_stride = a.batch.page_stride, f.shift = a.batch.page_shift;
   f.pages = a.batch.pages, f.entries = a.batch.table_pages;
-  const int last = min(b1 * (kBlockKeys<C> / KEYS), (seq.length + KEYS - 1) / KEYS);
-  f.first = b0 * (kBlockKeys<C> / KEYS) + wave, f.stride = kFewWaves;
-  f.steps = last > f.first ? (last - f.first + kFewWaves - 1) / kFewWaves : 0;
+  const int last = min(b1 * (kBlockKeys<C, W> / KEYS), (seq.length + KEYS - 1) / KEYS);
+  f.first = b0 * (kBlockKeys<C, W> / KEYS) + wave, f.stride = W;
+  f.steps = last > f.first ? (last - f.first + W - 1) / W : 0;
   const int limit = min(seq.base + col / a.group + 1, seq.length);
   const int all_see = min(seq.base + 1, seq.length);  // keys that every row sees
 
@@ -923,7 +923,7 @@ __device__ __forceinline__ void few_part(const Attention &a, const PagedSequence
   // The waves' sums, scaled to the largest of their maxima.
   __syncthreads();
   float *sums = reinterpret_cast<float *>(lds);  // [wave][row][D + 4]
-  float *ml = sums + kFewWaves * kFewRows * (D + 4);  // [wave][row] maxima, then sums
+  float *ml = sums + W * kFewRows * (D + 4);  // [wave][row] maxima, then sums
   st.l = across32(across16(st.l, Add()), Add());
 #pragma unroll
   for (int i = 0; i < D / 16; ++i)
@@ -931,19 +931,19 @@ __device__ __forceinline__ void few_part(const Attention &a, const PagedSequence
         st.o[i];
   if (lane < 16) {
     ml[wave * kFewRows + lane] = st.m;
-    ml[(kFewWaves + wave) * kFewRows + lane] = st.l;
+    ml[(W + wave) * kFewRows + lane] = st.l;
   }
   __syncthreads();
-  for (int i = tid; i < rows * (D / 4); i += 256) {
+  for (int i = tid; i < rows * (D / 4); i += W * 64) {
     const int c = i / (D / 4), d = i % (D / 4) * 4;
     float m = ml[c], l = 0.0f;
 #pragma unroll
-    for (int w = 1; w < kFewWaves; ++w) m = fmaxf(m, ml[w * kFewRows + c]);
+    for (int w = 1; w < W; ++w) m = fmaxf(m, ml[w * kFewRows + c]);
     f32x4 o = {};
 #pragma unroll
-    for (int w = 0; w < kFewWaves; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float k = decay(ml[w * kFewRows + c], m);
-      l += ml[(kFewWaves + w) * kFewRows + c] * k;
+      l += ml[(W + w) * kFewRows + c] * k;
       o += *reinterpret_cast<const f32x4 *>(sums + (w * kFewRows + c) * (D + 4) + d) * k;
     }
     if (part < 0) {
@@ -958,13 +958,13 @@ __device__ __forceinline__ void few_part(const Attention &a, const PagedSequence
 }
 
 // Workgroup `index` of those of few rows.
-template <typename T, int D, typename C, int STEPS>
+template <typename T, int D, typename C, int STEPS, int W>
 __device__ __forceinline__ void few_span(const Attention &a, int index, const PagedSequence &mine,
                                          char *lds) {
   int64_t *scratch = reinterpret_cast<int64_t *>(lds);
   const int kv = index % a.batch.kv_heads, span = index / a.batch.kv_heads;
   Find at;
-  const Spans sp = find_span<C>(a, span, mine, scratch, reinterpret_cast<Find *>(scratch + 8), at);
+  const Spans sp = find_span<C, W>(a, span, mine, scratch, reinterpret_cast<Find *>(scratch + 2 * W), at);
   if (at.s < 0) return;
   int64_t block = sp.start(span);
   const int64_t end = sp.start(span + 1);
@@ -973,12 +973,12 @@ __device__ __forceinline__ void few_span(const Attention &a, int index, const Pa
   bool later = false;
   for (; block < end && s < a.batch.sequences; ++s, done = 0) {
     const PagedSequence seq = sequence_at(a.batch, s, mine, a.tokens);
-    const int all = few_blocks<C>(a, seq);
+    const int all = few_blocks<C, W>(a, seq);
     const int take = __builtin_amdgcn_readfirstlane((int)min((int64_t)(all - done), end - block));
     if (take <= 0) continue;
     if (done == 0 && threadIdx.x == 0)  // where its parts are, for the kernel that joins them
       a.parts[s * a.batch.kv_heads + kv] = {span, later, sp.of(block + all - 1) - span + 1};
-    few_part<T, D, C, STEPS>(a, seq, s, kv, done, done + take,
+    few_part<T, D, C, STEPS, W>(a, seq, s, kv, done, done + take,
                       take == all ? -1 : part_row(a, span, later, kv), lds);
     block += take;
     later = true;
@@ -989,7 +989,7 @@ template <typename T, int D, typename C>
 __global__ __launch_bounds__(256, Cache<C>::kScaled ? 2 : 1) void attention_few_kernel(Attention a) {
   // One array: with several, the compiler waits for all direct loads at each LDS read.
   __shared__ __attribute__((aligned(16))) char lds[few_lds<D>()];
-  few_span<T, D, C, few_steps<D>()>(a, blockIdx.x, lane_sequence(a), lds);
+  few_span<T, D, C, few_steps<D>(), kFewWaves>(a, blockIdx.x, lane_sequence(a), lds);
 }
 
 // The sum of parts of a row: a thread's four channels, under the largest maximum so far.
@@ -1700,19 +1700,19 @@ __global__ __launch_bounds__((TileForm<D, C>::kWaves * 64), 2) void attention_ti
 }
 
 // ------------------------------------------------------------------ both in one launch
-// Spans of few rows and places of tiles of a call, for a key-value head.  All 256 threads; sums is
-// free again afterwards.
+// Spans of few rows and places of tiles of a call, for a key-value head.  All threads of the W
+// waves; sums is free again afterwards.
 struct Counts {
   int spans;
   int64_t places;
 };
-template <typename C>
+template <typename C, int W>
 __device__ Counts count_both(const Attention &a, const PagedSequence &mine, uint64_t *sums) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, S = a.batch.sequences;
   TileTotals total = {};
   if (S <= 64) {  // each wave for itself
     const int n = lane < S ? tile_count(a, mine) : 0;
-    const uint64_t blocks = wave_total((uint64_t)(lane < S ? few_blocks<C>(a, mine) : 0));
+    const uint64_t blocks = wave_total((uint64_t)(lane < S ? few_blocks<C, W>(a, mine) : 0));
     if (a.room) total = {(int)wave_total((uint64_t)n), wave_total(all_keys(a, mine, n))};
     const int m = a.room ? tile_places(a, total, mine, n) : 1;
     return {(int)min((uint64_t)a.shares, blocks), (int64_t)wave_total((uint64_t)n * m)};
@@ -1722,19 +1722,21 @@ __device__ Counts count_both(const Attention &a, const PagedSequence &mine, uint
     __syncthreads();
     if (lane == 0) sums[wave] = v;
     __syncthreads();
-    return sums[0] + sums[1] + sums[2] + sums[3];
+    v = 0;
+    for (int w = 0; w < W; ++w) v += sums[w];
+    return v;
   };
   uint64_t blocks = 0, tiles = 0, keys = 0, places = 0;
-  for (int c = tid; c < S; c += 256) {
+  for (int c = tid; c < S; c += W * 64) {
     const PagedSequence q = paged_sequences(a.batch, c, a.tokens);
     const int n = tile_count(a, q);
-    blocks += few_blocks<C>(a, q), tiles += n, keys += all_keys(a, q, n);
+    blocks += few_blocks<C, W>(a, q), tiles += n, keys += all_keys(a, q, n);
   }
   blocks = all(blocks), places = tiles = all(tiles);
   if (a.room) {
     total = {(int)tiles, all(keys)};
     places = 0;
-    for (int c = tid; c < S; c += 256) {
+    for (int c = tid; c < S; c += W * 64) {
       const PagedSequence q = paged_sequences(a.batch, c, a.tokens);
       const int n = tile_count(a, q);
       places += (uint64_t)n * tile_places(a, total, q, n);
@@ -1752,26 +1754,36 @@ __device__ Counts count_both(const Attention &a, const PagedSequence &mine, uint
 // 41 instead of 51 (64).  All of one kind first was better for some and 10 % worse than two
 // launches for others, as were places for the most that a call can have of each: those without
 // work then come before some with it.  Heads of 128 have a ring of one step here, so that three
-// workgroups still share a CU.  Heads of 256 have two launches: their tiles' workgroups have eight
-// waves.
+// workgroups still share a CU.  With heads of 256 few rows have eight waves as tiles do, one
+// workgroup a CU; of 8 bits 24 sequences of 2 to 24 tokens take 56 us instead of 63, 64 of one
+// beside two prompts 74 instead of 80, 16 prompts alone 75.5 instead of 73.5.  Of 16 bits the two
+// do not fit the registers there, and have two launches.
+template <int D, typename C>
+constexpr bool kBoth = D < 256 || Cache<C>::kScaled;
 constexpr int kTurn = 256;
 
 template <typename T, int D, typename C>
-__global__ __launch_bounds__(256, D == 64 ? 4 : 3) void attention_both_kernel(Attention a) {
-  constexpr int STEPS = D == 64 ? 2 : 1, FEW = few_lds<D, STEPS>(), TILE = tile_lds<D, C>();
+__global__ __launch_bounds__((TileForm<D, C>::kWaves * 64),
+                             (D == 64 ? 4 : D == 128 ? 3 : 2)) void attention_both_kernel(Attention a) {
+  constexpr int STEPS = D == 64 ? 2 : 1, W = TileForm<D, C>::kWaves;
+  constexpr int FEW = few_lds<D, STEPS, W>(), TILE = tile_lds<D, C>();
   // One array: with several, the compiler waits for all direct loads at each LDS read.
   __shared__ __attribute__((aligned(16))) char lds[FEW > TILE ? FEW : TILE];
   const PagedSequence mine = lane_sequence(a);
-  const Counts n = count_both<C>(a, mine, reinterpret_cast<uint64_t *>(lds));
+  const Counts n = count_both<C, W>(a, mine, reinterpret_cast<uint64_t *>(lds));
   const int few = n.spans * a.batch.kv_heads;
   const int64_t tiles = n.places * a.batch.kv_heads;
-  const int turns = (int)min((int64_t)(few + kTurn - 1) / kTurn, (tiles + kTurn - 1) / kTurn);
+  // the same for every lane, which the compiler cannot tell of what went through LDS
+  const int turns = __builtin_amdgcn_readfirstlane(
+      (int)min((int64_t)(few + kTurn - 1) / kTurn, (tiles + kTurn - 1) / kTurn));
   const int turn = blockIdx.x / kTurn, at = blockIdx.x % kTurn;
   const int index = (turn < 2 * turns ? turn / 2 : turn - turns) * kTurn + at;
-  if (turn < 2 * turns ? turn % 2 == 0 : tiles > few) {
-    if (index < tiles) tile_rows<T, D, C>(a, index, 0, mine, lds);
-  } else {
-    if (index < few) few_span<T, D, C, STEPS>(a, index, mine, lds);
+  const bool tile = turn < 2 * turns ? turn % 2 == 0 : tiles > few;
+  const int work = __builtin_amdgcn_readfirstlane(index >= (tile ? tiles : few) ? 0 : tile ? 2 : 1);
+  if (work == 2) {
+    tile_rows<T, D, C>(a, index, 0, mine, lds);
+  } else if (work == 1) {
+    few_span<T, D, C, STEPS, W>(a, index, mine, lds);
   }
 }
 
@@ -1835,14 +1847,16 @@ struct AttentionPlan {
 };
 
 AttentionPlan attention_plan(int64_t tokens, int64_t sequences, int64_t q_heads, int64_t kv_heads,
-                             int64_t head_dim, int64_t max_new, int64_t max_keys) {
+                             int64_t head_dim, int64_t max_new, int64_t max_keys,
+                             bool e4m3 = false) {
   AttentionPlan p = {};
   const int64_t group = q_heads / kv_heads;
   max_new = max_new < tokens ? max_new : tokens;
   p.tile = max_new * group > kFewRows;
   p.few = group <= kFewRows && !(p.tile && sequences == 1);  // one sequence: one of them
   if (p.few) {
-    const int64_t all = head_dim == 64 ? 768 : 512;  // workgroups that run at a time
+    // workgroups that run at a time
+    const int64_t all = head_dim == 64 ? 768 : head_dim == 256 && p.tile && e4m3 ? 256 : 512;
     p.shares = all / kv_heads > 1 ? all / kv_heads : 1;
     p.few_grid = p.shares * kv_heads;
     p.few_rows = 2 * p.shares * kv_heads * kFewRows;
@@ -1883,7 +1897,8 @@ int launch_attention(const AttentionPlan &p, Attention a, float *workspace, hipS
   a.row_parts = reinterpret_cast<int *>(a.parts + p.parts);
   a.shares = (int)p.shares, a.splits = (int)p.splits, a.room = (int)p.room;
   int64_t ys = 0, tile = 0;  // workgroups that join parts: ys for each of p.parts, and tile
-  const bool both = D < 256 && p.few && p.tile;
+  constexpr bool CAN = kBoth<D, C>;
+  const bool both = CAN && p.few && p.tile;
   if (p.few) {
     if (!both) {
       attention_few_kernel<T, D, C><<<(unsigned)p.few_grid, 256, 0, st>>>(a);
@@ -1903,9 +1918,9 @@ int launch_attention(const AttentionPlan &p, Attention a, float *workspace, hipS
     if (!both) {
       attention_tile_kernel<T, D, C><<<grid, TileForm<D, C>::kWaves * 64, 0, st>>>(a);
       if (const int rc = check_launch("attention_tile_kernel")) return rc;
-    } else if constexpr (D < 256) {  // of several sequences, whose parts have no dimension of the grid
+    } else if constexpr (CAN) {  // of several sequences, whose parts have no dimension of the grid
       const int64_t turns = (grid.x + kTurn - 1) / kTurn + (p.few_grid + kTurn - 1) / kTurn;
-      attention_both_kernel<T, D, C><<<(unsigned)(turns * kTurn), 256, 0, st>>>(a);
+      attention_both_kernel<T, D, C><<<(unsigned)(turns * kTurn), TileForm<D, C>::kWaves * 64, 0, st>>>(a);
       if (const int rc = check_launch("attention_both_kernel")) return rc;
     }
     if (p.splits > 1) tile = (int64_t)a.tokens * chunks;
@@ -1958,7 +1973,7 @@ int paged_attention(const void *q, int64_t q_token_stride, int64_t q_head_stride
                        gate_token_stride >= 0 && gate_head_stride >= 0),
              LM_EINVAL, "head rows must be 16-byte aligned");
   const AttentionPlan plan = attention_plan(tokens, sequences, q_heads, kv_heads, head_dim, max_new,
-                                            table_pages * page_size);
+                                            table_pages * page_size, E4M3_CACHE);
   // threads of the largest launches, below 2^32
   LM_REQUIRE(sequences * kv_heads < (1LL << 24) && plan.tiles * kv_heads < (1LL << 23), LM_EINVAL,
              "too many rows");
