@@ -1794,18 +1794,26 @@ __device__ __forceinline__ void combine_tile(const Attention &a, int block, int 
   const int t = block / chunks, lane = threadIdx.x & 63;
   const int i = block % chunks * 256 + threadIdx.x;
   const int head = i / (D / 4), d = i % (D / 4) * 4;
-  int s = -1;  // the token's sequence: a lane looks at one of 64
-  for (int c = 0; c < a.batch.sequences && s < 0; c += 64) {
-    const int k = c + lane;
-    const uint64_t hit = __ballot(k < a.batch.sequences && a.batch.starts[min(k, a.batch.sequences - 1)] <= t &&
-                                  t < a.batch.starts[min(k, a.batch.sequences - 1) + 1]);
-    if (hit) s = c + __builtin_ctzll(hit);
+  const int64_t rows = (int64_t)a.tokens * a.q_heads;
+  const int64_t row = (int64_t)t * a.q_heads + min(head, a.q_heads - 1);
+  // The token's sequence, of which a lane looks at one of 64, and the parts of its row are looked up
+  // together; left to itself, the compiler has a round of loads for each.
+  int parts = a.room ? a.row_parts[row] : a.splits, lo = 0, hi = 0;
+  for (int c = 0; c < a.batch.sequences; c += 64) {
+    const int k = min(c + lane, a.batch.sequences - 1);
+    int from = a.batch.starts[k], to = a.batch.starts[k + 1];
+    asm volatile("" : "+v"(from), "+v"(to), "+v"(parts));
+    const uint64_t hit = __ballot(c + lane < a.batch.sequences && from <= t && t < to);
+    if (hit) {
+      const int at = __builtin_ctzll(hit);
+      lo = __builtin_amdgcn_readlane(from, at), hi = __builtin_amdgcn_readlane(to, at);
+      break;
+    }
   }
-  if (s < 0 || head >= a.q_heads) return;
-  const PagedSequence seq = paged_sequence(a.batch, s, a.tokens);
-  if (t < seq.first || t >= seq.first + seq.count || (a.few && few_rows(seq, a.group))) return;
-  const int64_t rows = (int64_t)a.tokens * a.q_heads, row = (int64_t)t * a.q_heads + head;
-  const int parts = a.room ? min(a.row_parts[row], a.splits) : a.splits;
+  if (lo == hi || head >= a.q_heads) return;  // of no sequence
+  const PagedSequence seq = paged_sequence(a.batch, lo, hi, 0, a.tokens);
+  if (t >= seq.first + seq.count || (a.few && few_rows(seq, a.group))) return;
+  parts = min(parts, a.splits);
   if (parts < 2) return;  // written by its tile
   const uint2 gate = load_gate(a, {t, head}, d);
   PartSum sum;
