@@ -577,6 +577,44 @@ def test_captured_step_follows_its_batch(dev):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
 
 
+@pytest.mark.parametrize('eight', [False, True])
+@pytest.mark.parametrize('dim', [64, 128, 256])
+def test_captured_call_of_any_kind(dev, dim, eight):
+    """One captured call, replayed for prompts beside single tokens, one kind alone and no new token at
+    all: what the batch then holds decides, bit for bit as in a call of its own."""
+    gen, tokens, page = seeded(dim), 150, 16
+    kp, vp, scales = C.random_cache(gen, 500, 2, page, dim, BF16)
+    if not eight:
+        kp, vp = rand(gen, 500, 2, page, dim), rand(gen, 500, 2, page, dim)
+    kp, vp, q, gate = to(dev, kp, vp, rand(gen, tokens, 8, dim), rand(gen, tokens, 8, dim))
+    scales = scales.to(dev) if eight else None
+    table = torch.randperm(500, generator=gen)[:480].view(12, 40).to(I32).to(dev)
+    kinds = [[(1, 600 - 40 * i) for i in range(9)] + [(70, 100), (30, 500), (9, 9)],
+             [(1, 50 * i + 1) for i in range(12)], [(0, 7)] * 12,
+             [(40, 640), (0, 0), (50, 60)] + [(0, 3)] * 8 + [(60, 300)],
+             [(0, 0)] * 4 + [(2, 640)] * 4 + [(30, 31)] + [(1, 1)] * 3]
+    starts, lengths = torch.zeros(13, dtype=I32, device=dev), torch.zeros(12, dtype=I32, device=dev)
+    out = torch.zeros_like(q)
+
+    def call(o):
+        return A.paged_attention(q, kp, vp, starts, lengths, table, gate=gate, out=o, scales=scales)
+
+    call(out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(out)
+    for lens in kinds + kinds[::-1]:
+        starts.copy_(torch.tensor([0] + [n for n, _ in lens]).cumsum(0))
+        lengths.copy_(torch.tensor([n for _, n in lens]))
+        out.fill_(3.0)
+        graph.replay()
+        want = call(torch.full_like(q, 3.0))
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), lens
+        assert (out[int(starts[-1]):] == 3.0).all()
+
+
 def test_calls_on_two_streams(dev):
     """Two calls at once, each on its own stream and workspace, give what they give alone."""
     gen, args = seeded(13), []
