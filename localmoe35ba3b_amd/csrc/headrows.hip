@@ -360,10 +360,12 @@ __device__ __forceinline__ void block_rows(const HeadRows &a, const E4m3Pages &p
     Row8 raw[PASSES];
     load(d, raw);
     float *scale = p.scales + page * p.scale_stride + (2 * head + value) * nb + inside;
-    int least = kScaleLeast<T>;
+    // The exponent of the rows held already is the one that attention reads; another program may
+    // have left them one below the least, under which they are rounded again.
+    int least = kScaleLeast<T>, held = least;
     if (before > 0) {
-      const int held = (int)(__float_as_uint(*scale) >> 23 & 0xFFu) - 127;
-      least = min(max(held, kScaleLeast<T>), kScaleMost<T>);
+      held = min((int)(__float_as_uint(*scale) >> 23 & 0xFFu) - 127, kScaleMost<T>);
+      least = max(held, least);
     }
     const float *weight = value ? nullptr : a.k_w;
     float w0[4] = {}, w1[4] = {};
@@ -427,12 +429,12 @@ __device__ __forceinline__ void block_rows(const HeadRows &a, const E4m3Pages &p
     for (int i = 0; i < WAVES; ++i) e = max(e, largest[odd][wave / WAVES * WAVES + i]);
     uint8_t *rows = (value ? p.v : p.k) + page * a.batch.page_stride +
                     (((int64_t)head << a.batch.page_shift) + inside * kScaleKeys) * D;
-    const float inverse = power_of_two(-e), ratio = power_of_two(max(least - e, -126));
+    const float inverse = power_of_two(-e), ratio = power_of_two(max(held - e, -126));
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
       const int r = row + i * ROWS;
       if (r < before) {
-        if (e > least) {
+        if (e > held) {
           uint2 *b = reinterpret_cast<uint2 *>(rows + r * D + lane * 8);
           const uint2 old = *b;
           *b = uint2{rescale_e4m3(old.x, ratio), rescale_e4m3(old.y, ratio)};

@@ -242,9 +242,9 @@ def append(k_pages, v_pages, k, v, starts, lengths, table, inv_freq=None, k_weig
     (k_weight and inv_freq as in qk_norm_rope, by its position in its sequence, or by
     positions [T], or [A, T] with axes, which count for the rotation only).
     With scales, the pages hold 8 bits: each block of 16 positions takes the smallest power
-    of two that brings the values of its rows to 448 at most.  As later calls fill it, the
-    scale only grows; rows held already are then rounded again, which changes those below
-    2^-6 of it alone.  Rows of a block behind a sequence's last keep their bits, and where
+    of two that brings the values of its rows to 448 at most, from 2^-117 on (fp16: 2^-15).
+    As later calls fill it, the scale only grows; rows held already are then rounded again,
+    which changes those below 2^-6 of it alone.  Rows of a block behind a sequence's last keep their bits, and where
     positions are taken back inside a block, it keeps the scale that they needed.  A value is
     rounded once, from fp32; beyond 61440 in fp16 (0x1.Ep127 in bf16) it is held as that,
     infinities and NaN as NaN.

@@ -96,3 +96,37 @@ def test_append_leaves_what_is_held_beside_normed_keys(dev, dim, page, dtype):
                 assert torch.equal(after[number, :, at], bits[number, :, at]), (length, number, at)
         length += n
     assert grown > 0
+
+
+@TYPES
+@pytest.mark.parametrize('dim', [64, 128, 256])
+def test_append_into_blocks_of_small_scales(dev, dim, dtype):
+    """Scales below the least that an append makes, as another program may have written them: rows held
+    under them stay the values that attention reads, rounded under the new scale."""
+    gen, heads, page = seeded(dim + 7), 2, 32
+    exps = [-118, -121, -126] if dtype == BF16 else [-16, -20, -27]
+    for size in (0.0, 1e-6, 1.0):  # new rows that need the least scale, or more
+        kp, vp, scales = to(dev, *C.random_cache(gen, 4, heads, page, dim, dtype))
+        for number, e in zip((2, 0, 3), exps):
+            scales[number] = 2.0 ** e
+        want, scale64 = C.held(kp, vp, scales), [scales[:, :, s].cpu().double() for s in range(2)]
+        table = [2, 0, 3]
+        for base, n in ((5, 1), (6, 3), (page + 15, 2), (2 * page + 20, 4)):
+            k, v = ((torch.randn(n, heads, dim, generator=gen) * size).to(dtype) for _ in range(2))
+            plain_append((kp, vp, scales), want, scale64, k, v, base, table, page, dtype)
+
+
+def test_attention_before_and_after_an_append_to_a_small_scale(dev):
+    """What a row sees of the keys held before is the same before and after the append that lifts their
+    block's scale: fp16 values that 2^-15 still holds exactly."""
+    gen, page, dim = seeded(4), 16, 64
+    kp, vp, scales = to(dev, *C.random_cache(gen, 2, 1, page, dim, FP16))
+    vp[0] = (torch.randint(1, 15, (1, page, dim), generator=gen) * 32.0).to(dev).to(C.E4M3)  # 2^-15 of steps of 1
+    scales[0] = 2.0 ** -20
+    q = torch.zeros(1, 2, dim, dtype=FP16, device=dev)  # equal weights
+    batch = to(dev, ints(0, 1), ints(4), ints(0).view(1, 1))
+    a = A.paged_attention(q, kp, vp, *batch, scales=scales)
+    zero = torch.zeros(1, 1, dim, dtype=FP16, device=dev)
+    A.append(kp, vp, zero, zero, *to(dev, ints(0, 1), ints(5), ints(0).view(1, 1)), scales=scales)
+    assert scales[0].cpu().eq(2.0 ** -15).all()
+    assert torch.equal(A.paged_attention(q, kp, vp, *batch, scales=scales), a) and a.any()
