@@ -78,14 +78,13 @@ __global__ __launch_bounds__(256) void act_quant_kernel(const uint16_t *__restri
 // h := T(h + x), n = h rsqrt(mean h^2 + eps) (1 + w), s = max(amax |n|, 1e-10) fl(1/127) of each 128,
 // q = rint(n / s): n stays in fp32 until it is quantized.  A row lies in the registers of WAVES
 // waves, eight values a thread and chunk, a group of 128 in 16 lanes; it is read once.  Not finite
-// values leave a scale that is not.
+// values leave a scale that is not.  x may be h itself: a thread's loads come before its stores.
 //
 // Bound by its bytes, 7 a value: 2048 rows of 2048 7.5 us (29.5 MB, 3.9 TB/s with the start),
 // 8192 rows 19.8 us (5.9 TB/s); one row 2 us.  Divisions and a conversion for each byte took twice
 // that (14.0 and 44.5 us).  A wave a row of 2048, without a barrier, took 8.1 us.
 template <typename T, int WAVES, int CHUNKS, bool ADD>
-__global__ __launch_bounds__(256) void norm_quant_kernel(uint16_t *__restrict__ h,
-                                                         const uint16_t *__restrict__ x,
+__global__ __launch_bounds__(256) void norm_quant_kernel(uint16_t *h, const uint16_t *x,
                                                          const float *__restrict__ w,
                                                          int8_t *__restrict__ q,
                                                          float *__restrict__ s, int64_t rows, int n,
