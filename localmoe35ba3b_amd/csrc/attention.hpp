@@ -1896,6 +1896,38 @@ int64_t attention_bytes(const AttentionPlan &p, int64_t head_dim) {
          (p.parts * sizeof(Parts) + 15) / 16 * 16;
 }
 
+// Workgroups of attention_combine_kernel for a sequence's key-value head.  Where there are few
+// sequences, their rows and channels fill the chip.  Against twice as many workgroups at most, 24
+// sequences with 2 to 9 rows took 24.1 instead of 25.2 us and 16 of up to 300 new tokens 34.3 instead
+// of 35.6; with half as many, 24 of 2 to 24 (heads of 256), of which three are split in many parts,
+// took 69.0 instead of 63.5.
+int64_t pair_groups(const AttentionPlan &p, int64_t group, int64_t head_dim) {
+  const int64_t units = kFewRows / group * group * (head_dim / 64), some = 2048 / p.parts;
+  return some < 1 ? 1 : some < units ? some : units;
+}
+// And for a token's rows in tiles.
+int row_chunks(int64_t q_heads, int64_t head_dim) {
+  return (int)((q_heads * (head_dim / 4) + 255) / 256);
+}
+// Workgroups of attention_both_kernel.
+int64_t both_groups(const AttentionPlan &p, int64_t kv_heads) {
+  const int64_t tiles = p.tiles * kv_heads * p.splits;
+  return ((tiles + kTurn - 1) / kTurn + (p.few_grid + kTurn - 1) / kTurn) * kTurn;
+}
+// Whether the launches that take up more than a call's tiles or its sequences' key-value heads have
+// fewer than 2^32 threads: both kinds together, and the joining of both.
+template <bool E4M3_CACHE>
+bool attention_fits(const AttentionPlan &p, int64_t tokens, int64_t q_heads, int64_t kv_heads,
+                    int64_t head_dim) {
+  constexpr int64_t kThreads = 1LL << 32;
+  if (p.few && p.tile && (head_dim < 256 || E4M3_CACHE) &&
+      both_groups(p, kv_heads) * (head_dim == 256 ? 512 : 256) >= kThreads)
+    return false;
+  const int64_t few = p.few ? p.parts * pair_groups(p, q_heads / kv_heads, head_dim) : 0;
+  const int64_t tile = p.splits > 1 ? tokens * row_chunks(q_heads, head_dim) : 0;
+  return (few + tile) * 256 < kThreads;
+}
+
 template <typename T, int D, typename C>
 int launch_attention(const AttentionPlan &p, Attention a, float *workspace, hipStream_t st) {
   a.few = p.few;
@@ -1912,14 +1944,9 @@ int launch_attention(const AttentionPlan &p, Attention a, float *workspace, hipS
       attention_few_kernel<T, D, C><<<(unsigned)p.few_grid, 256, 0, st>>>(a);
       if (const int rc = check_launch("attention_few_kernel")) return rc;
     }
-    // Where there are few sequences, their rows and channels fill the chip.  Against twice as many
-    // workgroups at most, 24 sequences with 2 to 9 rows took 24.1 instead of 25.2 us and 16 of up to
-    // 300 new tokens 34.3 instead of 35.6; with half as many, 24 of 2 to 24 (heads of 256), of which
-    // three are split in many parts, took 69.0 instead of 63.5.
-    const int64_t units = kFewRows / a.group * a.group * (D / 64), some = 2048 / p.parts;
-    ys = some < 1 ? 1 : some < units ? some : units;
+    ys = pair_groups(p, a.group, D);
   }
-  const int chunks = (a.q_heads * (D / 4) + 255) / 256;
+  const int chunks = row_chunks(a.q_heads, D);
   if (p.tile) {
     const int64_t all = p.tiles * a.batch.kv_heads;
     const dim3 grid((unsigned)(p.room ? all * p.splits : all), (unsigned)(p.room ? 1 : p.splits));
@@ -1927,8 +1954,8 @@ int launch_attention(const AttentionPlan &p, Attention a, float *workspace, hipS
       attention_tile_kernel<T, D, C><<<grid, TileForm<D, C>::kWaves * 64, 0, st>>>(a);
       if (const int rc = check_launch("attention_tile_kernel")) return rc;
     } else if constexpr (CAN) {  // of several sequences, whose parts have no dimension of the grid
-      const int64_t turns = (grid.x + kTurn - 1) / kTurn + (p.few_grid + kTurn - 1) / kTurn;
-      attention_both_kernel<T, D, C><<<(unsigned)(turns * kTurn), TileForm<D, C>::kWaves * 64, 0, st>>>(a);
+      attention_both_kernel<T, D, C>
+          <<<(unsigned)both_groups(p, a.batch.kv_heads), TileForm<D, C>::kWaves * 64, 0, st>>>(a);
       if (const int rc = check_launch("attention_both_kernel")) return rc;
     }
     if (p.splits > 1) tile = (int64_t)a.tokens * chunks;
@@ -1982,9 +2009,9 @@ int paged_attention(const void *q, int64_t q_token_stride, int64_t q_head_stride
              LM_EINVAL, "head rows must be 16-byte aligned");
   const AttentionPlan plan = attention_plan(tokens, sequences, q_heads, kv_heads, head_dim, max_new,
                                             table_pages * page_size, E4M3_CACHE);
-  // threads of the largest launches, below 2^32
-  LM_REQUIRE(sequences * kv_heads < (1LL << 24) && plan.tiles * kv_heads < (1LL << 23), LM_EINVAL,
-             "too many rows");
+  LM_REQUIRE(sequences * kv_heads < (1LL << 24) && plan.tiles * kv_heads < (1LL << 23) &&
+                 attention_fits<E4M3_CACHE>(plan, tokens, q_heads, kv_heads, head_dim),
+             LM_EINVAL, "too many rows");
   const int64_t need = attention_bytes(plan, head_dim);
   LM_REQUIRE(need == 0 || (workspace && aligned16(workspace)), LM_EINVAL,
              "attention needs a 16-byte aligned workspace");
