@@ -109,6 +109,8 @@ class AttentionBlock:
             raise ValueError('expected rows [tokens, hidden]')
         if batch.max_new is not None and batch.max_new < 0:
             raise ValueError('invalid number of new tokens')
+        if self.w8a8 and h.dtype is not torch.bfloat16:  # norm_quantize takes fp16 too
+            raise ValueError('expected CUDA bf16 rows [tokens, hidden]')
 
     def forward_(self, h, batch):
         """h [T, H] bf16, updated in place: h += block(h); the new tokens' keys and values join
