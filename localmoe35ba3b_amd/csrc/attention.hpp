@@ -1700,22 +1700,35 @@ __global__ __launch_bounds__((TileForm<D, C>::kWaves * 64), 2) void attention_ti
 }
 
 // ------------------------------------------------------------------ both in one launch
-// Spans of few rows and places of tiles of a call, for a key-value head.  All threads of the W
-// waves; sums is free again afterwards.
+// What few rows read more of their keys than 1536 bytes for each key of a tile (in 512 bytes; the mean
+// of a sequence's tiles taken for all): few rows come first if it is positive for a call.
+template <int D, typename C, int W>
+__device__ __forceinline__ int64_t few_lead(const PagedSequence &q, int blocks, int tiles) {
+  constexpr int64_t kBlock = kBlockKeys<C, W> * D * Cache<C>::kBytes / 512;
+  return blocks * kBlock - (int64_t)tiles * max(q.length - q.count / 2, 0) * 3;
+}
+
+// Spans of few rows and places of tiles of a call, for a key-value head, and whether the former come
+// first.  All threads of the W waves; sums is free again afterwards.
 struct Counts {
   int spans;
   int64_t places;
+  bool few_first;
 };
-template <typename C, int W>
+template <int D, typename C, int W>
 __device__ Counts count_both(const Attention &a, const PagedSequence &mine, uint64_t *sums) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, S = a.batch.sequences;
   TileTotals total = {};
   if (S <= 64) {  // each wave for itself
     const int n = lane < S ? tile_count(a, mine) : 0;
-    const uint64_t blocks = wave_total((uint64_t)(lane < S ? few_blocks<C, W>(a, mine) : 0));
+    const int own = lane < S ? few_blocks<C, W>(a, mine) : 0;  // 64 of at most 2^25
+    const uint32_t blocks = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan((uint32_t)own), 63);
     if (a.room) total = {(int)wave_total((uint64_t)n), wave_total(all_keys(a, mine, n))};
     const int m = a.room ? tile_places(a, total, mine, n) : 1;
-    return {(int)min((uint64_t)a.shares, blocks), (int64_t)wave_total((uint64_t)n * m)};
+    int64_t lead = 0;
+    if (D < 256 && blocks && __any(n > 0))
+      lead = (int64_t)wave_total((uint64_t)few_lead<D, C, W>(mine, own, n));
+    return {(int)min((uint32_t)a.shares, blocks), (int64_t)wave_total((uint64_t)n * m), lead > 0};
   }
   auto all = [&](uint64_t v) {
     v = wave_total(v);
@@ -1726,13 +1739,17 @@ __device__ Counts count_both(const Attention &a, const PagedSequence &mine, uint
     for (int w = 0; w < W; ++w) v += sums[w];
     return v;
   };
-  uint64_t blocks = 0, tiles = 0, keys = 0, places = 0;
+  uint64_t blocks = 0, tiles = 0, keys = 0, places = 0, lead = 0;
   for (int c = tid; c < S; c += W * 64) {
     const PagedSequence q = paged_sequences(a.batch, c, a.tokens);
-    const int n = tile_count(a, q);
-    blocks += few_blocks<C, W>(a, q), tiles += n, keys += all_keys(a, q, n);
+    const int n = tile_count(a, q), own = few_blocks<C, W>(a, q);
+    blocks += own, tiles += n, keys += all_keys(a, q, n);
+    if (D < 256) lead += few_lead<D, C, W>(q, own, n);
   }
-  blocks = all(blocks), places = tiles = all(tiles);
+  // of a thread's blocks no more than the spans count: both sums in one word
+  tiles = all(min(blocks, (uint64_t)a.shares) << 40 | tiles);
+  blocks = tiles >> 40, places = tiles &= (1ULL << 40) - 1;
+  if (D < 256 && blocks && tiles) lead = all(lead);
   if (a.room) {
     total = {(int)tiles, all(keys)};
     places = 0;
@@ -1744,7 +1761,7 @@ __device__ Counts count_both(const Attention &a, const PagedSequence &mine, uint
     places = all(places);
   }
   __syncthreads();
-  return {(int)min((uint64_t)a.shares, blocks), (int64_t)places};
+  return {(int)min((uint64_t)a.shares, blocks), (int64_t)places, places && (int64_t)lead > 0};
 }
 
 // Workgroups of tiles and of few rows, kTurn of each in turn while there are both: the first bound
@@ -1753,7 +1770,15 @@ __device__ Counts count_both(const Attention &a, const PagedSequence &mine, uint
 // 8192 keys beside 32 of one 263 instead of 310 (64) and 380 instead of 463 (128), 24 of 2 to 24
 // 41 instead of 51 (64).  All of one kind first was better for some and 10 % worse than two
 // launches for others, as were places for the most that a call can have of each: those without
-// work then come before some with it.  Heads of 128 have a ring of one step here, so that three
+// work then come before some with it.
+// Only where few rows read far more than the tiles do (few_lead) all of them come first: in turn,
+// tiles hold places that the last spans wait for, which alone do not keep the memory busy.  64 of one
+// behind 1000 to 12000 keys beside short prompts with 1/32 of their keys (heads of 128) 324 us instead
+// of 377 and of 333 in two launches, 200 beside 8 prompts 233 instead of 260 and 236, with heads of 64
+// 221 instead of 247 and 224.  With 1/4 of the keys both orders took the same (128) or in turn 10 % less
+// (64); 100 beside three prompts behind up to 5000 keys 187 instead of 223.  Not with heads of 256,
+// where a workgroup has a CU to itself: one behind 200000 keys beside a prompt 63 instead of 56.
+// Heads of 128 have a ring of one step here, so that three
 // workgroups still share a CU.  With heads of 256 few rows have eight waves as tiles do, one
 // workgroup a CU; of 8 bits 24 sequences of 2 to 24 tokens take 56 us instead of 63, 64 of one
 // beside two prompts 74 instead of 80, 16 prompts alone 75.5 instead of 73.5.  Of 16 bits the two
@@ -1770,15 +1795,22 @@ __global__ __launch_bounds__((TileForm<D, C>::kWaves * 64),
   // One array: with several, the compiler waits for all direct loads at each LDS read.
   __shared__ __attribute__((aligned(16))) char lds[FEW > TILE ? FEW : TILE];
   const PagedSequence mine = lane_sequence(a);
-  const Counts n = count_both<C, W>(a, mine, reinterpret_cast<uint64_t *>(lds));
+  const Counts n = count_both<D, C, W>(a, mine, reinterpret_cast<uint64_t *>(lds));
   const int few = n.spans * a.batch.kv_heads;
   const int64_t tiles = n.places * a.batch.kv_heads;
   // the same for every lane, which the compiler cannot tell of what went through LDS
   const int turns = __builtin_amdgcn_readfirstlane(
       (int)min((int64_t)(few + kTurn - 1) / kTurn, (tiles + kTurn - 1) / kTurn));
-  const int turn = blockIdx.x / kTurn, at = blockIdx.x % kTurn;
-  const int index = (turn < 2 * turns ? turn / 2 : turn - turns) * kTurn + at;
-  const bool tile = turn < 2 * turns ? turn % 2 == 0 : tiles > few;
+  int turn = blockIdx.x / kTurn;
+  bool tile = turn < 2 * turns ? turn % 2 == 0 : tiles > few;
+  if (__builtin_amdgcn_readfirstlane(n.few_first)) {
+    const int own = (few + kTurn - 1) / kTurn;
+    tile = turn >= own;
+    turn -= tile ? own : 0;
+  } else {
+    turn = turn < 2 * turns ? turn / 2 : turn - turns;
+  }
+  const int index = turn * kTurn + blockIdx.x % kTurn;
   const int work = __builtin_amdgcn_readfirstlane(index >= (tile ? tiles : few) ? 0 : tile ? 2 : 1);
   if (work == 2) {
     tile_rows<T, D, C>(a, index, 0, mine, lds);
