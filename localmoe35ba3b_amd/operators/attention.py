@@ -141,7 +141,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, axes=N
     if several:
         positions, axes, places = _positions(positions, axes, pairs, tokens, device)
     else:
-        if positions.get_device() != device or positions.numel() != tokens:
+        if positions.get_device() != device:
             raise ValueError('Expected a CUDA position of every token')
         if positions.dtype is not torch.int64 or not positions.is_contiguous():
             positions = positions.to(torch.int64).contiguous()
@@ -184,9 +184,7 @@ def _page_strides(x):
 
 
 def _scales(scales, k_pages, device):
-    """The C arguments of a cache's scales, () for one of the rows' type."""
-    if scales is None:
-        return ()
+    """The C arguments of a cache's scales."""
     pages, heads, size, _ = k_pages.shape
     blocks = size // BLOCK
     if (scales.dtype is not torch.float32 or scales.get_device() != device
@@ -223,7 +221,8 @@ def check_batch(rows, k_pages, v_pages, starts, lengths, table, scales=None):
     cache's (kv_heads, head_dim)."""
     device = rows.get_device()
     _, _, heads, _, dim = _cache(k_pages, v_pages, rows.dtype if scales is None else _E4M3, device)
-    _scales(scales, k_pages, device)
+    if scales is not None:
+        _scales(scales, k_pages, device)
     _batch(device, starts, lengths, table)
     return heads, dim
 
@@ -244,10 +243,10 @@ def append(k_pages, v_pages, k, v, starts, lengths, table, inv_freq=None, k_weig
     With scales, the pages hold 8 bits: each block of 16 positions takes the smallest power
     of two that brings the values of its rows to 448 at most, from 2^-117 on (fp16: 2^-15).
     As later calls fill it, the scale only grows; rows held already are then rounded again,
-    which changes those below 2^-6 of it alone.  Rows of a block behind a sequence's last keep their bits, and where
-    positions are taken back inside a block, it keeps the scale that they needed.  A value is
-    rounded once, from fp32; beyond 61440 in fp16 (0x1.Ep127 in bf16) it is held as that,
-    infinities and NaN as NaN.
+    which changes those below 2^-6 of it alone.  Rows of a block behind a sequence's last keep
+    their bits, and where positions are taken back inside a block, it keeps the scale that they
+    needed.  A value is rounded once, from fp32; beyond 61440 in fp16 (0x1.Ep127 in bf16) it is
+    held as that, infinities and NaN as NaN.
     With q [T, q_heads, D], returns the queries normed and rotated for
     paged_attention, 0 in rows of no sequence.  The rows that a call writes must differ:
     no page twice among the new positions of its sequences."""
@@ -272,7 +271,7 @@ def append(k_pages, v_pages, k, v, starts, lengths, table, inv_freq=None, k_weig
         q_args = (q.data_ptr(), q_token, q_head, q_heads, q_w, q_out.data_ptr())
     k_weight, k_w = _weight(k_weight, dim, device)
     inv_freq, freq, pairs = _frequencies(inv_freq, dim, device)
-    name, places = 'lm_paged_append', ()
+    name, scale_args, places = 'lm_paged_append', (), ()
     if scales is not None or positions is not None or axes is not None:
         name, places = 'lm_paged_append_axes', (0, 0, 1, 0)
         if positions is not None:
@@ -280,11 +279,11 @@ def append(k_pages, v_pages, k, v, starts, lengths, table, inv_freq=None, k_weig
         elif axes is not None:
             raise ValueError('axes need positions')
         if scales is not None:
-            name = 'lm_paged_append_e4m3'
+            name, scale_args = 'lm_paged_append_e4m3', _scales(scales, k_pages, device)
     _lib.launch(device, name, k.data_ptr(), k_token, k_head, k_w, v.data_ptr(), v_token, v_head,
-                *q_args, k_pages.data_ptr(), v_pages.data_ptr(), *_scales(scales, k_pages, device),
-                pages, stride, heads, size, dim, *_batch(device, starts, lengths, table), *places,
-                freq, pairs, tokens, eps, _lib.dtype_code(dtype))
+                *q_args, k_pages.data_ptr(), v_pages.data_ptr(), *scale_args, pages, stride, heads,
+                size, dim, *_batch(device, starts, lengths, table), *places, freq, pairs, tokens,
+                eps, _lib.dtype_code(dtype))
     return q_out
 
 
@@ -335,9 +334,11 @@ def paged_attention(q, k_pages, v_pages, starts, lengths, table, scale=None, gat
         max_new = tokens
     need = _workspace_bytes(tokens, batch[5], q_heads, heads, dim, max_new, batch[4] * size)
     workspace = q.new_empty(need // 2) if need > 0 else None
-    _lib.launch(device, 'lm_paged_attention' if scales is None else 'lm_paged_attention_e4m3',
-                q.data_ptr(), q_token, q_head, q_heads, k_pages.data_ptr(), v_pages.data_ptr(),
-                *_scales(scales, k_pages, device), pages, stride, heads, size, dim, *batch, tokens,
+    name, scale_args = 'lm_paged_attention', ()
+    if scales is not None:
+        name, scale_args = 'lm_paged_attention_e4m3', _scales(scales, k_pages, device)
+    _lib.launch(device, name, q.data_ptr(), q_token, q_head, q_heads, k_pages.data_ptr(),
+                v_pages.data_ptr(), *scale_args, pages, stride, heads, size, dim, *batch, tokens,
                 max_new, dim ** -0.5 if scale is None else scale, *gate_args, out.data_ptr(),
                 _lib.ptr(workspace), need, _lib.dtype_code(dtype))
     return out
