@@ -83,6 +83,12 @@ def _check_rows(x):
         raise ValueError('Expected CUDA rows with K divisible by 128')
 
 
+def _check_bank(q, scale):
+    if (q.dtype is not torch.int8 or scale.dtype is not torch.float32
+            or not (q.is_cuda and scale.is_cuda)):
+        raise ValueError('Expected CUDA int8 weights and fp32 scales')
+
+
 def grouped_linear(x, table, experts, n, field, shared):
     """Grouped W8A8 decode GEMV; activation quantization is fused into the
     kernel.  x bf16 or fp16; the output is in x.dtype (w8a8.py:46)."""
@@ -119,6 +125,7 @@ def linear(x, q, scale, swiglu=False):
     m = x.shape[0]
     if k % 128 or x.shape[-1] != k or scale.shape != (n, k // 128):
         raise ValueError('Invalid INT8 group geometry')
+    _check_bank(q, scale)
     if m > 8:
         xq, xs = quantize(x)
         return gemm(xq, xs, q, scale, swiglu, out_dtype=x.dtype)
@@ -137,6 +144,8 @@ def gemm(xq, xs, q, scale, swiglu=False, out_dtype=torch.bfloat16):
     or, with swiglu, [M, N/2], in out_dtype (bf16 or fp16)."""
     if not (xq.is_cuda and q.is_cuda) or xq.dtype != torch.int8 or q.dtype != torch.int8:
         raise ValueError('Expected CUDA int8 rows and weights')
+    _check_bank(xq, xs)
+    _check_bank(q, scale)
     m, k = xq.shape
     n = q.shape[0]
     if (k % 128 or q.shape[1] != k or scale.shape != (n, k // 128)

@@ -1,0 +1,41 @@
+"""CPU checks of the W8A8 products' weights and scales: what a kernel would read as something else, or
+not at all, is refused before a launch."""
+import pytest
+import torch
+
+from localmoe35ba3b_amd import _lib
+from localmoe35ba3b_amd.operators import w8a8
+from tests.test_attention_checks import F32, gpu
+
+I8 = torch.int8
+
+
+def linear(rows=5, **change):
+    a = dict(x=gpu(rows, 256), q=gpu(32, 256, dtype=I8), scale=gpu(32, 2, dtype=F32))
+    a.update(change)
+    return w8a8.linear(**a)
+
+
+def gemm(**change):
+    a = dict(xq=gpu(5, 256, dtype=I8), xs=gpu(5, 2, dtype=F32), q=gpu(32, 256, dtype=I8),
+             scale=gpu(32, 2, dtype=F32))
+    a.update(change)
+    return w8a8.gemm(**a)
+
+
+@pytest.mark.parametrize('run,change', [
+    (linear, dict(scale=gpu(32, 2))), (linear, dict(scale=torch.zeros(32, 2))),
+    (linear, dict(q=gpu(32, 256))), (linear, dict(q=torch.zeros(32, 256, dtype=I8))),
+    (linear, dict(rows=20, scale=gpu(32, 2))), (linear, dict(rows=20, q=gpu(32, 256))),
+    (gemm, dict(scale=gpu(32, 2))), (gemm, dict(scale=torch.zeros(32, 2))),
+    (gemm, dict(xs=gpu(5, 2))), (gemm, dict(xs=torch.zeros(5, 2))), (gemm, dict(q=gpu(32, 256)))])
+def test_operators_refuse_other_banks(run, change, monkeypatch):
+    calls = []
+    monkeypatch.setattr(_lib, 'call', lambda name, *args: calls.append(name))
+    monkeypatch.setattr(_lib, 'stream', lambda device=None: 0)
+    run(**{n: v for n, v in change.items() if n == 'rows'})
+    assert calls
+    at = len(calls)
+    with pytest.raises(ValueError):
+        run(**change)
+    assert not any('gemm' in c or 'linear' in c for c in calls[at:])
