@@ -62,6 +62,9 @@ class AttentionBlock:
                 raise ValueError('projections have groups of 128')
             if tuple(bank['scale'].shape) != (bank['q'].shape[0], bank['q'].shape[1] // 128):
                 raise ValueError('the scales do not match their projection')
+            if (bank['q'].dtype != torch.int8 or bank['scale'].dtype != torch.float32
+                    or not qkv['q'].device == bank['q'].device == bank['scale'].device):
+                raise ValueError('expected int8 projections and fp32 scales on one device')
         for w, n in ((norm, qkv['q'].shape[1]), (q_norm, head_dim), (k_norm, head_dim)):
             if w is not None and w.numel() != n:
                 raise ValueError('norm weight does not match its rows')

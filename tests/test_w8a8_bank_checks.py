@@ -1,10 +1,11 @@
 """CPU checks of the W8A8 products' weights and scales: what a kernel would read as something else, or
-not at all, is refused before a launch."""
+not at all, is refused before a launch, by the operators and by the attention block."""
 import pytest
 import torch
 
 from localmoe35ba3b_amd import _lib
 from localmoe35ba3b_amd.operators import w8a8
+from localmoe35ba3b_amd.runtime.attention import AttentionBlock
 from tests.test_attention_checks import F32, gpu
 
 I8 = torch.int8
@@ -39,3 +40,19 @@ def test_operators_refuse_other_banks(run, change, monkeypatch):
     with pytest.raises(ValueError):
         run(**change)
     assert not any('gemm' in c or 'linear' in c for c in calls[at:])
+
+
+@pytest.mark.parametrize('w8a8', [False, True])
+@pytest.mark.parametrize('side,name,dtype', [('qkv', 'q', torch.uint8), ('qkv', 'scale', torch.bfloat16),
+                                             ('o', 'q', torch.uint8), ('o', 'scale', torch.float16)])
+def test_blocks_refuse_other_banks(side, name, dtype, w8a8):
+    banks = dict(qkv={'q': gpu(512, 256, dtype=I8), 'scale': gpu(512, 2, dtype=F32)},
+                 o={'q': gpu(256, 256, dtype=I8), 'scale': gpu(256, 2, dtype=F32)})
+    AttentionBlock(**banks, q_heads=4, kv_heads=2, head_dim=64, gated=False, w8a8=w8a8)
+    banks[side][name] = gpu(*banks[side][name].shape, dtype=dtype)
+    with pytest.raises(ValueError, match='int8 projections'):
+        AttentionBlock(**banks, q_heads=4, kv_heads=2, head_dim=64, gated=False, w8a8=w8a8)
+    banks[side][name] = torch.empty(banks[side][name].shape, device='meta',
+                                    dtype=I8 if name == 'q' else F32)  # stands for another device
+    with pytest.raises(ValueError, match='one device'):
+        AttentionBlock(**banks, q_heads=4, kv_heads=2, head_dim=64, gated=False, w8a8=w8a8)
