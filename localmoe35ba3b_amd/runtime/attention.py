@@ -71,8 +71,9 @@ class AttentionBlock:
         self.pairs = attention.check_frequencies(inv_freq, head_dim)
         if axes is not None and axes.numel() != self.pairs:
             raise ValueError('Expected an axis of every rotated pair')
-        if w8a8 and qkv['q'].shape[1] > 16384:
-            raise ValueError('W8A8 projections take rows of at most 16384 values')
+        if w8a8 and (qkv['q'].shape[1] > 16384 or o['q'].shape[1] > 65536):
+            raise ValueError('W8A8 projections take rows of at most 16384 values, the second one '
+                             'of 65536')
         self.k_pages = self.v_pages = self.scales = None
 
     def allocate(self, pages, page_size=64, dtype=torch.bfloat16):

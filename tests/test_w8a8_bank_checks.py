@@ -56,3 +56,12 @@ def test_blocks_refuse_other_banks(side, name, dtype, w8a8):
                                     dtype=I8 if name == 'q' else F32)  # stands for another device
     with pytest.raises(ValueError, match='one device'):
         AttentionBlock(**banks, q_heads=4, kv_heads=2, head_dim=64, gated=False, w8a8=w8a8)
+
+
+def test_blocks_refuse_rows_wider_than_their_second_product():
+    heads = 1028  # 65792 channels
+    banks = dict(qkv={'q': gpu(heads * 64 * 3, 128, dtype=I8), 'scale': gpu(heads * 64 * 3, 1, dtype=F32)},
+                 o={'q': gpu(128, heads * 64, dtype=I8), 'scale': gpu(128, heads // 2, dtype=F32)})
+    AttentionBlock(**banks, q_heads=heads, kv_heads=heads, head_dim=64, gated=False)
+    with pytest.raises(ValueError, match='65536'):
+        AttentionBlock(**banks, q_heads=heads, kv_heads=heads, head_dim=64, gated=False, w8a8=True)
