@@ -42,12 +42,12 @@
 //                         four waves on 32-key tiles.  Two tiles in LDS, one read
 //                         and one loaded.  Few tiles split their keys over workgroups
 //                         too.  2048 tokens of 16 heads of 256 (2 key-value heads)
-//                         behind 8192 keys: 293 to 302 us in a long run of calls,
-//                         1024 to 1054 TFLOP/s (1371 for a large library product);
-//                         without a history 64 us.
+//                         behind 8192 keys: 293 to 306 us on the same inputs, 320
+//                         on others each time, 966 to 1054 TFLOP/s (1372 for a
+//                         large library product); without a history 64 to 75 us.
 //  attention_both_kernel  the two in one launch, for calls that may have both (not with
 //                         heads of 256 in 16 bits).
-//  attention_combine_kernel  joins the parts of split keys, 4 to 12 us: the partial
+//  attention_combine_kernel  joins the parts of split keys, 3 to 10 us: the partial
 //                         sums are fp32, written and read once.
 //
 // A cache of 8 bits, e4m3 with a power of two for each 16 positions of a head, goes the
@@ -62,7 +62,7 @@
 // looked up with it, 64 blocks a wave at a time, as two exponents in a lane's register.
 // Times as above: 262144 keys 49 us (5.5 TB/s), 64 sequences 49 us (4.9 TB/s; of both
 // some 6 us are the chain from lengths to pages to rows, before which nothing is under
-// way), 2048 tokens behind 8192 keys 298 to 306 us.
+// way), 2048 tokens behind 8192 keys 298 to 316 us.
 #pragma once
 
 #include <cmath>
@@ -1778,11 +1778,11 @@ __device__ Counts count_both(const Attention &a, const PagedSequence &mine, uint
 // 221 instead of 247 and 224.  With 1/4 of the keys both orders took the same (128) or in turn 10 % less
 // (64); 100 beside three prompts behind up to 5000 keys 187 instead of 223.  Not with heads of 256,
 // where a workgroup has a CU to itself: one behind 200000 keys beside a prompt 63 instead of 56.
-// Heads of 128 have a ring of one step here, so that three
-// workgroups still share a CU.  With heads of 256 few rows have eight waves as tiles do, one
-// workgroup a CU; of 8 bits 24 sequences of 2 to 24 tokens take 56 us instead of 63, 64 of one
-// beside two prompts 74 instead of 80, 16 prompts alone 75.5 instead of 73.5.  Of 16 bits the two
-// do not fit the registers there, and have two launches.
+// Heads of 128 have a ring of one step here, so that three workgroups still share a CU.  With heads
+// of 256 few rows have eight waves as tiles do, one workgroup a CU; of 8 bits 24 sequences of 2 to 24
+// tokens take 56 us instead of 63, 64 of one beside two prompts 74 instead of 80, 16 prompts alone
+// 75.5 instead of 73.5, two of 1000 tokens (one behind 8000 keys) 254 instead of 245.  Of 16 bits the
+// two do not fit the registers there, and have two launches.
 template <int D, typename C>
 constexpr bool kBoth = D < 256 || Cache<C>::kScaled;
 constexpr int kTurn = 256;

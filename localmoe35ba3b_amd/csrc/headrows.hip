@@ -17,9 +17,10 @@
 // requested at the start, beside the position, whose lookups (sequence, length, page) are
 // the longest chain of a small call.
 //
-// Bound by the rows' bytes where there are many, by that chain where there are few.  18 heads
-// of 256: 4096 tokens 16 us (75.5 MB, 4.7 TB/s), one token 3 us, of three axes too; 64 tokens
-// into a cache 4 us; 3310 tokens into a cache (48 heads of 128) 18 us (81 MB, 4.5 TB/s).
+// Bound by the rows' bytes where there are many, by that chain where there are few.  From memory,
+// 18 heads of 256: 4096 tokens 18 us (75.5 MB, 4.2 TB/s; 16.5 us with the rows in the caches), one
+// token 3 us, of three axes too; 64 tokens into a cache 4 us; 3310 tokens into a cache (48 heads of
+// 128) 21.5 us (81 MB, 3.8 TB/s; 18.4).
 #include "paged.hpp"
 
 namespace lm {
@@ -227,9 +228,10 @@ __global__ __launch_bounds__(256) void head_rows_kernel(HeadRows a) {
 // (int8 under such scales would be rounded again in every row whenever one grows.)
 //
 // Blocks come first, as their chain is the longest: lengths, then page and rows, then the exchange
-// of the largest value; the queries' rows go as without a cache, a workgroup a token.  20 heads of
-// 256 (16 of them queries'): 64 tokens 4.9 us, 4096 tokens 20 us (79.7 MB, 4.0 TB/s), 16000 65 us
-// (4.8 TB/s); 3310 tokens, 48 heads of 128, 18 us (74.6 MB, 4.1 TB/s).  The next side's rows
+// of the largest value; the queries' rows go as without a cache, a workgroup a token.  From memory,
+// 20 heads of 256 (16 of them queries'): 64 tokens 4.7 us, 4096 tokens 21.6 us (79.7 MB, 3.7 TB/s;
+// 19.0 us with the rows in the caches), 16000 64.6 us (4.8 TB/s); 3310 tokens, 48 heads of 128,
+// 20.7 us (74.6 MB, 3.6 TB/s; 18.8).  The next side's rows
 // requested before the one at hand cost registers and gained nothing; the blocks' workgroups spread
 // among the queries' were slower.
 struct E4m3Pages {
@@ -330,7 +332,7 @@ __device__ __forceinline__ void block_rows(const HeadRows &a, const E4m3Pages &p
     bool value, rotated;
   };
   auto side = [&](int first) {
-    const int unit = min(first + wave / WAVES, 2 * a.k_heads - 1);  // the last one twice alike
+    const int unit = first + wave / WAVES;  // `first` is even where a workgroup has two at a time
     const bool value = unit >= a.k_heads, rotated = !value && lane * 8 < 2 * a.half;
     return Side{value ? unit - a.k_heads : unit, rotated ? lane * 4 : lane * 8,
                 rotated ? a.half + lane * 4 : lane * 8 + 4, value, rotated};

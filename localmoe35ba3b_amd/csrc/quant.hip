@@ -80,9 +80,10 @@ __global__ __launch_bounds__(256) void act_quant_kernel(const uint16_t *__restri
 // waves, eight values a thread and chunk, a group of 128 in 16 lanes; it is read once.  Not finite
 // values leave a scale that is not.  x may be h itself: a thread's loads come before its stores.
 //
-// Bound by its bytes, 7 a value: 2048 rows of 2048 7.5 us (29.5 MB, 3.9 TB/s with the start),
-// 8192 rows 19.8 us (5.9 TB/s); one row 2 us.  Divisions and a conversion for each byte took twice
-// that (14.0 and 44.5 us).  A wave a row of 2048, without a barrier, took 8.1 us.
+// Bound by its bytes, 7 a value, 3 without x, and by a launch's start and end: 2048 rows of 2048 take
+// 8.3 us from memory (29.5 MB, 3.6 TB/s; 6.4 us with the rows in the caches), without x 5.2 us; 8192
+// rows 22.1 us (5.3 TB/s), without x 13.2; one row 2 us.  Divisions and a conversion for each byte
+// took twice that.  A wave a row of 2048, without a barrier, took 8.1 us instead of 7.5.
 template <typename T, int WAVES, int CHUNKS, bool ADD>
 __global__ __launch_bounds__(256) void norm_quant_kernel(uint16_t *h, const uint16_t *x,
                                                          const float *__restrict__ w,
