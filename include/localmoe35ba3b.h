@@ -415,9 +415,10 @@ int lm_paged_append_axes(const void *k, int64_t k_token_stride, int64_t k_head_s
  * rows that the call writes to it (e at least -117 in bf16, -15 in fp16).  A block
  * that goes on keeps its e if that suffices (and is no less than those, where the
  * caller wrote it); otherwise e grows, and the rows held already are rounded again
- * to e4m3 (which changes only values below 2^-6 of the new scale).  Rows of a block behind its last position keep their bits.  Values
- * are rounded once, from fp32; sizes beyond four significant bits of `dtype` (61440
- * in fp16) are held as that, infinities and NaN as NaN. */
+ * to e4m3 (which changes only values below 2^-6 of the new scale).  Rows of a block
+ * behind its last position keep their bits.  Values are rounded once, from fp32;
+ * sizes beyond four significant bits of `dtype` (61440 in fp16) are held as that,
+ * infinities and NaN as NaN. */
 int lm_paged_append_e4m3(const void *k, int64_t k_token_stride, int64_t k_head_stride,
                          const float *k_weight, const void *v, int64_t v_token_stride,
                          int64_t v_head_stride, const void *q, int64_t q_token_stride,

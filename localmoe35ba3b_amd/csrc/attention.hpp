@@ -1946,12 +1946,13 @@ int64_t both_groups(const AttentionPlan &p, int64_t kv_heads) {
   const int64_t tiles = p.tiles * kv_heads * p.splits;
   return ((tiles + kTurn - 1) / kTurn + (p.few_grid + kTurn - 1) / kTurn) * kTurn;
 }
-// Whether the launches that take up more than a call's tiles or its sequences' key-value heads have
-// fewer than 2^32 threads: both kinds together, and the joining of both.
+// Whether a call's largest launches have fewer than 2^32 threads: of tiles, of sequences' key-value
+// heads, of both kinds together, and of the joining of both.
 template <bool E4M3_CACHE>
 bool attention_fits(const AttentionPlan &p, int64_t tokens, int64_t q_heads, int64_t kv_heads,
                     int64_t head_dim) {
   constexpr int64_t kThreads = 1LL << 32;
+  if (p.tiles * kv_heads * 512 >= kThreads) return false;
   if (p.few && p.tile && (head_dim < 256 || E4M3_CACHE) &&
       both_groups(p, kv_heads) * (head_dim == 256 ? 512 : 256) >= kThreads)
     return false;
@@ -2041,7 +2042,7 @@ int paged_attention(const void *q, int64_t q_token_stride, int64_t q_head_stride
              LM_EINVAL, "head rows must be 16-byte aligned");
   const AttentionPlan plan = attention_plan(tokens, sequences, q_heads, kv_heads, head_dim, max_new,
                                             table_pages * page_size, E4M3_CACHE);
-  LM_REQUIRE(sequences * kv_heads < (1LL << 24) && plan.tiles * kv_heads < (1LL << 23) &&
+  LM_REQUIRE(sequences * kv_heads < (1LL << 24) &&
                  attention_fits<E4M3_CACHE>(plan, tokens, q_heads, kv_heads, head_dim),
              LM_EINVAL, "too many rows");
   const int64_t need = attention_bytes(plan, head_dim);

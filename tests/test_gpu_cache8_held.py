@@ -56,6 +56,21 @@ def test_append_leaves_what_is_held(dev, dim, heads, page, dtype):
         length += n
 
 
+@pytest.mark.parametrize('dim,heads', [(64, 20), (128, 9), (256, 12)])
+def test_append_of_many_blocks_and_heads(dev, dim, heads):
+    """Workgroups that take several sides of a block, one after another: a chunk that goes on inside a
+    block of other sizes, and one behind it."""
+    gen, page = seeded(dim + heads), 64
+    kp, vp, scales = to(dev, *C.random_cache(gen, 28, heads, page, dim, BF16))
+    want, scale64 = C.held(kp, vp, scales), [scales[:, :, s].cpu().double() for s in range(2)]
+    table, length = torch.randperm(28, generator=gen)[:26].tolist(), 0
+    for n in (5, 1500, 90):
+        sizes = torch.exp2(torch.randint(-7, 8, (2, n, heads, 1), generator=gen).float())
+        k, v = ((torch.randn(n, heads, dim, generator=gen) * s).to(BF16) for s in sizes)
+        plain_append((kp, vp, scales), want, scale64, k, v, length, table, page, BF16)
+        length += n
+
+
 @TYPES
 @pytest.mark.parametrize('dim,page', [(64, 16), (128, 64), (256, 32)])
 def test_append_leaves_what_is_held_beside_normed_keys(dev, dim, page, dtype):
